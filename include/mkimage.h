@@ -64,8 +64,8 @@ mk_status mk_event_elapsed_ms(void* start, void* stop, float* ms);
  * reference's Tensor with dims[0] = in features, qwen_image.cpp:79-111); bf16 = uint16 bit patterns; fp8 = OCP e4m3.
  * ------------------------------------------------------------------------------------------------------------ */
 
-enum mk_dtype { MK_F32 = 0, MK_BF16 = 1, MK_FP8_E4M3 = 2, MK_F16 = 3, MK_DTYPE_OTHER = 255 /* a file dtype the
-                                                                                          kernels do not take */ };
+enum mk_dtype { MK_F32 = 0, MK_BF16 = 1, MK_FP8_E4M3 = 2, MK_F16 = 3, MK_I8 = 4 /* rows and matrices of the 8-bit
+                integer path (mk_gemm_i8) */, MK_DTYPE_OTHER = 255 /* a file dtype the kernels do not take */ };
 
 /* The GEMM's fused epilogue: what happens to acc = A W^T (* wscale[n]) + bias[n]. */
 enum mk_epilogue {
@@ -177,6 +177,22 @@ typedef struct mk_conv_args {
 } mk_conv_args;
 mk_status mk_conv3x3(const mk_conv_args* a, void* stream);
 
+/* proj in 8-bit integers: C = epilogue(sum_k A[r][k] W[n][k] * ascale[r] * wscale[n] + bias[n]), A and W int8 with one
+ * fp32 scale a row of A (a token) and a row of W (an output channel), the sum exact (int32), the rest in fp32. No
+ * counterpart in the reference (its 8-bit weights are widened before the product).
+ *   a: int8 [batch][M][lda], w: int8 [N][K], w_dtype MK_I8; lda and stride_a in elements; rows as mk_quantize_i8_rows and
+ *      mk_gate_norm write them, but any int8 value, -128 too, is taken;
+ *   ascale: [batch][M] (row b M + r), wscale: [N], both required;
+ *   the rest as in mk_gemm, epilogues STORE, GELU_TANH, SILU, SWIGLU, GEGLU (C f32, bf16 or f16), GATE_ADD, GATE_TANH
+ *   and ADD (C the fp32 residual). HEADS and PAIR_SUM are MK_ERR_UNSUPPORTED: store q|k|v and pack it with mk_heads.
+ * K is a multiple of 16 up to 131056 (the sum of K products of 8 bits fits int32), N of 4 (SWIGLU, GEGLU: of 8), M any;
+ * lda and stride_a multiples of 16, ldc, stride_c and gate_alt of 4; A, W, wscale, bias and gate are 16-byte aligned, C
+ * for 4 of its elements, ascale for one. C must not overlap an input. Columns N .. ldc - 1 of C are left as they were. A
+ * row's values do not depend on the launch's other rows: integer sums have no order, and the rest is one expression of
+ * the row's and the channel's numbers. Allocates nothing and keeps no workspace: it may be captured, and may run on
+ * several streams at once. */
+mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void* stream);
+
 /* GEMV for a few rows (the time embedding and modulation projections, rows <= 4):
  * y[r][n] = sum_k W[n][k] bf16(x'[r][k]) + b[n] with x' = silu(x) when silu_x (silu(temb) is the modulation
  * layers' input), else x; x fp32 [rows][K], W bf16 [N][K], y fp32. The activation is rounded to bf16 as every GEMM's
@@ -193,6 +209,47 @@ mk_status mk_ln_modulate(const float* x, uint32_t rows, uint32_t n, const float*
  * [rows][n]; row selection of the gate as in mk_ln_modulate. */
 mk_status mk_gate_add(float* x, const void* y, uint32_t y_dtype, uint32_t rows, uint32_t n, const float* gate,
                       int64_t alt, uint32_t split, uint32_t seg_rows, int tanh_gate, void* stream);
+
+/* A block's end and the next one's start in one pass over the residual stream (no counterpart in the reference, which
+ * runs gate_add and ln_modulate, and has no norm after a block):
+ *   v  = norm1(y)                                     the block's output; norm1 NONE, RMS or LAYER with w1, b1
+ *   x' = residual_scale x + g v                       g = gate[c], tanh(gate[c]) with tanh_gate, or 1 without a gate
+ *   h  = norm2(x') (1 + scale[c]) + shift[c]          norm2 NONE, RMS or LAYER with w2, b2
+ * x' goes to x_out in fp32 and h to out: f32, bf16 or f16, or int8 rows with their scales (the rule of
+ * mk_quantize_i8_rows on the fp32 h) for mk_gemm_i8. RMS: v rsqrt(mean v^2 + eps) w; LAYER: (v - mean) rsqrt(var + eps) w +
+ * b; statistics and everything before out in fp32.
+ * Row r is row i = r % seg_rows of segment r / seg_rows (seg_rows 0: all rows are one segment); gate, scale and shift are read
+ * at + segment * mod_stride, + alt too where i < split: one modulation row for each sample of a batch, another for its
+ * first rows. */
+enum mk_norm { MK_NORM_NONE = 0, MK_NORM_RMS = 1, MK_NORM_LAYER = 2 };
+typedef struct mk_gate_norm_args {
+    const float* x;       /* [rows][ldx] */
+    float* x_out;         /* [rows][ldx]: x', may be x itself; NULL: x' is not stored */
+    const void* y;        /* [rows][ldy] f32, bf16 or f16 (y_dtype); NULL: x' = x, only the norm (then no norm1, gate,
+                             residual_scale or x_out) */
+    void* out;            /* [rows][ldo] out_dtype; NULL: only the residual (then no norm2, scale or shift) */
+    float* out_scale;     /* [rows], for out_dtype MK_I8 */
+    const float* w1;      /* [n] or NULL (1); b1, b2: LAYER only, [n] or NULL (0) */
+    const float* b1;
+    const float* w2;
+    const float* b2;
+    const float* gate;    /* [n] a modulation row, or NULL */
+    const float* scale;
+    const float* shift;
+    int64_t ldx, ldy, ldo; /* elements between rows, >= n, multiples of 4 */
+    int64_t alt, mod_stride; /* floats, multiples of 4 */
+    uint32_t rows, n;     /* n a multiple of 4 up to 16384 */
+    uint32_t y_dtype, out_dtype;
+    uint32_t norm1, norm2; /* mk_norm */
+    uint32_t tanh_gate;
+    uint32_t split, seg_rows;
+    float residual_scale; /* 0: 1 */
+    float eps1, eps2;
+} mk_gate_norm_args;
+/* The vectors, x and x_out are 16-byte aligned, y and out for 4 of their elements, out_scale for one. Apart from x_out == x
+ * no output overlaps an input or another output. Infinities and NaNs stay in their row. Allocates nothing and keeps no
+ * workspace: it may be captured, and may run on several streams at once. */
+mk_status mk_gate_norm(const mk_gate_norm_args* a, void* stream);
 
 /* heads_norm_half / heads_half (qwen_image.cpp:226-250, sdxl.cpp:439-448): per (row, head) of x bf16
  * [batch][rows][ld] at column col0 + head * d: optional RMSNorm * w, RoPE from table rows rope[row0 + r], written
@@ -267,6 +324,13 @@ uint64_t mk_tensor_key(uint64_t seed, const char* name);
 /* Per-output-row fp8 quantisation: scale[r] = max|W[r]| / 448 (1 for a zero row), dst[r][c] = e4m3(W[r][c] /
  * scale[r]) rounded to nearest even, saturating; src bf16 [rows][cols]. */
 mk_status mk_quantize_fp8_rows(const void* src, uint64_t rows, uint64_t cols, void* dst, float* scale, void* stream);
+/* Per-row int8 quantisation, of weights once and of activations on the way into mk_gemm_i8: with a = max|src[r]|,
+ * scale[r] = a / 127 and dst[r][c] = 127 src[r][c] / a rounded to nearest, ties to even, decided exactly (values in
+ * -127 .. 127). A row of a < 2^-100 counts as zero: dst 0, scale 1. A row with an infinity or a NaN: dst 0, scale NaN, so
+ * its products are NaN and no other row's are. src f32, bf16 or f16 [rows][ld], dst int8 [rows][cols] (any cols; a multiple
+ * of 16 with 16-byte aligned src rows is the fast path). Allocates nothing. No counterpart in the reference. */
+mk_status mk_quantize_i8_rows(const void* src, uint32_t src_dtype, uint64_t rows, uint64_t cols, int64_t ld, void* dst,
+                              float* scale, void* stream);
 /* fp32 <-> bf16 conversions on the device */
 mk_status mk_f32_to_bf16(const float* x, size_t n, void* y, void* stream);
 mk_status mk_bf16_to_f32(const void* x, size_t n, float* y, void* stream);

@@ -14,9 +14,10 @@ import numpy as np
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libmkimage.so"
 
-F32, BF16, FP8, F16, DTYPE_OTHER = 0, 1, 2, 3, 255
+F32, BF16, FP8, F16, I8, DTYPE_OTHER = 0, 1, 2, 3, 4, 255
 EPI_STORE, EPI_GELU_TANH, EPI_GATE_ADD, EPI_GATE_TANH, EPI_SILU, EPI_ADD, EPI_HEADS, EPI_SWIGLU, EPI_GEGLU, \
     EPI_PAIR_SUM = range(10)
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
 FAMILY_DUAL, FAMILY_Q21, FAMILY_SDXL = 0, 1, 2
 
 _vp, _sz, _u32, _u64, _i64, _f, _d, _i = (C.c_void_p, C.c_size_t, C.c_uint32, C.c_uint64, C.c_int64, C.c_float,
@@ -39,6 +40,14 @@ class GemmArgs(C.Structure):
                 ("gate_alt", _i64), ("split", _u32), ("seg_rows", _u32), ("M", _u32), ("N", _u32), ("K", _u32),
                 ("lda", _i64), ("ldc", _i64), ("stride_a", _i64), ("stride_c", _i64), ("batch", _u32),
                 ("w_dtype", _u32), ("c_dtype", _u32), ("epilogue", _u32), ("heads", C.POINTER(HeadsArgs))]
+
+
+class GateNormArgs(C.Structure):
+    _fields_ = [(n, _vp) for n in ("x", "x_out", "y", "out", "out_scale", "w1", "b1", "w2", "b2", "gate", "scale",
+                                   "shift")] + \
+               [(n, _i64) for n in ("ldx", "ldy", "ldo", "alt", "mod_stride")] + \
+               [(n, _u32) for n in ("rows", "n", "y_dtype", "out_dtype", "norm1", "norm2", "tanh_gate", "split",
+                                    "seg_rows")] + [(n, _f) for n in ("residual_scale", "eps1", "eps2")]
 
 
 class Config(C.Structure):
@@ -88,6 +97,9 @@ _SIGS = {
     "mk_event_elapsed_ms": (_i, [_vp, _vp, C.POINTER(_f)]),
     "mk_gemm": (_i, [C.POINTER(GemmArgs), _vp]),
     "mk_gemm_grouped": (_i, [_vp, _u32, _vp]),
+    "mk_gemm_i8": (_i, [C.POINTER(GemmArgs), _vp, _vp]),
+    "mk_gate_norm": (_i, [C.POINTER(GateNormArgs), _vp]),
+    "mk_quantize_i8_rows": (_i, [_vp, _u32, _u64, _u64, _i64, _vp, _vp, _vp]),
     "mk_gemm_set_wait_limit": (_i, [_u32]),
     "mk_gemm_plan": (_i, [_vp, _u32, _u32, C.POINTER(_u32)]),
     "mk_gemv": (_i, [_vp, _u32, _u32, _vp, _vp, _u32, _vp, _i, _vp]),
@@ -194,7 +206,8 @@ def call(name, *args):
 # device memory
 # ---------------------------------------------------------------------------------------------------------------
 
-_NP = {F32: np.float32, BF16: np.uint16, FP8: np.uint8, F16: np.uint16}
+_NP = {F32: np.float32, BF16: np.uint16, FP8: np.uint8, F16: np.uint16, I8: np.int8}
+_SIZE = {F32: 4, BF16: 2, FP8: 1, F16: 2, I8: 1}
 
 
 # Device memory of dropped Dev objects: freed only after a device-wide synchronisation, so a pointer taken from a
@@ -319,6 +332,47 @@ def _check_gemm_grouped(args, count, stream=None):
         gemm_extents(g, f"mk_gemm_grouped[{i}]")
 
 
+def _check_gemm_i8(args, ascale, stream=None):
+    g = _struct(args, GemmArgs)
+    if g.M == 0 or g.N == 0 or g.batch == 0:
+        return
+    glu = g.epilogue in (EPI_SWIGLU, EPI_GEGLU)
+    check_extent(g.a, (g.batch - 1) * g.stride_a + (g.M - 1) * g.lda + g.K, "mk_gemm_i8: A")
+    check_extent(g.w, g.N * g.K, "mk_gemm_i8: W")
+    check_extent(ascale, g.batch * g.M * 4, "mk_gemm_i8: ascale")
+    check_extent(g.wscale, g.N * 4, "mk_gemm_i8: wscale")
+    check_extent(g.bias, g.N * 4, "mk_gemm_i8: bias")
+    if g.epilogue in (EPI_GATE_ADD, EPI_GATE_TANH):
+        check_extent(g.gate, (g.N + (max(int(g.gate_alt), 0) if g.split else 0)) * 4, "mk_gemm_i8: gate")
+    check_extent(g.c, ((g.batch - 1) * g.stride_c + (g.M - 1) * g.ldc + (g.N // 2 if glu else g.N)) *
+                 _SIZE.get(g.c_dtype, 4), "mk_gemm_i8: C")
+
+
+def _check_gate_norm(args, stream=None):
+    g = _struct(args, GateNormArgs)
+    if g.rows == 0 or g.n == 0:
+        return
+    what = "mk_gate_norm: "
+    for name, ld, size in (("x", g.ldx, 4), ("x_out", g.ldx, 4), ("y", g.ldy, _SIZE.get(g.y_dtype, 4)),
+                           ("out", g.ldo, _SIZE.get(g.out_dtype, 4))):
+        check_extent(getattr(g, name), ((g.rows - 1) * ld + g.n) * size, what + name)
+    if g.out_dtype == I8:
+        check_extent(g.out_scale, g.rows * 4, what + "out_scale")
+    for name in ("w1", "b1", "w2", "b2"):
+        check_extent(getattr(g, name), g.n * 4, what + name)
+    seg = g.seg_rows or g.rows
+    last = (g.rows - 1) // seg * max(int(g.mod_stride), 0) + (max(int(g.alt), 0) if g.split else 0)
+    for name in ("gate", "scale", "shift"):
+        check_extent(getattr(g, name), (last + g.n) * 4, what + name)
+
+
+def _check_quantize_i8(src, dtype, rows, cols, ld, dst, scale, stream=None):
+    if rows and cols:
+        check_extent(src, ((rows - 1) * ld + cols) * _SIZE.get(dtype, 4), "mk_quantize_i8_rows: src")
+        check_extent(dst, rows * cols, "mk_quantize_i8_rows: dst")
+        check_extent(scale, rows * 4, "mk_quantize_i8_rows: scale")
+
+
 def _check_conv(args, stream=None):
     a = _struct(args, ConvArgs)
     grid = (a.h + 2) * (a.width + 2)
@@ -337,7 +391,8 @@ def _check_attention(q, k, vt, out, dtype, batch, heads, kv_heads, d, n_q, q_pad
 
 
 _EXTENT_CHECKS = {"mk_gemm": _check_gemm, "mk_gemm_grouped": _check_gemm_grouped, "mk_conv3x3": _check_conv,
-                  "mk_attention": _check_attention}
+                  "mk_attention": _check_attention, "mk_gemm_i8": _check_gemm_i8, "mk_gate_norm": _check_gate_norm,
+                  "mk_quantize_i8_rows": _check_quantize_i8}
 
 
 class Dev:
