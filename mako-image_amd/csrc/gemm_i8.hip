@@ -22,71 +22,517 @@ struct I8P {
     uint32_t epi, c_dtype;
 };
 
-// The scaled sums of four channels: float(sum) ascale wscale + bias, the same expression everywhere, so a value does not
-// depend on which kernel made it.
-__device__ inline f32x4 i8_scaled(const int (&s)[4], float as, const f32x4& ws, const f32x4& b)
-{
-    f32x4 v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        v[e] = fmaf(float(s[e]) * as, ws[e], b[e]);
-    return v;
-}
-
 __device__ inline f32x4 load4(const float* p, uint32_t c, float none)
 {
     return p ? *reinterpret_cast<const f32x4*>(p + c) : f32x4{none, none, none, none};
 }
 
-// A thread computes one token's four channels (with a gated unit, of both parts) straight from memory.
-__global__ __launch_bounds__(256) void gemm_i8_plain_kernel(I8P p)
+// Epilogue classes (template): a plain store, an activation, the fp32 residual, a gated unit.
+enum { EC_STORE, EC_ACT, EC_RMW, EC_GLU };
+constexpr int epi_class(uint32_t epi)
 {
-    const bool glu = p.epi == MK_EPI_SWIGLU || p.epi == MK_EPI_GEGLU;
-    const uint32_t cols = glu ? p.N / 2 : p.N;
-    const uint32_t r = blockIdx.x * 16 + threadIdx.x / 16, c = (blockIdx.y * 16 + threadIdx.x % 16) * 4, z = blockIdx.z;
-    if (r >= p.M || c >= cols)
-        return;
-    const int8_t* a = p.a + int64_t(z) * p.sa + int64_t(r) * p.lda;
-    const int8_t* w = p.w + uint64_t(c) * p.K;
-    int s[2][4] = {};
-    for (uint32_t k = 0; k < p.K; k += 16) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(a + k);
-        for (int h = 0; h < (glu ? 2 : 1); ++h)
+    return epi == MK_EPI_STORE                                 ? EC_STORE
+           : epi == MK_EPI_GELU_TANH || epi == MK_EPI_SILU      ? EC_ACT
+           : epi == MK_EPI_SWIGLU || epi == MK_EPI_GEGLU        ? EC_GLU
+                                                                : EC_RMW;
+}
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+__device__ inline i32x4 mfma_i8(const i32x4& w, const i32x4& a, const i32x4& c)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, a, c, 0, 0, 0);
+#else
+    return c;
+#endif
+}
+
+// What a lane's four channels need: scales, bias, the gate rows (g1 for rows below the split; tanh applied).
+struct Ch4 {
+    f32x4 ws, b, g0, g1;
+};
+__device__ inline Ch4 channels4(const I8P& p, uint32_t c)
+{
+    Ch4 k;
+    k.ws = *reinterpret_cast<const f32x4*>(p.wscale + c);
+    k.b = load4(p.bias, c, 0.0f);
+    k.g0 = load4(p.gate, c, 1.0f);
+    k.g1 = p.gate && p.split ? *reinterpret_cast<const f32x4*>(p.gate + p.gate_alt + c) : k.g0;
+    if (p.epi == MK_EPI_GATE_TANH)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const u32x4 y = *reinterpret_cast<const u32x4*>(w + (uint64_t(h) * cols + e) * p.K + k);
+        for (int e = 0; e < 4; ++e) {
+            k.g0[e] = tanh_f(k.g0[e]);
+            k.g1[e] = tanh_f(k.g1[e]);
+        }
+    return k;
+}
+// sum * ascale (t) to the channel's value: one rounding for the product with wscale and the bias, everywhere
+__device__ inline f32x4 scaled(const f32x4& t, const f32x4& ws, const f32x4& b)
+{
+    f32x4 v;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[h][e] = __builtin_amdgcn_sdot4(int(x[i]), int(y[i]), s[h][e], false);
+    for (int e = 0; e < 4; ++e)
+        v[e] = fmaf(t[e], ws[e], b[e]);
+    return v;
+}
+template <bool GELU> __device__ inline f32x4 act4(const f32x4& v)
+{
+    f32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        o[e] = GELU ? gelu_tanh_f(v[e]) : silu_f(v[e]);
+    return o;
+}
+template <bool SWI> __device__ inline float glu1(float a, float g)
+{
+    return SWI ? silu_f(a) * g : a * (0.5f * g * (1.0f + erf_fit(g * 0.70710678f)));
+}
+__device__ inline f32x4 residual4(const I8P& p, uint32_t row, const f32x4& x, const f32x4& v, const Ch4& k)
+{
+    const f32x4 g = row % p.seg_rows < p.split ? k.g1 : k.g0;
+    f32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        o[e] = fmaf(g[e], v[e], x[e]);
+    return o;
+}
+// f(std::bool_constant<flag>{}): one branch on a uniform flag around code specialised for each value
+template <class F> __device__ inline void with_flag(bool flag, F&& f)
+{
+    if (flag)
+        f(std::true_type{});
+    else
+        f(std::false_type{});
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Tiles. The weight is the matrix cores' A operand (its rows are output channels), the activation the B operand, so a lane
+// of v_mfma_i32_16x16x64_i8 holds 4 consecutive channels of one token. NW waves, 2 along the channels.
+// ------------------------------------------------------------------------------------------------------------
+
+// LDS rows are 128 bytes of k, 8 chunks of 16. A 16-byte read serves 16 lanes a cycle, here 16 consecutive rows at one
+// chunk; rows r and r + 1 fall in opposite halves of the 64 banks, so the chunk is XOR-ed with (row >> 1) & 7.
+__device__ inline int swz_chunk(int row, int kc) { return kc ^ ((row >> 1) & 7); }
+__device__ inline int swz(int row, int kc) { return row * 128 + (swz_chunk(row, kc) << 4); }
+// s_waitcnt immediate: vmcnt vm, lgkmcnt 0 (vmcnt's bits 3:0 and 15:14, expcnt not waited for)
+constexpr int wait_vm(int vm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4); }
+
+template <int BM, int BN, int NW, int NSTG> constexpr int tile_lds()
+{
+    constexpr int ops = NSTG * (BM + BN) * 128, epi = NW * 32 * (BN / 2 + 4) * 4;
+    return ops > epi ? ops : epi;
+}
+
+template <int BM, int BN, int NW, int NSTG, int EC>
+__global__ __launch_bounds__(64 * NW, 1) __attribute__((amdgpu_waves_per_eu(
+    NW == 8 || tile_lds<BM, BN, NW, NSTG>() <= 80 * 1024 ? 2 : 1,
+    NW == 8 || tile_lds<BM, BN, NW, NSTG>() <= 80 * 1024 ? 2 : 1))) void gemm_i8_kernel(I8P p, uint32_t tiles_m,
+                                                                                      uint32_t tiles_n)
+{
+    constexpr bool GLU = EC == EC_GLU;
+    constexpr int NT = 64 * NW, WM = BM / (NW / 2), WC = BN / 2, TB = WM / 16, CB = WC / 16;
+    constexpr int RA = BM * 8 / NT, RW = BN * 8 / NT, ND = RA + RW; // direct loads a thread makes a k step
+    constexpr int LDW = WC + 4;
+    static_assert((NSTG - 2) * ND <= 63 && WM % 32 == 0, "");
+    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<BM, BN, NW, NSTG>()];
+    int8_t(*sW)[BN * 128] = reinterpret_cast<int8_t(*)[BN * 128]>(smem);
+    int8_t(*sA)[BM * 128] = reinterpret_cast<int8_t(*)[BM * 128]>(smem + NSTG * BN * 128);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave & 1, wm = wave >> 1;
+
+    // workgroup i runs on XCD i % 8: each XCD takes a run of tiles, 8 token tiles at a time, which share weight panels in
+    // its L2
+    uint32_t z, tm, tn;
+    {
+        const uint32_t n = gridDim.x, x = blockIdx.x % 8, q = n / 8, t = x * q + min(x, n % 8) + blockIdx.x / 8;
+        const uint32_t per = tiles_m * tiles_n, pid = t % per, in_group = 8 * tiles_n;
+        z = t / per;
+        const uint32_t first = pid / in_group * 8, g = min(tiles_m - first, 8u), i = pid % in_group;
+        tm = first + i % g;
+        tn = i / g;
+    }
+    const int m0 = int(tm) * BM, cols = int(GLU ? p.N / 2 : p.N);
+    // GLU: the tile makes channels n0 .. n0 + BN / 2, a wave's rows are WC / 2 rows of the first part and the same
+    // channels' rows of the second, so a lane's blocks cb and cb + CB / 2 are the two operands of one output.
+    const int n0 = int(tn) * (GLU ? BN / 2 : BN), nr = min(cols - n0, GLU ? BN / 2 : BN);
+
+    // Direct loads: wave w's round i fills LDS chunks (i NW + w) 64 + lane; chunk P holds row P / 8 and k chunk
+    // swz_chunk(row, P % 8). Buffer loads: the resource spans the tile's rows, the lane's byte offset selects row and
+    // chunk, the k offset is a scalar; rows past the end read the last one. Chunks past K (in the last k step) read out of
+    // the resource's range, which gives zeros.
+    const int8_t* gA = p.a + int64_t(z) * p.sa + int64_t(m0) * p.lda;
+    const int8_t* gW = p.w + uint64_t(n0) * p.K;
+    const int mr = min(int(p.M) - m0, BM);
+    const BufRes rsA = buf_res(gA, uint32_t(int64_t(mr - 1) * p.lda + p.K));
+    const BufRes rsW0 = buf_res(gW, uint32_t(nr) * p.K);
+    const BufRes rsW1 = buf_res(GLU ? gW + uint64_t(cols) * p.K : gW, uint32_t(nr) * p.K);
+    const int kc = (lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7); // the lane's k chunk, the same in every round
+    static_assert(NW % 2 == 0, "a round's rows are a multiple of 16");
+    uint32_t oa[RA], ow[RW];
+#pragma unroll
+    for (int i = 0; i < RA; ++i) {
+        const int row = (i * NW + wave) * 8 + (lane >> 3);
+        oa[i] = uint32_t(min(row, mr - 1)) * uint32_t(p.lda) + kc * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const int r = (i * NW + wave) * 8 + (lane >> 3);
+        ow[i] = uint32_t(min(GLU ? (r / WC) * (WC / 2) + r % (WC / 2) : r, nr - 1)) * p.K + kc * 16;
+    }
+    static_assert(!GLU || (WC / 2) % (8 * NW) == 0 || (8 * NW) % WC == 0, "");
+    // direct load i (activation rounds first) of k step kt into stage buf; past: what leaves the range in the last, partial
+    // step for the lanes whose chunk lies past K
+    auto dma1 = [&](int kt, uint32_t past, int buf, int i) {
+        if (i < RA)
+            buf_load_lds16(rsA, (lds_void*)&sA[buf][(i * NW + wave) * 1024], oa[i] + past, uint32_t(kt) * 128);
+        else {
+            const bool second = GLU && ((i - RA) * NW * 8 + wave * 8) % WC >= WC / 2;
+            buf_load_lds16(second ? rsW1 : rsW0, (lds_void*)&sW[buf][((i - RA) * NW + wave) * 1024], ow[i - RA] + past,
+                           uint32_t(kt) * 128);
+        }
+    };
+    const int ke = int((p.K + 127) / 128), kfull = int(p.K / 128);
+    const uint32_t tail = kc * 16 >= int(p.K) - kfull * 128 ? 0x80000000u : 0u;
+    auto past = [&](int kt) { return kt < kfull ? 0u : tail; };
+
+    i32x4 acc[CB][TB];
+#pragma unroll
+    for (int i = 0; i < CB; ++i)
+#pragma unroll
+        for (int j = 0; j < TB; ++j)
+            acc[i][j] = i32x4{0, 0, 0, 0};
+
+    // lane (r16, g4) supplies row r16 of a 16-row block and k bytes 16 g4 .. + 15 of a 64-deep substep, and holds channels
+    // 4 g4 .. + 3 of token r16
+    const int r16 = lane & 15, g4 = lane >> 4;
+    i32x4 wf[CB], af0[TB], af1[TB];
+    // (blocks are 16 rows apart, so the swizzle is the lane's: an address is one of two registers plus a constant)
+    const int fw[2] = {swz(wn * WC + r16, g4), swz(wn * WC + r16, 4 + g4)};
+    const int fa[2] = {swz(wm * WM + r16, g4), swz(wm * WM + r16, 4 + g4)};
+    auto rdw = [&](int buf, int ks, int cb) { wf[cb] = *reinterpret_cast<const i32x4*>(&sW[buf][fw[ks] + cb * 2048]); };
+    auto rda = [&](int buf, int ks, int tb, i32x4(&af)[TB]) {
+        af[tb] = *reinterpret_cast<const i32x4*>(&sA[buf][fa[ks] + tb * 2048]);
+    };
+    // A substep: the weight fragments are single-buffered, each next one read into its registers right after the last
+    // product that uses it; the next token fragments go to the other buffer with the first channel block; the direct loads
+    // of step gkt (into stage gbuf) follow one product each. Every instruction is fenced: the order is this one.
+    auto substep = [&](const i32x4(&af)[TB], int nbuf, int nks, i32x4(&naf)[TB], int gkt, int gbuf, bool load) {
+        const uint32_t gp = past(gkt);
+#pragma unroll
+        for (int i = 0; i < CB * TB; ++i) {
+            const int cb = i / TB, tb = i % TB;
+            acc[cb][tb] = mfma_i8(wf[cb], af[tb], acc[cb][tb]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (cb == 0) {
+                rda(nbuf, nks, tb, naf);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (tb == TB - 1) {
+                rdw(nbuf, nks, cb);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (load && i < ND) {
+                dma1(gkt, gp, gbuf, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (load)
+#pragma unroll
+            for (int i = CB * TB; i < ND; ++i)
+                dma1(gkt, gp, gbuf, i);
+    };
+
+    // k steps 0 .. NSTG - 1 on their way; past-the-end steps reload the last one (nobody reads them)
+#pragma unroll
+    for (int s = 0; s < NSTG; ++s) {
+        const int kt = min(s, ke - 1);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+            dma1(kt, past(kt), s, i);
     }
-    const float as = p.ascale[uint64_t(z) * p.M + r];
-    f32x4 v = i8_scaled(s[0], as, load4(p.wscale, c, 1.0f), load4(p.bias, c, 0.0f));
-    if (glu) {
-        const f32x4 g = i8_scaled(s[1], as, load4(p.wscale, cols + c, 1.0f), load4(p.bias, cols + c, 0.0f));
+    __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 1) * ND > 63 ? 63 : (NSTG - 1) * ND));
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+        rdw(0, 0, cb);
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb)
+        rda(0, 0, tb, af0);
+    // k step kt in stage `buf` (a constant: the loop is unrolled by NSTG): the first substep reads the second's fragments;
+    // then step kt + 1 has landed (later ones may be in flight) and, after the barrier, in every wave, and every wave has
+    // read this stage, so the second substep loads step kt + NSTG into it and reads step kt + 1's first fragments
+    auto step = [&](int kt, auto buf_c) {
+        constexpr int buf = decltype(buf_c)::value, nb = (buf + 1) % NSTG;
+        substep(af0, buf, 1, af1, 0, 0, false);
+        __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
+        __builtin_amdgcn_s_barrier();
+        substep(af1, nb, 0, af0, min(kt + NSTG, ke - 1), buf, true);
+    };
+    int kt = 0;
+    for (; kt + NSTG - 1 < ke; kt += NSTG) {
+        step(kt, std::integral_constant<int, 0>{});
+        step(kt + 1, std::integral_constant<int, 1>{});
+        if constexpr (NSTG > 2)
+            step(kt + 2, std::integral_constant<int, 2 % NSTG>{});
+        if constexpr (NSTG > 3)
+            step(kt + 3, std::integral_constant<int, 3 % NSTG>{});
+    }
+    if (kt < ke)
+        step(kt, std::integral_constant<int, 0>{});
+    if (NSTG > 2 && kt + 1 < ke)
+        step(kt + 1, std::integral_constant<int, 1>{});
+    if (NSTG > 3 && kt + 2 < ke)
+        step(kt + 2, std::integral_constant<int, 2 % NSTG>{});
+    __builtin_amdgcn_s_waitcnt(0); // the last loads land before the LDS is reused
+    __syncthreads();
+
+    // Epilogue: a wave stages 32 tokens at a time (fp32, times their scales) in LDS of its own and reads them back with its
+    // lanes along the channels, so that its stores are whole row segments. A wave's LDS operations complete in order:
+    // no barrier.
+    float* st = reinterpret_cast<float*>(smem) + wave * 32 * LDW;
+    const float* as = p.ascale + uint64_t(z) * p.M;
+    const int t0 = m0 + wm * WM;
+    float sc[TB];
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb)
+        sc[tb] = as[min(t0 + tb * 16 + r16, int(p.M) - 1)];
+    constexpr int WO = GLU ? WC / 2 : WC; // channels a wave writes
+    constexpr int LPR = WO / 4, RPI = 64 / LPR, NI = 32 / RPI; // lanes a row, rows an instruction, rows a lane
+    const int c0 = n0 + wn * WO;
+    auto stage = [&](int s) {
+#pragma unroll
+        for (int cb = 0; cb < WO / 16; ++cb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int a = acc[cb][2 * s + h][e];
+                    v[e] = GLU ? __builtin_bit_cast(float, a) : float(a) * sc[2 * s + h];
+                }
+                *reinterpret_cast<f32x4*>(st + (16 * h + r16) * LDW + cb * 16 + 4 * g4) = v;
+            }
+    };
+    if constexpr (GLU) {
+        with_flag(p.epi == MK_EPI_SWIGLU, [&](auto swi) {
+#pragma unroll
+            for (int cb = 0; cb < CB / 2; ++cb) {
+                const int c = min(c0 + cb * 16 + 4 * g4, cols - 4);
+                const f32x4 s1 = *reinterpret_cast<const f32x4*>(p.wscale + c);
+                const f32x4 s2 = *reinterpret_cast<const f32x4*>(p.wscale + cols + c);
+                const f32x4 b1 = load4(p.bias, c, 0.0f), b2 = load4(p.bias, cols + c, 0.0f);
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = fmaf(float(acc[cb][tb][e]) * sc[tb], s1[e], b1[e]);
+                        const float g = fmaf(float(acc[cb + CB / 2][tb][e]) * sc[tb], s2[e], b2[e]);
+                        acc[cb][tb][e] = __builtin_bit_cast(int, glu1<decltype(swi)::value>(a, g));
+                    }
+            }
+        });
+    }
+    const int lc = lane % LPR, lr = lane / LPR, ch = c0 + 4 * lc;
+    const bool mine = ch < cols; // (cols is a multiple of 4)
+    Ch4 k{};
+    if (!GLU)
+        k = channels4(p, min(ch, cols - 4));
+#pragma unroll
+    for (int s = 0; s < WM / 32; ++s) {
+        stage(s);
+        const int tok = t0 + 32 * s + lr;
+        const int64_t at = int64_t(z) * p.sc + int64_t(tok) * p.ldc + ch, step = int64_t(RPI) * p.ldc;
+        f32x4 v[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            v[i] = *reinterpret_cast<const f32x4*>(st + (lr + RPI * i) * LDW + 4 * lc);
+            if (!GLU)
+                v[i] = scaled(v[i], k.ws, k.b);
+        }
+        if constexpr (EC == EC_ACT)
+            with_flag(p.epi == MK_EPI_GELU_TANH, [&](auto gelu) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    v[i] = act4<decltype(gelu)::value>(v[i]);
+            });
+        // rows of the slice past M: the whole slices' stores have no guard between them
+        auto rows = [&](auto&& store) {
+            if (!mine)
+                return;
+            if (t0 + 32 * s + 32 <= int(p.M)) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    store(i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    if (tok + RPI * i < int(p.M))
+                        store(i);
+            }
+        };
+        if constexpr (EC == EC_RMW) {
+            float* c = static_cast<float*>(p.c) + at;
+            f32x4 x[NI];
+            rows([&](int i) { x[i] = *reinterpret_cast<const f32x4*>(c + i * step); });
+            rows([&](int i) { *reinterpret_cast<f32x4*>(c + i * step) = residual4(p, uint32_t(tok + RPI * i), x[i], v[i], k); });
+        } else if (p.c_dtype == MK_F32) {
+            float* c = static_cast<float*>(p.c) + at;
+            rows([&](int i) { *reinterpret_cast<f32x4*>(c + i * step) = v[i]; });
+        } else {
+            uint16_t* c = static_cast<uint16_t*>(p.c) + at;
+            u32x2 o[NI];
+            with_flag(p.c_dtype == MK_F16, [&](auto h) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    o[i] = u32x2{pack_x2(v[i][0], v[i][1], decltype(h)::value), pack_x2(v[i][2], v[i][3], decltype(h)::value)};
+            });
+            rows([&](int i) { *reinterpret_cast<u32x2*>(c + i * step) = o[i]; });
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Few rows (up to 16 TB): a workgroup makes 16 channels of all rows, its 8 waves every eighth 256 bytes of k each,
+// straight from memory: nothing of the weight is read twice, and all of a launch's loads are in flight at once. The sums
+// meet in LDS.
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kFewWaves = 8, kFewUnit = 256;
+
+template <int TB, int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_kernel(I8P p)
+{
+    constexpr bool GLU = EC == EC_GLU;
+    constexpr int CB = GLU ? 2 : 1, NS = kFewUnit / 64;
+    __shared__ i32x4 red[kFewWaves][CB * TB][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g4 = lane >> 4, cols = int(GLU ? p.N / 2 : p.N), n0 = blockIdx.x * 16;
+    const uint32_t z = blockIdx.y;
+    const int nr = min(cols - n0, 16), M = int(p.M);
+    const int8_t* gA = p.a + int64_t(z) * p.sa;
+    const int8_t* gW = p.w + uint64_t(n0) * p.K;
+    const BufRes rsA = buf_res(gA, uint32_t(int64_t(M - 1) * p.lda + p.K));
+    const BufRes rsW[2] = {buf_res(gW, uint32_t(nr) * p.K), buf_res(GLU ? gW + uint64_t(cols) * p.K : gW, uint32_t(nr) * p.K)};
+    const uint32_t ow = uint32_t(min(r16, nr - 1)) * p.K + g4 * 16;
+    uint32_t oa[TB];
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb)
+        oa[tb] = uint32_t(min(tb * 16 + r16, M - 1)) * uint32_t(p.lda) + g4 * 16;
+    i32x4 acc[CB][TB] = {};
+    struct Unit {
+        i32x4 w[NS][CB], a[NS][TB];
+    };
+    auto load = [&](uint32_t k, Unit& f) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            // chunks past K: out of range, zeros
+            const bool in = k + s * 64 + g4 * 16 < p.K;
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+                f.w[s][c] = __builtin_bit_cast(i32x4, buf_load16(rsW[c], in ? ow + s * 64 : 0xfffffff0u, in ? k : 0));
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+                f.a[s][tb] = __builtin_bit_cast(i32x4, buf_load16(rsA, in ? oa[tb] + s * 64 : 0xfffffff0u, in ? k : 0));
+        }
+    };
+    auto mul = [&](const Unit& f) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb)
+                    acc[c][tb] = mfma_i8(f.w[s][c], f.a[s][tb], acc[c][tb]);
+    };
+    constexpr uint32_t kStep = kFewWaves * kFewUnit;
+    Unit f[2];
+    uint32_t k = uint32_t(wave) * kFewUnit;
+    if (k < p.K) {
+        load(k, f[0]);
+        for (; k + kStep < p.K; k += kStep) {
+            load(k + kStep, f[1]);
+            mul(f[0]);
+            f[0] = f[1];
+        }
+        mul(f[0]);
+    }
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+            red[wave][c * TB + tb][lane] = acc[c][tb];
+    __syncthreads();
+    // wave tb finishes tokens 16 tb .. + 15
+    for (int tb = wave; tb < TB; tb += kFewWaves) {
+        const int tok = tb * 16 + r16, ch = n0 + 4 * g4;
+        i32x4 s[CB] = {};
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w)
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+                s[c] += red[w][c * TB + tb][lane];
+        if (tok >= M || ch >= cols)
+            continue;
+        const float as = p.ascale[uint64_t(z) * p.M + tok];
+        const Ch4 kc = channels4(p, ch);
+        f32x4 t;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            v[e] = p.epi == MK_EPI_SWIGLU ? silu_f(v[e]) * g[e] : v[e] * (0.5f * g[e] * (1.0f + erf_fit(g[e] * 0.70710678f)));
-    } else if (p.epi == MK_EPI_GELU_TANH || p.epi == MK_EPI_SILU) {
+            t[e] = float(s[0][e]) * as;
+        f32x4 v = scaled(t, kc.ws, kc.b);
+        if constexpr (GLU) {
+            f32x4 g;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            v[e] = p.epi == MK_EPI_SILU ? silu_f(v[e]) : gelu_tanh_f(v[e]);
-    }
-    const int64_t at = int64_t(z) * p.sc + int64_t(r) * p.ldc + c;
-    if (p.epi == MK_EPI_GATE_ADD || p.epi == MK_EPI_GATE_TANH || p.epi == MK_EPI_ADD) {
-        f32x4* x = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
-        f32x4 o = *x;
-        const f32x4 g = load4(p.gate, (r % p.seg_rows < p.split ? p.gate_alt : 0) + c, 1.0f);
+            for (int e = 0; e < 4; ++e)
+                t[e] = float(s[CB - 1][e]) * as;
+            g = scaled(t, *reinterpret_cast<const f32x4*>(p.wscale + cols + ch), load4(p.bias, cols + ch, 0.0f));
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            o[e] = fmaf(p.epi == MK_EPI_ADD ? 1.0f : p.epi == MK_EPI_GATE_TANH ? tanh_f(g[e]) : g[e], v[e], o[e]);
-        *x = o;
-    } else if (p.c_dtype == MK_F32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at) = v;
-    } else {
-        const bool h = p.c_dtype == MK_F16;
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.c) + at) = u32x2{pack_x2(v[0], v[1], h), pack_x2(v[2], v[3], h)};
+            for (int e = 0; e < 4; ++e)
+                v[e] = p.epi == MK_EPI_SWIGLU ? glu1<true>(v[e], g[e]) : glu1<false>(v[e], g[e]);
+        } else if constexpr (EC == EC_ACT) {
+            v = p.epi == MK_EPI_GELU_TANH ? act4<true>(v) : act4<false>(v);
+        }
+        const int64_t at = int64_t(z) * p.sc + int64_t(tok) * p.ldc + ch;
+        if constexpr (EC == EC_RMW) {
+            f32x4* x = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
+            *x = residual4(p, uint32_t(tok), *x, v, kc);
+        } else if (p.c_dtype == MK_F32) {
+            *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at) = v;
+        } else {
+            const bool h = p.c_dtype == MK_F16;
+            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.c) + at) = u32x2{pack_x2(v[0], v[1], h), pack_x2(v[2], v[3], h)};
+        }
     }
+}
+
+template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const I8P& p, hipStream_t s)
+{
+    const uint32_t cols = EC == EC_GLU ? p.N / 2 : p.N, tm = cdiv(p.M, BM), tn = cdiv(cols, EC == EC_GLU ? BN / 2 : BN);
+    const uint64_t tiles = uint64_t(tm) * tn * p.batch;
+    if (tiles > 0x7fffffffu)
+        return fail(MK_ERR_ARG, "gemm_i8: too many tiles");
+    gemm_i8_kernel<BM, BN, NW, NSTG, EC><<<uint32_t(tiles), 64 * NW, 0, s>>>(p, tm, tn);
+    MK_LAUNCH_CHECK("gemm_i8");
+    return MK_OK;
+}
+
+template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
+{
+    const uint32_t cols = EC == EC_GLU ? p.N / 2 : p.N;
+    if (p.M <= 64) {
+        const dim3 grid(cdiv(cols, 16), p.batch);
+        if (p.M <= 16)
+            gemm_i8_few_kernel<1, EC><<<grid, 64 * kFewWaves, 0, s>>>(p);
+        else if (p.M <= 32)
+            gemm_i8_few_kernel<2, EC><<<grid, 64 * kFewWaves, 0, s>>>(p);
+        else
+            gemm_i8_few_kernel<4, EC><<<grid, 64 * kFewWaves, 0, s>>>(p);
+        MK_LAUNCH_CHECK("gemm_i8");
+        return MK_OK;
+    }
+    const uint64_t big = uint64_t(cdiv(p.M, 256)) * cdiv(p.N, 256) * p.batch;
+    if (big >= cus)
+        return launch_tile<256, 256, 8, 2, EC>(p, s);
+    return launch_tile<128, 128, 4, 2, EC>(p, s);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -154,7 +600,14 @@ extern "C" mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void
                 a->epilogue,
                 a->c_dtype};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    gemm_i8_plain_kernel<<<dim3(cdiv(p.M, 16), cdiv(cols, 64), p.batch), 256, 0, s>>>(p);
-    MK_LAUNCH_CHECK("gemm_i8");
-    return MK_OK;
+    int dev = 0, cus = 0;
+    MK_HIP(hipGetDevice(&dev));
+    MK_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    const uint32_t n = cus > 0 ? uint32_t(cus) : 1;
+    switch (epi_class(p.epi)) {
+    case EC_STORE: return launch<EC_STORE>(p, n, s);
+    case EC_ACT: return launch<EC_ACT>(p, n, s);
+    case EC_GLU: return launch<EC_GLU>(p, n, s);
+    default: return launch<EC_RMW>(p, n, s);
+    }
 }
