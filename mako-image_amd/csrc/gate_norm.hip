@@ -55,145 +55,332 @@ __device__ inline uint32_t quant_pack(const f32x4& v, const Quant& q)
 }
 __device__ inline uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-__device__ inline f32x4 load_row4(const void* p, uint64_t at, uint32_t dtype)
+// f(std::integral_constant<uint32_t, t>{}) for the float type t: one branch around code specialised for each
+template <class F> __device__ inline void with_type(uint32_t t, F&& f)
 {
-    if (dtype == MK_F32)
+    if (t == MK_BF16)
+        f(std::integral_constant<uint32_t, MK_BF16>{});
+    else if (t == MK_F16)
+        f(std::integral_constant<uint32_t, MK_F16>{});
+    else
+        f(std::integral_constant<uint32_t, MK_F32>{});
+}
+template <uint32_t T> __device__ inline float widen(uint16_t h) { return T == MK_BF16 ? bf2f_bits(h) : h2f_bits(h); }
+// 4 elements of type T as floats
+template <uint32_t T> __device__ inline f32x4 load4(const void* p, uint64_t at)
+{
+    if constexpr (T == MK_F32) {
         return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
-    const u32x2 v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p) + at);
-    f32x4 o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint16_t h = uint16_t(v[e >> 1] >> (16 * (e & 1)));
-        o[e] = dtype == MK_BF16 ? bf2f_bits(h) : h2f_bits(h);
+    } else {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p) + at);
+        return f32x4{widen<T>(uint16_t(v[0])), widen<T>(uint16_t(v[0] >> 16)), widen<T>(uint16_t(v[1])),
+                     widen<T>(uint16_t(v[1] >> 16))};
     }
-    return o;
+}
+template <uint32_t T> __device__ inline float load1(const void* p, uint64_t at)
+{
+    if constexpr (T == MK_F32)
+        return static_cast<const float*>(p)[at];
+    else
+        return widen<T>(static_cast<const uint16_t*>(p)[at]);
 }
 
-// Sum over a workgroup of 256, every thread gets it.
-__device__ inline float block_sum(float v, float* red)
+__device__ inline uint32_t wave_max_bits(uint32_t v)
 {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-        red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
-}
-__device__ inline uint32_t block_max(uint32_t v, float* red)
-{
-    for (int m = 32; m; m >>= 1)
-        v = max(v, uint32_t(__shfl_xor(int(v), m)));
-    uint32_t* r = reinterpret_cast<uint32_t*>(red);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-        r[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return max(max(r[0], r[1]), max(r[2], r[3]));
+#if defined(__HIP_DEVICE_COMPILE__)
+    // the VALU ladder of wave_reduce, on the bits
+    return __builtin_bit_cast(uint32_t, wave_reduce(__builtin_bit_cast(float, v), [](float a, float b) {
+                                  return __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, a),
+                                                                       __builtin_bit_cast(uint32_t, b)));
+                              }));
+#else
+    return v;
+#endif
 }
 
-__device__ inline f32x4 vec4(const float* p, uint64_t at, float none)
+// Reductions over the W waves of a row, every thread gets the result. Each reduction of a kernel has a slot of its own in
+// LDS, so it takes one barrier; the waves' sums are added in their order.
+template <int W> struct RowRed {
+    float* slots; // W floats a reduction
+    __device__ float sum(float v, int i)
+    {
+        v = wave_sum(v);
+        if constexpr (W > 1) {
+            float* s = slots + i * W;
+            if ((threadIdx.x & 63) == 0)
+                s[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                v += s[w];
+        }
+        return v;
+    }
+    __device__ uint32_t max_bits(uint32_t v, int i)
+    {
+        v = wave_max_bits(v);
+        if constexpr (W > 1) {
+            uint32_t* s = reinterpret_cast<uint32_t*>(slots + i * W);
+            if ((threadIdx.x & 63) == 0)
+                s[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                v = max(v, s[w]);
+        }
+        return v;
+    }
+};
+
+__device__ inline f32x4 vec4(const float* p, int64_t at, float none)
 {
     return p ? *reinterpret_cast<const f32x4*>(p + at) : f32x4{none, none, none, none};
 }
 
-// The row in LDS, normed in place: each thread owns the float4s threadIdx.x + 256 i.
-__device__ inline void norm_row(f32x4* row, uint32_t nv, uint32_t n, uint32_t kind, const float* w, const float* b,
-                                float eps, float* red)
+// A row's norm in registers: each thread holds NV float4s, c = first + 64 W i of the row's nv (zeros past its end).
+template <int W, int NV>
+__device__ inline void norm_row(f32x4 (&v)[NV], uint32_t c0, uint32_t nv, uint32_t n, uint32_t kind, const float* w,
+                                const float* b, float eps, RowRed<W>& red, int slot)
 {
     if (kind == MK_NORM_NONE)
         return;
     float mean = 0.0f, s = 0.0f;
     if (kind == MK_NORM_LAYER) {
-        for (uint32_t c = threadIdx.x; c < nv; c += 256)
-            s += row[c][0] + row[c][1] + row[c][2] + row[c][3];
-        mean = block_sum(s, red) / float(n);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            s += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
+        mean = red.sum(s, slot) / float(n);
     }
     s = 0.0f;
-    for (uint32_t c = threadIdx.x; c < nv; c += 256)
-        for (int e = 0; e < 4; ++e)
-            s += (row[c][e] - mean) * (row[c][e] - mean);
-    const float inv = rsqrtf(block_sum(s, red) / float(n) + eps);
-    for (uint32_t c = threadIdx.x; c < nv; c += 256) {
-        const f32x4 ww = vec4(w, 4 * c, 1.0f), bb = vec4(b, 4 * c, 0.0f);
-        for (int e = 0; e < 4; ++e)
-            row[c][e] = (row[c][e] - mean) * inv * ww[e] + bb[e];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (c0 + 64 * W * i < nv) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[i][e] -= mean;
+                s = fmaf(v[i][e], v[i][e], s);
+            }
+        }
+    const float inv = rsqrtf(red.sum(s, slot + 1) / float(n) + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t c = c0 + 64 * W * i;
+        if (c < nv) {
+            const f32x4 ww = vec4(w, 4 * int64_t(c), 1.0f), bb = vec4(b, 4 * int64_t(c), 0.0f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[i][e] = fmaf(v[i][e] * inv, ww[e], bb[e]);
+        }
     }
 }
 
-__global__ __launch_bounds__(256) void gate_norm_kernel(mk_gate_norm_args g)
+// W waves a row (W = 1: four rows a workgroup), NV float4s a thread.
+template <int W, int NV>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gate_norm_args g)
 {
-    extern __shared__ f32x4 row[];
-    __shared__ float red[4];
-    const uint32_t r = blockIdx.x, nv = g.n / 4;
-    const uint32_t seg = r / g.seg_rows, i = r - seg * g.seg_rows;
-    const int64_t mod = int64_t(seg) * g.mod_stride + (i < g.split ? g.alt : 0);
-    const f32x4* x = reinterpret_cast<const f32x4*>(g.x + uint64_t(r) * g.ldx);
+    __shared__ float slots[5 * W];
+    RowRed<W> red{slots};
+    const uint32_t r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (W == 1 && r >= g.rows)
+        return;
+    const uint32_t nv = g.n / 4, c0 = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const uint32_t seg = r / g.seg_rows, at = r - seg * g.seg_rows;
+    const int64_t mod = int64_t(seg) * g.mod_stride + (at < g.split ? g.alt : 0);
+    const float* x = g.x + uint64_t(r) * g.ldx;
+    f32x4 v[NV];
     if (g.y) {
-        for (uint32_t c = threadIdx.x; c < nv; c += 256)
-            row[c] = load_row4(g.y, uint64_t(r) * g.ldy + 4 * c, g.y_dtype);
-        norm_row(row, nv, g.n, g.norm1, g.w1, g.b1, g.eps1, red);
-        for (uint32_t c = threadIdx.x; c < nv; c += 256) {
-            const f32x4 gt = vec4(g.gate, mod + 4 * c, 1.0f), xv = x[c];
-            f32x4 o;
+        f32x4 xv[NV], gt[NV];
+        with_type(g.y_dtype, [&](auto t) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t c = c0 + 64 * W * i;
+                v[i] = c < nv ? load4<decltype(t)::value>(g.y, uint64_t(r) * g.ldy + 4 * c) : f32x4{0, 0, 0, 0};
+            }
+        });
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t c = c0 + 64 * W * i;
+            xv[i] = c < nv ? *reinterpret_cast<const f32x4*>(x + 4 * c) : f32x4{0, 0, 0, 0};
+            gt[i] = c < nv ? vec4(g.gate, mod + 4 * c, 1.0f) : f32x4{0, 0, 0, 0};
+        }
+        norm_row<W, NV>(v, c0, nv, g.n, g.norm1, g.w1, g.b1, g.eps1, red, 0);
+        if (g.gate && g.tanh_gate)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    gt[i][e] = tanh_f(gt[i][e]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t c = c0 + 64 * W * i;
+#pragma unroll
             for (int e = 0; e < 4; ++e)
-                o[e] = fmaf(g.gate && g.tanh_gate ? tanh_f(gt[e]) : gt[e], row[c][e], g.residual_scale * xv[e]);
-            row[c] = o;
-            if (g.x_out)
-                reinterpret_cast<f32x4*>(g.x_out + uint64_t(r) * g.ldx)[c] = o;
+                v[i][e] = fmaf(gt[i][e], v[i][e], g.residual_scale * xv[i][e]);
+            if (g.x_out && c < nv)
+                *reinterpret_cast<f32x4*>(g.x_out + uint64_t(r) * g.ldx + 4 * c) = v[i];
         }
     } else {
-        for (uint32_t c = threadIdx.x; c < nv; c += 256)
-            row[c] = x[c];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t c = c0 + 64 * W * i;
+            v[i] = c < nv ? *reinterpret_cast<const f32x4*>(x + 4 * c) : f32x4{0, 0, 0, 0};
+        }
     }
     if (!g.out)
         return;
-    norm_row(row, nv, g.n, g.norm2, g.w2, g.b2, g.eps2, red);
-    uint32_t m = 0;
-    for (uint32_t c = threadIdx.x; c < nv; c += 256) {
-        const f32x4 sc = vec4(g.scale, mod + 4 * c, 0.0f), sh = vec4(g.shift, mod + 4 * c, 0.0f);
-        f32x4 h = row[c];
-        for (int e = 0; e < 4; ++e) {
-            h[e] = fmaf(h[e], 1.0f + sc[e], sh[e]);
-            m = max(m, abs_bits(h[e]));
-        }
-        const uint64_t at = uint64_t(r) * g.ldo + 4 * c;
-        row[c] = h;
-        if (g.out_dtype == MK_F32)
-            *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = h;
-        else if (g.out_dtype != MK_I8)
-            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(g.out) + at) =
-                u32x2{pack_x2(h[0], h[1], g.out_dtype == MK_F16), pack_x2(h[2], h[3], g.out_dtype == MK_F16)};
+    f32x4 sc[NV], sh[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t c = c0 + 64 * W * i;
+        sc[i] = c < nv ? vec4(g.scale, mod + 4 * c, 0.0f) : f32x4{0, 0, 0, 0};
+        sh[i] = c < nv ? vec4(g.shift, mod + 4 * c, 0.0f) : f32x4{0, 0, 0, 0};
     }
-    if (g.out_dtype != MK_I8)
+    norm_row<W, NV>(v, c0, nv, g.n, g.norm2, g.w2, g.b2, g.eps2, red, 2);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[i][e] = fmaf(v[i][e], 1.0f + sc[i][e], sh[i][e]);
+    if (g.out_dtype == MK_I8) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (c0 + 64 * W * i < nv)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    m = max(m, abs_bits(v[i][e]));
+        const Quant q = quant_of(red.max_bits(m, 4));
+        int8_t* o = static_cast<int8_t*>(g.out) + uint64_t(r) * g.ldo;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (c0 + 64 * W * i < nv)
+                *reinterpret_cast<uint32_t*>(o + 4 * (c0 + 64 * W * i)) = quant_pack(v[i], q);
+        if (c0 == 0)
+            g.out_scale[r] = q.scale;
         return;
-    const Quant q = quant_of(block_max(m, red));
-    for (uint32_t c = threadIdx.x; c < nv; c += 256)
-        *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(g.out) + uint64_t(r) * g.ldo + 4 * c) = quant_pack(row[c], q);
-    if (threadIdx.x == 0)
-        g.out_scale[r] = q.scale;
+    }
+    with_type(g.out_dtype, [&](auto t) {
+        constexpr uint32_t T = decltype(t)::value;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t c = c0 + 64 * W * i;
+            if (c < nv) {
+                const uint64_t o = uint64_t(r) * g.ldo + 4 * c;
+                if constexpr (T == MK_F32)
+                    *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + o) = v[i];
+                else
+                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(g.out) + o) =
+                        u32x2{pack_x2(v[i][0], v[i][1], T == MK_F16), pack_x2(v[i][2], v[i][3], T == MK_F16)};
+            }
+        }
+    });
 }
 
-__device__ inline float load1(const void* p, uint64_t at, uint32_t dtype)
+// The kernel of W waves a row with the fewest float4s a thread that hold it
+template <int W, int NV = 1> void launch_gate_norm(const mk_gate_norm_args& g, hipStream_t s)
 {
-    if (dtype == MK_F32)
-        return static_cast<const float*>(p)[at];
-    const uint16_t h = static_cast<const uint16_t*>(p)[at];
-    return dtype == MK_BF16 ? bf2f_bits(h) : h2f_bits(h);
+    constexpr int kMost = W == 16 ? 4 : W == 4 ? 16 : 4;
+    if constexpr (NV < kMost) {
+        if (g.n > uint32_t(NV) * 256 * W)
+            return launch_gate_norm<W, NV + 1>(g, s);
+    }
+    gate_norm_kernel<W, NV><<<W == 1 ? cdiv(g.rows, 4) : g.rows, W == 1 ? 256 : 64 * W, 0, s>>>(g);
 }
 
-__global__ __launch_bounds__(256) void quantize_i8_kernel(const void* src, uint32_t dtype, uint64_t cols, int64_t ld,
-                                                          int8_t* dst, float* scale)
+// int8 rows from rows of 8 elements times 64 W NV threads: the row stays in registers between its maximum and its codes.
+// 8 elements of T, as loaded
+template <uint32_t T> struct Raw8 {
+    u32x4 w[T == MK_F32 ? 2 : 1];
+    __device__ f32x4 half(int h) const
+    {
+        if constexpr (T == MK_F32) {
+            return __builtin_bit_cast(f32x4, w[h]);
+        } else {
+            const uint32_t a = w[0][2 * h], b = w[0][2 * h + 1];
+            return f32x4{widen<T>(uint16_t(a)), widen<T>(uint16_t(a >> 16)), widen<T>(uint16_t(b)), widen<T>(uint16_t(b >> 16))};
+        }
+    }
+};
+
+template <uint32_t T, int W, int NV>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_i8_kernel(const void* src, uint32_t rows, uint32_t nv,
+                                                                             int64_t ld, int8_t* dst, float* scale)
 {
-    __shared__ float red[4];
+    __shared__ float slots[W];
+    RowRed<W> red{slots};
+    const uint32_t r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (W == 1 && r >= rows)
+        return;
+    const uint32_t c0 = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const char* s = static_cast<const char*>(src) + uint64_t(r) * ld * (T == MK_F32 ? 4 : 2);
+    Raw8<T> v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t c = c0 + 64 * W * i;
+        v[i] = c < nv ? *reinterpret_cast<const Raw8<T>*>(s + uint64_t(c) * sizeof(Raw8<T>)) : Raw8<T>{};
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 f = v[i].half(h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                m = max(m, abs_bits(f[e]));
+        }
+    const Quant q = quant_of(red.max_bits(m, 0));
+    u32x2* d = reinterpret_cast<u32x2*>(dst + uint64_t(r) * nv * 8);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t c = c0 + 64 * W * i;
+        if (c < nv)
+            d[c] = u32x2{quant_pack(v[i].half(0), q), quant_pack(v[i].half(1), q)};
+    }
+    if (c0 == 0)
+        scale[r] = q.scale;
+}
+
+// Rows of any width and alignment, read twice.
+template <uint32_t T>
+__global__ __launch_bounds__(256) void quantize_i8_any_kernel(const void* src, uint64_t cols, int64_t ld, int8_t* dst,
+                                                              float* scale)
+{
+    __shared__ float slots[4];
+    RowRed<4> red{slots};
     const uint64_t r = blockIdx.x;
     uint32_t m = 0;
     for (uint64_t c = threadIdx.x; c < cols; c += 256)
-        m = max(m, abs_bits(load1(src, r * ld + c, dtype)));
-    const Quant q = quant_of(block_max(m, red));
+        m = max(m, abs_bits(load1<T>(src, r * ld + c)));
+    const Quant q = quant_of(red.max_bits(m, 0));
     for (uint64_t c = threadIdx.x; c < cols; c += 256)
-        dst[r * cols + c] = q.inv == 0.0f ? int8_t(0) : int8_t(quant_code(load1(src, r * ld + c, dtype), q));
+        dst[r * cols + c] = q.inv == 0.0f ? int8_t(0) : int8_t(quant_code(load1<T>(src, r * ld + c), q));
     if (threadIdx.x == 0)
         scale[r] = q.scale;
+}
+
+template <uint32_t T, int W, int NV = 1>
+void launch_quantize(const void* src, uint32_t rows, uint32_t cols, int64_t ld, int8_t* dst, float* scale, hipStream_t s)
+{
+    if constexpr (NV < 8) {
+        if (cols > uint32_t(NV) * 512 * W)
+            return launch_quantize<T, W, NV + 1>(src, rows, cols, ld, dst, scale, s);
+    }
+    quantize_i8_kernel<T, W, NV><<<W == 1 ? cdiv(rows, 4) : rows, W == 1 ? 256 : 64 * W, 0, s>>>(src, rows, cols / 8, ld, dst,
+                                                                                                scale);
+}
+template <uint32_t T>
+void quantize_rows(const void* src, uint32_t rows, uint64_t cols, int64_t ld, int8_t* dst, float* scale, bool vector,
+                   hipStream_t s)
+{
+    if (!vector || cols > 16384)
+        quantize_i8_any_kernel<T><<<rows, 256, 0, s>>>(src, cols, ld, dst, scale);
+    else if (cols <= 4096 && rows >= 2048)
+        launch_quantize<T, 1>(src, rows, uint32_t(cols), ld, dst, scale, s);
+    else
+        launch_quantize<T, 4>(src, rows, uint32_t(cols), ld, dst, scale, s);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -247,7 +434,11 @@ mk_status mk_gate_norm(const mk_gate_norm_args* a, void* stream)
         g.seg_rows = 0xffffffffu;
     if (g.residual_scale == 0.0f)
         g.residual_scale = 1.0f;
-    gate_norm_kernel<<<g.rows, 256, g.n * sizeof(float), static_cast<hipStream_t>(stream)>>>(g);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (g.n <= 1024)
+        launch_gate_norm<1>(g, s);
+    else
+        launch_gate_norm<4>(g, s);
     MK_LAUNCH_CHECK("gate_norm");
     return MK_OK;
 }
@@ -265,8 +456,16 @@ mk_status mk_quantize_i8_rows(const void* src, uint32_t src_dtype, uint64_t rows
         return fail(MK_ERR_ARG, "quantize_i8_rows: src and scale must be aligned for an element");
     if (!rows)
         return MK_OK;
-    quantize_i8_kernel<<<uint32_t(rows), 256, 0, static_cast<hipStream_t>(stream)>>>(src, src_dtype, cols, ld,
-                                                                                    static_cast<int8_t*>(dst), scale);
+    // 16-byte loads and 8-byte stores: rows of a multiple of 16 elements, 16-byte aligned
+    const bool vector = cols % 16 == 0 && aligned(src, 16) && aligned(dst, 8) && ld % (src_dtype == MK_F32 ? 4 : 8) == 0;
+    int8_t* d = static_cast<int8_t*>(dst);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (src_dtype == MK_F32)
+        quantize_rows<MK_F32>(src, uint32_t(rows), cols, ld, d, scale, vector, s);
+    else if (src_dtype == MK_BF16)
+        quantize_rows<MK_BF16>(src, uint32_t(rows), cols, ld, d, scale, vector, s);
+    else
+        quantize_rows<MK_F16>(src, uint32_t(rows), cols, ld, d, scale, vector, s);
     MK_LAUNCH_CHECK("quantize_i8_rows");
     return MK_OK;
 }
