@@ -3,6 +3,7 @@
 
 #include <string>
 #include <type_traits>
+#include <utility>
 
 namespace mk {
 
@@ -84,10 +85,18 @@ template <bool GELU> __device__ inline f32x4 act4(const f32x4& v)
         o[e] = GELU ? gelu_tanh_f(v[e]) : silu_f(v[e]);
     return o;
 }
-template <bool SWI> __device__ inline float glu1(float a, float g)
+// g Phi(g), Phi the normal distribution: Phi(-z) = e^(-z^2 / 2) t (a1 + t (a2 + ..)) / 2, t = 1 / (1 + p z / sqrt(2)), for z >= 0
+// (Abramowitz and Stegun 7.1.26, erf within 1.5e-7). erf_fit's longer series and its IEEE division cost 26 us of VALU
+// time at 3952 x 5120 outputs, as much as the product's matrix instructions.
+__device__ inline float gelu_erf_f(float g)
 {
-    return SWI ? silu_f(a) * g : a * (0.5f * g * (1.0f + erf_fit(g * 0.70710678f)));
+    constexpr float p = 0.231641888f, c = -0.72134752f; // 0.3275911 / sqrt(2); -log2(e) / 2
+    const float z = fabsf(g), t = __builtin_amdgcn_rcpf(fmaf(p, z, 1.0f));
+    const float s = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.530702714f, -0.726576013f), 0.710706870f), -0.142248368f), 0.127414796f);
+    const float h = s * __builtin_amdgcn_exp2f(z * z * c);
+    return g * (g < 0.0f ? h : 1.0f - h);
 }
+template <bool SWI> __device__ inline float glu1(float a, float g) { return SWI ? silu_f(a) * g : a * gelu_erf_f(g); }
 __device__ inline f32x4 residual4(const I8P& p, uint32_t row, const f32x4& x, const f32x4& v, const Ch4& k)
 {
     const f32x4 g = row % p.seg_rows < p.split ? k.g1 : k.g0;
@@ -124,38 +133,30 @@ template <int BM, int BN, int NW, int NSTG> constexpr int tile_lds()
     return ops > epi ? ops : epi;
 }
 
+// f(std::integral_constant<int, 0>{}), f(1), ..
+template <class F, int... I> __device__ __forceinline__ void for_each_int(F&& f, std::integer_sequence<int, I...>)
+{
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+// One tile: tokens m0 .. m0 + BM of batch item z, output channels from n0.
 template <int BM, int BN, int NW, int NSTG, int EC>
-__global__ __launch_bounds__(64 * NW, 1) __attribute__((amdgpu_waves_per_eu(
-    NW == 8 || tile_lds<BM, BN, NW, NSTG>() <= 80 * 1024 ? 2 : 1,
-    NW == 8 || tile_lds<BM, BN, NW, NSTG>() <= 80 * 1024 ? 2 : 1))) void gemm_i8_kernel(I8P p, uint32_t tiles_m,
-                                                                                      uint32_t tiles_n)
+__device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0, int8_t* smem)
 {
     constexpr bool GLU = EC == EC_GLU;
     constexpr int NT = 64 * NW, WM = BM / (NW / 2), WC = BN / 2, TB = WM / 16, CB = WC / 16;
     constexpr int RA = BM * 8 / NT, RW = BN * 8 / NT, ND = RA + RW; // direct loads a thread makes a k step
     constexpr int LDW = WC + 4;
     static_assert((NSTG - 2) * ND <= 63 && WM % 32 == 0, "");
-    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<BM, BN, NW, NSTG>()];
     int8_t(*sW)[BN * 128] = reinterpret_cast<int8_t(*)[BN * 128]>(smem);
     int8_t(*sA)[BM * 128] = reinterpret_cast<int8_t(*)[BM * 128]>(smem + NSTG * BN * 128);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave & 1, wm = wave >> 1;
 
-    // workgroup i runs on XCD i % 8: each XCD takes a run of tiles, 8 token tiles at a time, which share weight panels in
-    // its L2
-    uint32_t z, tm, tn;
-    {
-        const uint32_t n = gridDim.x, x = blockIdx.x % 8, q = n / 8, t = x * q + min(x, n % 8) + blockIdx.x / 8;
-        const uint32_t per = tiles_m * tiles_n, pid = t % per, in_group = 8 * tiles_n;
-        z = t / per;
-        const uint32_t first = pid / in_group * 8, g = min(tiles_m - first, 8u), i = pid % in_group;
-        tm = first + i % g;
-        tn = i / g;
-    }
-    const int m0 = int(tm) * BM, cols = int(GLU ? p.N / 2 : p.N);
+    const int cols = int(GLU ? p.N / 2 : p.N);
     // GLU: the tile makes channels n0 .. n0 + BN / 2, a wave's rows are WC / 2 rows of the first part and the same
     // channels' rows of the second, so a lane's blocks cb and cb + CB / 2 are the two operands of one output.
-    const int n0 = int(tn) * (GLU ? BN / 2 : BN), nr = min(cols - n0, GLU ? BN / 2 : BN);
+    const int nr = min(cols - n0, GLU ? BN / 2 : BN);
 
     // Direct loads: wave w's round i fills LDS chunks (i NW + w) 64 + lane; chunk P holds row P / 8 and k chunk
     // swz_chunk(row, P % 8). Buffer loads: the resource spans the tile's rows, the lane's byte offset selects row and
@@ -180,7 +181,6 @@ __global__ __launch_bounds__(64 * NW, 1) __attribute__((amdgpu_waves_per_eu(
         const int r = (i * NW + wave) * 8 + (lane >> 3);
         ow[i] = uint32_t(min(GLU ? (r / WC) * (WC / 2) + r % (WC / 2) : r, nr - 1)) * p.K + kc * 16;
     }
-    static_assert(!GLU || (WC / 2) % (8 * NW) == 0 || (8 * NW) % WC == 0, "");
     // direct load i (activation rounds first) of k step kt into stage buf; past: what leaves the range in the last, partial
     // step for the lanes whose chunk lies past K
     auto dma1 = [&](int kt, uint32_t past, int buf, int i) {
@@ -217,7 +217,8 @@ __global__ __launch_bounds__(64 * NW, 1) __attribute__((amdgpu_waves_per_eu(
     // A substep: the weight fragments are single-buffered, each next one read into its registers right after the last
     // product that uses it; the next token fragments go to the other buffer with the first channel block; the direct loads
     // of step gkt (into stage gbuf) follow one product each. Every instruction is fenced: the order is this one.
-    auto substep = [&](const i32x4(&af)[TB], int nbuf, int nks, i32x4(&naf)[TB], int gkt, int gbuf, bool load) {
+    auto substep = [&](const i32x4(&af)[TB], int nbuf, int nks, i32x4(&naf)[TB], int gkt, int gbuf,
+                       bool load) __attribute__((always_inline)) {
         const uint32_t gp = past(gkt);
 #pragma unroll
         for (int i = 0; i < CB * TB; ++i) {
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(64 * NW, 1) __attribute__((amdgpu_waves_per_eu(
     // k step kt in stage `buf` (a constant: the loop is unrolled by NSTG): the first substep reads the second's fragments;
     // then step kt + 1 has landed (later ones may be in flight) and, after the barrier, in every wave, and every wave has
     // read this stage, so the second substep loads step kt + NSTG into it and reads step kt + 1's first fragments
-    auto step = [&](int kt, auto buf_c) {
+    auto step = [&](int kt, auto buf_c) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value, nb = (buf + 1) % NSTG;
         substep(af0, buf, 1, af1, 0, 0, false);
         __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
@@ -270,20 +271,14 @@ __global__ __launch_bounds__(64 * NW, 1) __attribute__((amdgpu_waves_per_eu(
         substep(af1, nb, 0, af0, min(kt + NSTG, ke - 1), buf, true);
     };
     int kt = 0;
-    for (; kt + NSTG - 1 < ke; kt += NSTG) {
-        step(kt, std::integral_constant<int, 0>{});
-        step(kt + 1, std::integral_constant<int, 1>{});
-        if constexpr (NSTG > 2)
-            step(kt + 2, std::integral_constant<int, 2 % NSTG>{});
-        if constexpr (NSTG > 3)
-            step(kt + 3, std::integral_constant<int, 3 % NSTG>{});
-    }
-    if (kt < ke)
-        step(kt, std::integral_constant<int, 0>{});
-    if (NSTG > 2 && kt + 1 < ke)
-        step(kt + 1, std::integral_constant<int, 1>{});
-    if (NSTG > 3 && kt + 2 < ke)
-        step(kt + 2, std::integral_constant<int, 2 % NSTG>{});
+    for (; kt + NSTG - 1 < ke; kt += NSTG)
+        for_each_int([&](auto i) __attribute__((always_inline)) { step(kt + decltype(i)::value, i); }, std::make_integer_sequence<int, NSTG>{});
+    for_each_int(
+        [&](auto i) __attribute__((always_inline)) {
+            if (kt + decltype(i)::value < ke)
+                step(kt + decltype(i)::value, i);
+        },
+        std::make_integer_sequence<int, NSTG - 1>{});
     __builtin_amdgcn_s_waitcnt(0); // the last loads land before the LDS is reused
     __syncthreads();
 
@@ -392,6 +387,62 @@ __global__ __launch_bounds__(64 * NW, 1) __attribute__((amdgpu_waves_per_eu(
     }
 }
 
+// Workgroup i runs on XCD i % 8 and each XCD has an L2 of its own: of n workgroups XCD x takes a run.
+__device__ inline uint32_t xcd_run(uint32_t i, uint32_t n)
+{
+    const uint32_t x = i % 8;
+    return x * (n / 8) + min(x, n % 8) + i / 8;
+}
+// Tile t of the launch, 8 token tiles at a time, so that a run of tiles shares weight panels
+__device__ inline void locate(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, uint32_t& z, uint32_t& tm, uint32_t& tn)
+{
+    const uint32_t per = tiles_m * tiles_n, in_group = 8 * tiles_n;
+    z = t / per;
+    t %= per;
+    const uint32_t first = t / in_group * 8, g = min(tiles_m - first, 8u), i = t % in_group;
+    tm = first + i % g;
+    tn = i / g;
+}
+
+// waves a SIMD: two where 8 waves share the LDS, or two workgroups of 4 fit it
+template <int BM, int BN, int NW, int NSTG> constexpr int tile_waves()
+{
+    return NW == 8 || tile_lds<BM, BN, NW, NSTG>() <= 80 * 1024 ? 2 : 1;
+}
+
+template <int BM, int BN, int NW, int NSTG, int EC>
+__global__ __launch_bounds__(64 * NW, (tile_waves<BM, BN, NW, NSTG>())) __attribute__((amdgpu_waves_per_eu(
+    tile_waves<BM, BN, NW, NSTG>(), tile_waves<BM, BN, NW, NSTG>()))) void gemm_i8_kernel(I8P p, uint32_t tiles_m,
+                                                                                          uint32_t tiles_n)
+{
+    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<BM, BN, NW, NSTG>()];
+    uint32_t z, tm, tn;
+    locate(xcd_run(blockIdx.x, gridDim.x), tiles_m, tiles_n, z, tm, tn);
+    i8_tile<BM, BN, NW, NSTG, EC>(p, z, int(tm) * BM, int(tn) * (EC == EC_GLU ? BN / 2 : BN), smem);
+}
+
+// 256 x 256 tiles, the first `whole` of them one a workgroup, the rest a quarter (128 x 128) a workgroup: whole rounds of the
+// chip take the large tile, the last, partial one spreads over all of it.
+template <int EC>
+__global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_mixed_kernel(
+    I8P p, uint32_t tiles_m, uint32_t tiles_n, uint32_t whole)
+{
+    constexpr int BO = EC == EC_GLU ? 128 : 256; // output channels of a tile
+    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<256, 256, 8, 2>()];
+    static_assert(tile_lds<128, 128, 8, 4>() <= tile_lds<256, 256, 8, 2>(), "");
+    uint32_t z, tm, tn;
+    if (blockIdx.x < whole) {
+        locate(xcd_run(blockIdx.x, whole), tiles_m, tiles_n, z, tm, tn);
+        i8_tile<256, 256, 8, 2, EC>(p, z, int(tm) * 256, int(tn) * BO, smem);
+        return;
+    }
+    const uint32_t i = xcd_run(blockIdx.x - whole, gridDim.x - whole);
+    locate(whole + i / 4, tiles_m, tiles_n, z, tm, tn);
+    const uint32_t m0 = tm * 256 + (i & 2) * 64, n0 = tn * BO + (i & 1) * (BO / 2);
+    if (m0 < p.M && n0 < (EC == EC_GLU ? p.N / 2 : p.N))
+        i8_tile<128, 128, 8, 4, EC>(p, z, int(m0), int(n0), smem);
+}
+
 // ------------------------------------------------------------------------------------------------------------
 // Few rows (up to 16 TB): a workgroup makes 16 channels of all rows, its 8 waves every eighth 256 bytes of k each,
 // straight from memory: nothing of the weight is read twice, and all of a launch's loads are in flight at once. The sums
@@ -443,17 +494,21 @@ template <int TB, int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm
                 for (int tb = 0; tb < TB; ++tb)
                     acc[c][tb] = mfma_i8(f.w[s][c], f.a[s][tb], acc[c][tb]);
     };
+    // two units in turn, each loaded while the other one is multiplied
     constexpr uint32_t kStep = kFewWaves * kFewUnit;
-    Unit f[2];
+    Unit f0, f1;
     uint32_t k = uint32_t(wave) * kFewUnit;
-    if (k < p.K) {
-        load(k, f[0]);
-        for (; k + kStep < p.K; k += kStep) {
-            load(k + kStep, f[1]);
-            mul(f[0]);
-            f[0] = f[1];
-        }
-        mul(f[0]);
+    if (k < p.K)
+        load(k, f0);
+    for (; k < p.K; k += 2 * kStep) {
+        if (k + kStep < p.K)
+            load(k + kStep, f1);
+        mul(f0);
+        if (k + kStep >= p.K)
+            break;
+        if (k + 2 * kStep < p.K)
+            load(k + 2 * kStep, f0);
+        mul(f1);
     }
 #pragma unroll
     for (int c = 0; c < CB; ++c)
@@ -515,6 +570,22 @@ template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const 
     return MK_OK;
 }
 
+int tile_of(const I8P& p, bool, uint32_t cus)
+{
+    return uint64_t(cdiv(p.M, 256)) * cdiv(p.N, 256) * p.batch >= cus ? 0 : 1;
+}
+
+template <int EC> mk_status launch_mixed(const I8P& p, uint32_t cus, hipStream_t s)
+{
+    const uint32_t tm = cdiv(p.M, 256), tn = cdiv(p.N, 256);
+    const uint64_t tiles = uint64_t(tm) * tn * p.batch, whole = tiles / cus * cus;
+    if (tiles > 0x7fffffffu)
+        return fail(MK_ERR_ARG, "gemm_i8: too many tiles");
+    gemm_i8_mixed_kernel<EC><<<uint32_t(whole + (tiles - whole) * 4), 512, 0, s>>>(p, tm, tn, uint32_t(whole));
+    MK_LAUNCH_CHECK("gemm_i8");
+    return MK_OK;
+}
+
 template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
 {
     const uint32_t cols = EC == EC_GLU ? p.N / 2 : p.N;
@@ -529,10 +600,18 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
         MK_LAUNCH_CHECK("gemm_i8");
         return MK_OK;
     }
-    const uint64_t big = uint64_t(cdiv(p.M, 256)) * cdiv(p.N, 256) * p.batch;
-    if (big >= cus)
-        return launch_tile<256, 256, 8, 2, EC>(p, s);
-    return launch_tile<128, 128, 4, 2, EC>(p, s);
+    switch (tile_of(p, EC == EC_GLU, cus)) {
+    case 0: return launch_tile<256, 256, 8, 2, EC>(p, s);
+    case 1: return launch_tile<128, 128, 4, 2, EC>(p, s);
+    case 2: return launch_tile<128, 128, 4, 4, EC>(p, s);
+    case 3: return launch_tile<64, 128, 4, 6, EC>(p, s);
+    case 4: return launch_tile<64, 64, 4, 8, EC>(p, s);
+    case 5: return launch_tile<64, 64, 4, 4, EC>(p, s);
+    case 6: return launch_tile<128, 256, 8, 3, EC>(p, s);
+    case 7: return launch_tile<256, 128, 8, 3, EC>(p, s);
+    case 9: return launch_mixed<EC>(p, cus, s);
+    default: return launch_tile<64, 128, 4, 3, EC>(p, s);
+    }
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

@@ -350,20 +350,27 @@ def _check_gemm_i8(args, ascale, stream=None):
 
 def _check_gate_norm(args, stream=None):
     g = _struct(args, GateNormArgs)
-    if g.rows == 0 or g.n == 0:
+    rows, n = g.rows, g.n
+    if rows == 0 or n == 0:
         return
-    what = "mk_gate_norm: "
-    for name, ld, size in (("x", g.ldx, 4), ("x_out", g.ldx, 4), ("y", g.ldy, _SIZE.get(g.y_dtype, 4)),
-                           ("out", g.ldo, _SIZE.get(g.out_dtype, 4))):
-        check_extent(getattr(g, name), ((g.rows - 1) * ld + g.n) * size, what + name)
-    if g.out_dtype == I8:
-        check_extent(g.out_scale, g.rows * 4, what + "out_scale")
-    for name in ("w1", "b1", "w2", "b2"):
-        check_extent(getattr(g, name), g.n * 4, what + name)
-    seg = g.seg_rows or g.rows
-    last = (g.rows - 1) // seg * max(int(g.mod_stride), 0) + (max(int(g.alt), 0) if g.split else 0)
-    for name in ("gate", "scale", "shift"):
-        check_extent(getattr(g, name), (last + g.n) * 4, what + name)
+    x = ((rows - 1) * g.ldx + n) * 4
+    check_extent(g.x, x, "mk_gate_norm: x")
+    check_extent(g.x_out, x, "mk_gate_norm: x_out")
+    check_extent(g.y, ((rows - 1) * g.ldy + n) * _SIZE.get(g.y_dtype, 4), "mk_gate_norm: y")
+    dt = g.out_dtype
+    check_extent(g.out, ((rows - 1) * g.ldo + n) * _SIZE.get(dt, 4), "mk_gate_norm: out")
+    if dt == I8:
+        check_extent(g.out_scale, rows * 4, "mk_gate_norm: out_scale")
+    for name in ("w1", "b1", "w2", "b2") if g.norm1 or g.norm2 else ():
+        p = getattr(g, name)
+        if p:
+            check_extent(p, n * 4, "mk_gate_norm: " + name)
+    gate, scale, shift = g.gate, g.scale, g.shift
+    if gate or scale or shift:
+        last = (rows - 1) // (g.seg_rows or rows) * max(g.mod_stride, 0) + (max(g.alt, 0) if g.split else 0)
+        check_extent(gate, (last + n) * 4, "mk_gate_norm: gate")
+        check_extent(scale, (last + n) * 4, "mk_gate_norm: scale")
+        check_extent(shift, (last + n) * 4, "mk_gate_norm: shift")
 
 
 def _check_quantize_i8(src, dtype, rows, cols, ld, dst, scale, stream=None):
