@@ -1,6 +1,7 @@
 // proj in 8-bit integers: C = epilogue(ascale[r] wscale[n] sum_k A[r][k] W[n][k] + bias[n]), int32 sums.
 #include "common.hpp"
 
+#include <algorithm>
 #include <string>
 #include <type_traits>
 #include <utility>
@@ -206,7 +207,12 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
     // lane (r16, g4) supplies row r16 of a 16-row block and k bytes 16 g4 .. + 15 of a 64-deep substep, and holds channels
     // 4 g4 .. + 3 of token r16
     const int r16 = lane & 15, g4 = lane >> 4;
+    // Two schedules. A small wave tile (at most 16 blocks) has too few products in a substep to cover the LDS's latency:
+    // it reads a whole k step's fragments one step ahead (WIDE; two sets of registers). A large one reads a substep ahead.
+    constexpr bool WIDE = CB * TB <= 16;
+    static_assert(!WIDE || NSTG % 2 == 0, "a step's register set is its parity");
     i32x4 wf[CB], af0[TB], af1[TB];
+    i32x4 fr[2][2][WIDE ? CB + TB : 1]; // [parity][substep][weight blocks, then token blocks]
     // (blocks are 16 rows apart, so the swizzle is the lane's: an address is one of two registers plus a constant)
     const int fw[2] = {swz(wn * WC + r16, g4), swz(wn * WC + r16, 4 + g4)};
     const int fa[2] = {swz(wm * WM + r16, g4), swz(wm * WM + r16, 4 + g4)};
@@ -254,17 +260,55 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
     }
     __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 1) * ND > 63 ? 63 : (NSTG - 1) * ND));
     __builtin_amdgcn_s_barrier();
+    // fragment j of a step in the order of use: substep j / (CB + TB)
+    auto frag = [&](int buf, int j, i32x4(&f)[2][WIDE ? CB + TB : 1]) {
+        const int ks = j / (CB + TB), i = j % (CB + TB);
+        f[ks][i] = *reinterpret_cast<const i32x4*>(i < CB ? &sW[buf][fw[ks] + i * 2048] : &sA[buf][fa[ks] + (i - CB) * 2048]);
+    };
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb)
-        rdw(0, 0, cb);
+        for (int j = 0; j < 2 * (CB + TB); ++j)
+            frag(0, j, fr[0]);
+    } else {
 #pragma unroll
-    for (int tb = 0; tb < TB; ++tb)
-        rda(0, 0, tb, af0);
+        for (int cb = 0; cb < CB; ++cb)
+            rdw(0, 0, cb);
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+            rda(0, 0, tb, af0);
+    }
     // k step kt in stage `buf` (a constant: the loop is unrolled by NSTG): the first substep reads the second's fragments;
     // then step kt + 1 has landed (later ones may be in flight) and, after the barrier, in every wave, and every wave has
     // read this stage, so the second substep loads step kt + NSTG into it and reads step kt + 1's first fragments
     auto step = [&](int kt, auto buf_c) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value, nb = (buf + 1) % NSTG;
+        if constexpr (WIDE) {
+            // this step's fragments are in registers (read before the barrier), step kt + 1 has landed: its fragments
+            // are read and step kt + NSTG goes into this stage while this step's products run
+            constexpr int NM = 2 * CB * TB, NF = 2 * (CB + TB), RPM = (2 * NF + NM - 1) / NM, LPM = (2 * ND + NM - 1) / NM;
+            __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
+            __builtin_amdgcn_s_barrier();
+            const int kl = min(kt + NSTG, ke - 1);
+            const uint32_t gp = past(kl);
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+                const int ks = i / (CB * TB), cb = i % (CB * TB) / TB, tb = i % TB;
+                acc[cb][tb] = mfma_i8(fr[buf % 2][ks][cb], fr[buf % 2][ks][CB + tb], acc[cb][tb]);
+                __builtin_amdgcn_sched_barrier(0);
+                // the reads in the first half of the products, the loads behind them
+#pragma unroll
+                for (int j = i * RPM; j < (i + 1) * RPM && j < NF; ++j) {
+                    frag(nb, j, fr[(buf + 1) % 2]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int j = i * LPM; j < (i + 1) * LPM && j < ND; ++j) {
+                    dma1(kl, gp, buf, j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            return;
+        }
         substep(af0, buf, 1, af1, 0, 0, false);
         __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
         __builtin_amdgcn_s_barrier();
@@ -437,40 +481,44 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         return;
     }
     const uint32_t i = xcd_run(blockIdx.x - whole, gridDim.x - whole);
-    locate(whole + i / 4, tiles_m, tiles_n, z, tm, tn);
-    const uint32_t m0 = tm * 256 + (i & 2) * 64, n0 = tn * BO + (i & 1) * (BO / 2);
+    uint32_t m0, n0;
+    if (whole) {
+        locate(whole + i / 4, tiles_m, tiles_n, z, tm, tn);
+        m0 = tm * 256 + (i & 2) * 64;
+        n0 = tn * BO + (i & 1) * (BO / 2);
+    } else { // less than a round: the launch's tiles are the small ones
+        locate(i, tiles_m, tiles_n, z, tm, tn);
+        m0 = tm * 128;
+        n0 = tn * (BO / 2);
+    }
     if (m0 < p.M && n0 < (EC == EC_GLU ? p.N / 2 : p.N))
         i8_tile<128, 128, 8, 4, EC>(p, z, int(m0), int(n0), smem);
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Few rows (up to 16 TB): a workgroup makes 16 channels of all rows, its 8 waves every eighth 256 bytes of k each,
-// straight from memory: nothing of the weight is read twice, and all of a launch's loads are in flight at once. The sums
-// meet in LDS.
+// Up to 16 rows: a workgroup makes 16 channels of all rows, its 8 waves every eighth 256 bytes of k each, straight from
+// memory to registers; nothing of the weight is read twice. The sums meet in LDS.
 // ------------------------------------------------------------------------------------------------------------
-constexpr int kFewWaves = 8, kFewUnit = 256;
+constexpr int kFewWaves = 8;
 
-template <int TB, int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_kernel(I8P p)
+template <int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_kernel(I8P p)
 {
     constexpr bool GLU = EC == EC_GLU;
-    constexpr int CB = GLU ? 2 : 1, NS = kFewUnit / 64;
-    __shared__ i32x4 red[kFewWaves][CB * TB][64];
+    constexpr int CB = GLU ? 2 : 1, NS = 4;
+    constexpr uint32_t kUnit = 64 * NS, kStep = kFewWaves * kUnit;
+    __shared__ i32x4 red[kFewWaves][CB][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r16 = lane & 15, g4 = lane >> 4, cols = int(GLU ? p.N / 2 : p.N), n0 = blockIdx.x * 16;
+    const int r16 = lane & 15, g4 = lane >> 4, cols = int(GLU ? p.N / 2 : p.N), n0 = int(blockIdx.x) * 16;
     const uint32_t z = blockIdx.y;
     const int nr = min(cols - n0, 16), M = int(p.M);
     const int8_t* gA = p.a + int64_t(z) * p.sa;
     const int8_t* gW = p.w + uint64_t(n0) * p.K;
     const BufRes rsA = buf_res(gA, uint32_t(int64_t(M - 1) * p.lda + p.K));
     const BufRes rsW[2] = {buf_res(gW, uint32_t(nr) * p.K), buf_res(GLU ? gW + uint64_t(cols) * p.K : gW, uint32_t(nr) * p.K)};
-    const uint32_t ow = uint32_t(min(r16, nr - 1)) * p.K + g4 * 16;
-    uint32_t oa[TB];
-#pragma unroll
-    for (int tb = 0; tb < TB; ++tb)
-        oa[tb] = uint32_t(min(tb * 16 + r16, M - 1)) * uint32_t(p.lda) + g4 * 16;
-    i32x4 acc[CB][TB] = {};
+    const uint32_t ow = uint32_t(min(r16, nr - 1)) * p.K + g4 * 16, oa = uint32_t(min(r16, M - 1)) * uint32_t(p.lda) + g4 * 16;
+    i32x4 acc[CB] = {};
     struct Unit {
-        i32x4 w[NS][CB], a[NS][TB];
+        i32x4 w[NS][CB], a[NS];
     };
     auto load = [&](uint32_t k, Unit& f) {
 #pragma unroll
@@ -480,9 +528,7 @@ template <int TB, int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm
 #pragma unroll
             for (int c = 0; c < CB; ++c)
                 f.w[s][c] = __builtin_bit_cast(i32x4, buf_load16(rsW[c], in ? ow + s * 64 : 0xfffffff0u, in ? k : 0));
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-                f.a[s][tb] = __builtin_bit_cast(i32x4, buf_load16(rsA, in ? oa[tb] + s * 64 : 0xfffffff0u, in ? k : 0));
+            f.a[s] = __builtin_bit_cast(i32x4, buf_load16(rsA, in ? oa + s * 64 : 0xfffffff0u, in ? k : 0));
         }
     };
     auto mul = [&](const Unit& f) {
@@ -490,14 +536,11 @@ template <int TB, int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int c = 0; c < CB; ++c)
-#pragma unroll
-                for (int tb = 0; tb < TB; ++tb)
-                    acc[c][tb] = mfma_i8(f.w[s][c], f.a[s][tb], acc[c][tb]);
+                acc[c] = mfma_i8(f.w[s][c], f.a[s], acc[c]);
     };
     // two units in turn, each loaded while the other one is multiplied
-    constexpr uint32_t kStep = kFewWaves * kFewUnit;
     Unit f0, f1;
-    uint32_t k = uint32_t(wave) * kFewUnit;
+    uint32_t k = uint32_t(wave) * kUnit;
     if (k < p.K)
         load(k, f0);
     for (; k < p.K; k += 2 * kStep) {
@@ -512,50 +555,44 @@ template <int TB, int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm
     }
 #pragma unroll
     for (int c = 0; c < CB; ++c)
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-            red[wave][c * TB + tb][lane] = acc[c][tb];
+        red[wave][c][lane] = acc[c];
     __syncthreads();
-    // wave tb finishes tokens 16 tb .. + 15
-    for (int tb = wave; tb < TB; tb += kFewWaves) {
-        const int tok = tb * 16 + r16, ch = n0 + 4 * g4;
-        i32x4 s[CB] = {};
+    const int tok = r16, ch = n0 + 4 * g4;
+    if (wave || tok >= M || ch >= cols)
+        return;
+    i32x4 s[CB] = {};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w)
+    for (int w = 0; w < kFewWaves; ++w)
 #pragma unroll
-            for (int c = 0; c < CB; ++c)
-                s[c] += red[w][c * TB + tb][lane];
-        if (tok >= M || ch >= cols)
-            continue;
-        const float as = p.ascale[uint64_t(z) * p.M + tok];
-        const Ch4 kc = channels4(p, ch);
-        f32x4 t;
+        for (int c = 0; c < CB; ++c)
+            s[c] += red[w][c][lane];
+    const float as = p.ascale[uint64_t(z) * p.M + tok];
+    const Ch4 kc = channels4(p, ch);
+    f32x4 t;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        t[e] = float(s[0][e]) * as;
+    f32x4 v = scaled(t, kc.ws, kc.b);
+    if constexpr (GLU) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            t[e] = float(s[0][e]) * as;
-        f32x4 v = scaled(t, kc.ws, kc.b);
-        if constexpr (GLU) {
-            f32x4 g;
+            t[e] = float(s[CB - 1][e]) * as;
+        const f32x4 g = scaled(t, *reinterpret_cast<const f32x4*>(p.wscale + cols + ch), load4(p.bias, cols + ch, 0.0f));
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                t[e] = float(s[CB - 1][e]) * as;
-            g = scaled(t, *reinterpret_cast<const f32x4*>(p.wscale + cols + ch), load4(p.bias, cols + ch, 0.0f));
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = p.epi == MK_EPI_SWIGLU ? glu1<true>(v[e], g[e]) : glu1<false>(v[e], g[e]);
-        } else if constexpr (EC == EC_ACT) {
-            v = p.epi == MK_EPI_GELU_TANH ? act4<true>(v) : act4<false>(v);
-        }
-        const int64_t at = int64_t(z) * p.sc + int64_t(tok) * p.ldc + ch;
-        if constexpr (EC == EC_RMW) {
-            f32x4* x = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
-            *x = residual4(p, uint32_t(tok), *x, v, kc);
-        } else if (p.c_dtype == MK_F32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at) = v;
-        } else {
-            const bool h = p.c_dtype == MK_F16;
-            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.c) + at) = u32x2{pack_x2(v[0], v[1], h), pack_x2(v[2], v[3], h)};
-        }
+        for (int e = 0; e < 4; ++e)
+            v[e] = p.epi == MK_EPI_SWIGLU ? glu1<true>(v[e], g[e]) : glu1<false>(v[e], g[e]);
+    } else if constexpr (EC == EC_ACT) {
+        v = p.epi == MK_EPI_GELU_TANH ? act4<true>(v) : act4<false>(v);
+    }
+    const int64_t at = int64_t(z) * p.sc + int64_t(tok) * p.ldc + ch;
+    if constexpr (EC == EC_RMW) {
+        f32x4* x = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
+        *x = residual4(p, uint32_t(tok), *x, v, kc);
+    } else if (p.c_dtype == MK_F32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at) = v;
+    } else {
+        const bool h = p.c_dtype == MK_F16;
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.c) + at) = u32x2{pack_x2(v[0], v[1], h), pack_x2(v[2], v[3], h)};
     }
 }
 
@@ -570,48 +607,71 @@ template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const 
     return MK_OK;
 }
 
-int tile_of(const I8P& p, bool, uint32_t cus)
-{
-    return uint64_t(cdiv(p.M, 256)) * cdiv(p.N, 256) * p.batch >= cus ? 0 : 1;
-}
+// The kernel of a launch: the one with the least estimated time in us, beside a launch's own. A tile takes its k steps of
+// 128 at the rate its CU brings operands in (64 x 32: 0.09, 64 x 64: 0.14, 128 x 128: 0.36 a step) or, where all CUs load, at the
+// 22.4 TB/s that they take from the L2s together; 256 x 256 tiles are bound by the matrix cores (1.54 a step, 7.7 for the
+// epilogue that nothing overlaps). Fitted to the four kernels' times at 198 shapes (rows 1 .. 4096, N and K 256 .. 12288); the choice is
+// within 0.3% of the best of the four in the mean, 13% at worst (16 x 4096 x 12288: 13.3 us against 11.8). Measured, us, few /
+// 64 x 32 / 64 x 64 / mixed: 1 x 4096 x 4096 4.5 / 6.1 / 7.6 / 14.1, 1 x 12288 x 4096 14.0 / 10.6 / 9.7 / 14.2, 77 x 2560 x 2048
+// - / 4.4 / 5.0 / 9.0, 300 x 4096 x 12288 - / 38.0 / 35.2 / 36.4, 1024 x 4096 x 4096 - / 35.8 / 26.9 / 19.1.
+enum { K_FEW, K_64X32, K_64X64, K_MIXED };
 
-template <int EC> mk_status launch_mixed(const I8P& p, uint32_t cus, hipStream_t s)
+int kernel_of(const I8P& p, bool glu, uint32_t cus)
 {
-    const uint32_t tm = cdiv(p.M, 256), tn = cdiv(p.N, 256);
-    const uint64_t tiles = uint64_t(tm) * tn * p.batch, whole = tiles / cus * cus;
-    if (tiles > 0x7fffffffu)
-        return fail(MK_ERR_ARG, "gemm_i8: too many tiles");
-    gemm_i8_mixed_kernel<EC><<<uint32_t(whole + (tiles - whole) * 4), 512, 0, s>>>(p, tm, tn, uint32_t(whole));
-    MK_LAUNCH_CHECK("gemm_i8");
-    return MK_OK;
+    const double steps = double(cdiv(p.K, 128));
+    auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t(cdiv(p.M, bm)) * cdiv(p.N, bn) * p.batch; };
+    auto rounds = [&](uint64_t n) { return double((n + cus - 1) / cus); };
+    auto small = [&](uint32_t bm, uint32_t bn, double step, double end) {
+        const uint64_t n = tiles(bm, bn);
+        return std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / 22.4e6 * 256 / cus);
+    };
+    double best = 1e30;
+    int kernel = K_MIXED;
+    auto consider = [&](int k, double t) {
+        if (t < best) {
+            best = t;
+            kernel = k;
+        }
+    };
+    if (p.M <= 16)
+        consider(K_FEW, std::max(rounds(tiles(16, 16)) * p.K * 3.4e-4, double(p.N) * p.K * p.batch * 0.174e-6) + 0.3);
+    if (!glu) // (its two parts are 16 channels of a wave each)
+        consider(K_64X32, small(64, 32, 0.0891, 0.734));
+    consider(K_64X64, small(64, 64, 0.144, 0.692));
+    const uint64_t big = tiles(256, 256), whole = big / cus;
+    const double quarter = steps * 0.359 + 1.25;
+    consider(K_MIXED, whole ? double(whole) * (steps * 1.54 + 7.7) + rounds((big - whole * cus) * 4) * quarter
+                            : rounds(tiles(128, 128)) * quarter);
+    return kernel;
 }
 
 template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
 {
-    const uint32_t cols = EC == EC_GLU ? p.N / 2 : p.N;
-    if (p.M <= 64) {
-        const dim3 grid(cdiv(cols, 16), p.batch);
-        if (p.M <= 16)
-            gemm_i8_few_kernel<1, EC><<<grid, 64 * kFewWaves, 0, s>>>(p);
-        else if (p.M <= 32)
-            gemm_i8_few_kernel<2, EC><<<grid, 64 * kFewWaves, 0, s>>>(p);
-        else
-            gemm_i8_few_kernel<4, EC><<<grid, 64 * kFewWaves, 0, s>>>(p);
-        MK_LAUNCH_CHECK("gemm_i8");
-        return MK_OK;
+    switch (kernel_of(p, EC == EC_GLU, cus)) {
+    case K_FEW:
+        gemm_i8_few_kernel<EC><<<dim3(cdiv(EC == EC_GLU ? p.N / 2 : p.N, 16), p.batch), 64 * kFewWaves, 0, s>>>(p);
+        break;
+    case K_64X32:
+        if constexpr (EC != EC_GLU)
+            return launch_tile<64, 32, 4, 6, EC>(p, s);
+    case K_64X64:
+        return launch_tile<64, 64, 4, 4, EC>(p, s);
+    default: {
+        uint32_t tm = cdiv(p.M, 256), tn = cdiv(p.N, 256);
+        const uint64_t tiles = uint64_t(tm) * tn * p.batch, whole = tiles / cus * cus;
+        uint64_t grid = whole + (tiles - whole) * 4;
+        if (!whole) {
+            tm = cdiv(p.M, 128);
+            tn = cdiv(p.N, 128);
+            grid = uint64_t(tm) * tn * p.batch;
+        }
+        if (grid > 0x7fffffffu)
+            return fail(MK_ERR_ARG, "gemm_i8: too many tiles");
+        gemm_i8_mixed_kernel<EC><<<uint32_t(grid), 512, 0, s>>>(p, tm, tn, uint32_t(whole));
     }
-    switch (tile_of(p, EC == EC_GLU, cus)) {
-    case 0: return launch_tile<256, 256, 8, 2, EC>(p, s);
-    case 1: return launch_tile<128, 128, 4, 2, EC>(p, s);
-    case 2: return launch_tile<128, 128, 4, 4, EC>(p, s);
-    case 3: return launch_tile<64, 128, 4, 6, EC>(p, s);
-    case 4: return launch_tile<64, 64, 4, 8, EC>(p, s);
-    case 5: return launch_tile<64, 64, 4, 4, EC>(p, s);
-    case 6: return launch_tile<128, 256, 8, 3, EC>(p, s);
-    case 7: return launch_tile<256, 128, 8, 3, EC>(p, s);
-    case 9: return launch_mixed<EC>(p, cus, s);
-    default: return launch_tile<64, 128, 4, 3, EC>(p, s);
     }
+    MK_LAUNCH_CHECK("gemm_i8");
+    return MK_OK;
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
