@@ -2,6 +2,7 @@
 #include "common.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <type_traits>
 #include <utility>
@@ -674,6 +675,24 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
     return MK_OK;
 }
 
+// Compute units of the current device, asked once a device (the question costs as much as a launch).
+mk_status compute_units(uint32_t& n)
+{
+    static std::atomic<int> known[64];
+    int dev = 0, cus = 0;
+    MK_HIP(hipGetDevice(&dev));
+    if (dev >= 0 && dev < 64)
+        cus = known[dev].load(std::memory_order_relaxed);
+    if (!cus) {
+        MK_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+        cus = std::max(cus, 1);
+        if (dev >= 0 && dev < 64)
+            known[dev].store(cus, std::memory_order_relaxed);
+    }
+    n = uint32_t(cus);
+    return MK_OK;
+}
+
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 } // namespace
@@ -739,10 +758,8 @@ extern "C" mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void
                 a->epilogue,
                 a->c_dtype};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    int dev = 0, cus = 0;
-    MK_HIP(hipGetDevice(&dev));
-    MK_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-    const uint32_t n = cus > 0 ? uint32_t(cus) : 1;
+    uint32_t n = 0;
+    MK_TRY(compute_units(n));
     switch (epi_class(p.epi)) {
     case EC_STORE: return launch<EC_STORE>(p, n, s);
     case EC_ACT: return launch<EC_ACT>(p, n, s);
