@@ -139,6 +139,21 @@ __device__ inline f32x4 vec4(const float* p, int64_t at, float none)
     return p ? *reinterpret_cast<const f32x4*>(p + at) : f32x4{none, none, none, none};
 }
 
+// The thread's NV float4s of a vector (`none` without one, zeros past its end)
+template <int W, int NV>
+__device__ inline void load_vec(f32x4 (&o)[NV], const float* p, int64_t at, uint32_t c0, uint32_t nv, float none)
+{
+    if (p) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            o[i] = c0 + 64 * W * i < nv ? *reinterpret_cast<const f32x4*>(p + at + 4 * (c0 + 64 * W * i)) : f32x4{0, 0, 0, 0};
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            o[i] = f32x4{none, none, none, none};
+    }
+}
+
 // A row's norm in registers: each thread holds NV float4s, c = first + 64 W i of the row's nv (zeros past its end).
 template <int W, int NV>
 __device__ inline void norm_row(f32x4 (&v)[NV], uint32_t c0, uint32_t nv, uint32_t n, uint32_t kind, const float* w,
@@ -176,7 +191,13 @@ __device__ inline void norm_row(f32x4 (&v)[NV], uint32_t c0, uint32_t nv, uint32
     }
 }
 
-// W waves a row (W = 1: four rows a workgroup), NV float4s a thread.
+// mk_gate_norm, one pass: the row of x and y in registers (W waves a row, NV float4s a thread; W = 1: four rows a workgroup),
+// the statistics two-pass over them (the mean first, then the squares about it: a variance far below the mean's square keeps
+// its digits). Bound by HBM: 8 bytes of residual, 2 of y and 2 (int8: 1) of out an element. Measured with three sets of
+// buffers in turn: 4352 x 4096 38.3 us (5.6 TB/s), 32768 x 4096 296 us (5.4), 32768 x 1280 88 us (5.7), to int8 4352 x
+// 4096 38.2 us; a copy runs at 5.0. The residual's nontemporal loads and stores are worth 47 -> 38 us of the first; y is the
+// last product's output and out the next one's input, which the caches may hold. Loading the vectors (w, scale, shift) with
+// the row costs the registers of half the waves: 47 -> 53 us.
 template <int W, int NV>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gate_norm_args g)
 {
@@ -189,9 +210,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gat
     const uint32_t seg = r / g.seg_rows, at = r - seg * g.seg_rows;
     const int64_t mod = int64_t(seg) * g.mod_stride + (at < g.split ? g.alt : 0);
     const float* x = g.x + uint64_t(r) * g.ldx;
-    f32x4 v[NV];
-    if (g.y) {
-        f32x4 xv[NV], gt[NV];
+    f32x4 v[NV], xv[NV], gt[NV];
+    if (g.y)
         with_type(g.y_dtype, [&](auto t) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -199,12 +219,15 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gat
                 v[i] = c < nv ? load4<decltype(t)::value>(g.y, uint64_t(r) * g.ldy + 4 * c) : f32x4{0, 0, 0, 0};
             }
         });
+    // the residual is not used again before the next block's end: its loads and stores pass the caches by
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = c0 + 64 * W * i;
-            xv[i] = c < nv ? *reinterpret_cast<const f32x4*>(x + 4 * c) : f32x4{0, 0, 0, 0};
-            gt[i] = c < nv ? vec4(g.gate, mod + 4 * c, 1.0f) : f32x4{0, 0, 0, 0};
-        }
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t c = c0 + 64 * W * i;
+        xv[i] = c < nv ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(x + 4 * c)) : f32x4{0, 0, 0, 0};
+    }
+    if (g.y)
+        load_vec<W, NV>(gt, g.gate, mod, c0, nv, 1.0f);
+    if (g.y) {
         norm_row<W, NV>(v, c0, nv, g.n, g.norm1, g.w1, g.b1, g.eps1, red, 0);
         if (g.gate && g.tanh_gate)
 #pragma unroll
@@ -219,30 +242,25 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gat
             for (int e = 0; e < 4; ++e)
                 v[i][e] = fmaf(gt[i][e], v[i][e], g.residual_scale * xv[i][e]);
             if (g.x_out && c < nv)
-                *reinterpret_cast<f32x4*>(g.x_out + uint64_t(r) * g.ldx + 4 * c) = v[i];
+                __builtin_nontemporal_store(v[i], reinterpret_cast<f32x4*>(g.x_out + uint64_t(r) * g.ldx + 4 * c));
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = c0 + 64 * W * i;
-            v[i] = c < nv ? *reinterpret_cast<const f32x4*>(x + 4 * c) : f32x4{0, 0, 0, 0};
-        }
+        for (int i = 0; i < NV; ++i)
+            v[i] = xv[i];
     }
     if (!g.out)
         return;
-    f32x4 sc[NV], sh[NV];
+    norm_row<W, NV>(v, c0, nv, g.n, g.norm2, g.w2, g.b2, g.eps2, red, 2);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const uint32_t c = c0 + 64 * W * i;
-        sc[i] = c < nv ? vec4(g.scale, mod + 4 * c, 0.0f) : f32x4{0, 0, 0, 0};
-        sh[i] = c < nv ? vec4(g.shift, mod + 4 * c, 0.0f) : f32x4{0, 0, 0, 0};
-    }
-    norm_row<W, NV>(v, c0, nv, g.n, g.norm2, g.w2, g.b2, g.eps2, red, 2);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+        const f32x4 s = c < nv ? vec4(g.scale, mod + 4 * c, 0.0f) : f32x4{0, 0, 0, 0};
+        const f32x4 h = c < nv ? vec4(g.shift, mod + 4 * c, 0.0f) : f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            v[i][e] = fmaf(v[i][e], 1.0f + sc[i][e], sh[i][e]);
+            v[i][e] = fmaf(v[i][e], 1.0f + s[e], h[e]);
+    }
     if (g.out_dtype == MK_I8) {
         uint32_t m = 0;
 #pragma unroll
@@ -278,11 +296,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gat
     });
 }
 
-// The kernel of W waves a row with the fewest float4s a thread that hold it
 template <int W, int NV = 1> void launch_gate_norm(const mk_gate_norm_args& g, hipStream_t s)
 {
-    constexpr int kMost = W == 16 ? 4 : W == 4 ? 16 : 4;
-    if constexpr (NV < kMost) {
+    if constexpr (NV < 4) {
         if (g.n > uint32_t(NV) * 256 * W)
             return launch_gate_norm<W, NV + 1>(g, s);
     }
@@ -383,6 +399,24 @@ void quantize_rows(const void* src, uint32_t rows, uint64_t cols, int64_t ld, in
         launch_quantize<T, 4>(src, rows, uint32_t(cols), ld, dst, scale, s);
 }
 
+void launch_rows(const mk_gate_norm_args& g, hipStream_t s)
+{
+    // the fewest waves that hold the row in 4 float4s a thread: more of them wait at barriers (32768 x 1280, 2 / 4 / 8 waves: 95 /
+    // 108 / 155 us); in 2 float4s where few rows leave compute units idle (1 x 4096, 4 / 8 waves: 5.1 / 3.9 us, 300 x 4096 7.2 /
+    // 6.3, 600 x 4096 10.2 / 9.5, 4352 x 4096 47.1 / 46.9)
+    const uint32_t waves = cdiv(g.n, g.rows <= 512 ? 512 : 1024);
+    if (waves <= 1)
+        launch_gate_norm<1>(g, s);
+    else if (waves <= 2)
+        launch_gate_norm<2>(g, s);
+    else if (waves <= 4)
+        launch_gate_norm<4>(g, s);
+    else if (waves <= 8)
+        launch_gate_norm<8>(g, s);
+    else
+        launch_gate_norm<16>(g, s);
+}
+
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool float_type(uint32_t t) { return t == MK_F32 || t == MK_BF16 || t == MK_F16; }
 
@@ -435,10 +469,7 @@ mk_status mk_gate_norm(const mk_gate_norm_args* a, void* stream)
     if (g.residual_scale == 0.0f)
         g.residual_scale = 1.0f;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (g.n <= 1024)
-        launch_gate_norm<1>(g, s);
-    else
-        launch_gate_norm<4>(g, s);
+    launch_rows(g, s);
     MK_LAUNCH_CHECK("gate_norm");
     return MK_OK;
 }
