@@ -609,67 +609,77 @@ template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const 
 }
 
 // The kernel of a launch: the one with the least estimated time in us, beside a launch's own. A tile takes its k steps of
-// 128 at the rate its CU brings operands in (64 x 32: 0.09, 64 x 64: 0.14, 128 x 128: 0.36 a step) or, where all CUs load, at the
-// 22.4 TB/s that they take from the L2s together; 256 x 256 tiles are bound by the matrix cores (1.54 a step, 7.7 for the
-// epilogue that nothing overlaps). Fitted to the four kernels' times at 198 shapes (rows 1 .. 4096, N and K 256 .. 12288); the choice is
-// within 0.3% of the best of the four in the mean, 13% at worst (16 x 4096 x 12288: 13.3 us against 11.8). Measured, us, few /
-// 64 x 32 / 64 x 64 / mixed: 1 x 4096 x 4096 4.5 / 6.1 / 7.6 / 14.1, 1 x 12288 x 4096 14.0 / 10.6 / 9.7 / 14.2, 77 x 2560 x 2048
-// - / 4.4 / 5.0 / 9.0, 300 x 4096 x 12288 - / 38.0 / 35.2 / 36.4, 1024 x 4096 x 4096 - / 35.8 / 26.9 / 19.1.
-enum { K_FEW, K_64X32, K_64X64, K_MIXED };
+// 128 at the rate its CU brings operands in (64 x 32: 0.096, 64 x 64: 0.15, 64 x 128: 0.26, 128 x 128: 0.37 a step) or, where
+// all CUs load, at the 19 to 22 TB/s that they take from the L2s together; 256 x 256 tiles are bound by the matrix cores
+// (1.5 a step, 7.6 for the pipeline's start and the epilogue, which nothing overlaps; 1.2 where the round is not full and
+// the clock higher). Fitted to the kernels' times at 436 shapes (rows 1 .. 4096, N and K 256 .. 12288); the choice is within 0.2%
+// of the best in the mean, 13% at worst (16 x 4096 x 12288: 13.3 us against 11.8). Measured, us, few / 64 x 32 / 64 x 64 /
+// 64 x 128 / mixed: 1 x 4096 x 4096 4.5 / 6.1 / 7.6 / 11 / 14, 1 x 12288 x 4096 14 / 10.6 / 9.7 / 11 / 14, 77 x 2560 x 2048 - / 4.4 /
+// 5.0 / 7.4 / 9.0, 300 x 4096 x 12288 - / 38 / 35 / 29 / 36, 1024 x 4096 x 4096 - / 36 / 27 / 24 / 19.
+// The mixed kernel's last, partial round takes quarter tiles up to two rounds of them (4352 x 4096 x 12288, 16 tiles left: 207 us
+// against 259; 4352 x 5120 x 4096, 84 left: 91 and 95; 1024 x 8192 x 4096, 128: 40 and 44), then whole ones (1024 x 9216 x 4096,
+// 144: 54 and 44; 4352 x 7168 x 4096, 220: 131 and 112).
+struct Plan {
+    int kernel;
+    uint32_t tiles_m, tiles_n, whole, grid; // of the mixed kernel
+};
+enum { K_FEW, K_64X32, K_64X64, K_64X128, K_MIXED };
 
-int kernel_of(const I8P& p, bool glu, uint32_t cus)
+Plan plan_of(const I8P& p, bool glu, uint32_t cus)
 {
     const double steps = double(cdiv(p.K, 128));
     auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t(cdiv(p.M, bm)) * cdiv(p.N, bn) * p.batch; };
     auto rounds = [&](uint64_t n) { return double((n + cus - 1) / cus); };
-    auto small = [&](uint32_t bm, uint32_t bn, double step, double end) {
-        const uint64_t n = tiles(bm, bn);
-        return std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / 22.4e6 * 256 / cus);
-    };
-    double best = 1e30;
-    int kernel = K_MIXED;
+    Plan best{K_MIXED, 0, 0, 0, 0};
+    double least = 1e30;
     auto consider = [&](int k, double t) {
-        if (t < best) {
-            best = t;
-            kernel = k;
+        if (t < least) {
+            least = t;
+            best.kernel = k;
         }
     };
+    auto small = [&](int k, uint32_t bm, uint32_t bn, double step, double end, double tbs) {
+        const uint64_t n = tiles(bm, bn);
+        consider(k, std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / (tbs * 1e6) * 256 / cus));
+    };
     if (p.M <= 16)
-        consider(K_FEW, std::max(rounds(tiles(16, 16)) * p.K * 3.4e-4, double(p.N) * p.K * p.batch * 0.174e-6) + 0.3);
+        consider(K_FEW, std::max(rounds(tiles(16, 16)) * p.K * 3.5e-4, double(p.N) * p.K * p.batch * 0.172e-6) + 0.3);
     if (!glu) // (its two parts are 16 channels of a wave each)
-        consider(K_64X32, small(64, 32, 0.0891, 0.734));
-    consider(K_64X64, small(64, 64, 0.144, 0.692));
-    const uint64_t big = tiles(256, 256), whole = big / cus;
-    const double quarter = steps * 0.359 + 1.25;
-    consider(K_MIXED, whole ? double(whole) * (steps * 1.54 + 7.7) + rounds((big - whole * cus) * 4) * quarter
-                            : rounds(tiles(128, 128)) * quarter);
-    return kernel;
+        small(K_64X32, 64, 32, 0.0957, 0.762, 22.5);
+    small(K_64X64, 64, 64, 0.15, 0.682, 21.4);
+    small(K_64X128, 64, 128, 0.259, 1.43, 19.0);
+    const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = whole ? (big - whole) * 4 : tiles(128, 128);
+    const bool quarters = rest <= 2 * uint64_t(cus);
+    consider(K_MIXED, double(whole / cus) * (steps * 1.5 + 7.6) +
+                          (quarters ? rounds(rest) * (steps * 0.372 + 1.32) : steps * 1.2 + 7.6));
+    const bool all_quarters = quarters && !whole;
+    const uint64_t w = quarters ? whole : big, g = quarters ? whole + rest : big;
+    best.tiles_m = cdiv(p.M, all_quarters ? 128 : 256);
+    best.tiles_n = cdiv(p.N, all_quarters ? 128 : 256);
+    best.whole = uint32_t(std::min<uint64_t>(w, 0x7fffffffu));
+    best.grid = g <= 0x7fffffffu ? uint32_t(g) : 0;
+    return best;
 }
 
 template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
 {
-    switch (kernel_of(p, EC == EC_GLU, cus)) {
+    const Plan plan = plan_of(p, EC == EC_GLU, cus);
+    switch (plan.kernel) {
     case K_FEW:
         gemm_i8_few_kernel<EC><<<dim3(cdiv(EC == EC_GLU ? p.N / 2 : p.N, 16), p.batch), 64 * kFewWaves, 0, s>>>(p);
         break;
     case K_64X32:
         if constexpr (EC != EC_GLU)
             return launch_tile<64, 32, 4, 6, EC>(p, s);
+        return fail(MK_ERR_UNSUPPORTED, "gemm_i8: no gated 64 x 32 tiles");
     case K_64X64:
         return launch_tile<64, 64, 4, 4, EC>(p, s);
-    default: {
-        uint32_t tm = cdiv(p.M, 256), tn = cdiv(p.N, 256);
-        const uint64_t tiles = uint64_t(tm) * tn * p.batch, whole = tiles / cus * cus;
-        uint64_t grid = whole + (tiles - whole) * 4;
-        if (!whole) {
-            tm = cdiv(p.M, 128);
-            tn = cdiv(p.N, 128);
-            grid = uint64_t(tm) * tn * p.batch;
-        }
-        if (grid > 0x7fffffffu)
+    case K_64X128:
+        return launch_tile<64, 128, 4, 4, EC>(p, s);
+    default:
+        if (!plan.grid)
             return fail(MK_ERR_ARG, "gemm_i8: too many tiles");
-        gemm_i8_mixed_kernel<EC><<<uint32_t(grid), 512, 0, s>>>(p, tm, tn, uint32_t(whole));
-    }
+        gemm_i8_mixed_kernel<EC><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole);
     }
     MK_LAUNCH_CHECK("gemm_i8");
     return MK_OK;
