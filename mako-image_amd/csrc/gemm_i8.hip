@@ -1,4 +1,11 @@
-// proj in 8-bit integers: C = epilogue(ascale[r] wscale[n] sum_k A[r][k] W[n][k] + bias[n]), int32 sums.
+// proj in 8-bit integers on gfx950: C = epilogue(ascale[r] wscale[n] sum_k A[r][k] W[n][k] + bias[n]), the sums exact in
+// int32 (v_mfma_i32_16x16x64_i8), so their order, and with it the kernel that a launch takes, does not show in a result.
+//
+// What bounds it: up to 16 rows the weight's bytes (1 x 12288 x 4096: 9.7 us, 5.2 TB/s with a launch's own time); tens to
+// hundreds of rows what a CU takes from its L2 (80 to 110 bytes a ns); from about 1000 rows the matrix cores at the clock that the
+// power limit leaves: 8192^3 at 2.6 POP/s with them 68% busy at 1.87 GHz, 32768 x 12288 x 4096 2.4 POP/s with 60% at 1.4 to 1.6 GHz
+// (rocprofv3 counters; no LDS bank conflicts). There neither the waves' priority nor fragments read further ahead
+// changed the time, within 0.5%.
 #include "common.hpp"
 
 #include <algorithm>
@@ -223,7 +230,9 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
     };
     // A substep: the weight fragments are single-buffered, each next one read into its registers right after the last
     // product that uses it; the next token fragments go to the other buffer with the first channel block; the direct loads
-    // of step gkt (into stage gbuf) follow one product each. Every instruction is fenced: the order is this one.
+    // of step gkt (into stage gbuf) follow every second product (0.8% faster than every one). Every instruction is fenced:
+    // the order is this one.
+    static_assert(WIDE || ND <= CB * TB / 2, "a load after every second product");
     auto substep = [&](const i32x4(&af)[TB], int nbuf, int nks, i32x4(&naf)[TB], int gkt, int gbuf,
                        bool load) __attribute__((always_inline)) {
         const uint32_t gp = past(gkt);
@@ -240,15 +249,11 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
                 rdw(nbuf, nks, cb);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (load && i < ND) {
-                dma1(gkt, gp, gbuf, i);
+            if (load && i % 2 && i / 2 < ND) {
+                dma1(gkt, gp, gbuf, i / 2);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (load)
-#pragma unroll
-            for (int i = CB * TB; i < ND; ++i)
-                dma1(gkt, gp, gbuf, i);
     };
 
     // k steps 0 .. NSTG - 1 on their way; past-the-end steps reload the last one (nobody reads them)
