@@ -503,7 +503,11 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 
 // ------------------------------------------------------------------------------------------------------------
 // Up to 16 rows: a workgroup makes 16 channels of all rows, its 8 waves every eighth 256 bytes of k each, straight from
-// memory to registers; nothing of the weight is read twice. The sums meet in LDS.
+// memory to registers (the rows of a product's operand lie in 64-byte pieces of 16 rows a load: about 40 bytes a ns and CU,
+// enough where every CU has a workgroup or two); nothing of the weight is read twice. The sums meet in LDS. Bound by the
+// weight's bytes: 1 x 4096 x 4096 5.0 us, 1 x 4096 x 12288 9.9 us, a launch alone 3. 4 or 16 waves, 128 or 512 bytes a
+// turn: within 15%. Two or four of these rows' blocks (17 to 64 rows) are slower than 64 x 32 tiles (32 x 4096 x 4096 7.9 and
+// 6.3 us).
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kFewWaves = 8;
 
@@ -529,12 +533,12 @@ template <int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_
     auto load = [&](uint32_t k, Unit& f) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            // chunks past K: out of range, zeros
+            // chunks past K: out of range, zeros (k itself stays in a scalar register)
             const bool in = k + s * 64 + g4 * 16 < p.K;
 #pragma unroll
             for (int c = 0; c < CB; ++c)
-                f.w[s][c] = __builtin_bit_cast(i32x4, buf_load16(rsW[c], in ? ow + s * 64 : 0xfffffff0u, in ? k : 0));
-            f.a[s] = __builtin_bit_cast(i32x4, buf_load16(rsA, in ? oa + s * 64 : 0xfffffff0u, in ? k : 0));
+                f.w[s][c] = __builtin_bit_cast(i32x4, buf_load16(rsW[c], in ? ow + s * 64 : 0x80000000u, k));
+            f.a[s] = __builtin_bit_cast(i32x4, buf_load16(rsA, in ? oa + s * 64 : 0x80000000u, k));
         }
     };
     auto mul = [&](const Unit& f) {
@@ -605,10 +609,7 @@ template <int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_
 template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const I8P& p, hipStream_t s)
 {
     const uint32_t cols = EC == EC_GLU ? p.N / 2 : p.N, tm = cdiv(p.M, BM), tn = cdiv(cols, EC == EC_GLU ? BN / 2 : BN);
-    const uint64_t tiles = uint64_t(tm) * tn * p.batch;
-    if (tiles > 0x7fffffffu)
-        return fail(MK_ERR_ARG, "gemm_i8: too many tiles");
-    gemm_i8_kernel<BM, BN, NW, NSTG, EC><<<uint32_t(tiles), 64 * NW, 0, s>>>(p, tm, tn);
+    gemm_i8_kernel<BM, BN, NW, NSTG, EC><<<tm * tn * p.batch, 64 * NW, 0, s>>>(p, tm, tn);
     MK_LAUNCH_CHECK("gemm_i8");
     return MK_OK;
 }
@@ -628,41 +629,45 @@ struct Plan {
     int kernel;
     uint32_t tiles_m, tiles_n, whole, grid; // of the mixed kernel
 };
-enum { K_FEW, K_64X32, K_64X64, K_64X128, K_MIXED };
+enum { K_NONE = -1, K_FEW, K_64X32, K_64X64, K_64X128, K_MIXED };
 
 Plan plan_of(const I8P& p, bool glu, uint32_t cus)
 {
     const double steps = double(cdiv(p.K, 128));
     auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t(cdiv(p.M, bm)) * cdiv(p.N, bn) * p.batch; };
     auto rounds = [&](uint64_t n) { return double((n + cus - 1) / cus); };
-    Plan best{K_MIXED, 0, 0, 0, 0};
+    Plan best{K_NONE, 0, 0, 0, 0};
     double least = 1e30;
-    auto consider = [&](int k, double t) {
-        if (t < least) {
+    // a grid dimension holds fewer than 2^32 threads
+    auto consider = [&](int k, double t, uint64_t threads) {
+        if (t < least && threads < (uint64_t(1) << 32)) {
             least = t;
             best.kernel = k;
         }
     };
     auto small = [&](int k, uint32_t bm, uint32_t bn, double step, double end, double tbs) {
         const uint64_t n = tiles(bm, bn);
-        consider(k, std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / (tbs * 1e6) * 256 / cus));
+        consider(k, std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / (tbs * 1e6) * 256 / cus),
+                 n * 256);
     };
     if (p.M <= 16)
-        consider(K_FEW, std::max(rounds(tiles(16, 16)) * p.K * 3.5e-4, double(p.N) * p.K * p.batch * 0.172e-6) + 0.3);
+        consider(K_FEW, std::max(rounds(tiles(16, 16)) * p.K * 3.5e-4, double(p.N) * p.K * p.batch * 0.172e-6) + 0.3,
+                 uint64_t(cdiv(p.N, 16)) * 512);
     if (!glu) // (its two parts are 16 channels of a wave each)
         small(K_64X32, 64, 32, 0.0957, 0.762, 22.5);
     small(K_64X64, 64, 64, 0.15, 0.682, 21.4);
     small(K_64X128, 64, 128, 0.259, 1.43, 19.0);
     const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = whole ? (big - whole) * 4 : tiles(128, 128);
     const bool quarters = rest <= 2 * uint64_t(cus);
-    consider(K_MIXED, double(whole / cus) * (steps * 1.5 + 7.6) +
-                          (quarters ? rounds(rest) * (steps * 0.372 + 1.32) : steps * 1.2 + 7.6));
-    const bool all_quarters = quarters && !whole;
-    const uint64_t w = quarters ? whole : big, g = quarters ? whole + rest : big;
-    best.tiles_m = cdiv(p.M, all_quarters ? 128 : 256);
-    best.tiles_n = cdiv(p.N, all_quarters ? 128 : 256);
-    best.whole = uint32_t(std::min<uint64_t>(w, 0x7fffffffu));
-    best.grid = g <= 0x7fffffffu ? uint32_t(g) : 0;
+    const uint64_t groups = quarters ? whole + rest : big;
+    consider(K_MIXED,
+             double(whole / cus) * (steps * 1.5 + 7.6) + (quarters ? rounds(rest) * (steps * 0.372 + 1.32) : steps * 1.2 + 7.6),
+             groups * 512);
+    const uint32_t side = quarters && !whole ? 128 : 256;
+    best.tiles_m = cdiv(p.M, side);
+    best.tiles_n = cdiv(p.N, side);
+    best.whole = uint32_t(quarters ? whole : big);
+    best.grid = uint32_t(groups);
     return best;
 }
 
@@ -681,9 +686,9 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
         return launch_tile<64, 64, 4, 4, EC>(p, s);
     case K_64X128:
         return launch_tile<64, 128, 4, 4, EC>(p, s);
+    case K_NONE:
+        return fail(MK_ERR_ARG, "gemm_i8: a launch of more than 2^32 threads");
     default:
-        if (!plan.grid)
-            return fail(MK_ERR_ARG, "gemm_i8: too many tiles");
         gemm_i8_mixed_kernel<EC><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole);
     }
     MK_LAUNCH_CHECK("gemm_i8");
@@ -750,8 +755,8 @@ extern "C" mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void
                                 "multiple of 4");
     if (!a->M || !a->batch)
         return MK_OK;
-    if (a->M > 0x7fffff00u || a->batch > 65535)
-        return fail(MK_ERR_ARG, "gemm_i8: more than 2^31 - 256 rows or 65535 batch items");
+    if (a->M > 0x7fffff00u || a->N > 0x7fffff00u || a->batch > 65535)
+        return fail(MK_ERR_ARG, "gemm_i8: more than 2^31 - 256 rows or channels or 65535 batch items");
     const I8P p{static_cast<const int8_t*>(a->a),
                 static_cast<const int8_t*>(a->w),
                 ascale,

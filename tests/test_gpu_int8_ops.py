@@ -9,6 +9,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
+from scipy.special import erf
 
 import mkimage as M
 
@@ -76,7 +77,8 @@ def quantize(bits, dt, rows, cols, ld, stream=None, offset=0):
 @pytest.mark.parametrize("dt", [M.F32, M.BF16, M.F16])
 @pytest.mark.parametrize("rows, cols, pad, offset", [
     (1, 1, 0, 0), (1, 16, 0, 0), (3, 5, 2, 0), (2, 64, 0, 0), (7, 1000, 0, 0), (5, 4096, 0, 0), (300, 272, 16, 0),
-    (4, 12288, 0, 0), (3, 16400, 0, 0), (2, 40000, 0, 0), (2, 33333, 3, 0), (9, 256, 0, 1), (2, 1024, 8, 4), (1100, 80, 0, 0)])
+    (4, 12288, 0, 0), (3, 16400, 0, 0), (5, 1536, 0, 0), (3, 1552, 16, 0), (3, 3056, 0, 0),
+    (2, 8192, 0, 0), (2, 24576, 0, 0), (1, 65536, 0, 0), (1, 65552, 0, 0), (2, 40000, 0, 0), (2, 33333, 3, 0), (9, 256, 0, 1), (2, 1024, 8, 4), (1100, 80, 0, 0)])
 def test_quantize_rows_equal_the_definition(gpu, dt, rows, cols, pad, offset):
     rng = np.random.default_rng(rows * 7 + cols)
     x = rng.standard_normal((rows, cols + pad)) * np.exp(rng.standard_normal((rows, 1)) * 3)
@@ -180,10 +182,8 @@ class Product:
             if self.epi == M.EPI_SWIGLU:
                 s = a / (1 + np.exp(-a))
                 return s * b, np.abs(b) * (1.1 * ea + np.abs(s) * (8 + 4 * np.abs(a)) * u) + np.abs(s) * eb + 4 * u * np.abs(s * b)
-            from math import erf
-            er = np.vectorize(erf)(b * np.sqrt(0.5))
-            g = 0.5 * b * (1 + er)
-            # the erf fit is within 1.2e-7 and a few roundings of its exp's argument (z^2 + 1.27 below 15 where it counts)
+            g = 0.5 * b * (1 + erf(b * np.sqrt(0.5)))
+            # the erf series is within 1.5e-7, its five terms, exp2 and rcp add a few roundings of values below 1
             return a * g, np.abs(g) * ea + np.abs(a) * (1.13 * eb + 0.5 * np.abs(b) * (2e-7 + 32 * u)) + 4 * u * np.abs(a * g)
         if self.rmw:
             row = np.arange(self.m) % (self.seg or 1 << 32)
@@ -281,7 +281,9 @@ def test_product_batches_and_strides(gpu, m, n, k):
     Product(m, 2 * n, k, epi=M.EPI_SWIGLU, batch=2, lda=k + 16, ldc=n + 20, c=M.F16, bias=False).check()
 
 
-@pytest.mark.parametrize("m, n", [(4400, 1028), (2048, 2304), (1537, 4100)])
+# (on 256 compute units: 128 x 128 tiles in one and two rounds; 256 x 256 ones in a partial round, in a whole round and a few
+# quarters of tiles, in a whole round and a partial one)
+@pytest.mark.parametrize("m, n", [(4400, 1028), (2048, 2304), (1537, 4100), (4400, 2304), (4400, 4100), (4400, 6000)])
 @pytest.mark.parametrize("epi, c", [(M.EPI_STORE, M.BF16), (M.EPI_GEGLU, M.F16), (M.EPI_GATE_TANH, M.F32)])
 def test_product_many_tiles(gpu, m, n, epi, c):
     n -= n % 8 if epi == M.EPI_GEGLU else 0
@@ -507,6 +509,12 @@ WIDTHS = [4, 8, 64, 252, 256, 260, 516, 1024, 1280, 2048, 4096, 4100, 5120, 8192
 def test_gate_norm_widths(gpu, n, rows):
     GateNorm(rows, n).check()
     GateNorm(rows, n, out=M.I8, norm1=M.NORM_RMS, norm2=M.NORM_RMS, alpha=0.5).check()
+
+
+@pytest.mark.parametrize("n", [512, 1024, 1280, 2048, 4096, 6144, 8192, 16384])
+def test_gate_norm_many_rows(gpu, n):
+    # beyond 512 rows a row takes fewer waves
+    GateNorm(517, n, out=M.I8, norm1=M.NORM_RMS, split=20, seg=260, samples=2).check()
 
 
 @pytest.mark.parametrize("y", [M.F32, M.BF16, M.F16])
