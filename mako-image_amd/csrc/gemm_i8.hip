@@ -136,10 +136,16 @@ __device__ inline int swz(int row, int kc) { return row * 128 + (swz_chunk(row, 
 // s_waitcnt immediate: vmcnt vm, lgkmcnt 0 (vmcnt's bits 3:0 and 15:14, expcnt not waited for)
 constexpr int wait_vm(int vm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4); }
 
-template <int BM, int BN, int NW, int NSTG> constexpr int tile_lds()
+// Channels that a wave stages at a time in the epilogue, 16 tokens of them (64 at most, 4 KB; a gated unit writes half)
+constexpr int epi_channels(int bn, bool glu)
 {
-    constexpr int ops = NSTG * (BM + BN) * 128, epi = NW * 32 * (BN / 2 + 4) * 4;
-    return ops > epi ? ops : epi;
+    const int wo = glu ? bn / 4 : bn / 2;
+    return wo < 64 ? wo : 64;
+}
+// LDS bytes of a tile: the stages; behind them, for a chain of tiles, the epilogue's staging, which else reuses them.
+template <int BM, int BN, int NW, int NSTG, bool CHAIN> constexpr int tile_lds()
+{
+    return NSTG * (BM + BN) * 128 + (CHAIN ? NW * 16 * epi_channels(BN, false) * 4 : 0);
 }
 
 // f(std::integral_constant<int, 0>{}), f(1), ..
@@ -148,15 +154,16 @@ template <class F, int... I> __device__ __forceinline__ void for_each_int(F&& f,
     (f(std::integral_constant<int, I>{}), ...);
 }
 
-// One tile: tokens m0 .. m0 + BM of batch item z, output channels from n0.
-template <int BM, int BN, int NW, int NSTG, int EC>
-__device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0, int8_t* smem)
+// Tiles of BM tokens x BN channels, `count` of them one after the other: at(i, z, m0, n0) gives the i-th's batch item, first
+// token and first output channel. CHAIN: the last k steps of a tile load the first ones of the next, and the epilogue
+// stages in LDS of its own, so that a workgroup's next tile starts where the last one ends.
+template <int BM, int BN, int NW, int NSTG, int EC, bool CHAIN, class At>
+__device__ __forceinline__ void i8_tiles(const I8P& p, int8_t* smem, uint32_t count, At at)
 {
     constexpr bool GLU = EC == EC_GLU;
     constexpr int NT = 64 * NW, WM = BM / (NW / 2), WC = BN / 2, TB = WM / 16, CB = WC / 16;
     constexpr int RA = BM * 8 / NT, RW = BN * 8 / NT, ND = RA + RW; // direct loads a thread makes a k step
-    constexpr int LDW = WC + 4;
-    static_assert((NSTG - 2) * ND <= 63 && WM % 32 == 0, "");
+    static_assert((NSTG - 1) * ND <= 63 && (!CHAIN || NSTG == 2), "");
     int8_t(*sW)[BN * 128] = reinterpret_cast<int8_t(*)[BN * 128]>(smem);
     int8_t(*sA)[BM * 128] = reinterpret_cast<int8_t(*)[BM * 128]>(smem + NSTG * BN * 128);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -165,34 +172,46 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
     const int cols = int(GLU ? p.N / 2 : p.N);
     // GLU: the tile makes channels n0 .. n0 + BN / 2, a wave's rows are WC / 2 rows of the first part and the same
     // channels' rows of the second, so a lane's blocks cb and cb + CB / 2 are the two operands of one output.
-    const int nr = min(cols - n0, GLU ? BN / 2 : BN);
 
+    // The lane, as a value that the compiler does not know: what is derived from it is computed where it stands, not ahead of
+    // the k loop, whose registers are all taken.
+    auto here = [&]() __attribute__((always_inline)) {
+        int l = lane;
+        if (CHAIN)
+            asm volatile("" : "+v"(l));
+        return l;
+    };
     // Direct loads: wave w's round i fills LDS chunks (i NW + w) 64 + lane; chunk P holds row P / 8 and k chunk
     // swz_chunk(row, P % 8). Buffer loads: the resource spans the tile's rows, the lane's byte offset selects row and
-    // chunk, the k offset is a scalar; rows past the end read the last one. Chunks past K (in the last k step) read out of
+    // chunk, the k offset is a scalar; rows past the end read the last one. Chunks past K (in the last k steps) read out of
     // the resource's range, which gives zeros.
-    const int8_t* gA = p.a + int64_t(z) * p.sa + int64_t(m0) * p.lda;
-    const int8_t* gW = p.w + uint64_t(n0) * p.K;
-    const int mr = min(int(p.M) - m0, BM);
-    const BufRes rsA = buf_res(gA, uint32_t(int64_t(mr - 1) * p.lda + p.K));
-    const BufRes rsW0 = buf_res(gW, uint32_t(nr) * p.K);
-    const BufRes rsW1 = buf_res(GLU ? gW + uint64_t(cols) * p.K : gW, uint32_t(nr) * p.K);
-    const int kc = (lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7); // the lane's k chunk, the same in every round
     static_assert(NW % 2 == 0, "a round's rows are a multiple of 16");
-    uint32_t oa[RA], ow[RW];
+    const int kc = (lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7); // the lane's k chunk, the same in every round
+    uint32_t z, oa[RA], ow[RW];
+    int m0, n0;
+    BufRes rsA, rsW0, rsW1;
+    auto set = [&](uint32_t tile) __attribute__((always_inline)) {
+        at(tile, z, m0, n0);
+        const int lane = here();
+        const int nr = min(cols - n0, GLU ? BN / 2 : BN), mr = min(int(p.M) - m0, BM);
+        const int8_t* gW = p.w + uint64_t(n0) * p.K;
+        rsA = buf_res(p.a + int64_t(z) * p.sa + int64_t(m0) * p.lda, uint32_t(int64_t(mr - 1) * p.lda + p.K));
+        rsW0 = buf_res(gW, uint32_t(nr) * p.K);
+        rsW1 = buf_res(GLU ? gW + uint64_t(cols) * p.K : gW, uint32_t(nr) * p.K);
 #pragma unroll
-    for (int i = 0; i < RA; ++i) {
-        const int row = (i * NW + wave) * 8 + (lane >> 3);
-        oa[i] = uint32_t(min(row, mr - 1)) * uint32_t(p.lda) + kc * 16;
-    }
+        for (int i = 0; i < RA; ++i) {
+            const int row = (i * NW + wave) * 8 + (lane >> 3);
+            oa[i] = uint32_t(min(row, mr - 1)) * uint32_t(p.lda) + kc * 16;
+        }
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        const int r = (i * NW + wave) * 8 + (lane >> 3);
-        ow[i] = uint32_t(min(GLU ? (r / WC) * (WC / 2) + r % (WC / 2) : r, nr - 1)) * p.K + kc * 16;
-    }
-    // direct load i (activation rounds first) of k step kt into stage buf; past: what leaves the range in the last, partial
-    // step for the lanes whose chunk lies past K
-    auto dma1 = [&](int kt, uint32_t past, int buf, int i) {
+        for (int i = 0; i < RW; ++i) {
+            const int r = (i * NW + wave) * 8 + (lane >> 3);
+            ow[i] = uint32_t(min(GLU ? (r / WC) * (WC / 2) + r % (WC / 2) : r, nr - 1)) * p.K + kc * 16;
+        }
+    };
+    // direct load i (activation rounds first) of k step kt into stage buf; past: what leaves the range for the lanes whose
+    // chunk lies past K
+    auto dma1 = [&](int kt, uint32_t past, int buf, int i) __attribute__((always_inline)) {
         if (i < RA)
             buf_load_lds16(rsA, (lds_void*)&sA[buf][(i * NW + wave) * 1024], oa[i] + past, uint32_t(kt) * 128);
         else {
@@ -201,17 +220,11 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
                            uint32_t(kt) * 128);
         }
     };
-    const int ke = int((p.K + 127) / 128), kfull = int(p.K / 128);
-    const uint32_t tail = kc * 16 >= int(p.K) - kfull * 128 ? 0x80000000u : 0u;
-    auto past = [&](int kt) { return kt < kfull ? 0u : tail; };
+    // (a chain takes an even number of steps, so that every tile starts in stage 0: one of zeros where K has an odd one)
+    const int kn = int((p.K + 127) / 128), ke = CHAIN ? (kn + 1) & ~1 : kn;
+    auto past = [&](int kt) { return kc * 16 >= int(p.K) - kt * 128 ? 0x80000000u : 0u; };
 
     i32x4 acc[CB][TB];
-#pragma unroll
-    for (int i = 0; i < CB; ++i)
-#pragma unroll
-        for (int j = 0; j < TB; ++j)
-            acc[i][j] = i32x4{0, 0, 0, 0};
-
     // lane (r16, g4) supplies row r16 of a 16-row block and k bytes 16 g4 .. + 15 of a 64-deep substep, and holds channels
     // 4 g4 .. + 3 of token r16
     const int r16 = lane & 15, g4 = lane >> 4;
@@ -256,37 +269,16 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
         }
     };
 
-    // k steps 0 .. NSTG - 1 on their way; past-the-end steps reload the last one (nobody reads them)
-#pragma unroll
-    for (int s = 0; s < NSTG; ++s) {
-        const int kt = min(s, ke - 1);
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-            dma1(kt, past(kt), s, i);
-    }
-    __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 1) * ND > 63 ? 63 : (NSTG - 1) * ND));
-    __builtin_amdgcn_s_barrier();
     // fragment j of a step in the order of use: substep j / (CB + TB)
     auto frag = [&](int buf, int j, i32x4(&f)[2][WIDE ? CB + TB : 1]) {
         const int ks = j / (CB + TB), i = j % (CB + TB);
         f[ks][i] = *reinterpret_cast<const i32x4*>(i < CB ? &sW[buf][fw[ks] + i * 2048] : &sA[buf][fa[ks] + (i - CB) * 2048]);
     };
-    if constexpr (WIDE) {
-#pragma unroll
-        for (int j = 0; j < 2 * (CB + TB); ++j)
-            frag(0, j, fr[0]);
-    } else {
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-            rdw(0, 0, cb);
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-            rda(0, 0, tb, af0);
-    }
     // k step kt in stage `buf` (a constant: the loop is unrolled by NSTG): the first substep reads the second's fragments;
     // then step kt + 1 has landed (later ones may be in flight) and, after the barrier, in every wave, and every wave has
-    // read this stage, so the second substep loads step kt + NSTG into it and reads step kt + 1's first fragments
-    auto step = [&](int kt, auto buf_c) __attribute__((always_inline)) {
+    // read this stage, so the second substep loads into it and reads step kt + 1's first fragments. The loads are those of step kt + NSTG
+    // of that tile, from k step kl.
+    auto step = [&](int kl, auto buf_c) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value, nb = (buf + 1) % NSTG;
         if constexpr (WIDE) {
             // this step's fragments are in registers (read before the barrier), step kt + 1 has landed: its fragments
@@ -294,7 +286,6 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
             constexpr int NM = 2 * CB * TB, NF = 2 * (CB + TB), RPM = (2 * NF + NM - 1) / NM, LPM = (2 * ND + NM - 1) / NM;
             __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
             __builtin_amdgcn_s_barrier();
-            const int kl = min(kt + NSTG, ke - 1);
             const uint32_t gp = past(kl);
 #pragma unroll
             for (int i = 0; i < NM; ++i) {
@@ -318,122 +309,199 @@ __device__ __forceinline__ void i8_tile(const I8P& p, uint32_t z, int m0, int n0
         substep(af0, buf, 1, af1, 0, 0, false);
         __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
         __builtin_amdgcn_s_barrier();
-        substep(af1, nb, 0, af0, min(kt + NSTG, ke - 1), buf, true);
+        substep(af1, nb, 0, af0, kl, buf, true);
     };
-    int kt = 0;
-    for (; kt + NSTG - 1 < ke; kt += NSTG)
-        for_each_int([&](auto i) __attribute__((always_inline)) { step(kt + decltype(i)::value, i); }, std::make_integer_sequence<int, NSTG>{});
-    for_each_int(
-        [&](auto i) __attribute__((always_inline)) {
-            if (kt + decltype(i)::value < ke)
-                step(kt + decltype(i)::value, i);
-        },
-        std::make_integer_sequence<int, NSTG - 1>{});
-    __builtin_amdgcn_s_waitcnt(0); // the last loads land before the LDS is reused
-    __syncthreads();
 
-    // Epilogue: a wave stages 32 tokens at a time (fp32, times their scales) in LDS of its own and reads them back with its
-    // lanes along the channels, so that its stores are whole row segments. A wave's LDS operations complete in order:
-    // no barrier.
-    float* st = reinterpret_cast<float*>(smem) + wave * 32 * LDW;
-    const float* as = p.ascale + uint64_t(z) * p.M;
-    const int t0 = m0 + wm * WM;
-    float sc[TB];
+    // Epilogue: a wave stages ST tokens x up to 64 channels at a time (fp32, times the tokens' scales) in LDS of its own and
+    // reads them back with its lanes along the channels, so that its stores are whole row segments. A wave's LDS operations
+    // complete in order: no barrier. Rows of SC floats, their 16-byte chunks XOR-ed so that 16 rows at a chunk cover all banks.
+    // (32 tokens keep more stores in flight; a chain has LDS for 16, the residual registers.)
+    constexpr int WO = GLU ? WC / 2 : WC, SC = epi_channels(BN, GLU), NH = WO / SC; // channels a wave writes, stages at a time
+    constexpr int ST = CHAIN || EC == EC_RMW ? 16 : 32, NCH = SC / 4, RPI = 64 / NCH, NI = ST / RPI; // chunks a row, rows an instruction, a lane
+    auto epilogue = [&](uint32_t ez, int em0, int en0) __attribute__((always_inline)) {
+        const int lane = here(), r16 = lane & 15, g4 = lane >> 4;
+        float* st = reinterpret_cast<float*>(smem + (CHAIN ? NSTG * (BM + BN) * 128 : 0)) + wave * ST * SC;
+        auto swap = [](int row) { return row / (64 / SC) % NCH; };
+        const float* as = p.ascale + uint64_t(ez) * p.M;
+        const int t0 = em0 + wm * WM, c0 = en0 + wn * WO;
+        float sc[TB];
 #pragma unroll
-    for (int tb = 0; tb < TB; ++tb)
-        sc[tb] = as[min(t0 + tb * 16 + r16, int(p.M) - 1)];
-    constexpr int WO = GLU ? WC / 2 : WC; // channels a wave writes
-    constexpr int LPR = WO / 4, RPI = 64 / LPR, NI = 32 / RPI; // lanes a row, rows an instruction, rows a lane
-    const int c0 = n0 + wn * WO;
-    auto stage = [&](int s) {
+        for (int tb = 0; tb < TB; ++tb)
+            sc[tb] = as[min(t0 + tb * 16 + r16, int(p.M) - 1)];
+        const int lc = lane % NCH, lr = lane / NCH;
+        Ch4 k[NH];
+        if constexpr (!GLU)
 #pragma unroll
-        for (int cb = 0; cb < WO / 16; ++cb)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int a = acc[cb][2 * s + h][e];
-                    v[e] = GLU ? __builtin_bit_cast(float, a) : float(a) * sc[2 * s + h];
-                }
-                *reinterpret_cast<f32x4*>(st + (16 * h + r16) * LDW + cb * 16 + 4 * g4) = v;
-            }
-    };
-    if constexpr (GLU) {
-        with_flag(p.epi == MK_EPI_SWIGLU, [&](auto swi) {
-#pragma unroll
-            for (int cb = 0; cb < CB / 2; ++cb) {
-                const int c = min(c0 + cb * 16 + 4 * g4, cols - 4);
-                const f32x4 s1 = *reinterpret_cast<const f32x4*>(p.wscale + c);
-                const f32x4 s2 = *reinterpret_cast<const f32x4*>(p.wscale + cols + c);
-                const f32x4 b1 = load4(p.bias, c, 0.0f), b2 = load4(p.bias, cols + c, 0.0f);
-#pragma unroll
-                for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float a = fmaf(float(acc[cb][tb][e]) * sc[tb], s1[e], b1[e]);
-                        const float g = fmaf(float(acc[cb + CB / 2][tb][e]) * sc[tb], s2[e], b2[e]);
-                        acc[cb][tb][e] = __builtin_bit_cast(int, glu1<decltype(swi)::value>(a, g));
-                    }
-            }
-        });
-    }
-    const int lc = lane % LPR, lr = lane / LPR, ch = c0 + 4 * lc;
-    const bool mine = ch < cols; // (cols is a multiple of 4)
-    Ch4 k{};
-    if (!GLU)
-        k = channels4(p, min(ch, cols - 4));
-#pragma unroll
-    for (int s = 0; s < WM / 32; ++s) {
-        stage(s);
-        const int tok = t0 + 32 * s + lr;
-        const int64_t at = int64_t(z) * p.sc + int64_t(tok) * p.ldc + ch, step = int64_t(RPI) * p.ldc;
-        f32x4 v[NI];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            v[i] = *reinterpret_cast<const f32x4*>(st + (lr + RPI * i) * LDW + 4 * lc);
-            if (!GLU)
-                v[i] = scaled(v[i], k.ws, k.b);
-        }
-        if constexpr (EC == EC_ACT)
-            with_flag(p.epi == MK_EPI_GELU_TANH, [&](auto gelu) {
-#pragma unroll
-                for (int i = 0; i < NI; ++i)
-                    v[i] = act4<decltype(gelu)::value>(v[i]);
-            });
-        // rows of the slice past M: the whole slices' stores have no guard between them
-        auto rows = [&](auto&& store) {
-            if (!mine)
+            for (int h = 0; h < NH; ++h)
+                k[h] = channels4(p, min(c0 + h * SC + 4 * lc, cols - 4)); // (cols is a multiple of 4)
+        // slice s: tokens ST (s / NH) .. + ST - 1, channels SC (s % NH) .. + SC - 1
+        constexpr int NSL = WM / ST * NH;
+        auto token = [&](int s, int i) { return t0 + s / NH * ST + lr + RPI * i; };
+        auto place = [&](int s) { return int64_t(ez) * p.sc + int64_t(token(s, 0)) * p.ldc + c0 + s % NH * SC + 4 * lc; };
+        const int64_t next = int64_t(RPI) * p.ldc;
+        // f(i) for the lane's rows of a slice that are C's; a whole slice has no guard between them
+        auto rows = [&](int s, auto&& f) __attribute__((always_inline)) {
+            if (c0 + s % NH * SC + 4 * lc >= cols)
                 return;
-            if (t0 + 32 * s + 32 <= int(p.M)) {
+            if (t0 + s / NH * ST + ST <= int(p.M)) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
-                    store(i);
+                    f(i);
             } else {
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
-                    if (tok + RPI * i < int(p.M))
-                        store(i);
+                    if (token(s, i) < int(p.M))
+                        f(i);
             }
         };
-        if constexpr (EC == EC_RMW) {
-            float* c = static_cast<float*>(p.c) + at;
-            f32x4 x[NI];
-            rows([&](int i) { x[i] = *reinterpret_cast<const f32x4*>(c + i * step); });
-            rows([&](int i) { *reinterpret_cast<f32x4*>(c + i * step) = residual4(p, uint32_t(tok + RPI * i), x[i], v[i], k); });
-        } else if (p.c_dtype == MK_F32) {
-            float* c = static_cast<float*>(p.c) + at;
-            rows([&](int i) { *reinterpret_cast<f32x4*>(c + i * step) = v[i]; });
-        } else {
-            uint16_t* c = static_cast<uint16_t*>(p.c) + at;
-            u32x2 o[NI];
-            with_flag(p.c_dtype == MK_F16, [&](auto h) {
+        // the residual's rows of a slice are loaded while the slice before it is added and stored
+        f32x4 x[2][EC == EC_RMW ? NI : 1];
+        auto residual = [&](int s) __attribute__((always_inline)) {
+            const float* c = static_cast<const float*>(p.c) + place(s);
+            rows(s, [&](int i) { x[s % 2][i] = *reinterpret_cast<const f32x4*>(c + i * next); });
+        };
+        if constexpr (EC == EC_RMW)
+            residual(0);
+        if constexpr (CHAIN)
+            __builtin_amdgcn_s_waitcnt(wait_vm(0)); // the next tile's first steps have landed in this wave
+        if constexpr (GLU) {
+            with_flag(p.epi == MK_EPI_SWIGLU, [&](auto swi) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < NI; ++i)
-                    o[i] = u32x2{pack_x2(v[i][0], v[i][1], decltype(h)::value), pack_x2(v[i][2], v[i][3], decltype(h)::value)};
+                for (int cb = 0; cb < CB / 2; ++cb) {
+                    const int c = min(c0 + cb * 16 + 4 * g4, cols - 4);
+                    const f32x4 s1 = *reinterpret_cast<const f32x4*>(p.wscale + c);
+                    const f32x4 s2 = *reinterpret_cast<const f32x4*>(p.wscale + cols + c);
+                    const f32x4 b1 = load4(p.bias, c, 0.0f), b2 = load4(p.bias, cols + c, 0.0f);
+#pragma unroll
+                    for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float a = fmaf(float(acc[cb][tb][e]) * sc[tb], s1[e], b1[e]);
+                            const float g = fmaf(float(acc[cb + CB / 2][tb][e]) * sc[tb], s2[e], b2[e]);
+                            acc[cb][tb][e] = __builtin_bit_cast(int, glu1<decltype(swi)::value>(a, g));
+                        }
+                }
             });
-            rows([&](int i) { *reinterpret_cast<u32x2*>(c + i * step) = o[i]; });
         }
+#pragma unroll
+        for (int s = 0; s < NSL; ++s) {
+            const int h = s % NH;
+#pragma unroll
+            for (int cb = 0; cb < SC / 16; ++cb)
+#pragma unroll
+                for (int t = 0; t < ST / 16; ++t) {
+                    const int tb = s / NH * (ST / 16) + t, row = 16 * t + r16;
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int a = acc[h * (SC / 16) + cb][tb][e];
+                        v[e] = GLU ? __builtin_bit_cast(float, a) : float(a) * sc[tb];
+                    }
+                    *reinterpret_cast<f32x4*>(st + row * SC + 4 * ((cb * 4 + g4) ^ swap(row))) = v;
+                }
+            f32x4 v[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int row = lr + RPI * i;
+                v[i] = *reinterpret_cast<const f32x4*>(st + row * SC + 4 * (lc ^ swap(row)));
+                if constexpr (!GLU)
+                    v[i] = scaled(v[i], k[h].ws, k[h].b);
+            }
+            if constexpr (EC == EC_ACT)
+                with_flag(p.epi == MK_EPI_GELU_TANH, [&](auto gelu) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < NI; ++i)
+                        v[i] = act4<decltype(gelu)::value>(v[i]);
+                });
+            if constexpr (EC == EC_RMW) {
+                if (s + 1 < NSL)
+                    residual(s + 1);
+                float* c = static_cast<float*>(p.c) + place(s);
+                rows(s, [&](int i) {
+                    *reinterpret_cast<f32x4*>(c + i * next) = residual4(p, uint32_t(token(s, i)), x[s % 2][i], v[i], k[h]);
+                });
+            } else if (p.c_dtype == MK_F32) {
+                float* c = static_cast<float*>(p.c) + place(s);
+                rows(s, [&](int i) { *reinterpret_cast<f32x4*>(c + i * next) = v[i]; });
+            } else {
+                uint16_t* c = static_cast<uint16_t*>(p.c) + place(s);
+                u32x2 o[NI];
+                with_flag(p.c_dtype == MK_F16, [&](auto f16) {
+#pragma unroll
+                    for (int i = 0; i < NI; ++i)
+                        o[i] = u32x2{pack_x2(v[i][0], v[i][1], decltype(f16)::value),
+                                     pack_x2(v[i][2], v[i][3], decltype(f16)::value)};
+                });
+                rows(s, [&](int i) { *reinterpret_cast<u32x2*>(c + i * next) = o[i]; });
+            }
+        }
+    };
+
+    // k steps 0 .. NSTG - 1 of the first tile on their way
+    set(0);
+#pragma unroll
+    for (int s = 0; s < NSTG; ++s) {
+        const int kt = min(s, ke - 1);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+            dma1(kt, past(kt), s, i);
+    }
+    for (uint32_t tile = 0;;) {
+        // step 0 in LDS: of the first tile, this wave's loads of it have landed; of later ones, all (before its stores)
+        if (!CHAIN || !tile)
+            __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 1) * ND));
+        __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int i = 0; i < CB; ++i)
+#pragma unroll
+            for (int j = 0; j < TB; ++j)
+                acc[i][j] = i32x4{0, 0, 0, 0};
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int j = 0; j < 2 * (CB + TB); ++j)
+                frag(0, j, fr[0]);
+        } else {
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+                rdw(0, 0, cb);
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+                rda(0, 0, tb, af0);
+        }
+        int kt = 0;
+        uint32_t ez = z;
+        int em0 = m0, en0 = n0;
+        bool more = false;
+        if constexpr (CHAIN) {
+            using S0 = std::integral_constant<int, 0>;
+            using S1 = std::integral_constant<int, 1>;
+            for (; kt + 2 < ke; kt += 2) {
+                step(kt + 2, S0{});
+                step(kt + 3, S1{});
+            }
+            // the last two steps load the next tile's first two (the last tile's own, which nobody reads)
+            more = ++tile < count;
+            if (more)
+                set(tile);
+            step(0, S0{});
+            step(1, S1{});
+        } else {
+            // past-the-end steps reload the last one (nobody reads them)
+            for (; kt + NSTG - 1 < ke; kt += NSTG)
+                for_each_int([&](auto i) __attribute__((always_inline)) { step(min(kt + decltype(i)::value + NSTG, ke - 1), i); },
+                             std::make_integer_sequence<int, NSTG>{});
+            for_each_int(
+                [&](auto i) __attribute__((always_inline)) {
+                    if (kt + decltype(i)::value < ke)
+                        step(ke - 1, i);
+                },
+                std::make_integer_sequence<int, NSTG - 1>{});
+            __builtin_amdgcn_s_waitcnt(0); // the last loads land before the LDS is reused
+            __syncthreads();
+        }
+        epilogue(ez, em0, en0);
+        if (!more)
+            break;
     }
 }
 
@@ -457,7 +525,7 @@ __device__ inline void locate(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, ui
 // waves a SIMD: two where 8 waves share the LDS, or two workgroups of 4 fit it
 template <int BM, int BN, int NW, int NSTG> constexpr int tile_waves()
 {
-    return NW == 8 || tile_lds<BM, BN, NW, NSTG>() <= 80 * 1024 ? 2 : 1;
+    return NW == 8 || tile_lds<BM, BN, NW, NSTG, false>() <= 80 * 1024 ? 2 : 1;
 }
 
 template <int BM, int BN, int NW, int NSTG, int EC>
@@ -465,40 +533,53 @@ __global__ __launch_bounds__(64 * NW, (tile_waves<BM, BN, NW, NSTG>())) __attrib
     tile_waves<BM, BN, NW, NSTG>(), tile_waves<BM, BN, NW, NSTG>()))) void gemm_i8_kernel(I8P p, uint32_t tiles_m,
                                                                                           uint32_t tiles_n)
 {
-    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<BM, BN, NW, NSTG>()];
-    uint32_t z, tm, tn;
-    locate(xcd_run(blockIdx.x, gridDim.x), tiles_m, tiles_n, z, tm, tn);
-    i8_tile<BM, BN, NW, NSTG, EC>(p, z, int(tm) * BM, int(tn) * (EC == EC_GLU ? BN / 2 : BN), smem);
+    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<BM, BN, NW, NSTG, false>()];
+    i8_tiles<BM, BN, NW, NSTG, EC, false>(p, smem, 1, [&](uint32_t, uint32_t& z, int& m0, int& n0) {
+        uint32_t tm, tn;
+        locate(xcd_run(blockIdx.x, gridDim.x), tiles_m, tiles_n, z, tm, tn);
+        m0 = int(tm) * BM;
+        n0 = int(tn) * (EC == EC_GLU ? BN / 2 : BN);
+    });
 }
 
-// 256 x 256 tiles, the first `whole` of them one a workgroup, the rest a quarter (128 x 128) a workgroup: whole rounds of the
-// chip take the large tile, the last, partial one spreads over all of it.
-template <int EC>
+// 256 x 256 tiles, the first `whole` of them in `chains` workgroups (CHAIN: one a compute unit, which go from tile to tile;
+// else as many as tiles), the rest a quarter (128 x 128) a workgroup: whole rounds of the chip take the large tile, the
+// last, partial one spreads over all of it. A chain saves 1.8 us a tile (32768 x 12288 x 4096 1343 -> 1298 us) where the number of k
+// steps is even; the gated epilogues have no registers for it (4352 x 24576 x 4096 SwiGLU 372 -> 398).
+template <int EC, bool CHAIN>
 __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_mixed_kernel(
-    I8P p, uint32_t tiles_m, uint32_t tiles_n, uint32_t whole)
+    I8P p, uint32_t tiles_m, uint32_t tiles_n, uint32_t whole, uint32_t chains)
 {
     constexpr int BO = EC == EC_GLU ? 128 : 256; // output channels of a tile
-    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<256, 256, 8, 2>()];
-    static_assert(tile_lds<128, 128, 8, 4>() <= tile_lds<256, 256, 8, 2>(), "");
-    uint32_t z, tm, tn;
-    if (blockIdx.x < whole) {
-        locate(xcd_run(blockIdx.x, whole), tiles_m, tiles_n, z, tm, tn);
-        i8_tile<256, 256, 8, 2, EC>(p, z, int(tm) * 256, int(tn) * BO, smem);
+    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<256, 256, 8, 2, CHAIN>()];
+    static_assert(tile_lds<128, 128, 8, 4, false>() <= tile_lds<256, 256, 8, 2, CHAIN>(), "");
+    if (blockIdx.x < chains) {
+        i8_tiles<256, 256, 8, 2, EC, CHAIN>(p, smem, CHAIN ? (whole - blockIdx.x - 1) / chains + 1 : 1,
+                                            [&](uint32_t i, uint32_t& z, int& m0, int& n0) {
+                                                uint32_t tm, tn;
+                                                locate(xcd_run(blockIdx.x + i * chains, whole), tiles_m, tiles_n, z, tm, tn);
+                                                m0 = int(tm) * 256;
+                                                n0 = int(tn) * BO;
+                                            });
         return;
     }
-    const uint32_t i = xcd_run(blockIdx.x - whole, gridDim.x - whole);
-    uint32_t m0, n0;
+    const uint32_t i = xcd_run(blockIdx.x - chains, gridDim.x - chains);
+    uint32_t bz, tm, tn, bm, bn;
     if (whole) {
-        locate(whole + i / 4, tiles_m, tiles_n, z, tm, tn);
-        m0 = tm * 256 + (i & 2) * 64;
-        n0 = tn * BO + (i & 1) * (BO / 2);
+        locate(whole + i / 4, tiles_m, tiles_n, bz, tm, tn);
+        bm = tm * 256 + (i & 2) * 64;
+        bn = tn * BO + (i & 1) * (BO / 2);
     } else { // less than a round: the launch's tiles are the small ones
-        locate(i, tiles_m, tiles_n, z, tm, tn);
-        m0 = tm * 128;
-        n0 = tn * (BO / 2);
+        locate(i, tiles_m, tiles_n, bz, tm, tn);
+        bm = tm * 128;
+        bn = tn * (BO / 2);
     }
-    if (m0 < p.M && n0 < (EC == EC_GLU ? p.N / 2 : p.N))
-        i8_tile<128, 128, 8, 4, EC>(p, z, int(m0), int(n0), smem);
+    if (bm < p.M && bn < (EC == EC_GLU ? p.N / 2 : p.N))
+        i8_tiles<128, 128, 8, 4, EC, false>(p, smem, 1, [&](uint32_t, uint32_t& z, int& m0, int& n0) {
+            z = bz;
+            m0 = int(bm);
+            n0 = int(bn);
+        });
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -627,7 +708,8 @@ template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const 
 // 144: 54 and 44; 4352 x 7168 x 4096, 220: 131 and 112).
 struct Plan {
     int kernel;
-    uint32_t tiles_m, tiles_n, whole, grid; // of the mixed kernel
+    bool chain; // these of the mixed kernel
+    uint32_t tiles_m, tiles_n, whole, chains, grid;
 };
 enum { K_NONE = -1, K_FEW, K_64X32, K_64X64, K_64X128, K_MIXED };
 
@@ -636,7 +718,7 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
     const double steps = double(cdiv(p.K, 128));
     auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t(cdiv(p.M, bm)) * cdiv(p.N, bn) * p.batch; };
     auto rounds = [&](uint64_t n) { return double((n + cus - 1) / cus); };
-    Plan best{K_NONE, 0, 0, 0, 0};
+    Plan best{K_NONE, false, 0, 0, 0, 0, 0};
     double least = 1e30;
     // a grid dimension holds fewer than 2^32 threads
     auto consider = [&](int k, double t, uint64_t threads) {
@@ -659,14 +741,18 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
     small(K_64X128, 64, 128, 0.259, 1.43, 19.0);
     const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = whole ? (big - whole) * 4 : tiles(128, 128);
     const bool quarters = rest <= 2 * uint64_t(cus);
-    const uint64_t groups = quarters ? whole + rest : big;
+    const uint64_t tiled = quarters ? whole : big;
+    best.chain = !glu && tiled > cus && cdiv(p.K, 128) % 2 == 0;
+    const uint64_t chains = best.chain ? cus : tiled;
+    const uint64_t groups = chains + (quarters ? rest : 0);
     consider(K_MIXED,
              double(whole / cus) * (steps * 1.5 + 7.6) + (quarters ? rounds(rest) * (steps * 0.372 + 1.32) : steps * 1.2 + 7.6),
              groups * 512);
     const uint32_t side = quarters && !whole ? 128 : 256;
     best.tiles_m = cdiv(p.M, side);
     best.tiles_n = cdiv(p.N, side);
-    best.whole = uint32_t(quarters ? whole : big);
+    best.whole = uint32_t(tiled);
+    best.chains = uint32_t(chains);
     best.grid = uint32_t(groups);
     return best;
 }
@@ -689,7 +775,12 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
     case K_NONE:
         return fail(MK_ERR_ARG, "gemm_i8: a launch of more than 2^32 threads");
     default:
-        gemm_i8_mixed_kernel<EC><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole);
+        if constexpr (EC != EC_GLU)
+            if (plan.chain) {
+                gemm_i8_mixed_kernel<EC, true><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole, plan.chains);
+                break;
+            }
+        gemm_i8_mixed_kernel<EC, false><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole, plan.chains);
     }
     MK_LAUNCH_CHECK("gemm_i8");
     return MK_OK;
