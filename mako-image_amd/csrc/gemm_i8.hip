@@ -94,16 +94,16 @@ template <bool GELU> __device__ inline f32x4 act4(const f32x4& v)
         o[e] = GELU ? gelu_tanh_f(v[e]) : silu_f(v[e]);
     return o;
 }
-// g Phi(g), Phi the normal distribution: Phi(-z) = e^(-z^2 / 2) t (a1 + t (a2 + ..)) / 2, t = 1 / (1 + p z / sqrt(2)), for z >= 0
-// (Abramowitz and Stegun 7.1.26, erf within 1.5e-7). erf_fit's longer series and its IEEE division cost 26 us of VALU
-// time at 3952 x 5120 outputs, as much as the product's matrix instructions.
+// g Phi(g), Phi the normal distribution: max(g, 0) - |g| Phi(-|g|), with Phi(-z) = e^(-z^2 / 2) t (a1 + t (a2 + ..)) / 2, t = 1 / (1 +
+// p z / sqrt(2)) for z >= 0 (Abramowitz and Stegun 7.1.26, erf within 1.5e-7). In a tile's epilogue these instructions run
+// alone: erf_fit's longer series and its IEEE division make 3952 x 10240 x 1280 GEGLU 79 us, this 67.
 __device__ inline float gelu_erf_f(float g)
 {
     constexpr float p = 0.231641888f, c = -0.72134752f; // 0.3275911 / sqrt(2); -log2(e) / 2
     const float z = fabsf(g), t = __builtin_amdgcn_rcpf(fmaf(p, z, 1.0f));
     const float s = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.530702714f, -0.726576013f), 0.710706870f), -0.142248368f), 0.127414796f);
     const float h = s * __builtin_amdgcn_exp2f(z * z * c);
-    return g * (g < 0.0f ? h : 1.0f - h);
+    return fmaf(-z, h, fmaxf(g, 0.0f));
 }
 template <bool SWI> __device__ inline float glu1(float a, float g) { return SWI ? silu_f(a) * g : a * gelu_erf_f(g); }
 __device__ inline f32x4 residual4(const I8P& p, uint32_t row, const f32x4& x, const f32x4& v, const Ch4& k)
@@ -317,7 +317,7 @@ __device__ __forceinline__ void i8_tiles(const I8P& p, int8_t* smem, uint32_t co
     // complete in order: no barrier. Rows of SC floats, their 16-byte chunks XOR-ed so that 16 rows at a chunk cover all banks.
     // (32 tokens keep more stores in flight; a chain has LDS for 16, the residual registers.)
     constexpr int WO = GLU ? WC / 2 : WC, SC = epi_channels(BN, GLU), NH = WO / SC; // channels a wave writes, stages at a time
-    constexpr int ST = CHAIN || EC == EC_RMW ? 16 : 32, NCH = SC / 4, RPI = 64 / NCH, NI = ST / RPI; // chunks a row, rows an instruction, a lane
+    constexpr int ST = CHAIN || EC == EC_RMW || WM < 32 ? 16 : 32, NCH = SC / 4, RPI = 64 / NCH, NI = ST / RPI; // chunks a row, rows an instruction, a lane
     auto epilogue = [&](uint32_t ez, int em0, int en0) __attribute__((always_inline)) {
         const int lane = here(), r16 = lane & 15, g4 = lane >> 4;
         float* st = reinterpret_cast<float*>(smem + (CHAIN ? NSTG * (BM + BN) * 128 : 0)) + wave * ST * SC;
@@ -543,16 +543,16 @@ __global__ __launch_bounds__(64 * NW, (tile_waves<BM, BN, NW, NSTG>())) __attrib
 }
 
 // 256 x 256 tiles, the first `whole` of them in `chains` workgroups (CHAIN: one a compute unit, which go from tile to tile;
-// else as many as tiles), the rest a quarter (128 x 128) a workgroup: whole rounds of the chip take the large tile, the
-// last, partial one spreads over all of it. A chain saves 1.8 us a tile (32768 x 12288 x 4096 1343 -> 1298 us) where the number of k
+// else as many as tiles), the rest in parts of side x side (128 or 64) a workgroup: whole rounds of the chip take the large
+// tile, the last, partial one spreads over all of it. A chain saves 1.8 us a tile (32768 x 12288 x 4096 1343 -> 1298 us) where the number of k
 // steps is even; the gated epilogues have no registers for it (4352 x 24576 x 4096 SwiGLU 372 -> 398).
 template <int EC, bool CHAIN>
 __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_mixed_kernel(
-    I8P p, uint32_t tiles_m, uint32_t tiles_n, uint32_t whole, uint32_t chains)
+    I8P p, uint32_t tiles_m, uint32_t tiles_n, uint32_t whole, uint32_t chains, uint32_t side)
 {
     constexpr int BO = EC == EC_GLU ? 128 : 256; // output channels of a tile
     __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<256, 256, 8, 2, CHAIN>()];
-    static_assert(tile_lds<128, 128, 8, 4, false>() <= tile_lds<256, 256, 8, 2, CHAIN>(), "");
+    static_assert(tile_lds<128, 128, 8, 4, false>() <= sizeof(smem) && tile_lds<64, 64, 8, 8, false>() <= sizeof(smem), "");
     if (blockIdx.x < chains) {
         i8_tiles<256, 256, 8, 2, EC, CHAIN>(p, smem, CHAIN ? (whole - blockIdx.x - 1) / chains + 1 : 1,
                                             [&](uint32_t i, uint32_t& z, int& m0, int& n0) {
@@ -566,20 +566,26 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     const uint32_t i = xcd_run(blockIdx.x - chains, gridDim.x - chains);
     uint32_t bz, tm, tn, bm, bn;
     if (whole) {
-        locate(whole + i / 4, tiles_m, tiles_n, bz, tm, tn);
-        bm = tm * 256 + (i & 2) * 64;
-        bn = tn * BO + (i & 1) * (BO / 2);
-    } else { // less than a round: the launch's tiles are the small ones
+        const uint32_t n = 256 / side, part = i % (n * n);
+        locate(whole + i / (n * n), tiles_m, tiles_n, bz, tm, tn);
+        bm = tm * 256 + part / n * side;
+        bn = tn * BO + part % n * (side * BO / 256);
+    } else { // less than a round: the launch's tiles are 128 x 128
         locate(i, tiles_m, tiles_n, bz, tm, tn);
         bm = tm * 128;
         bn = tn * (BO / 2);
     }
-    if (bm < p.M && bn < (EC == EC_GLU ? p.N / 2 : p.N))
-        i8_tiles<128, 128, 8, 4, EC, false>(p, smem, 1, [&](uint32_t, uint32_t& z, int& m0, int& n0) {
-            z = bz;
-            m0 = int(bm);
-            n0 = int(bn);
-        });
+    if (bm >= p.M || bn >= (EC == EC_GLU ? p.N / 2 : p.N))
+        return;
+    auto at = [&](uint32_t, uint32_t& z, int& m0, int& n0) {
+        z = bz;
+        m0 = int(bm);
+        n0 = int(bn);
+    };
+    if (side == 128)
+        i8_tiles<128, 128, 8, 4, EC, false>(p, smem, 1, at);
+    else
+        i8_tiles<64, 64, 8, 8, EC, false>(p, smem, 1, at);
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -709,7 +715,7 @@ template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const 
 struct Plan {
     int kernel;
     bool chain; // these of the mixed kernel
-    uint32_t tiles_m, tiles_n, whole, chains, grid;
+    uint32_t tiles_m, tiles_n, whole, chains, side, grid;
 };
 enum { K_NONE = -1, K_FEW, K_64X32, K_64X64, K_64X128, K_MIXED };
 
@@ -718,7 +724,7 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
     const double steps = double(cdiv(p.K, 128));
     auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t(cdiv(p.M, bm)) * cdiv(p.N, bn) * p.batch; };
     auto rounds = [&](uint64_t n) { return double((n + cus - 1) / cus); };
-    Plan best{K_NONE, false, 0, 0, 0, 0, 0};
+    Plan best{K_NONE, false, 0, 0, 0, 0, 0, 0};
     double least = 1e30;
     // a grid dimension holds fewer than 2^32 threads
     auto consider = [&](int k, double t, uint64_t threads) {
@@ -739,18 +745,35 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
         small(K_64X32, 64, 32, 0.0957, 0.762, 22.5);
     small(K_64X64, 64, 64, 0.15, 0.682, 21.4);
     small(K_64X128, 64, 128, 0.259, 1.43, 19.0);
-    const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = whole ? (big - whole) * 4 : tiles(128, 128);
-    const bool quarters = rest <= 2 * uint64_t(cus);
-    const uint64_t tiled = quarters ? whole : big;
+    // whole rounds of 256 x 256 tiles and the rest: as it is, in 128 x 128 parts up to two rounds of them, or in 64 x 64 ones
+    // up to one
+    const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = big - whole;
+    double last = steps * 1.2 + 7.6;
+    uint64_t parts = 0;
+    best.side = 128;
+    if (rest) {
+        const uint64_t n128 = whole ? rest * 4 : tiles(128, 128);
+        const double t128 = rounds(n128) * (steps * 0.372 + 1.32), t64 = steps * 0.15 + 0.7;
+        if (n128 <= 2 * uint64_t(cus) && t128 < last) {
+            last = t128;
+            parts = n128;
+        }
+        if (whole && rest * 16 <= cus && t64 < last) {
+            last = t64;
+            parts = rest * 16;
+            best.side = 64;
+        }
+    } else {
+        last = 0.0;
+    }
+    const uint64_t tiled = parts ? whole : big;
     best.chain = !glu && tiled > cus && cdiv(p.K, 128) % 2 == 0;
     const uint64_t chains = best.chain ? cus : tiled;
-    const uint64_t groups = chains + (quarters ? rest : 0);
-    consider(K_MIXED,
-             double(whole / cus) * (steps * 1.5 + 7.6) + (quarters ? rounds(rest) * (steps * 0.372 + 1.32) : steps * 1.2 + 7.6),
-             groups * 512);
-    const uint32_t side = quarters && !whole ? 128 : 256;
-    best.tiles_m = cdiv(p.M, side);
-    best.tiles_n = cdiv(p.N, side);
+    const uint64_t groups = chains + parts;
+    consider(K_MIXED, double(whole / cus) * (steps * 1.5 + 7.6) + last, groups * 512);
+    const uint32_t tile = parts && !whole ? 128 : 256;
+    best.tiles_m = cdiv(p.M, tile);
+    best.tiles_n = cdiv(p.N, tile);
     best.whole = uint32_t(tiled);
     best.chains = uint32_t(chains);
     best.grid = uint32_t(groups);
@@ -777,10 +800,12 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
     default:
         if constexpr (EC != EC_GLU)
             if (plan.chain) {
-                gemm_i8_mixed_kernel<EC, true><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole, plan.chains);
+                gemm_i8_mixed_kernel<EC, true><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole, plan.chains,
+                                                                   plan.side);
                 break;
             }
-        gemm_i8_mixed_kernel<EC, false><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole, plan.chains);
+        gemm_i8_mixed_kernel<EC, false><<<plan.grid, 512, 0, s>>>(p, plan.tiles_m, plan.tiles_n, plan.whole, plan.chains,
+                                                                   plan.side);
     }
     MK_LAUNCH_CHECK("gemm_i8");
     return MK_OK;

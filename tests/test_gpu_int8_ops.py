@@ -281,13 +281,14 @@ def test_product_batches_and_strides(gpu, m, n, k):
     Product(m, 2 * n, k, epi=M.EPI_SWIGLU, batch=2, lda=k + 16, ldc=n + 20, c=M.F16, bias=False).check()
 
 
-# (on 256 compute units: 128 x 128 tiles in one and two rounds; 256 x 256 ones in a partial round, in a whole round and a few
-# quarters of tiles, in a whole round and a partial one)
-@pytest.mark.parametrize("m, n", [(4400, 1028), (2048, 2304), (1537, 4100), (4400, 2304), (4400, 4100), (4400, 6000)])
+# (on 256 compute units: 128 x 128 tiles in one and two rounds; 256 x 256 ones in a partial round; in a whole round and 128 x
+# 128 parts, 64 x 64 parts, a partial round; chains of two, of one or two tiles; an odd number of k steps, which is never chained)
+@pytest.mark.parametrize("m, n, k", [(4400, 1028, 176), (2048, 2304, 176), (1537, 4100, 176), (4400, 2304, 176), (4400, 4100, 176),
+                                     (4300, 4096, 176), (4400, 6000, 176), (8300, 4100, 176), (4400, 6000, 80), (8300, 4100, 336)])
 @pytest.mark.parametrize("epi, c", [(M.EPI_STORE, M.BF16), (M.EPI_GEGLU, M.F16), (M.EPI_GATE_TANH, M.F32)])
-def test_product_many_tiles(gpu, m, n, epi, c):
+def test_product_many_tiles(gpu, m, n, k, epi, c):
     n -= n % 8 if epi == M.EPI_GEGLU else 0
-    Product(m, n, 176, epi, c, split=100, seg=m).check()
+    Product(m, n, k, epi, c, split=100, seg=m).check()
 
 
 @pytest.mark.parametrize("m", [1, 20, 130])
