@@ -241,29 +241,43 @@ __device__ __forceinline__ void i8_tiles(const I8P& p, int8_t* smem, uint32_t co
     auto rda = [&](int buf, int ks, int tb, i32x4(&af)[TB]) {
         af[tb] = *reinterpret_cast<const i32x4*>(&sA[buf][fa[ks] + tb * 2048]);
     };
-    // A substep: the weight fragments are single-buffered, each next one read into its registers right after the last
-    // product that uses it; the next token fragments go to the other buffer with the first channel block; the direct loads
-    // of step gkt (into stage gbuf) follow every second product (0.8% faster than every one). Every instruction is fenced:
-    // the order is this one.
-    static_assert(WIDE || ND <= CB * TB / 2, "a load after every second product");
+    // A substep: the weight fragments are single-buffered, each next one read into its registers after the last product that
+    // uses it; the next token fragments go to the other buffer with the first channel block. The second substep (`load`) has
+    // the step's barrier after its first TB products, whose fragments are there, and the direct loads of step gkt into
+    // stage gbuf after every second product behind it. (The barrier behind four products, not before them, is 0.5% faster; a
+    // load after every second product, not every one, 0.8%.) Every instruction is fenced: the order is this one.
+    static_assert(WIDE || ND <= (CB - 1) * TB / 2, "a load after every second product");
     auto substep = [&](const i32x4(&af)[TB], int nbuf, int nks, i32x4(&naf)[TB], int gkt, int gbuf,
                        bool load) __attribute__((always_inline)) {
         const uint32_t gp = past(gkt);
+        const int from = load ? TB : 0;
 #pragma unroll
         for (int i = 0; i < CB * TB; ++i) {
             const int cb = i / TB, tb = i % TB;
+            if (load && i == TB) {
+                // step kt + 1 has landed (later ones may be in flight), and this stage is read
+                __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+            }
             acc[cb][tb] = mfma_i8(wf[cb], af[tb], acc[cb][tb]);
             __builtin_amdgcn_sched_barrier(0);
-            if (cb == 0) {
-                rda(nbuf, nks, tb, naf);
+            if (i < from)
+                continue;
+            if (i < from + TB) {
+                rda(nbuf, nks, i - from, naf);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (load && i == TB) {
+                rdw(nbuf, nks, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (tb == TB - 1) {
                 rdw(nbuf, nks, cb);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (load && i % 2 && i / 2 < ND) {
-                dma1(gkt, gp, gbuf, i / 2);
+            if (load && (i - TB) % 2 && (i - TB) / 2 < ND) {
+                dma1(gkt, gp, gbuf, (i - TB) / 2);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -274,10 +288,10 @@ __device__ __forceinline__ void i8_tiles(const I8P& p, int8_t* smem, uint32_t co
         const int ks = j / (CB + TB), i = j % (CB + TB);
         f[ks][i] = *reinterpret_cast<const i32x4*>(i < CB ? &sW[buf][fw[ks] + i * 2048] : &sA[buf][fa[ks] + (i - CB) * 2048]);
     };
-    // k step kt in stage `buf` (a constant: the loop is unrolled by NSTG): the first substep reads the second's fragments;
-    // then step kt + 1 has landed (later ones may be in flight) and, after the barrier, in every wave, and every wave has
-    // read this stage, so the second substep loads into it and reads step kt + 1's first fragments. The loads are those of step kt + NSTG
-    // of that tile, from k step kl.
+    // k step kt in stage `buf` (a constant: the loop is unrolled by NSTG): the first substep reads the second's fragments.
+    // Where step kt + 1 has landed and, behind the barrier, in every wave, and every wave has read this stage, the second
+    // one loads into it and reads step kt + 1's first fragments. The loads are those of k step kl: kt + NSTG, or the
+    // next tile's.
     auto step = [&](int kl, auto buf_c) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value, nb = (buf + 1) % NSTG;
         if constexpr (WIDE) {
@@ -307,8 +321,6 @@ __device__ __forceinline__ void i8_tiles(const I8P& p, int8_t* smem, uint32_t co
             return;
         }
         substep(af0, buf, 1, af1, 0, 0, false);
-        __builtin_amdgcn_s_waitcnt(wait_vm((NSTG - 2) * ND));
-        __builtin_amdgcn_s_barrier();
         substep(af1, nb, 0, af0, kl, buf, true);
     };
 
