@@ -247,7 +247,8 @@ typedef struct mk_gate_norm_args {
     float eps1, eps2;
 } mk_gate_norm_args;
 /* The vectors, x and x_out are 16-byte aligned, y and out for 4 of their elements, out_scale for one. Apart from x_out == x
- * no output overlaps an input or another output. Infinities and NaNs stay in their row. Allocates nothing and keeps no
+ * no output overlaps an input or another output. Infinities and NaNs stay in their row, and a row's bits do not depend on
+ * the rows beside it. Allocates nothing and keeps no
  * workspace: it may be captured, and may run on several streams at once. */
 mk_status mk_gate_norm(const mk_gate_norm_args* a, void* stream);
 

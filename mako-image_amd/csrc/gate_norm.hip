@@ -208,8 +208,8 @@ __device__ inline void norm_row(f32x4 (&v)[NV], uint32_t c0, uint32_t nv, uint32
 // mk_gate_norm, one pass: the row of x and y in registers (W waves a row, NV float4s a thread; W = 1: four rows a workgroup),
 // the statistics two-pass over them (the mean first, then the squares about it: a variance far below the mean's square keeps
 // its digits). Bound by HBM: 8 bytes of residual, 2 of y and 2 (int8: 1) of out an element. Measured with three sets of
-// buffers in turn: 4352 x 4096 38.3 us (5.6 TB/s), 32768 x 4096 296 us (5.4), 32768 x 1280 88 us (5.7), to int8 4352 x
-// 4096 38.2 us; a copy runs at 5.0. The residual's nontemporal loads and stores are worth 47 -> 38 us of the first; y is the
+// buffers in turn: 4352 x 4096 38.3 us (5.6 TB/s), 32768 x 4096 294 us (5.5), 32768 x 1280 88 us (5.7), to int8 4352 x
+// 4096 37.5 us; a copy runs at 5.0. The residual's nontemporal loads and stores are worth 47 -> 38 us of the first; y is the
 // last product's output and out the next one's input, which the caches may hold. Loading the vectors (w, scale, shift) with
 // the row costs the registers of half the waves: 47 -> 53 us.
 template <int W, int NV>
@@ -239,9 +239,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gat
         const uint32_t c = c0 + 64 * W * i;
         xv[i] = c < nv ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(x + 4 * c)) : f32x4{0, 0, 0, 0};
     }
-    if (g.y)
-        load_vec<W, NV>(gt, g.gate, mod, c0, nv, 1.0f);
     if (g.y) {
+        load_vec<W, NV>(gt, g.gate, mod, c0, nv, 1.0f);
         norm_row<W, NV>(v, c0, nv, g.n, g.norm1, g.w1, g.b1, g.eps1, red, 0);
         if (g.gate && g.tanh_gate)
 #pragma unroll
@@ -430,17 +429,17 @@ void quantize_rows(const void* src, uint32_t rows, uint64_t cols, int64_t ld, in
 
 void launch_rows(const mk_gate_norm_args& g, hipStream_t s)
 {
-    // the fewest waves that hold the row in 4 float4s a thread: more of them wait at barriers (32768 x 1280, 2 / 4 / 8 waves: 95 /
-    // 108 / 155 us); in 2 float4s where few rows leave compute units idle (1 x 4096, 4 / 8 waves: 5.1 / 3.9 us, 300 x 4096 7.2 /
-    // 6.3, 600 x 4096 10.2 / 9.5, 4352 x 4096 47.1 / 46.9)
-    const uint32_t waves = cdiv(g.n, g.rows <= 512 ? 512 : 1024);
-    if (waves <= 1)
+    // waves a row by its width alone, so that a row's sums, and its bits, do not depend on the rows beside it. More waves than
+    // that wait at barriers (us on 1 / 2 / 4 / 8 / 16 waves: 32768 x 512 46 / 44 / 66, 32768 x 1280 - / 95 / 108 / 155, 10000 x
+    // 2560 - / 65 / 62 / 69), fewer hold too few rows' loads in flight (32768 x 4096 - / - / 303 / 298 / 355, 9000 x 8192 - / - / - /
+    // 171 / 179) and take longer over a single one (1 x 4096 - / - / 5.1 / 3.9 / 3.4).
+    if (g.n <= 512)
         launch_gate_norm<1>(g, s);
-    else if (waves <= 2)
+    else if (g.n <= 1536)
         launch_gate_norm<2>(g, s);
-    else if (waves <= 4)
+    else if (g.n <= 3328)
         launch_gate_norm<4>(g, s);
-    else if (waves <= 8)
+    else if (g.n <= 8192)
         launch_gate_norm<8>(g, s);
     else
         launch_gate_norm<16>(g, s);

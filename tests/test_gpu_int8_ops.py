@@ -512,10 +512,15 @@ def test_gate_norm_widths(gpu, n, rows):
     GateNorm(rows, n, out=M.I8, norm1=M.NORM_RMS, norm2=M.NORM_RMS, alpha=0.5).check()
 
 
-@pytest.mark.parametrize("n", [512, 1024, 1280, 2048, 4096, 6144, 8192, 16384])
+@pytest.mark.parametrize("n", [512, 1024, 1280, 1540, 2048, 3332, 4096, 6144, 8192, 8196, 16384])
 def test_gate_norm_many_rows(gpu, n):
-    # beyond 512 rows a row takes fewer waves
-    GateNorm(517, n, out=M.I8, norm1=M.NORM_RMS, split=20, seg=260, samples=2).check()
+    g = GateNorm(517, n, out=M.I8, norm1=M.NORM_RMS, split=20, seg=260, samples=2)
+    g.check()
+    x, h, s = g.read()
+    for rows in (300, 5, 1):  # the first rows alone: the same bits
+        g.rows, g.x, g.ybits = rows, g.x[:rows], g.ybits[:rows]
+        x1, h1, s1 = g.run()
+        assert np.array_equal(x1, x[:rows]) and np.array_equal(h1, h[:rows]) and np.array_equal(s1, s[:rows])
 
 
 @pytest.mark.parametrize("y", [M.F32, M.BF16, M.F16])
