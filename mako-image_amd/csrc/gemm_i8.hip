@@ -94,16 +94,22 @@ template <bool GELU> __device__ inline f32x4 act4(const f32x4& v)
         o[e] = GELU ? gelu_tanh_f(v[e]) : silu_f(v[e]);
     return o;
 }
-// g Phi(g), Phi the normal distribution: max(g, 0) - |g| Phi(-|g|), with Phi(-z) = e^(-z^2 / 2) t (a1 + t (a2 + ..)) / 2, t = 1 / (1 +
-// p z / sqrt(2)) for z >= 0 (Abramowitz and Stegun 7.1.26, erf within 1.5e-7). In a tile's epilogue these instructions run
-// alone: erf_fit's longer series and its IEEE division make 3952 x 10240 x 1280 GEGLU 79 us, this 67.
+// g Phi(g), Phi the normal distribution: max(g, 0) - |g| Phi(-|g|). log2 Phi(-z) for z >= 0 is a polynomial of degree 8, fitted here
+// by iterated least squares to Phi's own error on [0, 5.8] (Phi within 2.7e-7, z Phi(-z) within 8.5e-8, Phi(-z) to 8e-5 of itself up
+// to z = 5.5); beyond, it falls faster than Phi does. In a tile's epilogue these instructions run alone: with erf_fit's longer
+// series and its IEEE division 3952 x 10240 x 1280 GEGLU took 79 us, with a rational form (a reciprocal more) 68, so 66.
 __device__ inline float gelu_erf_f(float g)
 {
-    constexpr float p = 0.231641888f, c = -0.72134752f; // 0.3275911 / sqrt(2); -log2(e) / 2
-    const float z = fabsf(g), t = __builtin_amdgcn_rcpf(fmaf(p, z, 1.0f));
-    const float s = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.530702714f, -0.726576013f), 0.710706870f), -0.142248368f), 0.127414796f);
-    const float h = s * __builtin_amdgcn_exp2f(z * z * c);
-    return fmaf(-z, h, fmaxf(g, 0.0f));
+    const float z = fabsf(g);
+    float q = fmaf(-5.577092e-07f, z, 9.50235062e-06f);
+    q = fmaf(q, z, -3.01707514e-05f);
+    q = fmaf(q, z, -0.0005522336f);
+    q = fmaf(q, z, 0.0076639154f);
+    q = fmaf(q, z, -0.052960813f);
+    q = fmaf(q, z, -0.459032208f);
+    q = fmaf(q, z, -1.15113127f);
+    q = fmaf(q, z, -0.999999285f);
+    return fmaf(-z, __builtin_amdgcn_exp2f(q), fmaxf(g, 0.0f));
 }
 template <bool SWI> __device__ inline float glu1(float a, float g) { return SWI ? silu_f(a) * g : a * gelu_erf_f(g); }
 __device__ inline f32x4 residual4(const I8P& p, uint32_t row, const f32x4& x, const f32x4& v, const Ch4& k)
@@ -601,26 +607,25 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Up to 16 rows: a workgroup makes 16 channels of all rows, its 8 waves every eighth 256 bytes of k each, straight from
-// memory to registers (the rows of a product's operand lie in 64-byte pieces of 16 rows a load: about 40 bytes a ns and CU,
-// enough where every CU has a workgroup or two); nothing of the weight is read twice. The sums meet in LDS. Bound by the
-// weight's bytes: 1 x 4096 x 4096 5.0 us, 1 x 4096 x 12288 9.9 us, a launch alone 3. 4 or 16 waves, 128 or 512 bytes a
-// turn: within 15%. Two or four of these rows' blocks (17 to 64 rows) are slower than 64 x 32 tiles (32 x 4096 x 4096 7.9 and
-// 6.3 us).
+// 16 rows x 16 channels a workgroup, its 8 waves every eighth 256 bytes of k each, straight from memory to registers: for few
+// rows (up to 16 read the weight once) and for small products of long k, whose few larger tiles leave the chip idle. The
+// rows of an operand lie in 64-byte pieces of 16 rows a load, which brings 40 to 60 bytes a ns and CU, half of what the direct
+// loads of a tile do. The sums meet in LDS. Up to 16 rows bound by the weight's bytes: 1 x 4096 x 4096 5.0 us, 1 x 4096 x 12288 9.9
+// us, a launch alone 3; 98 x 176 x 11344 9.6 us, on 64 x 32 tiles 19.4. 4 or 16 waves, 128 or 512 bytes a turn: within 15%.
 // ------------------------------------------------------------------------------------------------------------
-constexpr int kFewWaves = 8;
+constexpr int k16Waves = 8;
 
-template <int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_kernel(I8P p)
+template <int EC> __global__ __launch_bounds__(64 * k16Waves) void gemm_i8_16_kernel(I8P p)
 {
     constexpr bool GLU = EC == EC_GLU;
     constexpr int CB = GLU ? 2 : 1, NS = 4;
-    constexpr uint32_t kUnit = 64 * NS, kStep = kFewWaves * kUnit;
-    __shared__ i32x4 red[kFewWaves][CB][64];
+    constexpr uint32_t kUnit = 64 * NS, kStep = k16Waves * kUnit;
+    __shared__ i32x4 red[k16Waves][CB][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g4 = lane >> 4, cols = int(GLU ? p.N / 2 : p.N), n0 = int(blockIdx.x) * 16;
     const uint32_t z = blockIdx.y;
-    const int nr = min(cols - n0, 16), M = int(p.M);
-    const int8_t* gA = p.a + int64_t(z) * p.sa;
+    const int m0 = int(blockIdx.z) * 16, nr = min(cols - n0, 16), M = min(int(p.M) - m0, 16);
+    const int8_t* gA = p.a + int64_t(z) * p.sa + int64_t(m0) * p.lda;
     const int8_t* gW = p.w + uint64_t(n0) * p.K;
     const BufRes rsA = buf_res(gA, uint32_t(int64_t(M - 1) * p.lda + p.K));
     const BufRes rsW[2] = {buf_res(gW, uint32_t(nr) * p.K), buf_res(GLU ? gW + uint64_t(cols) * p.K : gW, uint32_t(nr) * p.K)};
@@ -671,11 +676,11 @@ template <int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_
         return;
     i32x4 s[CB] = {};
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w)
+    for (int w = 0; w < k16Waves; ++w)
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             s[c] += red[w][c][lane];
-    const float as = p.ascale[uint64_t(z) * p.M + tok];
+    const float as = p.ascale[uint64_t(z) * p.M + m0 + tok];
     const Ch4 kc = channels4(p, ch);
     f32x4 t;
 #pragma unroll
@@ -693,10 +698,10 @@ template <int EC> __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few_
     } else if constexpr (EC == EC_ACT) {
         v = p.epi == MK_EPI_GELU_TANH ? act4<true>(v) : act4<false>(v);
     }
-    const int64_t at = int64_t(z) * p.sc + int64_t(tok) * p.ldc + ch;
+    const int64_t at = int64_t(z) * p.sc + int64_t(m0 + tok) * p.ldc + ch;
     if constexpr (EC == EC_RMW) {
         f32x4* x = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
-        *x = residual4(p, uint32_t(tok), *x, v, kc);
+        *x = residual4(p, uint32_t(m0 + tok), *x, v, kc);
     } else if (p.c_dtype == MK_F32) {
         *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at) = v;
     } else {
@@ -714,22 +719,23 @@ template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const 
 }
 
 // The kernel of a launch: the one with the least estimated time in us, beside a launch's own. A tile takes its k steps of
-// 128 at the rate its CU brings operands in (64 x 32: 0.096, 64 x 64: 0.15, 64 x 128: 0.26, 128 x 128: 0.37 a step) or, where
-// all CUs load, at the 19 to 22 TB/s that they take from the L2s together; 256 x 256 tiles are bound by the matrix cores
-// (1.5 a step, 7.6 for the pipeline's start and the epilogue, which nothing overlaps; 1.2 where the round is not full and
-// the clock higher). Fitted to the kernels' times at 436 shapes (rows 1 .. 4096, N and K 256 .. 12288); the choice is within 0.2%
-// of the best in the mean, 13% at worst (16 x 4096 x 12288: 13.3 us against 11.8). Measured, us, few / 64 x 32 / 64 x 64 /
-// 64 x 128 / mixed: 1 x 4096 x 4096 4.5 / 6.1 / 7.6 / 11 / 14, 1 x 12288 x 4096 14 / 10.6 / 9.7 / 11 / 14, 77 x 2560 x 2048 - / 4.4 /
-// 5.0 / 7.4 / 9.0, 300 x 4096 x 12288 - / 38 / 35 / 29 / 36, 1024 x 4096 x 4096 - / 36 / 27 / 24 / 19.
-// The mixed kernel's last, partial round takes quarter tiles up to two rounds of them (4352 x 4096 x 12288, 16 tiles left: 207 us
-// against 259; 4352 x 5120 x 4096, 84 left: 91 and 95; 1024 x 8192 x 4096, 128: 40 and 44), then whole ones (1024 x 9216 x 4096,
-// 144: 54 and 44; 4352 x 7168 x 4096, 220: 131 and 112).
+// 128 at the rate its CU brings operands in (64 x 32: 0.096, 64 x 64: 0.15, 64 x 128: 0.26, 128 x 128: 0.37 a step; 16 x 16 rows
+// 40 bytes a ns, or all weights 5.8 TB/s) or, where all CUs load, at the 19 to 22 TB/s that they take from the L2s together; 256
+// x 256 tiles are bound by the matrix cores (1.5 a step, 7.6 for the pipeline's start and the epilogue, which nothing overlaps;
+// 1.2 where the round is not full and the clock higher). Fitted to the kernels' times at 436 shapes (rows 1 .. 4096, N and K 256 ..
+// 12288); at 238 others (rows 1 .. 5000, N from 64, K from 256) the choice is within 0.7% of the best in the mean, 17% at worst
+// (450 x 176 x 11344: 20.6 us, 17.6). Measured, us, 16 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / mixed: 1 x 4096 x 4096 5.0 / 6.1 / 7.6 /
+// 11 / 14, 1 x 12288 x 4096 12.5 / 10.6 / 9.6 / 11 / 14, 98 x 176 x 11344 9.6 / 19 / 28 / 40 / -, 77 x 2560 x 2048 9.3 / 4.3 / 4.8 / 7.1 /
+// 9.0, 300 x 4096 x 12288 - / 38 / 35 / 29 / 36, 1024 x 4096 x 4096 - / 36 / 27 / 24 / 19.
+// The mixed kernel's last, partial round takes 128 x 128 parts up to two rounds of them (4352 x 5120 x 4096, 84 tiles left: 91 us
+// against 95 in whole tiles; 1024 x 8192 x 4096, 128: 40 and 44), then whole tiles (1024 x 9216 x 4096, 144: 54 and 44; 4352 x 7168
+// x 4096, 220: 131 and 112); 64 x 64 parts where they fit one round (4352 x 4096 x 12288, 16 left: 185 us, 210 in 128 x 128, 259 whole).
 struct Plan {
     int kernel;
     bool chain; // these of the mixed kernel
     uint32_t tiles_m, tiles_n, whole, chains, side, grid;
 };
-enum { K_NONE = -1, K_FEW, K_64X32, K_64X64, K_64X128, K_MIXED };
+enum { K_NONE = -1, K_16X16, K_64X32, K_64X64, K_64X128, K_MIXED };
 
 Plan plan_of(const I8P& p, bool glu, uint32_t cus)
 {
@@ -750,8 +756,10 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
         consider(k, std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / (tbs * 1e6) * 256 / cus),
                  n * 256);
     };
-    if (p.M <= 16)
-        consider(K_FEW, std::max(rounds(tiles(16, 16)) * p.K * 3.5e-4, double(p.N) * p.K * p.batch * 0.172e-6) + 0.3,
+    if (p.M <= 16 * 65535)
+        consider(K_16X16,
+                 std::max(rounds(tiles(16, 16)) * (p.K * (16.0 + std::min(p.M, 16u)) * 2.4e-5 + 0.3),
+                          double(p.N) * p.K * p.batch * 0.172e-6),
                  uint64_t(cdiv(p.N, 16)) * 512);
     if (!glu) // (its two parts are 16 channels of a wave each)
         small(K_64X32, 64, 32, 0.0957, 0.762, 22.5);
@@ -796,8 +804,9 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
 {
     const Plan plan = plan_of(p, EC == EC_GLU, cus);
     switch (plan.kernel) {
-    case K_FEW:
-        gemm_i8_few_kernel<EC><<<dim3(cdiv(EC == EC_GLU ? p.N / 2 : p.N, 16), p.batch), 64 * kFewWaves, 0, s>>>(p);
+    case K_16X16:
+        gemm_i8_16_kernel<EC><<<dim3(cdiv(EC == EC_GLU ? p.N / 2 : p.N, 16), p.batch, cdiv(p.M, 16)), 64 * k16Waves, 0,
+                                 s>>>(p);
         break;
     case K_64X32:
         if constexpr (EC != EC_GLU)
