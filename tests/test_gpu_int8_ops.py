@@ -281,6 +281,13 @@ def test_product_batches_and_strides(gpu, m, n, k):
     Product(m, 2 * n, k, epi=M.EPI_SWIGLU, batch=2, lda=k + 16, ldc=n + 20, c=M.F16, bias=False).check()
 
 
+@pytest.mark.parametrize("epi, c", [(M.EPI_STORE, M.F16), (M.EPI_GELU_TANH, M.BF16), (M.EPI_SWIGLU, M.BF16), (M.EPI_GEGLU, M.F32),
+                                    (M.EPI_GATE_TANH, M.F32), (M.EPI_ADD, M.F32)])
+@pytest.mark.parametrize("m, n, k", [(1, 72, 8208), (17, 72, 8208), (61, 136, 6160)])
+def test_product_small_with_long_k(gpu, m, n, k, epi, c):
+    Product(m, n, k, epi, c, batch=2, lda=k + 16, ldc=n + 4, split=5, seg=16).check()
+
+
 # (on 256 compute units: 128 x 128 tiles in one and two rounds; 256 x 256 ones in a partial round; in a whole round and 128 x
 # 128 parts, 64 x 64 parts, a partial round; chains of two, of one or two tiles; an odd number of k steps, which is never chained)
 @pytest.mark.parametrize("m, n, k", [(4400, 1028, 176), (2048, 2304, 176), (1537, 4100, 176), (4400, 2304, 176), (4400, 4100, 176),
