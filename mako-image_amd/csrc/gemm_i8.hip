@@ -109,7 +109,8 @@ __device__ inline float gelu_erf_f(float g)
     q = fmaf(q, z, -0.459032208f);
     q = fmaf(q, z, -1.15113127f);
     q = fmaf(q, z, -0.999999285f);
-    return fmaf(-z, __builtin_amdgcn_exp2f(q), fmaxf(g, 0.0f));
+    // (the factor is bounded where Phi has long been 0: an infinite g gives g or 0, a NaN stays one by q)
+    return fmaf(-fminf(z, 1e4f), __builtin_amdgcn_exp2f(q), fmaxf(g, 0.0f));
 }
 template <bool SWI> __device__ inline float glu1(float a, float g) { return SWI ? silu_f(a) * g : a * gelu_erf_f(g); }
 __device__ inline f32x4 residual4(const I8P& p, uint32_t row, const f32x4& x, const f32x4& v, const Ch4& k)
@@ -226,8 +227,7 @@ __device__ __forceinline__ void i8_tiles(const I8P& p, int8_t* smem, uint32_t co
                            uint32_t(kt) * 128);
         }
     };
-    // (a chain takes an even number of steps, so that every tile starts in stage 0: one of zeros where K has an odd one)
-    const int kn = int((p.K + 127) / 128), ke = CHAIN ? (kn + 1) & ~1 : kn;
+    const int ke = int((p.K + 127) / 128); // a chain's is even: every tile starts in stage 0
     auto past = [&](int kt) { return kc * 16 >= int(p.K) - kt * 128 ? 0x80000000u : 0u; };
 
     i32x4 acc[CB][TB];

@@ -183,7 +183,7 @@ class Product:
                 s = a / (1 + np.exp(-a))
                 return s * b, np.abs(b) * (1.1 * ea + np.abs(s) * (8 + 4 * np.abs(a)) * u) + np.abs(s) * eb + 4 * u * np.abs(s * b)
             g = 0.5 * b * (1 + erf(b * np.sqrt(0.5)))
-            # the erf series is within 1.5e-7, its five terms, exp2 and rcp add a few roundings of values below 1
+            # z Phi(-z) is fitted within 8.5e-8; exp2 and the polynomial's roundings add less than 16 u of values below z / 2
             return a * g, np.abs(g) * ea + np.abs(a) * (1.13 * eb + 0.5 * np.abs(b) * (2e-7 + 32 * u)) + 4 * u * np.abs(a * g)
         if self.rmw:
             row = np.arange(self.m) % (self.seg or 1 << 32)
@@ -332,6 +332,18 @@ def test_product_nonfinite_scales_stay_in_their_row(gpu, m, n, k):
     keep = [r for r in range(m) if r not in (3, m - 1)]
     w, e = p.want()
     assert (np.abs(got[keep] - w[0, keep]) <= e[0, keep] + HALF[M.BF16] * (np.abs(w[0, keep]) + e[0, keep])).all()
+
+
+@pytest.mark.parametrize("m, n, k", [(3, 24, 48), (70, 264, 208), (300, 1032, 336)])
+def test_geglu_of_infinite_gates(gpu, m, n, k):
+    # b Phi(b) is b at +inf and 0 at -inf; a NaN stays in its column
+    p = Product(m, n, k, M.EPI_GEGLU)
+    f = n // 2
+    p.bias[f + 1], p.bias[f + 2], p.bias[f + 3] = np.inf, -np.inf, np.nan
+    got, a = p.run()[0], p.pre[0, :, 1]
+    assert (np.abs(a) > p.mag[0, :, 1] * 4 * u).all()
+    assert np.array_equal(got[:, 1], np.copysign(np.inf, a)) and (got[:, 2] == 0).all() and np.isnan(got[:, 3]).all()
+    assert np.isfinite(np.delete(got, [1, 2, 3], 1)).all()
 
 
 def test_product_empty(gpu):
