@@ -722,9 +722,9 @@ template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const 
 // 128 at the rate its CU brings operands in (64 x 32: 0.096, 64 x 64: 0.15, 64 x 128: 0.26, 128 x 128: 0.37 a step; 16 x 16 rows
 // 40 bytes a ns, or all weights 5.8 TB/s) or, where all CUs load, at the 19 to 22 TB/s that they take from the L2s together; 256
 // x 256 tiles are bound by the matrix cores (1.5 a step, 7.6 for the pipeline's start and the epilogue, which nothing overlaps;
-// 1.2 where the round is not full and the clock higher). Fitted to the kernels' times at 436 shapes (rows 1 .. 4096, N and K 256 ..
-// 12288); at 238 others (rows 1 .. 5000, N from 64, K from 256) the choice is within 0.7% of the best in the mean, 17% at worst
-// (450 x 176 x 11344: 20.6 us, 17.6). Measured, us, 16 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / mixed: 1 x 4096 x 4096 5.0 / 6.1 / 7.6 /
+// 1.2 and 5.9 where the round is not full and the clock higher). Fitted to the kernels' times at 1020 shapes and epilogues (rows 1 .. 9000, N
+// from 64, K from 128): the choice is within 0.3% of the best in the mean for STORE, 0.9% for GELU and GEGLU, 17% at worst (450 x 176 x
+// 11344: 20.6 us, 17.6). Measured, us, 16 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / mixed: 1 x 4096 x 4096 5.0 / 6.1 / 7.6 /
 // 11 / 14, 1 x 12288 x 4096 12.5 / 10.6 / 9.6 / 11 / 14, 98 x 176 x 11344 9.6 / 19 / 28 / 40 / -, 77 x 2560 x 2048 9.3 / 4.3 / 4.8 / 7.1 /
 // 9.0, 300 x 4096 x 12288 - / 38 / 35 / 29 / 36, 1024 x 4096 x 4096 - / 36 / 27 / 24 / 19.
 // The mixed kernel's last, partial round takes 128 x 128 parts up to two rounds of them (4352 x 5120 x 4096, 84 tiles left: 91 us
@@ -756,42 +756,43 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
         consider(k, std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / (tbs * 1e6) * 256 / cus),
                  n * 256);
     };
+    const uint32_t parts = glu ? 2 : 1; // of the weight
     if (p.M <= 16 * 65535)
         consider(K_16X16,
-                 std::max(rounds(tiles(16, 16)) * (p.K * (16.0 + std::min(p.M, 16u)) * 2.4e-5 + 0.3),
+                 std::max(rounds(tiles(16, 16 * parts)) * (p.K * (16.0 * parts + std::min(p.M, 16u)) * 2.4e-5 + 0.05),
                           double(p.N) * p.K * p.batch * 0.172e-6),
-                 uint64_t(cdiv(p.N, 16)) * 512);
+                 uint64_t(cdiv(p.N, 16 * parts)) * 512);
     if (!glu) // (its two parts are 16 channels of a wave each)
-        small(K_64X32, 64, 32, 0.0957, 0.762, 22.5);
-    small(K_64X64, 64, 64, 0.15, 0.682, 21.4);
-    small(K_64X128, 64, 128, 0.259, 1.43, 19.0);
+        small(K_64X32, 64, 32, 0.0957, 0.53, 22.5);
+    small(K_64X64, 64, 64, 0.15, 0.69, 21.4);
+    small(K_64X128, 64, 128, 0.259, 1.6, 19.0);
     // whole rounds of 256 x 256 tiles and the rest: as it is, in 128 x 128 parts up to two rounds of them, or in 64 x 64 ones
     // up to one
     const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = big - whole;
-    double last = steps * 1.2 + 7.6;
-    uint64_t parts = 0;
+    double last = steps * 1.2 + 5.9;
+    uint64_t tail = 0;
     best.side = 128;
     if (rest) {
         const uint64_t n128 = whole ? rest * 4 : tiles(128, 128);
-        const double t128 = rounds(n128) * (steps * 0.372 + 1.32), t64 = steps * 0.15 + 0.7;
+        const double t128 = rounds(n128) * (steps * 0.372 + 2.05), t64 = steps * 0.15 + 0.7;
         if (n128 <= 2 * uint64_t(cus) && t128 < last) {
             last = t128;
-            parts = n128;
+            tail = n128;
         }
         if (whole && rest * 16 <= cus && t64 < last) {
             last = t64;
-            parts = rest * 16;
+            tail = rest * 16;
             best.side = 64;
         }
     } else {
         last = 0.0;
     }
-    const uint64_t tiled = parts ? whole : big;
+    const uint64_t tiled = tail ? whole : big;
     best.chain = !glu && tiled > cus && cdiv(p.K, 128) % 2 == 0;
     const uint64_t chains = best.chain ? cus : tiled;
-    const uint64_t groups = chains + parts;
+    const uint64_t groups = chains + tail;
     consider(K_MIXED, double(whole / cus) * (steps * 1.5 + 7.6) + last, groups * 512);
-    const uint32_t tile = parts && !whole ? 128 : 256;
+    const uint32_t tile = tail && !whole ? 128 : 256;
     best.tiles_m = cdiv(p.M, tile);
     best.tiles_n = cdiv(p.N, tile);
     best.whole = uint32_t(tiled);

@@ -288,9 +288,9 @@ def test_product_small_with_long_k(gpu, m, n, k, epi, c):
     Product(m, n, k, epi, c, batch=2, lda=k + 16, ldc=n + 4, split=5, seg=16).check()
 
 
-# (on 256 compute units: 128 x 128 tiles in one and two rounds; 256 x 256 ones in a partial round; in a whole round and 128 x
+# (on 256 compute units: 64 x 64 tiles; 128 x 128 ones in one and two rounds; 256 x 256 ones in a partial round; in a whole round and 128 x
 # 128 parts, 64 x 64 parts, a partial round; chains of two, of one or two tiles; an odd number of k steps, which is never chained)
-@pytest.mark.parametrize("m, n, k", [(4400, 1028, 176), (2048, 2304, 176), (1537, 4100, 176), (4400, 2304, 176), (4400, 4100, 176),
+@pytest.mark.parametrize("m, n, k", [(4400, 1028, 176), (2048, 2304, 176), (2040, 2044, 336), (1537, 4100, 176), (4400, 2304, 176), (4400, 4100, 176),
                                      (4300, 4096, 176), (4400, 6000, 176), (8300, 4100, 176), (4400, 6000, 80), (8300, 4100, 336)])
 @pytest.mark.parametrize("epi, c", [(M.EPI_STORE, M.BF16), (M.EPI_GEGLU, M.F16), (M.EPI_GATE_TANH, M.F32)])
 def test_product_many_tiles(gpu, m, n, k, epi, c):
