@@ -540,19 +540,18 @@ __device__ inline void locate(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, ui
     tn = i / g;
 }
 
-// waves a SIMD: two where 8 waves share the LDS, or two workgroups of 4 fit it
-template <int BM, int BN, int NW, int NSTG> constexpr int tile_waves()
-{
-    return NW == 8 || tile_lds<BM, BN, NW, NSTG, false>() <= 80 * 1024 ? 2 : 1;
-}
+// A tile a workgroup of 4 waves (one a SIMD), as many workgroups on a CU as its 160 KB of LDS hold. One with stages in flight (64 x
+// 128 of 4) takes a long k fastest; with 2 stages and two or three workgroups on the CU, one's loads, epilogue and stores go on
+// under the others' products, which is what counts over a short k (7431 x 768 x 96 GEGLU 9.7 -> 6.0 us, 896 x 4928 x 176 8.9 -> 6.4,
+// 4400 x 1024 x 384 ADD 14.2 -> 11.2, 1700 x 2560 x 2560 24.4 -> 20.7 with 128 x 128).
+template <int BM, int BN, int NSTG> constexpr int resident() { return 160 * 1024 / tile_lds<BM, BN, 4, NSTG, false>(); }
 
-template <int BM, int BN, int NW, int NSTG, int EC>
-__global__ __launch_bounds__(64 * NW, (tile_waves<BM, BN, NW, NSTG>())) __attribute__((amdgpu_waves_per_eu(
-    tile_waves<BM, BN, NW, NSTG>(), tile_waves<BM, BN, NW, NSTG>()))) void gemm_i8_kernel(I8P p, uint32_t tiles_m,
-                                                                                          uint32_t tiles_n)
+template <int BM, int BN, int NSTG, int EC>
+__global__ __launch_bounds__(256, (resident<BM, BN, NSTG>())) __attribute__((amdgpu_waves_per_eu(
+    resident<BM, BN, NSTG>(), resident<BM, BN, NSTG>()))) void gemm_i8_kernel(I8P p, uint32_t tiles_m, uint32_t tiles_n)
 {
-    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<BM, BN, NW, NSTG, false>()];
-    i8_tiles<BM, BN, NW, NSTG, EC, false>(p, smem, 1, [&](uint32_t, uint32_t& z, int& m0, int& n0) {
+    __shared__ __attribute__((aligned(16))) int8_t smem[tile_lds<BM, BN, 4, NSTG, false>()];
+    i8_tiles<BM, BN, 4, NSTG, EC, false>(p, smem, 1, [&](uint32_t, uint32_t& z, int& m0, int& n0) {
         uint32_t tm, tn;
         locate(xcd_run(blockIdx.x, gridDim.x), tiles_m, tiles_n, z, tm, tn);
         m0 = int(tm) * BM;
@@ -710,32 +709,44 @@ template <int EC> __global__ __launch_bounds__(64 * k16Waves) void gemm_i8_16_ke
     }
 }
 
-template <int BM, int BN, int NW, int NSTG, int EC> mk_status launch_tile(const I8P& p, hipStream_t s)
+template <int BM, int BN, int NSTG, int EC> mk_status launch_tile(const I8P& p, hipStream_t s)
 {
     const uint32_t cols = EC == EC_GLU ? p.N / 2 : p.N, tm = cdiv(p.M, BM), tn = cdiv(cols, EC == EC_GLU ? BN / 2 : BN);
-    gemm_i8_kernel<BM, BN, NW, NSTG, EC><<<tm * tn * p.batch, 64 * NW, 0, s>>>(p, tm, tn);
+    gemm_i8_kernel<BM, BN, NSTG, EC><<<tm * tn * p.batch, 256, 0, s>>>(p, tm, tn);
     MK_LAUNCH_CHECK("gemm_i8");
     return MK_OK;
 }
 
-// The kernel of a launch: the one with the least estimated time in us, beside a launch's own. A tile takes its k steps of
-// 128 at the rate its CU brings operands in (64 x 32: 0.096, 64 x 64: 0.15, 64 x 128: 0.26, 128 x 128: 0.37 a step; 16 x 16 rows
-// 40 bytes a ns, or all weights 5.8 TB/s) or, where all CUs load, at the 19 to 22 TB/s that they take from the L2s together; 256
-// x 256 tiles are bound by the matrix cores (1.5 a step, 7.6 for the pipeline's start and the epilogue, which nothing overlaps;
-// 1.2 and 5.9 where the round is not full and the clock higher). Fitted to the kernels' times at 1020 shapes and epilogues (rows 1 .. 9000, N
-// from 64, K from 128): the choice is within 0.3% of the best in the mean for STORE, 0.9% for GELU and GEGLU, 17% at worst (450 x 176 x
-// 11344: 20.6 us, 17.6). Measured, us, 16 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / mixed: 1 x 4096 x 4096 5.0 / 6.1 / 7.6 /
-// 11 / 14, 1 x 12288 x 4096 12.5 / 10.6 / 9.6 / 11 / 14, 98 x 176 x 11344 9.6 / 19 / 28 / 40 / -, 77 x 2560 x 2048 9.3 / 4.3 / 4.8 / 7.1 /
-// 9.0, 300 x 4096 x 12288 - / 38 / 35 / 29 / 36, 1024 x 4096 x 4096 - / 36 / 27 / 24 / 19.
+// The kernel of a launch: the one with the least estimated time in us, beside a launch's own. A round of tiles, a workgroup
+// of the kernel in every place that a CU has for one, takes so much a k step of 128 and so much beside (a start, an epilogue); the
+// last round has 1, 2 or 3 workgroups on a CU. 16 x 16 rows come at 45 bytes a ns and CU, or all weights at 6.3 TB/s. A round of
+// 256 x 256 tiles is bound by the matrix cores (1.6 a step; 1.2 where it is not full and the clock higher).
+// Fitted to the kernels' times at 1900 shapes and epilogues (rows 1 .. 16000, N from 64, K from 96): the choice is within 0.6% of the
+// best in the mean, 22% at worst. Measured, us, 16 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / the same in 2 stages / 128 x 128 / mixed: 1 x
+// 4096 x 4096 5.0 / 6.1 / 7.6 / 11 / - / - / 14, 98 x 176 x 11344 9.6 / 19 / 28 / 40 / - / - / -, 77 x 2560 x 2048 9.3 / 4.3 / 4.8 / 7.1 / - / - /
+// 9.0, 300 x 4096 x 12288 - / 38 / 35 / 28 / 51 / 56 / 36, 896 x 4928 x 176 GEGLU - / - / 9.0 / 11 / 6.4 / 7.4 / 10, 1700 x 2560 x 2560 - / - /
+// 24 / 26 / 23 / 21 / 25, 1024 x 4096 x 4096 - / 36 / 28 / 24 / 23 / 24 / 19.
 // The mixed kernel's last, partial round takes 128 x 128 parts up to two rounds of them (4352 x 5120 x 4096, 84 tiles left: 91 us
 // against 95 in whole tiles; 1024 x 8192 x 4096, 128: 40 and 44), then whole tiles (1024 x 9216 x 4096, 144: 54 and 44; 4352 x 7168
 // x 4096, 220: 131 and 112); 64 x 64 parts where they fit one round (4352 x 4096 x 12288, 16 left: 185 us, 210 in 128 x 128, 259 whole).
+enum { K_NONE = -1, K_16X16, K_64X32, K_64X64, K_64X128, K_64X128_2, K_128X128_2, K_MIXED };
+struct TileCost {
+    int kernel;
+    uint32_t bm, bn, resident;
+    double step[3], end[3]; // of a round with 1, 2, 3 workgroups on a CU
+};
+constexpr TileCost kTiles[] = {
+    {K_64X32, 64, 32, resident<64, 32, 6>(), {0.084, 0.40, 0}, {0.84, 1.9, 0}},
+    {K_64X64, 64, 64, resident<64, 64, 4>(), {0.132, 0.40, 0}, {0.85, 2.1, 0}},
+    {K_64X128, 64, 128, resident<64, 128, 4>(), {0.295, 0, 0}, {2.4, 0, 0}},
+    {K_64X128_2, 64, 128, resident<64, 128, 2>(), {0.51, 0.57, 0.96}, {0.84, 1.7, 3.7}},
+    {K_128X128_2, 128, 128, resident<128, 128, 2>(), {0.57, 0.88, 0}, {2.3, 4.3, 0}},
+};
 struct Plan {
     int kernel;
     bool chain; // these of the mixed kernel
     uint32_t tiles_m, tiles_n, whole, chains, side, grid;
 };
-enum { K_NONE = -1, K_16X16, K_64X32, K_64X64, K_64X128, K_MIXED };
 
 Plan plan_of(const I8P& p, bool glu, uint32_t cus)
 {
@@ -751,30 +762,28 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
             best.kernel = k;
         }
     };
-    auto small = [&](int k, uint32_t bm, uint32_t bn, double step, double end, double tbs) {
-        const uint64_t n = tiles(bm, bn);
-        consider(k, std::max(rounds(n) * (steps * step + end), double(n) * steps * (bm + bn) * 128 / (tbs * 1e6) * 256 / cus),
-                 n * 256);
-    };
     const uint32_t parts = glu ? 2 : 1; // of the weight
     if (p.M <= 16 * 65535)
         consider(K_16X16,
-                 std::max(rounds(tiles(16, 16 * parts)) * (p.K * (16.0 * parts + std::min(p.M, 16u)) * 2.4e-5 + 0.05),
-                          double(p.N) * p.K * p.batch * 0.172e-6),
+                 std::max(rounds(tiles(16, 16 * parts)) * (p.K * (16.0 * parts + std::min(p.M, 16u)) * 2.2e-5 + 0.16),
+                          double(p.N) * p.K * p.batch * 0.16e-6),
                  uint64_t(cdiv(p.N, 16 * parts)) * 512);
-    if (!glu) // (its two parts are 16 channels of a wave each)
-        small(K_64X32, 64, 32, 0.0957, 0.53, 22.5);
-    small(K_64X64, 64, 64, 0.15, 0.69, 21.4);
-    small(K_64X128, 64, 128, 0.259, 1.6, 19.0);
+    for (const TileCost& c : kTiles) {
+        if (glu && c.kernel == K_64X32) // (its two parts are 16 channels of a wave each)
+            continue;
+        const uint64_t n = tiles(c.bm, c.bn), round = uint64_t(c.resident) * cus, last = (n % round + cus - 1) / cus;
+        auto time = [&](uint64_t w) { return steps * c.step[w - 1] + c.end[w - 1]; };
+        consider(c.kernel, double(n / round) * time(c.resident) + (last ? time(last) : 0.0), n * 256);
+    }
     // whole rounds of 256 x 256 tiles and the rest: as it is, in 128 x 128 parts up to two rounds of them, or in 64 x 64 ones
     // up to one
     const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = big - whole;
-    double last = steps * 1.2 + 5.9;
+    double last = steps * 1.2 + 7.9;
     uint64_t tail = 0;
     best.side = 128;
     if (rest) {
         const uint64_t n128 = whole ? rest * 4 : tiles(128, 128);
-        const double t128 = rounds(n128) * (steps * 0.372 + 2.05), t64 = steps * 0.15 + 0.7;
+        const double t128 = rounds(n128) * (steps * 0.43 + 2.75), t64 = steps * 0.15 + 0.7;
         if (n128 <= 2 * uint64_t(cus) && t128 < last) {
             last = t128;
             tail = n128;
@@ -791,7 +800,7 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
     best.chain = !glu && tiled > cus && cdiv(p.K, 128) % 2 == 0;
     const uint64_t chains = best.chain ? cus : tiled;
     const uint64_t groups = chains + tail;
-    consider(K_MIXED, double(whole / cus) * (steps * 1.5 + 7.6) + last, groups * 512);
+    consider(K_MIXED, double(whole / cus) * (steps * 1.6 + 9.5) + last, groups * 512);
     const uint32_t tile = tail && !whole ? 128 : 256;
     best.tiles_m = cdiv(p.M, tile);
     best.tiles_n = cdiv(p.N, tile);
@@ -811,12 +820,16 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
         break;
     case K_64X32:
         if constexpr (EC != EC_GLU)
-            return launch_tile<64, 32, 4, 6, EC>(p, s);
+            return launch_tile<64, 32, 6, EC>(p, s);
         return fail(MK_ERR_UNSUPPORTED, "gemm_i8: no gated 64 x 32 tiles");
     case K_64X64:
-        return launch_tile<64, 64, 4, 4, EC>(p, s);
+        return launch_tile<64, 64, 4, EC>(p, s);
     case K_64X128:
-        return launch_tile<64, 128, 4, 4, EC>(p, s);
+        return launch_tile<64, 128, 4, EC>(p, s);
+    case K_64X128_2:
+        return launch_tile<64, 128, 2, EC>(p, s);
+    case K_128X128_2:
+        return launch_tile<128, 128, 2, EC>(p, s);
     case K_NONE:
         return fail(MK_ERR_ARG, "gemm_i8: a launch of more than 2^32 threads");
     default:
