@@ -248,8 +248,7 @@ typedef struct mk_gate_norm_args {
 } mk_gate_norm_args;
 /* The vectors, x and x_out are 16-byte aligned, y and out for 4 of their elements, out_scale for one. Apart from x_out == x
  * no output overlaps an input or another output. Infinities and NaNs stay in their row, and a row's bits do not depend on
- * the rows beside it. Allocates nothing and keeps no
- * workspace: it may be captured, and may run on several streams at once. */
+ * the rows beside it. Allocates nothing and keeps no workspace: it may be captured, and may run on several streams at once. */
 mk_status mk_gate_norm(const mk_gate_norm_args* a, void* stream);
 
 /* heads_norm_half / heads_half (qwen_image.cpp:226-250, sdxl.cpp:439-448): per (row, head) of x bf16
@@ -329,7 +328,8 @@ mk_status mk_quantize_fp8_rows(const void* src, uint64_t rows, uint64_t cols, vo
  * scale[r] = a / 127 and dst[r][c] = 127 src[r][c] / a rounded to nearest, ties to even, decided exactly (values in
  * -127 .. 127). A row of a < 2^-100 counts as zero: dst 0, scale 1. A row with an infinity or a NaN: dst 0, scale NaN, so
  * its products are NaN and no other row's are. src f32, bf16 or f16 [rows][ld], dst int8 [rows][cols] (any cols; a multiple
- * of 16 with 16-byte aligned src rows is the fast path). Allocates nothing. No counterpart in the reference. */
+ * of 16 with 16-byte aligned src rows is the fast path). No output overlaps src or the other output. Allocates nothing and
+ * keeps no workspace: it may be captured, and may run on several streams at once. No counterpart in the reference. */
 mk_status mk_quantize_i8_rows(const void* src, uint32_t src_dtype, uint64_t rows, uint64_t cols, int64_t ld, void* dst,
                               float* scale, void* stream);
 /* fp32 <-> bf16 conversions on the device */

@@ -1,11 +1,11 @@
 // proj in 8-bit integers on gfx950: C = epilogue(ascale[r] wscale[n] sum_k A[r][k] W[n][k] + bias[n]), the sums exact in
 // int32 (v_mfma_i32_16x16x64_i8), so their order, and with it the kernel that a launch takes, does not show in a result.
 //
-// What bounds it: up to 16 rows the weight's bytes (1 x 12288 x 4096: 9.7 us, 5.2 TB/s with a launch's own time); tens to
-// hundreds of rows what a CU takes from its L2 (80 to 110 bytes a ns); from about 1000 rows the matrix cores at the clock that the
-// power limit leaves: 8192^3 at 2.6 POP/s with them 68% busy at 1.87 GHz, 32768 x 12288 x 4096 2.4 POP/s with 60% at 1.4 to 1.6 GHz
-// (rocprofv3 counters; no LDS bank conflicts). There neither the waves' priority nor fragments read further ahead
-// changed the time, within 0.5%.
+// What bounds it: up to 16 rows the weight's bytes (1 x 12288 x 4096: 9.5 us, 5.3 TB/s with a launch's own time); tens to
+// hundreds of rows what a CU takes from its L2 (80 to 110 bytes a ns); over a short k the epilogue; from about 1000 rows the
+// matrix cores at the clock that the power limit leaves: 8192^3 at 2.6 POP/s with them 68% busy at 1.87 GHz, 32768 x 12288 x 4096
+// 2.4 POP/s with 60% at 1.4 to 1.6 GHz (rocprofv3 counters; no LDS bank conflicts). There neither the waves' priority nor
+// fragments read further ahead changed the time, within 0.5%.
 #include "common.hpp"
 
 #include <algorithm>
