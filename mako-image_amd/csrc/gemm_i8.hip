@@ -540,7 +540,9 @@ __device__ inline void locate(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, ui
     tn = i / g;
 }
 
-// A tile a workgroup of 4 waves (one a SIMD), as many workgroups on a CU as its 160 KB of LDS hold. One with stages in flight (64 x
+// A tile a workgroup of 4 waves (one a SIMD), as many workgroups on a CU as its 160 KB of LDS hold. Few rows or narrow outputs
+// take small tiles (32 x 32; 32 x 64 for a gated unit), which spread over more CUs: 208 x 1040 x 10288 18 -> 11.7 us, 16 x 4096 x 12288 11.7
+// -> 9.8, 77 x 2560 x 2048 4.3 -> 3.8. One with stages in flight (64 x
 // 128 of 4) takes a long k fastest; with 2 stages and two or three workgroups on the CU, one's loads, epilogue and stores go on
 // under the others' products, which is what counts over a short k (7431 x 768 x 96 GEGLU 9.7 -> 6.0 us, 896 x 4928 x 176 8.9 -> 6.4,
 // 4400 x 1024 x 384 ADD 14.2 -> 11.2, 1700 x 2560 x 2560 24.4 -> 20.7 with 128 x 128).
@@ -719,28 +721,31 @@ template <int BM, int BN, int NSTG, int EC> mk_status launch_tile(const I8P& p, 
 
 // The kernel of a launch: the one with the least estimated time in us, beside a launch's own. A round of tiles, a workgroup
 // of the kernel in every place that a CU has for one, takes so much a k step of 128 and so much beside (a start, an epilogue); the
-// last round has 1, 2 or 3 workgroups on a CU. 16 x 16 rows come at 45 bytes a ns and CU, or all weights at 6.3 TB/s. A round of
-// 256 x 256 tiles is bound by the matrix cores (1.6 a step; 1.2 where it is not full and the clock higher).
-// Fitted to the kernels' times at 1900 shapes and epilogues (rows 1 .. 16000, N from 64, K from 96): the choice is within 0.6% of the
-// best in the mean, 22% at worst. Measured, us, 16 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / the same in 2 stages / 128 x 128 / mixed: 1 x
-// 4096 x 4096 5.0 / 6.1 / 7.6 / 11 / - / - / 14, 98 x 176 x 11344 9.6 / 19 / 28 / 40 / - / - / -, 77 x 2560 x 2048 9.3 / 4.3 / 4.8 / 7.1 / - / - /
-// 9.0, 300 x 4096 x 12288 - / 38 / 35 / 28 / 51 / 56 / 36, 896 x 4928 x 176 GEGLU - / - / 9.0 / 11 / 6.4 / 7.4 / 10, 1700 x 2560 x 2560 - / - /
-// 24 / 26 / 23 / 21 / 25, 1024 x 4096 x 4096 - / 36 / 28 / 24 / 23 / 24 / 19.
+// last round has 1, 2 or 3 workgroups on a CU. 16 x 16 rows come at 48 bytes a ns and CU, or all weights at 6.3 TB/s. A round of
+// 256 x 256 tiles is bound by the matrix cores (1.5 a step; 0.95 where it is not full and the clock higher).
+// Fitted to the kernels' times at 1500 shapes and epilogues (rows 1 .. 16000, N from 64, K from 96): the choice is within 0.7% of the
+// best in the mean, 33% at worst (4000 x 1040 x 10288: 100 us, 76 in 128 x 128 tiles). Measured, us, 16 x 16 / 32 x 32 / 64 x 32 / 64 x 64 / 64
+// x 128 / the same in 2 stages / 128 x 128 / mixed: 1 x 4096 x 4096 5.0 / - / 6.1 / 7.6 / 11 / - / - / 14, 77 x 2560 x 2048 9.3 / 3.9 / 4.3 / 4.8 / 7.1 / -
+// / - / 9.0, 208 x 1040 x 10288 33 / 12 / 18 / 26 / 36 / - / - / -, 130 x 2560 x 2560 16 / 6.0 / 5.2 / 6.1 / 9.1 / - / - / -, 300 x 4096 x 12288 - / 47 /
+// 38 / 35 / 28 / 51 / 56 / 36, 1700 x 2560 x 2560 - / - / - / 24 / 26 / 23 / 21 / 25, 1024 x 4096 x 4096 - / - / 36 / 28 / 24 / 23 / 24 / 19; GEGLU (32 x 64 for
+// 32 x 32) 896 x 4928 x 176 - / - / - / 9.0 / 11 / 6.4 / 7.4 / 10, 300 x 1024 x 4096 18 / 7.1 / - / 8.4 / 12 / - / - / -.
 // The mixed kernel's last, partial round takes 128 x 128 parts up to two rounds of them (4352 x 5120 x 4096, 84 tiles left: 91 us
 // against 95 in whole tiles; 1024 x 8192 x 4096, 128: 40 and 44), then whole tiles (1024 x 9216 x 4096, 144: 54 and 44; 4352 x 7168
 // x 4096, 220: 131 and 112); 64 x 64 parts where they fit one round (4352 x 4096 x 12288, 16 left: 185 us, 210 in 128 x 128, 259 whole).
-enum { K_NONE = -1, K_16X16, K_64X32, K_64X64, K_64X128, K_64X128_2, K_128X128_2, K_MIXED };
+enum { K_NONE = -1, K_16X16, K_32X32, K_32X64, K_64X32, K_64X64, K_64X128, K_64X128_2, K_128X128_2, K_MIXED };
 struct TileCost {
     int kernel;
     uint32_t bm, bn, resident;
     double step[3], end[3]; // of a round with 1, 2, 3 workgroups on a CU
 };
 constexpr TileCost kTiles[] = {
-    {K_64X32, 64, 32, resident<64, 32, 6>(), {0.084, 0.40, 0}, {0.84, 1.9, 0}},
-    {K_64X64, 64, 64, resident<64, 64, 4>(), {0.132, 0.40, 0}, {0.85, 2.1, 0}},
-    {K_64X128, 64, 128, resident<64, 128, 4>(), {0.295, 0, 0}, {2.4, 0, 0}},
-    {K_64X128_2, 64, 128, resident<64, 128, 2>(), {0.51, 0.57, 0.96}, {0.84, 1.7, 3.7}},
-    {K_128X128_2, 128, 128, resident<128, 128, 2>(), {0.57, 0.88, 0}, {2.3, 4.3, 0}},
+    {K_128X128_2, 128, 128, resident<128, 128, 2>(), {0.5, 0.81, 0}, {1.8, 4.4, 0}},
+    {K_64X128_2, 64, 128, resident<64, 128, 2>(), {0.44, 0.53, 0.97}, {0.7, 1.5, 3.4}},
+    {K_64X128, 64, 128, resident<64, 128, 4>(), {0.26, 0, 0}, {2.4, 0, 0}},
+    {K_64X64, 64, 64, resident<64, 64, 4>(), {0.15, 0.35, 0}, {0.66, 2.0, 0}},
+    {K_64X32, 64, 32, resident<64, 32, 6>(), {0.077, 0.25, 0}, {0.64, 1.5, 0}},
+    {K_32X64, 32, 64, resident<32, 64, 6>(), {0.11, 0.25, 0}, {0.48, 1.3, 0}},
+    {K_32X32, 32, 32, resident<32, 32, 8>(), {0.069, 0.115, 0}, {0.65, 0.77, 0}},
 };
 struct Plan {
     int kernel;
@@ -750,7 +755,9 @@ struct Plan {
 
 Plan plan_of(const I8P& p, bool glu, uint32_t cus)
 {
-    const double steps = double(cdiv(p.K, 128));
+    // rows that start inside a cache line (inside a 64-byte half of one) cost the loads 1.2 (1.4) times as much
+    const uint32_t inside = uint32_t(p.K | p.lda) % 128;
+    const double slow = !inside ? 1.0 : inside == 64 ? 1.2 : 1.4, steps = slow * cdiv(p.K, 128);
     auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t(cdiv(p.M, bm)) * cdiv(p.N, bn) * p.batch; };
     auto rounds = [&](uint64_t n) { return double((n + cus - 1) / cus); };
     Plan best{K_NONE, false, 0, 0, 0, 0, 0, 0};
@@ -762,28 +769,33 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
             best.kernel = k;
         }
     };
+    // its bytes from the large cache, whatever the kernel; of kernels that wait for them the largest tile (1 x 12288 x 4096 9.5 us on 64
+    // x 64 tiles, 9.9 on 32 x 32)
+    const double weights = double(p.N) * p.K * p.batch * 0.13e-6;
     const uint32_t parts = glu ? 2 : 1; // of the weight
     if (p.M <= 16 * 65535)
         consider(K_16X16,
-                 std::max(rounds(tiles(16, 16 * parts)) * (p.K * (16.0 * parts + std::min(p.M, 16u)) * 2.2e-5 + 0.16),
-                          double(p.N) * p.K * p.batch * 0.16e-6),
+                 std::max(rounds(tiles(16, 16 * parts)) * (p.K * (16.0 * parts + std::min(p.M, 16u)) * 2.1e-5 + 0.15),
+                          1.25 * weights),
                  uint64_t(cdiv(p.N, 16 * parts)) * 512);
     for (const TileCost& c : kTiles) {
-        if (glu && c.kernel == K_64X32) // (its two parts are 16 channels of a wave each)
+        // (a gated unit's two parts are blocks of 16 channels of a wave: 64 a tile at least)
+        if (glu ? c.bn < 64 : c.kernel == K_32X64)
             continue;
         const uint64_t n = tiles(c.bm, c.bn), round = uint64_t(c.resident) * cus, last = (n % round + cus - 1) / cus;
         auto time = [&](uint64_t w) { return steps * c.step[w - 1] + c.end[w - 1]; };
-        consider(c.kernel, double(n / round) * time(c.resident) + (last ? time(last) : 0.0), n * 256);
+        consider(c.kernel, std::max(double(n / round) * time(c.resident) + (last ? time(last) : 0.0), weights), n * 256);
     }
     // whole rounds of 256 x 256 tiles and the rest: as it is, in 128 x 128 parts up to two rounds of them, or in 64 x 64 ones
     // up to one
     const uint64_t big = tiles(256, 256), whole = big / cus * cus, rest = big - whole;
-    double last = steps * 1.2 + 7.9;
+    const double msteps = (0.6 + 0.4 / slow) * steps;
+    double last = msteps * 0.95 + 7.9;
     uint64_t tail = 0;
     best.side = 128;
     if (rest) {
         const uint64_t n128 = whole ? rest * 4 : tiles(128, 128);
-        const double t128 = rounds(n128) * (steps * 0.43 + 2.75), t64 = steps * 0.15 + 0.7;
+        const double t128 = rounds(n128) * (msteps * 0.43 + 2.4), t64 = msteps * 0.13 + 0.7;
         if (n128 <= 2 * uint64_t(cus) && t128 < last) {
             last = t128;
             tail = n128;
@@ -800,7 +812,7 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
     best.chain = !glu && tiled > cus && cdiv(p.K, 128) % 2 == 0;
     const uint64_t chains = best.chain ? cus : tiled;
     const uint64_t groups = chains + tail;
-    consider(K_MIXED, double(whole / cus) * (steps * 1.6 + 9.5) + last, groups * 512);
+    consider(K_MIXED, double(whole / cus) * (msteps * 1.5 + 9.5) + last, groups * 512);
     const uint32_t tile = tail && !whole ? 128 : 256;
     best.tiles_m = cdiv(p.M, tile);
     best.tiles_n = cdiv(p.N, tile);
@@ -818,10 +830,15 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
         gemm_i8_16_kernel<EC><<<dim3(cdiv(EC == EC_GLU ? p.N / 2 : p.N, 16), p.batch, cdiv(p.M, 16)), 64 * k16Waves, 0,
                                  s>>>(p);
         break;
+    case K_32X32:
     case K_64X32:
         if constexpr (EC != EC_GLU)
-            return launch_tile<64, 32, 6, EC>(p, s);
-        return fail(MK_ERR_UNSUPPORTED, "gemm_i8: no gated 64 x 32 tiles");
+            return plan.kernel == K_32X32 ? launch_tile<32, 32, 8, EC>(p, s) : launch_tile<64, 32, 6, EC>(p, s);
+        return fail(MK_ERR_UNSUPPORTED, "gemm_i8: no gated tiles of 32 channels");
+    case K_32X64:
+        if constexpr (EC == EC_GLU)
+            return launch_tile<32, 64, 6, EC>(p, s);
+        return fail(MK_ERR_UNSUPPORTED, "gemm_i8: 32 x 64 tiles are the gated units'");
     case K_64X64:
         return launch_tile<64, 64, 4, EC>(p, s);
     case K_64X128:

@@ -288,13 +288,14 @@ def test_product_small_with_long_k(gpu, m, n, k, epi, c):
     Product(m, n, k, epi, c, batch=2, lda=k + 16, ldc=n + 4, split=5, seg=16).check()
 
 
-# On 256 compute units: 64 x 32 tiles (64 x 64 for GEGLU), 64 x 64, 64 x 128 in 4 stages and in 2, 128 x 128 in one round, in several;
-# the mixed kernel's 128 x 128 tiles, 256 x 256 ones in a partial round; a whole round and one and two rounds of 128 x 128 parts,
-# 64 x 64 parts; chains and a partial round, 128 x 128 parts, 64 x 64 parts; two whole rounds of an odd number of k steps.
+# On 256 compute units: 32 x 32 (GEGLU: 32 x 64), 64 x 32 and 64 x 64 tiles, 64 x 128 in 4 stages and in 2, 128 x 128; the mixed
+# kernel's 128 x 128 tiles in one and two rounds, 256 x 256 ones in a partial round; a whole round and one and two rounds of 128 x
+# 128 parts, 64 x 64 parts; chains and a partial round, 128 x 128 parts, 64 x 64 parts; two whole rounds of an odd number of k steps.
 @pytest.mark.parametrize("m, n, k", [(257, 516, 336), (150, 3076, 176), (150, 6000, 1040), (150, 6000, 176), (2048, 2304, 176),
                                      (1030, 6000, 176), (8300, 4100, 336), (2040, 1028, 1040), (1537, 8200, 176), (2818, 6000, 592),
                                      (4300, 5124, 2064), (2040, 8200, 176), (6200, 4100, 720), (8300, 4100, 720), (6200, 5124, 2192),
-                                     (8300, 4100, 592)])
+                                     (8300, 4100, 592), (50, 1028, 720), (200, 1040, 4112), (50, 4100, 176), (50, 8200, 176),
+                                     (100, 8200, 1040), (515, 8200, 720)])
 @pytest.mark.parametrize("epi, c", [(M.EPI_STORE, M.BF16), (M.EPI_GELU_TANH, M.F16), (M.EPI_GEGLU, M.F16), (M.EPI_GATE_TANH, M.F32)])
 def test_product_many_tiles(gpu, m, n, k, epi, c):
     n -= n % 8 if epi == M.EPI_GEGLU else 0
