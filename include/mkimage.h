@@ -187,9 +187,9 @@ mk_status mk_conv3x3(const mk_conv_args* a, void* stream);
  *   and ADD (C the fp32 residual). HEADS and PAIR_SUM are MK_ERR_UNSUPPORTED: store q|k|v and pack it with mk_heads.
  * K is a multiple of 16 up to 131056 (the sum of K products of 8 bits fits int32), N of 4 (SWIGLU, GEGLU: of 8), M any;
  * lda and stride_a multiples of 16, ldc, stride_c and gate_alt of 4; A, W, wscale, bias and gate are 16-byte aligned, C
- * for 4 of its elements, ascale for one. (Rows that start at multiples of 128 bytes, so K and lda multiples of 128, are fastest:
- * others cross a cache line in every step of 128, 15 to 40% where the loads bind. Zero columns of A and W up to the next
- * multiple change nothing but that.) C must not overlap an input. Columns N .. ldc - 1 of C are left as they were. A
+ * for 4 of its elements, ascale for one. (Rows that start at multiples of 128 bytes, so K and lda multiples of 128, are
+ * fastest: others cross a cache line in every step of 128, 15 to 40% where the loads bind. Zero columns of A and W up to
+ * the next multiple change nothing but that.) C must not overlap an input. Columns N .. ldc - 1 of C are left as they were. A
  * row's values do not depend on the launch's other rows: integer sums have no order, and the rest is one expression of
  * the row's and the channel's numbers. Allocates nothing and keeps no workspace: it may be captured, and may run on
  * several streams at once. */

@@ -2,10 +2,10 @@
 // int32 (v_mfma_i32_16x16x64_i8), so their order, and with it the kernel that a launch takes, does not show in a result.
 //
 // What bounds it: up to 16 rows the weight's bytes (1 x 12288 x 4096: 9.5 us, 5.3 TB/s with a launch's own time); tens to
-// hundreds of rows what a CU takes from its L2 (80 to 110 bytes a ns); over a short k the epilogue; from about 1000 rows the
-// matrix cores at the clock that the power limit leaves: 8192^3 at 2.6 POP/s with them 68% busy at 1.87 GHz, 32768 x 12288 x 4096
-// 2.4 POP/s with 60% at 1.4 to 1.6 GHz (rocprofv3 counters; no LDS bank conflicts). There neither the waves' priority nor
-// fragments read further ahead changed the time, within 0.5%.
+// hundreds of rows what a CU takes from its L2 (80 to 110 bytes a ns); over a short k the epilogue; from about 1000 rows
+// the matrix cores at the clock that the power limit leaves: 8192^3 at 2.6 POP/s with them 68% busy at 1.87 GHz, 32768 x
+// 12288 x 4096 2.4 POP/s with 60% at 1.4 to 1.6 GHz (rocprofv3 counters; no LDS bank conflicts). There neither the waves'
+// priority nor fragments read further ahead changed the time, within 0.5%.
 #include "common.hpp"
 
 #include <algorithm>
@@ -94,10 +94,11 @@ template <bool GELU> __device__ inline f32x4 act4(const f32x4& v)
         o[e] = GELU ? gelu_tanh_f(v[e]) : silu_f(v[e]);
     return o;
 }
-// g Phi(g), Phi the normal distribution: max(g, 0) - |g| Phi(-|g|). log2 Phi(-z) for z >= 0 is a polynomial of degree 8, fitted here
-// by iterated least squares to Phi's own error on [0, 5.8] (Phi within 2.7e-7, z Phi(-z) within 8.5e-8, Phi(-z) to 8e-5 of itself up
-// to z = 5.5); beyond, it falls faster than Phi does. In a tile's epilogue these instructions run alone: with erf_fit's longer
-// series and its IEEE division 3952 x 10240 x 1280 GEGLU took 79 us, with a rational form (a reciprocal more) 68, so 66.
+// g Phi(g), Phi the normal distribution: max(g, 0) - |g| Phi(-|g|). log2 Phi(-z) for z >= 0 is a polynomial of degree 8,
+// fitted here by iterated least squares to Phi's own error on [0, 5.8] (Phi within 2.7e-7, z Phi(-z) within 8.5e-8, Phi(-z)
+// to 8e-5 of itself up to z = 5.5); beyond, it falls faster than Phi does. In a tile's epilogue these instructions run
+// alone: with erf_fit's longer series and its IEEE division 3952 x 10240 x 1280 GEGLU took 79 us, with a rational form (a
+// reciprocal more) 68, so 66.
 __device__ inline float gelu_erf_f(float g)
 {
     const float z = fabsf(g);
@@ -330,12 +331,13 @@ __device__ __forceinline__ void i8_tiles(const I8P& p, int8_t* smem, uint32_t co
         substep(af1, nb, 0, af0, kl, buf, true);
     };
 
-    // Epilogue: a wave stages ST tokens x up to 64 channels at a time (fp32, times the tokens' scales) in LDS of its own and
-    // reads them back with its lanes along the channels, so that its stores are whole row segments. A wave's LDS operations
-    // complete in order: no barrier. Rows of SC floats, their 16-byte chunks XOR-ed so that 16 rows at a chunk cover all banks.
-    // (32 tokens keep more stores in flight; a chain has LDS for 16, the residual registers.)
+    // Epilogue: a wave stages ST tokens x up to 64 channels at a time (fp32, times the tokens' scales) in LDS of its own
+    // and reads them back with its lanes along the channels, so that its stores are whole row segments. A wave's LDS
+    // operations complete in order: no barrier. Rows of SC floats, their 16-byte chunks XOR-ed so that 16 rows at a chunk
+    // cover all banks. (32 tokens keep more stores in flight; a chain has LDS for 16, the residual registers.)
     constexpr int WO = GLU ? WC / 2 : WC, SC = epi_channels(BN, GLU), NH = WO / SC; // channels a wave writes, stages at a time
-    constexpr int ST = CHAIN || EC == EC_RMW || WM < 32 ? 16 : 32, NCH = SC / 4, RPI = 64 / NCH, NI = ST / RPI; // chunks a row, rows an instruction, a lane
+    constexpr int ST = CHAIN || EC == EC_RMW || WM < 32 ? 16 : 32;
+    constexpr int NCH = SC / 4, RPI = 64 / NCH, NI = ST / RPI; // chunks a row, rows an instruction, rows a lane
     auto epilogue = [&](uint32_t ez, int em0, int en0) __attribute__((always_inline)) {
         const int lane = here(), r16 = lane & 15, g4 = lane >> 4;
         float* st = reinterpret_cast<float*>(smem + (CHAIN ? NSTG * (BM + BN) * 128 : 0)) + wave * ST * SC;
@@ -540,12 +542,12 @@ __device__ inline void locate(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, ui
     tn = i / g;
 }
 
-// A tile a workgroup of 4 waves (one a SIMD), as many workgroups on a CU as its 160 KB of LDS hold. Few rows or narrow outputs
-// take small tiles (32 x 32; 32 x 64 for a gated unit), which spread over more CUs: 208 x 1040 x 10288 18 -> 11.7 us, 16 x 4096 x 12288 11.7
-// -> 9.8, 77 x 2560 x 2048 4.3 -> 3.8. One with stages in flight (64 x
-// 128 of 4) takes a long k fastest; with 2 stages and two or three workgroups on the CU, one's loads, epilogue and stores go on
-// under the others' products, which is what counts over a short k (7431 x 768 x 96 GEGLU 9.7 -> 6.0 us, 896 x 4928 x 176 8.9 -> 6.4,
-// 4400 x 1024 x 384 ADD 14.2 -> 11.2, 1700 x 2560 x 2560 24.4 -> 20.7 with 128 x 128).
+// A tile a workgroup of 4 waves (one a SIMD), as many workgroups on a CU as its 160 KB of LDS hold. Few rows or narrow
+// outputs take small tiles (32 x 32; 32 x 64 for a gated unit), which spread over more CUs: 208 x 1040 x 10288 18 -> 11.7
+// us, 16 x 4096 x 12288 11.7 -> 9.8, 77 x 2560 x 2048 4.3 -> 3.8. One with stages in flight (64 x 128 of 4) takes a long k
+// fastest; with 2 stages and two or three workgroups on the CU, one's loads, epilogue and stores go on under the others'
+// products, which is what counts over a short k (7431 x 768 x 96 GEGLU 9.7 -> 6.0 us, 896 x 4928 x 176 8.9 -> 6.4, 4400 x
+// 1024 x 384 ADD 14.2 -> 11.2, 1700 x 2560 x 2560 24.4 -> 20.7 with 128 x 128).
 template <int BM, int BN, int NSTG> constexpr int resident() { return 160 * 1024 / tile_lds<BM, BN, 4, NSTG, false>(); }
 
 template <int BM, int BN, int NSTG, int EC>
@@ -563,8 +565,9 @@ __global__ __launch_bounds__(256, (resident<BM, BN, NSTG>())) __attribute__((amd
 
 // 256 x 256 tiles, the first `whole` of them in `chains` workgroups (CHAIN: one a compute unit, which go from tile to tile;
 // else as many as tiles), the rest in parts of side x side (128 or 64) a workgroup: whole rounds of the chip take the large
-// tile, the last, partial one spreads over all of it. A chain saves 1.8 us a tile (32768 x 12288 x 4096 1343 -> 1298 us) where the number of k
-// steps is even; the gated epilogues have no registers for it (4352 x 24576 x 4096 SwiGLU 372 -> 398).
+// tile, the last, partial one spreads over all of it. A chain saves 1.8 us a tile (32768 x 12288 x 4096 1343 -> 1298 us)
+// where the number of k steps is even; the gated epilogues have no registers for it (4352 x 24576 x 4096 SwiGLU 372 ->
+// 398).
 template <int EC, bool CHAIN>
 __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_mixed_kernel(
     I8P p, uint32_t tiles_m, uint32_t tiles_n, uint32_t whole, uint32_t chains, uint32_t side)
@@ -608,11 +611,12 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// 16 rows x 16 channels a workgroup, its 8 waves every eighth 256 bytes of k each, straight from memory to registers: for few
-// rows (up to 16 read the weight once) and for small products of long k, whose few larger tiles leave the chip idle. The
-// rows of an operand lie in 64-byte pieces of 16 rows a load, which brings 40 to 60 bytes a ns and CU, half of what the direct
-// loads of a tile do. The sums meet in LDS. Up to 16 rows bound by the weight's bytes: 1 x 4096 x 4096 5.0 us, 1 x 4096 x 12288 9.9
-// us, a launch alone 3; 98 x 176 x 11344 9.6 us, on 64 x 32 tiles 19.4. 4 or 16 waves, 128 or 512 bytes a turn: within 15%.
+// 16 rows x 16 channels a workgroup, its 8 waves every eighth 256 bytes of k each, straight from memory to registers: for
+// few rows (up to 16 read the weight once) and for small products of long k, whose few larger tiles leave the chip idle.
+// The rows of an operand lie in 64-byte pieces of 16 rows a load, which brings 40 to 60 bytes a ns and CU, half of what the
+// direct loads of a tile do. The sums meet in LDS. Up to 16 rows bound by the weight's bytes: 1 x 4096 x 4096 5.0 us, 1 x
+// 4096 x 12288 9.9 us, a launch alone 3; 98 x 176 x 11344 9.6 us, on 64 x 32 tiles 19.4. 4 or 16 waves, 128 or 512 bytes a
+// turn: within 15%.
 // ------------------------------------------------------------------------------------------------------------
 constexpr int k16Waves = 8;
 
@@ -720,18 +724,25 @@ template <int BM, int BN, int NSTG, int EC> mk_status launch_tile(const I8P& p, 
 }
 
 // The kernel of a launch: the one with the least estimated time in us, beside a launch's own. A round of tiles, a workgroup
-// of the kernel in every place that a CU has for one, takes so much a k step of 128 and so much beside (a start, an epilogue); the
-// last round has 1, 2 or 3 workgroups on a CU. 16 x 16 rows come at 48 bytes a ns and CU, or all weights at 6.3 TB/s. A round of
-// 256 x 256 tiles is bound by the matrix cores (1.5 a step; 0.95 where it is not full and the clock higher).
-// Fitted to the kernels' times at 1500 shapes and epilogues (rows 1 .. 16000, N from 64, K from 96): the choice is within 0.7% of the
-// best in the mean, 33% at worst (4000 x 1040 x 10288: 100 us, 76 in 128 x 128 tiles). Measured, us, 16 x 16 / 32 x 32 / 64 x 32 / 64 x 64 / 64
-// x 128 / the same in 2 stages / 128 x 128 / mixed: 1 x 4096 x 4096 5.0 / - / 6.1 / 7.6 / 11 / - / - / 14, 77 x 2560 x 2048 9.3 / 3.9 / 4.3 / 4.8 / 7.1 / -
-// / - / 9.0, 208 x 1040 x 10288 33 / 12 / 18 / 26 / 36 / - / - / -, 130 x 2560 x 2560 16 / 6.0 / 5.2 / 6.1 / 9.1 / - / - / -, 300 x 4096 x 12288 - / 47 /
-// 38 / 35 / 28 / 51 / 56 / 36, 1700 x 2560 x 2560 - / - / - / 24 / 26 / 23 / 21 / 25, 1024 x 4096 x 4096 - / - / 36 / 28 / 24 / 23 / 24 / 19; GEGLU (32 x 64 for
-// 32 x 32) 896 x 4928 x 176 - / - / - / 9.0 / 11 / 6.4 / 7.4 / 10, 300 x 1024 x 4096 18 / 7.1 / - / 8.4 / 12 / - / - / -.
-// The mixed kernel's last, partial round takes 128 x 128 parts up to two rounds of them (4352 x 5120 x 4096, 84 tiles left: 91 us
-// against 95 in whole tiles; 1024 x 8192 x 4096, 128: 40 and 44), then whole tiles (1024 x 9216 x 4096, 144: 54 and 44; 4352 x 7168
-// x 4096, 220: 131 and 112); 64 x 64 parts where they fit one round (4352 x 4096 x 12288, 16 left: 185 us, 210 in 128 x 128, 259 whole).
+// of the kernel in every place that a CU has for one, takes so much a k step of 128 and so much beside (a start, an
+// epilogue); the last round has 1, 2 or 3 workgroups on a CU. 16 x 16 rows come at 48 bytes a ns and CU, or all weights at
+// 6.3 TB/s. A round of 256 x 256 tiles is bound by the matrix cores (1.5 a step; 0.95 where it is not full and the clock
+// higher). Fitted to the kernels' times at 1500 shapes and epilogues (rows 1 .. 16000, N from 64, K from 96): the choice is
+// within 0.7% of the best in the mean, 33% at worst (4000 x 1040 x 10288: 100 us, 76 in 128 x 128 tiles). Measured, us:
+//                             16x16  32x32  64x32  64x64  64x128  64x128, 2 stages  128x128  mixed
+//   1 x 4096 x 4096             5.0           6.1    7.6      11                                14
+//   77 x 2560 x 2048            9.3    3.9    4.3    4.8     7.1                               9.0
+//   208 x 1040 x 10288           33     12     18     26      36
+//   130 x 2560 x 2560            16    6.0    5.2    6.1     9.1
+//   300 x 4096 x 12288                  47     38     35      28                51       56     36
+//   1700 x 2560 x 2560                                24      26                23       21     25
+//   1024 x 4096 x 4096                         36     28      24                23       24     19
+//   896 x 4928 x 176 GEGLU                           9.0      11               6.4      7.4     10
+//   300 x 1024 x 4096 GEGLU      18    7.1 (32x64)   8.4      12
+// The mixed kernel's last, partial round takes 128 x 128 parts up to two rounds of them (4352 x 5120 x 4096, 84 tiles left:
+// 91 us against 95 in whole tiles; 1024 x 8192 x 4096, 128: 40 and 44), then whole tiles (1024 x 9216 x 4096, 144: 54 and
+// 44; 4352 x 7168 x 4096, 220: 131 and 112); 64 x 64 parts where they fit one round (4352 x 4096 x 12288, 16 left: 185 us,
+// 210 in 128 x 128, 259 whole).
 enum { K_NONE = -1, K_16X16, K_32X32, K_32X64, K_64X32, K_64X64, K_64X128, K_64X128_2, K_128X128_2, K_MIXED };
 struct TileCost {
     int kernel;
@@ -769,8 +780,8 @@ Plan plan_of(const I8P& p, bool glu, uint32_t cus)
             best.kernel = k;
         }
     };
-    // its bytes from the large cache, whatever the kernel; of kernels that wait for them the largest tile (1 x 12288 x 4096 9.5 us on 64
-    // x 64 tiles, 9.9 on 32 x 32)
+    // its bytes from the large cache, whatever the kernel; of kernels that wait for them the largest tile (1 x 12288 x 4096
+    // 9.5 us on 64 x 64 tiles, 9.9 on 32 x 32)
     const double weights = double(p.N) * p.K * p.batch * 0.13e-6;
     const uint32_t parts = glu ? 2 : 1; // of the weight
     if (p.M <= 16 * 65535)

@@ -78,7 +78,8 @@ def quantize(bits, dt, rows, cols, ld, stream=None, offset=0):
 @pytest.mark.parametrize("rows, cols, pad, offset", [
     (1, 1, 0, 0), (1, 16, 0, 0), (3, 5, 2, 0), (2, 64, 0, 0), (7, 1000, 0, 0), (5, 4096, 0, 0), (300, 272, 16, 0),
     (4, 12288, 0, 0), (3, 16400, 0, 0), (5, 1536, 0, 0), (3, 1552, 16, 0), (3, 3056, 0, 0),
-    (2, 8192, 0, 0), (2, 24576, 0, 0), (1, 65536, 0, 0), (1, 65552, 0, 0), (2, 40000, 0, 0), (2, 33333, 3, 0), (9, 256, 0, 1), (2, 1024, 8, 4), (1100, 80, 0, 0)])
+    (2, 8192, 0, 0), (2, 24576, 0, 0), (1, 65536, 0, 0), (1, 65552, 0, 0), (2, 40000, 0, 0),
+    (2, 33333, 3, 0), (9, 256, 0, 1), (2, 1024, 8, 4), (1100, 80, 0, 0)])
 def test_quantize_rows_equal_the_definition(gpu, dt, rows, cols, pad, offset):
     rng = np.random.default_rng(rows * 7 + cols)
     x = rng.standard_normal((rows, cols + pad)) * np.exp(rng.standard_normal((rows, 1)) * 3)
