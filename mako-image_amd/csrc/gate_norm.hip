@@ -309,11 +309,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gate_norm_kernel(mk_gat
     });
 }
 
-template <int W, int NV = 1> void launch_gate_norm(const mk_gate_norm_args& g, hipStream_t s)
+// NV .. MOST: the float4s a thread that the rows of W waves need
+template <int W, int NV, int MOST> void launch_gate_norm(const mk_gate_norm_args& g, hipStream_t s)
 {
-    if constexpr (NV < 4) {
+    if constexpr (NV < MOST) {
         if (g.n > uint32_t(NV) * 256 * W)
-            return launch_gate_norm<W, NV + 1>(g, s);
+            return launch_gate_norm<W, NV + 1, MOST>(g, s);
     }
     gate_norm_kernel<W, NV><<<grid_of(W == 1 ? cdiv(g.rows, 4) : g.rows), W == 1 ? 256 : 64 * W, 0, s>>>(g);
 }
@@ -394,12 +395,13 @@ __global__ __launch_bounds__(256) void quantize_i8_any_kernel(const void* src, u
         scale[r] = q.scale;
 }
 
-template <uint32_t T, int W, int NV = 1>
+// NV .. MOST: the turns of 8 elements a thread that the rows of W waves need
+template <uint32_t T, int W, int NV, int MOST>
 void launch_quantize(const void* src, uint32_t rows, uint32_t cols, int64_t ld, int8_t* dst, float* scale, hipStream_t s)
 {
-    if constexpr (NV < (W == 16 ? 8 : 3)) {
+    if constexpr (NV < MOST) {
         if (cols > uint32_t(NV) * 512 * W)
-            return launch_quantize<T, W, NV + 1>(src, rows, cols, ld, dst, scale, s);
+            return launch_quantize<T, W, NV + 1, MOST>(src, rows, cols, ld, dst, scale, s);
     }
     quantize_i8_kernel<T, W, NV><<<grid_of(W == 1 ? cdiv(rows, 4) : rows), W == 1 ? 256 : 64 * W, 0, s>>>(
         src, rows, cols / 8, ld, dst, scale);
@@ -416,15 +418,15 @@ void quantize_rows(const void* src, uint32_t rows, uint64_t cols, int64_t ld, in
     // us; 4352 x 1280: 6.1 / 5.8 / 7.6 / 9.1; 4352 x 12288, 4 / 8 / 16: 32.9 / 30.7 / 30.0)
     const uint32_t n = uint32_t(cols), waves = cdiv(n, 1536);
     if (waves <= 1)
-        launch_quantize<T, 1>(src, rows, n, ld, dst, scale, s);
+        launch_quantize<T, 1, 1, 3>(src, rows, n, ld, dst, scale, s);
     else if (waves <= 2)
-        launch_quantize<T, 2>(src, rows, n, ld, dst, scale, s);
+        launch_quantize<T, 2, 2, 3>(src, rows, n, ld, dst, scale, s);
     else if (waves <= 4)
-        launch_quantize<T, 4>(src, rows, n, ld, dst, scale, s);
+        launch_quantize<T, 4, 2, 3>(src, rows, n, ld, dst, scale, s);
     else if (waves <= 8)
-        launch_quantize<T, 8>(src, rows, n, ld, dst, scale, s);
+        launch_quantize<T, 8, 2, 3>(src, rows, n, ld, dst, scale, s);
     else
-        launch_quantize<T, 16>(src, rows, n, ld, dst, scale, s);
+        launch_quantize<T, 16, 2, 8>(src, rows, n, ld, dst, scale, s);
 }
 
 void launch_rows(const mk_gate_norm_args& g, hipStream_t s)
@@ -434,15 +436,15 @@ void launch_rows(const mk_gate_norm_args& g, hipStream_t s)
     // 2560 - / 65 / 62 / 69), fewer hold too few rows' loads in flight (32768 x 4096 - / - / 303 / 298 / 355, 9000 x 8192 - / - / - /
     // 171 / 179) and take longer over a single one (1 x 4096 - / - / 5.1 / 3.9 / 3.4).
     if (g.n <= 512)
-        launch_gate_norm<1>(g, s);
+        launch_gate_norm<1, 1, 2>(g, s);
     else if (g.n <= 1536)
-        launch_gate_norm<2>(g, s);
+        launch_gate_norm<2, 2, 3>(g, s);
     else if (g.n <= 3328)
-        launch_gate_norm<4>(g, s);
+        launch_gate_norm<4, 2, 4>(g, s);
     else if (g.n <= 8192)
-        launch_gate_norm<8>(g, s);
+        launch_gate_norm<8, 2, 4>(g, s);
     else
-        launch_gate_norm<16>(g, s);
+        launch_gate_norm<16, 3, 4>(g, s);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
