@@ -194,6 +194,11 @@ mk_status mk_conv3x3(const mk_conv_args* a, void* stream);
  * the row's and the channel's numbers. Allocates nothing and keeps no workspace: it may be captured, and may run on
  * several streams at once. */
 mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void* stream);
+/* The plan of a mk_gemm_i8 launch on a device of cus compute units, without running it (host only; a test hook): out[0] x
+ * out[1] rows of A x rows of W a tile, out[2] steps of 128 k that a workgroup keeps in LDS (0: it takes its operands straight
+ * from memory), out[3] workgroups that go from tile to tile (0: each makes one), out[4] the side of the parts that a last,
+ * partial round of 256 x 256 tiles is cut into (0: whole tiles), out[5] workgroups. No counterpart in the reference. */
+mk_status mk_gemm_i8_plan(const mk_gemm_args* a, uint32_t cus, uint32_t* out);
 
 /* GEMV for a few rows (the time embedding and modulation projections, rows <= 4):
  * y[r][n] = sum_k W[n][k] bf16(x'[r][k]) + b[n] with x' = silu(x) when silu_x (silu(temb) is the modulation

@@ -746,17 +746,17 @@ template <int BM, int BN, int NSTG, int EC> mk_status launch_tile(const I8P& p, 
 enum { K_NONE = -1, K_16X16, K_32X32, K_32X64, K_64X32, K_64X64, K_64X128, K_64X128_2, K_128X128_2, K_MIXED };
 struct TileCost {
     int kernel;
-    uint32_t bm, bn, resident;
+    uint32_t bm, bn, stages, resident;
     double step[3], end[3]; // of a round with 1, 2, 3 workgroups on a CU
 };
 constexpr TileCost kTiles[] = {
-    {K_128X128_2, 128, 128, resident<128, 128, 2>(), {0.5, 0.81, 0}, {1.8, 4.4, 0}},
-    {K_64X128_2, 64, 128, resident<64, 128, 2>(), {0.44, 0.53, 0.97}, {0.7, 1.5, 3.4}},
-    {K_64X128, 64, 128, resident<64, 128, 4>(), {0.26, 0, 0}, {2.4, 0, 0}},
-    {K_64X64, 64, 64, resident<64, 64, 4>(), {0.15, 0.35, 0}, {0.66, 2.0, 0}},
-    {K_64X32, 64, 32, resident<64, 32, 6>(), {0.077, 0.25, 0}, {0.64, 1.5, 0}},
-    {K_32X64, 32, 64, resident<32, 64, 6>(), {0.11, 0.25, 0}, {0.48, 1.3, 0}},
-    {K_32X32, 32, 32, resident<32, 32, 8>(), {0.069, 0.115, 0}, {0.65, 0.77, 0}},
+    {K_128X128_2, 128, 128, 2, resident<128, 128, 2>(), {0.5, 0.81, 0}, {1.8, 4.4, 0}},
+    {K_64X128_2, 64, 128, 2, resident<64, 128, 2>(), {0.44, 0.53, 0.97}, {0.7, 1.5, 3.4}},
+    {K_64X128, 64, 128, 4, resident<64, 128, 4>(), {0.26, 0, 0}, {2.4, 0, 0}},
+    {K_64X64, 64, 64, 4, resident<64, 64, 4>(), {0.15, 0.35, 0}, {0.66, 2.0, 0}},
+    {K_64X32, 64, 32, 6, resident<64, 32, 6>(), {0.077, 0.25, 0}, {0.64, 1.5, 0}},
+    {K_32X64, 32, 64, 6, resident<32, 64, 6>(), {0.11, 0.25, 0}, {0.48, 1.3, 0}},
+    {K_32X32, 32, 32, 8, resident<32, 32, 8>(), {0.069, 0.115, 0}, {0.65, 0.77, 0}},
 };
 struct Plan {
     int kernel;
@@ -894,13 +894,8 @@ mk_status compute_units(uint32_t& n)
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-} // namespace
-
-} // namespace mk
-
-using namespace mk;
-
-extern "C" mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void* stream)
+// The checks of a call's arguments, and the kernels' (an empty product's, M or batch 0, too).
+mk_status prepare(const mk_gemm_args* a, const float* ascale, I8P& p)
 {
     if (!a || !a->a || !a->w || !a->c || !a->wscale || !ascale)
         return fail(MK_ERR_ARG, "gemm_i8: null argument (A, W, C, ascale and wscale are required)");
@@ -932,30 +927,49 @@ extern "C" mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void
         (gated && (!aligned(a->gate, 16) || a->gate_alt % 4)))
         return fail(MK_ERR_ARG, "gemm_i8: A, W, wscale, bias and gate must be 16-byte aligned, C for 4 elements, gate_alt a "
                                 "multiple of 4");
-    if (!a->M || !a->batch)
+    if (!a->M || !a->batch) {
+        p = {};
         return MK_OK;
+    }
     if (a->M > 0x7fffff00u || a->N > 0x7fffff00u || a->batch > 65535)
         return fail(MK_ERR_ARG, "gemm_i8: more than 2^31 - 256 rows or channels or 65535 batch items");
-    const I8P p{static_cast<const int8_t*>(a->a),
-                static_cast<const int8_t*>(a->w),
-                ascale,
-                a->wscale,
-                a->bias,
-                gated ? a->gate : nullptr,
-                a->c,
-                a->lda,
-                a->ldc,
-                a->batch > 1 ? a->stride_a : 0,
-                a->batch > 1 ? a->stride_c : 0,
-                a->gate_alt,
-                a->M,
-                a->N,
-                a->K,
-                a->batch,
-                a->split,
-                a->seg_rows ? a->seg_rows : 0xffffffffu,
-                a->epilogue,
-                a->c_dtype};
+    p = {static_cast<const int8_t*>(a->a),
+         static_cast<const int8_t*>(a->w),
+         ascale,
+         a->wscale,
+         a->bias,
+         gated ? a->gate : nullptr,
+         a->c,
+         a->lda,
+         a->ldc,
+         a->batch > 1 ? a->stride_a : 0,
+         a->batch > 1 ? a->stride_c : 0,
+         a->gate_alt,
+         a->M,
+         a->N,
+         a->K,
+         a->batch,
+         a->split,
+         a->seg_rows ? a->seg_rows : 0xffffffffu,
+         a->epilogue,
+         a->c_dtype};
+    return MK_OK;
+}
+
+} // namespace
+
+} // namespace mk
+
+using namespace mk;
+
+extern "C" {
+
+mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void* stream)
+{
+    I8P p;
+    MK_TRY(prepare(a, ascale, p));
+    if (!p.M)
+        return MK_OK;
     hipStream_t s = static_cast<hipStream_t>(stream);
     uint32_t n = 0;
     MK_TRY(compute_units(n));
@@ -966,3 +980,37 @@ extern "C" mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void
     default: return launch<EC_RMW>(p, n, s);
     }
 }
+
+mk_status mk_gemm_i8_plan(const mk_gemm_args* a, uint32_t cus, uint32_t* out)
+{
+    if (!a || !out || !cus)
+        return fail(MK_ERR_ARG, "gemm_i8_plan: null argument or no compute units");
+    I8P p;
+    MK_TRY(prepare(a, a->wscale, p));
+    if (!p.M)
+        return fail(MK_ERR_ARG, "gemm_i8_plan: empty product");
+    const bool glu = epi_class(p.epi) == EC_GLU;
+    const Plan plan = plan_of(p, glu, cus);
+    if (plan.kernel == K_NONE)
+        return fail(MK_ERR_ARG, "gemm_i8: a launch of more than 2^32 threads");
+    uint32_t o[6] = {16, glu ? 32u : 16u, 0, 0, 0, 0};
+    for (const TileCost& c : kTiles)
+        if (c.kernel == plan.kernel) {
+            o[0] = c.bm;
+            o[1] = c.bn;
+            o[2] = c.stages;
+        }
+    if (plan.kernel == K_MIXED) {
+        o[0] = o[1] = plan.whole ? 256 : 128;
+        o[2] = plan.whole ? 2 : 4;
+        o[3] = plan.chain ? plan.chains : 0;
+        o[4] = plan.whole && plan.grid > plan.chains ? plan.side : 0;
+        o[5] = plan.grid;
+    } else {
+        o[5] = cdiv(p.M, o[0]) * cdiv(p.N, o[1]) * p.batch;
+    }
+    std::copy(o, o + 6, out);
+    return MK_OK;
+}
+
+} // extern "C"

@@ -98,6 +98,7 @@ _SIGS = {
     "mk_gemm": (_i, [C.POINTER(GemmArgs), _vp]),
     "mk_gemm_grouped": (_i, [_vp, _u32, _vp]),
     "mk_gemm_i8": (_i, [C.POINTER(GemmArgs), _vp, _vp]),
+    "mk_gemm_i8_plan": (_i, [C.POINTER(GemmArgs), _u32, C.POINTER(_u32)]),
     "mk_gate_norm": (_i, [C.POINTER(GateNormArgs), _vp]),
     "mk_quantize_i8_rows": (_i, [_vp, _u32, _u64, _u64, _i64, _vp, _vp, _vp]),
     "mk_gemm_set_wait_limit": (_i, [_u32]),
