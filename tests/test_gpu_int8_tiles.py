@@ -1,0 +1,25 @@
+"""Every kernel of mk_gemm_i8 where its loops, batches and rows can go wrong, each shape checked to take the kernel it is
+meant for; tolerances are test_gpu_int8_ops.py's."""
+import pytest
+
+import mkimage as M
+from test_gpu_int8_ops import Product
+from test_int8_kernels import kind, kinds
+
+pytestmark = pytest.mark.gpu
+
+# tile: (m, n, k steps). The steps pass what a workgroup keeps in LDS and leave every remainder of it to the loop's end, so
+# that loads made inside the loop are used and each stage is loaded again.
+STEPS = {(32, 32, 8): (50, 1032, range(9, 17)), (64, 32, 6): (37, 4104, range(7, 13)), (32, 64, 6): (50, 2056, range(7, 13)),
+         (64, 64, 4): (37, 8200, range(5, 9)), (64, 128, 4): (100, 8200, range(7, 11)), (64, 128, 2): (100, 8200, range(3, 7)),
+         (128, 128, 2): (1537, 4104, range(3, 6)), (128, 128, 4): (200, 8200, range(5, 9)),
+         (256, "one", 0): (900, 8200, range(5, 7)), (256, "one", 128): (3100, 5128, (4, 5)),
+         (256, "chain", 0): (3100, 8200, (4,)), (256, "chain", 128): (4300, 8200, (4,))}
+
+
+@pytest.mark.parametrize("epi, tile, m, n, ke", [
+    (epi, t, m, n, ke) for epi in (M.EPI_STORE, M.EPI_SWIGLU) for t, (m, n, kes) in STEPS.items() for ke in kes if t in kinds(epi)])
+def test_product_loops_past_the_stages(gpu, epi, tile, m, n, ke):
+    k = 128 * ke - 48  # the last step is partial
+    assert kind(m, n, k, epi) == tile
+    Product(m, n, k, epi).check()
