@@ -4,7 +4,7 @@ import pytest
 
 import mkimage as M
 from test_gpu_int8_ops import Product
-from test_int8_kernels import kind, kinds
+from test_int8_kernels import GLU, SHAPES, kind, kinds
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +23,17 @@ def test_product_loops_past_the_stages(gpu, epi, tile, m, n, ke):
     k = 128 * ke - 48  # the last step is partial
     assert kind(m, n, k, epi) == tile
     Product(m, n, k, epi).check()
+
+
+# Every epilogue on every kernel, three batch items in padded rows of A and C, a split inside each item's segments: chains go
+# on from one item to the next, and so do the parts of the last round.
+EPILOGUES = [(M.EPI_STORE, M.BF16), (M.EPI_GELU_TANH, M.F32), (M.EPI_SILU, M.F16), (M.EPI_ADD, M.F32), (M.EPI_GATE_ADD, M.F32),
+             (M.EPI_GATE_TANH, M.F32), (M.EPI_SWIGLU, M.BF16), (M.EPI_GEGLU, M.F32)]
+
+
+@pytest.mark.parametrize("epi, c, tile", [(epi, c, tile) for epi, c in EPILOGUES for tile in kinds(epi)])
+def test_product_batches_on_every_kernel(gpu, epi, c, tile):
+    m, n, k = SHAPES[tile]
+    assert kind(m, n, k, epi, batch=3, lda=k + 16) == tile
+    cols = n // 2 if epi in GLU else n
+    Product(m, n, k, epi, c, batch=3, lda=k + 16, ldc=cols + 4, split=m // 3, seg=m // 2 + 1).check()
