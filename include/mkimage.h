@@ -191,7 +191,8 @@ mk_status mk_conv3x3(const mk_conv_args* a, void* stream);
  * fastest: others cross a cache line in every step of 128, 15 to 40% where the loads bind. Zero columns of A and W up to
  * the next multiple change nothing but that.) C must not overlap an input. Columns N .. ldc - 1 of C are left as they were. A
  * row's values do not depend on the launch's other rows: integer sums have no order, and the rest is one expression of
- * the row's and the channel's numbers. Allocates nothing and keeps no workspace: it may be captured, and may run on
+ * the row's and the channel's numbers. GEGLU's g Phi(g), Phi the normal distribution, has Phi within 2.7e-7 (mk_gemm's: 6e-8)
+ * and |g| Phi(-|g|) within 9e-8, for f32 outputs too. Allocates nothing and keeps no workspace: it may be captured, and may run on
  * several streams at once. */
 mk_status mk_gemm_i8(const mk_gemm_args* a, const float* ascale, void* stream);
 /* The plan of a mk_gemm_i8 launch on a device of cus compute units, without running it (host only; a test hook): out[0] x

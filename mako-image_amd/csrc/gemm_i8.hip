@@ -2,10 +2,12 @@
 // int32 (v_mfma_i32_16x16x64_i8), so their order, and with it the kernel that a launch takes, does not show in a result.
 //
 // What bounds it: up to 16 rows the weight's bytes (1 x 12288 x 4096: 9.5 us, 5.3 TB/s with a launch's own time); tens to
-// hundreds of rows what a CU takes from its L2 (80 to 110 bytes a ns); over a short k the epilogue; from about 1000 rows
-// the matrix cores at the clock that the power limit leaves: 8192^3 at 2.6 POP/s with them 68% busy at 1.87 GHz, 32768 x
-// 12288 x 4096 2.4 POP/s with 60% at 1.4 to 1.6 GHz (rocprofv3 counters; no LDS bank conflicts). There neither the waves'
-// priority nor fragments read further ahead changed the time, within 0.5%.
+// hundreds of rows what a CU takes from its L2 (80 to 110 bytes a ns); over a short k the epilogue, and most of all the fp32
+// residual's, 8 bytes an output with no product under them (4400 x 8192 x 2048 ADD 148 us, STORE 72); from about 2000 rows the
+// matrix cores at the clock that lasting load leaves: 8192^3 415 us (2.65 POP/s) with them 69% busy at 1.83 GHz, some launches
+// later 484 us (2.27), 75% at 1.44 GHz; 32768 x 12288 x 4096 1296 us (2.54), 64% at 1.89 GHz, and 1636 us (2.02), 73% at 1.32
+// GHz (rocprofv3 counters, each time from the launch that was counted; no LDS bank conflicts in the 256 x 256 tiles). There
+// neither the waves' priority nor fragments read further ahead changed the time, within 0.5%.
 #include "common.hpp"
 
 #include <algorithm>
@@ -543,11 +545,11 @@ __device__ inline void locate(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, ui
 }
 
 // A tile a workgroup of 4 waves (one a SIMD), as many workgroups on a CU as its 160 KB of LDS hold. Few rows or narrow
-// outputs take small tiles (32 x 32; 32 x 64 for a gated unit), which spread over more CUs: 208 x 1040 x 10288 18 -> 11.7
-// us, 16 x 4096 x 12288 11.7 -> 9.8, 77 x 2560 x 2048 4.3 -> 3.8. One with stages in flight (64 x 128 of 4) takes a long k
+// outputs take small tiles (32 x 32; 32 x 64 for a gated unit), which spread over more CUs: 208 x 1040 x 10288 18 -> 11.6
+// us, 16 x 4096 x 12288 12.8 -> 9.9, 77 x 2560 x 2048 4.3 -> 3.9. One with stages in flight (64 x 128 of 4) takes a long k
 // fastest; with 2 stages and two or three workgroups on the CU, one's loads, epilogue and stores go on under the others'
-// products, which is what counts over a short k (7431 x 768 x 96 GEGLU 9.7 -> 6.0 us, 896 x 4928 x 176 8.9 -> 6.4, 4400 x
-// 1024 x 384 ADD 14.2 -> 11.2, 1700 x 2560 x 2560 24.4 -> 20.7 with 128 x 128).
+// products, which is what counts over a short k (7431 x 768 x 96 GEGLU 9.7 -> 6.1 us, 896 x 4928 x 176 9.0 -> 6.5, 4400 x
+// 1024 x 384 ADD 14.2 -> 11.2, 1700 x 2560 x 2560 24.4 -> 20.1 with 128 x 128).
 template <int BM, int BN, int NSTG> constexpr int resident() { return 160 * 1024 / tile_lds<BM, BN, 4, NSTG, false>(); }
 
 template <int BM, int BN, int NSTG, int EC>
@@ -727,8 +729,9 @@ template <int BM, int BN, int NSTG, int EC> mk_status launch_tile(const I8P& p, 
 // of the kernel in every place that a CU has for one, takes so much a k step of 128 and so much beside (a start, an
 // epilogue); the last round has 1, 2 or 3 workgroups on a CU. 16 x 16 rows come at 48 bytes a ns and CU, or all weights at
 // 6.3 TB/s. A round of 256 x 256 tiles is bound by the matrix cores (1.5 a step; 0.95 where it is not full and the clock
-// higher). Fitted to the kernels' times at 1500 shapes and epilogues (rows 1 .. 16000, N from 64, K from 96): the choice is
-// within 0.7% of the best in the mean, 33% at worst (4000 x 1040 x 10288: 100 us, 76 in 128 x 128 tiles). Measured, us:
+// higher). Fitted to the kernels' times at 1500 shapes and epilogues (rows 1 .. 16000, N from 64, K from 96): on those the
+// choice is within 0.7% of the best in the mean, 33% at worst (4000 x 1040 x 10288: 100 us, 76 in 128 x 128 tiles). The
+// epilogue's bytes have no term (4400 x 8192 x 256 ADD: 74 us, 57 in 64 x 128 tiles of 2 stages). Measured, us:
 //                             16x16  32x32  64x32  64x64  64x128  64x128, 2 stages  128x128  mixed
 //   1 x 4096 x 4096             5.0           6.1    7.6      11                                14
 //   77 x 2560 x 2048            9.3    3.9    4.3    4.8     7.1                               9.0
