@@ -77,3 +77,15 @@ def test_product_sums_are_exact_at_the_largest_k_in_tiles(gpu, tile, m, n, epi):
     if epi == M.EPI_GEGLU:
         s = s * np.float32(128.0 * 128.0 * k)  # the gate's GELU is the gate itself: one more product
     assert np.array_equal(p.run(), np.broadcast_to(s.astype(np.float64), (1, m, p.cols)))
+
+
+# One and two k steps, no more than any kernel keeps in LDS, whole ones and parts.
+@pytest.mark.parametrize("epi", [M.EPI_STORE, M.EPI_GEGLU])
+@pytest.mark.parametrize("k", [16, 112, 128, 176, 256])
+def test_product_of_one_or_two_steps(gpu, k, epi):
+    seen = set()
+    for m, n in ((1, 8), (17, 6152), (17, 8200), (50, 4104), (50, 6152), (50, 8200), (100, 8200), (1537, 4104), (1537, 8200),
+                 (4300, 136), (4300, 8200)):
+        Product(m, n, k, epi).check()
+        seen.add(kind(m, n, k, epi))
+    assert seen >= {(64, 128, 2), (128, 128, 2), (256, "one", 0)} and len(seen) >= 5
