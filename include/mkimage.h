@@ -65,7 +65,7 @@ mk_status mk_event_elapsed_ms(void* start, void* stop, float* ms);
  * ------------------------------------------------------------------------------------------------------------ */
 
 enum mk_dtype { MK_F32 = 0, MK_BF16 = 1, MK_FP8_E4M3 = 2, MK_F16 = 3, MK_I8 = 4 /* rows and matrices of the 8-bit
-                integer path (mk_gemm_i8) */, MK_DTYPE_OTHER = 255 /* a file dtype the kernels do not take */ };
+                integer path (mk_gemm_i8) */, MK_I32 = 5 /* positions (mk_rope_rows) */, MK_DTYPE_OTHER = 255 /* a file dtype the kernels do not take */ };
 
 /* The GEMM's fused epilogue: what happens to acc = A W^T (* wscale[n]) + bias[n]. */
 enum mk_epilogue {
@@ -286,6 +286,117 @@ mk_status mk_attention(const void* q, const void* k, const void* vt, void* out, 
                        uint32_t heads, uint32_t kv_heads, uint32_t d, uint32_t n_q, uint32_t q_pad, uint32_t n_k,
                        uint32_t k_pad, int64_t ldo, int64_t stride_o, uint32_t q_pos0, uint32_t block, float scale,
                        const uint32_t* key_hole, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * Packed batches: the rows of several requests (images of different sizes, prompts of different lengths, each with a LoRA
+ * of its own or none) one after the other in one matrix, so that mk_gemm's projections run over all of them at once. The
+ * three operators below are what such a batch needs between the projections. No counterpart in the reference (it runs one
+ * request at a time; its adapters beside a projection, moss_image.cpp:435-624, are one LoRA for all rows).
+ *
+ * They allocate nothing and keep nothing between calls: what they need besides their operands is the caller's workspace. They
+ * may be captured, and may run on several streams at once, with a workspace each. They run on the current device. Host arrays
+ * are read during the call only (a graph keeps what they held at its capture). No output overlaps an input (but for the
+ * in-place forms named below), another output or the workspace. A call whose sizes leave nothing to do returns MK_OK.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* Attention of packed documents: query rows q_row .. q_row + q_rows - 1 attend to key rows k_row .. k_row + k_rows - 1, and
+ * to no others. Key c of a document has position c, its query row i position p = q_pos + i; the row sees the key iff
+ *   block == 0 or p >= block or c <= p or c < prefix
+ * (block 0: no mask; UINT32_MAX: causal; S: a causal text prefix, the rows behind it see every key, as mk_attention's block;
+ * prefix P with a causal block: the first P keys are seen by every row). q_pos may be negative: rows may see nothing. */
+typedef struct mk_attn_doc {
+    uint32_t q_row, q_rows;
+    uint32_t k_row, k_rows;
+    int32_t q_pos;
+    uint32_t block, prefix;
+} mk_attn_doc;
+typedef struct mk_attn_packed_args {
+    const void* q;       /* [rows][ldq] bf16 or f16, head h at column h d */
+    const void* k;       /* [rows][ldk], key / value head g at column g d; query head h reads g = h / (heads / kv_heads) */
+    const void* v;       /* [rows][ldv] */
+    void* out;           /* [rows][ldo] */
+    int64_t ldq, ldk, ldv, ldo; /* elements between rows, multiples of 8, less than 2^24 (q|k|v of one projection: its width) */
+    uint32_t dtype;      /* q, k, v: MK_BF16 or MK_F16 */
+    uint32_t out_dtype;  /* MK_BF16 or MK_F16 */
+    uint32_t heads, kv_heads, d; /* kv_heads divides heads (at most 65535), d 64 or 128 */
+    float scale;         /* s = scale q.k; finite, >= 0 (0 is 0: every seen key weighs the same) */
+    float cap;           /* > 0: s = cap tanh(s / cap); 0: none */
+    const float* slopes; /* device [heads] or NULL: s -= slopes[h] |p - c|, after the cap */
+    const mk_attn_doc* docs; /* host [n_docs], in any order; q rows of two documents must not overlap, k rows may */
+    uint32_t n_docs;
+    void* workspace;     /* 16-byte aligned, or NULL: few rows over many keys then run on few compute units */
+    uint64_t workspace_bytes; /* at least what mk_attention_packed_workspace says, when workspace is not NULL */
+} mk_attn_packed_args;
+/* out = softmax(s) v over the seen keys, sums and the softmax in fp32; the probabilities enter the second product in the inputs'
+ * type, rounded once. A row that sees no key, or only keys of score -inf, is zero. Rows outside every document are left as they were. What a row does not see does not
+ * reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees makes it NaN. All pointers
+ * 16-byte aligned (slopes 4). A row's bits may depend on the other documents of the call (their number decides how keys are
+ * split), not on their contents. */
+mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream);
+/* The workspace of that call on the current device, in bytes (0: none). Reads all of the arguments but the operands. */
+mk_status mk_attention_packed_workspace(const mk_attn_packed_args* a, uint64_t* bytes);
+
+/* Low-rank adapters of many requests beside a shared projection: with a = ids[r], and column n in part p = n / (N / parts),
+ *   c[r][n] = base[r][n] + scale[a] sum_j t[r][p rank + j] B[a][n][j],   t[r][i] = sum_k x[r][k] A[a][i][k]
+ * base is what the projection itself (mk_gemm) stored; parts are the modules of a fused matrix (q|k|v: 3, gate|up: 2), each
+ * with an A of its own. A row whose id is outside [0, adapters) (-1, say) has no adapter: c = base. Adapters of smaller ranks are
+ * filled up with zeros. To merge an adapter for good instead: mk_lora_merge. */
+typedef struct mk_lora_rows_args {
+    const void* x;       /* [rows][ldx] bf16 or f16: the projection's input */
+    const void* a;       /* [adapters][parts rank][K] */
+    const void* b;       /* [adapters][N][rank] */
+    const float* scale;  /* device [adapters] or NULL (1) */
+    const int32_t* ids;  /* device [rows] or NULL (all 0); rows of one adapter are fastest one after the other */
+    const void* base;    /* [rows][ldbase] or NULL (0); may be c itself (then ldbase == ldc) */
+    void* c;             /* [rows][ldc] */
+    int64_t ldx, ldbase, ldc; /* elements between rows, multiples of 8 */
+    uint32_t rows, K, N; /* K a multiple of 8, N of 8 parts */
+    uint32_t rank;       /* of each part, a multiple of 8 up to 256 */
+    uint32_t parts;      /* 1 to 4 */
+    uint32_t adapters;   /* at least 1 */
+    uint32_t dtype;      /* x, a, b: MK_BF16 or MK_F16 */
+    uint32_t c_dtype;    /* base and c: MK_F32, MK_BF16 or MK_F16 */
+    void* workspace;     /* 16-byte aligned */
+    uint64_t workspace_bytes; /* at least what mk_lora_rows_workspace says */
+} mk_lora_rows_args;
+/* Sums in fp32; t enters the second product as two values of the inputs' type (its rounding and the rest). Infinities and
+ * NaNs of a row or of an adapter reach that row, or that adapter's rows, alone. All pointers 16-byte aligned (scale and ids 4). */
+mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream);
+/* The workspace of that call on the current device, in bytes. Reads the sizes and types alone. */
+mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes);
+
+/* Rotary positions of several axes (text: one; an image's rows: height and width; a video's: time, height and width) on the
+ * query and key heads of packed rows, each head RMS-normed before (v rsqrt(mean v^2 + eps) w) where norm_q / norm_k is given:
+ * mk_heads without a table on the host, in the rows' own layout. Axis a turns axis_dims[a] of a head's d dims by angles
+ * pos[r][a] f, the axes one after the other from pair 0; dims behind the last axis' (d - sum of axis_dims) are not turned.
+ * series: MK_ROPE_OWN: pair j of axis a has f = theta^(-2 j / axis_dims[a]) (mk_rope_table's axes: 16, 56, 56);
+ *         MK_ROPE_SHARED: pair i of all has f = theta^(-2 i / R), R the sum of axis_dims: one series cut into sections.
+ * rope_mode: 1 pairs (i, i + R / 2), 2 pairs (2 i, 2 i + 1). Angles are exact to 2^-31 of a turn for int32 positions, and to
+ * (1 + |pos| 2^-20) times that for f32 ones up to 2^31 (an infinite or NaN position makes its pairs NaN). */
+enum mk_rope_series { MK_ROPE_OWN = 0, MK_ROPE_SHARED = 1 };
+typedef struct mk_rope_rows_args {
+    const void* q;       /* [rows][ldq], head h at column h d */
+    const void* k;       /* [rows][ldk] or NULL (then kv_heads 0) */
+    void* q_out;         /* [rows][ldqo]; q itself: in place (then out_dtype == dtype, ldqo == ldq) */
+    void* k_out;
+    int64_t ldq, ldk, ldqo, ldko; /* elements between rows, multiples of 4 */
+    uint32_t rows, heads, kv_heads, d; /* d 64 or 128 */
+    uint32_t dtype, out_dtype; /* MK_F32, MK_BF16 or MK_F16 each */
+    const float* norm_q; /* [d] or NULL */
+    const float* norm_k;
+    float eps;
+    float k_scale;       /* keys times this at the end (0: 1) */
+    const void* pos;     /* device [rows][pos_ld], one a row and axis */
+    int64_t pos_ld;      /* >= axes; 0: one row of positions for all rows */
+    uint32_t pos_dtype;  /* MK_I32 or MK_F32 */
+    uint32_t axes;       /* 1 to 4 */
+    uint32_t axis_dims[4]; /* each a multiple of 2, their sum R a multiple of 8 up to d */
+    double theta;        /* >= 1 */
+    uint32_t series;     /* mk_rope_series */
+    uint32_t rope_mode;  /* 1 or 2 */
+} mk_rope_rows_args;
+/* Everything in fp32, rounded once. q, k and the outputs are aligned for 4 of their elements, the rest for one. */
+mk_status mk_rope_rows(const mk_rope_rows_args* a, void* stream);
 
 /* Elementwise and norms (fp32 unless stated). */
 mk_status mk_silu(float* x, size_t n, void* stream);

@@ -14,10 +14,11 @@ import numpy as np
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libmkimage.so"
 
-F32, BF16, FP8, F16, I8, DTYPE_OTHER = 0, 1, 2, 3, 4, 255
+F32, BF16, FP8, F16, I8, I32, DTYPE_OTHER = 0, 1, 2, 3, 4, 5, 255
 EPI_STORE, EPI_GELU_TANH, EPI_GATE_ADD, EPI_GATE_TANH, EPI_SILU, EPI_ADD, EPI_HEADS, EPI_SWIGLU, EPI_GEGLU, \
     EPI_PAIR_SUM = range(10)
 NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
+ROPE_OWN, ROPE_SHARED = range(2)
 FAMILY_DUAL, FAMILY_Q21, FAMILY_SDXL = 0, 1, 2
 
 _vp, _sz, _u32, _u64, _i64, _f, _d, _i = (C.c_void_p, C.c_size_t, C.c_uint32, C.c_uint64, C.c_int64, C.c_float,
@@ -48,6 +49,33 @@ class GateNormArgs(C.Structure):
                [(n, _i64) for n in ("ldx", "ldy", "ldo", "alt", "mod_stride")] + \
                [(n, _u32) for n in ("rows", "n", "y_dtype", "out_dtype", "norm1", "norm2", "tanh_gate", "split",
                                     "seg_rows")] + [(n, _f) for n in ("residual_scale", "eps1", "eps2")]
+
+
+class AttnDoc(C.Structure):
+    _fields_ = [(n, _u32) for n in ("q_row", "q_rows", "k_row", "k_rows")] + [("q_pos", C.c_int32), ("block", _u32),
+                                                                              ("prefix", _u32)]
+
+
+class AttnPackedArgs(C.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "out")] + [(n, _i64) for n in ("ldq", "ldk", "ldv", "ldo")] + \
+               [(n, _u32) for n in ("dtype", "out_dtype", "heads", "kv_heads", "d")] + \
+               [("scale", _f), ("cap", _f), ("slopes", _vp), ("docs", C.POINTER(AttnDoc)), ("n_docs", _u32),
+                ("workspace", _vp), ("workspace_bytes", _u64)]
+
+
+class LoraRowsArgs(C.Structure):
+    _fields_ = [(n, _vp) for n in ("x", "a", "b", "scale", "ids", "base", "c")] + \
+               [(n, _i64) for n in ("ldx", "ldbase", "ldc")] + \
+               [(n, _u32) for n in ("rows", "K", "N", "rank", "parts", "adapters", "dtype", "c_dtype")] + \
+               [("workspace", _vp), ("workspace_bytes", _u64)]
+
+
+class RopeRowsArgs(C.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "k", "q_out", "k_out")] + [(n, _i64) for n in ("ldq", "ldk", "ldqo", "ldko")] + \
+               [(n, _u32) for n in ("rows", "heads", "kv_heads", "d", "dtype", "out_dtype")] + \
+               [("norm_q", _vp), ("norm_k", _vp), ("eps", _f), ("k_scale", _f), ("pos", _vp), ("pos_ld", _i64),
+                ("pos_dtype", _u32), ("axes", _u32), ("axis_dims", _u32 * 4), ("theta", _d), ("series", _u32),
+                ("rope_mode", _u32)]
 
 
 class Config(C.Structure):
@@ -110,6 +138,11 @@ _SIGS = {
                       _vp]),
     "mk_attention": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _i64, _i64, _u32,
                           _u32, _f, _vp, _vp]),
+    "mk_attention_packed": (_i, [C.POINTER(AttnPackedArgs), _vp]),
+    "mk_attention_packed_workspace": (_i, [C.POINTER(AttnPackedArgs), C.POINTER(_u64)]),
+    "mk_lora_rows": (_i, [C.POINTER(LoraRowsArgs), _vp]),
+    "mk_lora_rows_workspace": (_i, [C.POINTER(LoraRowsArgs), C.POINTER(_u64)]),
+    "mk_rope_rows": (_i, [C.POINTER(RopeRowsArgs), _vp]),
     "mk_silu": (_i, [_vp, _sz, _vp]),
     "mk_gelu_tanh": (_i, [_vp, _sz, _vp]),
     "mk_swiglu": (_i, [_vp, _u32, _u32, _u32, _vp, _vp]),
@@ -399,7 +432,52 @@ def _check_attention(q, k, vt, out, dtype, batch, heads, kv_heads, d, n_q, q_pad
         check_extent(out, ((batch - 1) * stride_o + (n_q - 1) * ldo + heads * d) * 2, "mk_attention: out")
 
 
-_EXTENT_CHECKS = {"mk_gemm": _check_gemm, "mk_gemm_grouped": _check_gemm_grouped, "mk_conv3x3": _check_conv,
+def _check_attention_packed(args, stream=None):
+    g = _struct(args, AttnPackedArgs)
+    docs = [g.docs[i] for i in range(g.n_docs)] if g.docs else []
+    q = max((d.q_row + d.q_rows for d in docs if d.q_rows), default=0)
+    k = max((d.k_row + d.k_rows for d in docs if d.q_rows and d.k_rows), default=0)
+    nq, nk = g.heads * g.d, g.kv_heads * g.d
+    if q:
+        check_extent(g.q, ((q - 1) * g.ldq + nq) * 2, "mk_attention_packed: q")
+        check_extent(g.out, ((q - 1) * g.ldo + nq) * 2, "mk_attention_packed: out")
+        check_extent(g.slopes, g.heads * 4, "mk_attention_packed: slopes")
+    if k:
+        check_extent(g.k, ((k - 1) * g.ldk + nk) * 2, "mk_attention_packed: k")
+        check_extent(g.v, ((k - 1) * g.ldv + nk) * 2, "mk_attention_packed: v")
+    check_extent(g.workspace, g.workspace_bytes, "mk_attention_packed: workspace")
+
+
+def _check_lora_rows(args, stream=None):
+    g = _struct(args, LoraRowsArgs)
+    if g.rows == 0 or g.K == 0 or g.N == 0:
+        return
+    size = _SIZE.get(g.c_dtype, 4)
+    check_extent(g.x, ((g.rows - 1) * g.ldx + g.K) * 2, "mk_lora_rows: x")
+    check_extent(g.a, g.adapters * g.parts * g.rank * g.K * 2, "mk_lora_rows: a")
+    check_extent(g.b, g.adapters * g.N * g.rank * 2, "mk_lora_rows: b")
+    check_extent(g.scale, g.adapters * 4, "mk_lora_rows: scale")
+    check_extent(g.ids, g.rows * 4, "mk_lora_rows: ids")
+    check_extent(g.base, ((g.rows - 1) * g.ldbase + g.N) * size, "mk_lora_rows: base")
+    check_extent(g.c, ((g.rows - 1) * g.ldc + g.N) * size, "mk_lora_rows: c")
+    check_extent(g.workspace, g.workspace_bytes, "mk_lora_rows: workspace")
+
+
+def _check_rope_rows(args, stream=None):
+    g = _struct(args, RopeRowsArgs)
+    if g.rows == 0:
+        return
+    for n, ld, heads, dt in (("q", g.ldq, g.heads, g.dtype), ("k", g.ldk, g.kv_heads, g.dtype),
+                             ("q_out", g.ldqo, g.heads, g.out_dtype), ("k_out", g.ldko, g.kv_heads, g.out_dtype)):
+        check_extent(getattr(g, n), ((g.rows - 1) * ld + heads * g.d) * _SIZE.get(dt, 4), "mk_rope_rows: " + n)
+    check_extent(g.norm_q, g.d * 4, "mk_rope_rows: norm_q")
+    check_extent(g.norm_k, g.d * 4, "mk_rope_rows: norm_k")
+    check_extent(g.pos, ((g.rows - 1) * g.pos_ld + g.axes) * 4, "mk_rope_rows: pos")
+
+
+_EXTENT_CHECKS = {"mk_attention_packed": _check_attention_packed, "mk_lora_rows": _check_lora_rows,
+                  "mk_rope_rows": _check_rope_rows,
+                  "mk_gemm": _check_gemm, "mk_gemm_grouped": _check_gemm_grouped, "mk_conv3x3": _check_conv,
                   "mk_attention": _check_attention, "mk_gemm_i8": _check_gemm_i8, "mk_gate_norm": _check_gate_norm,
                   "mk_quantize_i8_rows": _check_quantize_i8}
 
