@@ -349,8 +349,8 @@ typedef struct mk_lora_rows_args {
     const int32_t* ids;  /* device [rows] or NULL (all 0); rows of one adapter are fastest one after the other */
     const void* base;    /* [rows][ldbase] or NULL (0); may be c itself (then ldbase == ldc) */
     void* c;             /* [rows][ldc] */
-    int64_t ldx, ldbase, ldc; /* elements between rows, multiples of 8 */
-    uint32_t rows, K, N; /* K a multiple of 8, N of 8 parts */
+    int64_t ldx, ldbase, ldc; /* elements between rows, multiples of 8 below 2^23 */
+    uint32_t rows, K, N; /* K a multiple of 8, N of 8 parts, both up to 2^22; rows up to 2^28 */
     uint32_t rank;       /* of each part, a multiple of 8 up to 256 */
     uint32_t parts;      /* 1 to 4 */
     uint32_t adapters;   /* at least 1 */
@@ -359,7 +359,7 @@ typedef struct mk_lora_rows_args {
     void* workspace;     /* 16-byte aligned */
     uint64_t workspace_bytes; /* at least what mk_lora_rows_workspace says */
 } mk_lora_rows_args;
-/* Sums in fp32; t enters the second product as two values of the inputs' type (its rounding and the rest). Infinities and
+/* Sums in fp32; t enters the second product as two or three values of the inputs' type (its rounding and the rest). Infinities and
  * NaNs of a row or of an adapter reach that row, or that adapter's rows, alone. All pointers 16-byte aligned (scale and ids 4). */
 mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream);
 /* The workspace of that call on the current device, in bytes. Reads the sizes and types alone. */

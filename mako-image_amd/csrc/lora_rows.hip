@@ -1,11 +1,18 @@
 // mk_lora_rows: low-rank adapters of many requests beside a shared projection.
+//
+// Two launches: t = x A^T (the rows' own adapters) into the workspace, then c = base + scale t B^T. Bound by memory: x, base
+// and c once each, with 2 rank flops a value. t is a few values a row, so it goes through memory in fp32, as the
+// partial sums of the workgroups that share a row's K (no atomics: the second launch adds them in their order).
 #include "common.hpp"
 
 #include <type_traits>
+#include <utility>
 
 namespace mk {
 
 namespace {
+
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
 
 struct LoraP {
     const uint16_t *x, *a, *b;
@@ -13,63 +20,404 @@ struct LoraP {
     const int32_t* ids;
     const void* base;
     void* c;
-    float* t; // workspace: [rows][parts rank]
+    float* t; // workspace: [splits][rows][parts rank]
     int64_t ldx, ldbase, ldc;
     uint32_t rows, K, N, rank, parts, adapters;
+    uint32_t splits, split_k; // workgroups that share a row's K, and the k of each
+    uint32_t blocks;          // of 128 columns that a wave of the second product goes through
 };
 
 template <bool F16> __device__ inline float widen(uint16_t h) { return F16 ? h2f_bits(h) : bf2f_bits(h); }
+template <bool F16> __device__ inline void widen8(const u32x4& v, float (&f)[8])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[2 * j] = widen<F16>(uint16_t(v[j]));
+        f[2 * j + 1] = widen<F16>(uint16_t(v[j] >> 16));
+    }
+}
 // the adapter of a row, or -1
 __device__ inline int adapter_of(const LoraP& p, uint32_t row)
 {
     const int id = p.ids ? p.ids[row] : 0;
     return id >= 0 && uint32_t(id) < p.adapters ? id : -1;
 }
+// s_waitcnt immediate: vmcnt vm, lgkmcnt 0 (vmcnt's bits 3:0 and 15:14, expcnt not waited for)
+constexpr int wait_vm(int vm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4); }
 
-// t[row][i] = x[row] . A[a][i], a wave for each
-template <bool F16> __global__ __launch_bounds__(256) void shrink_kernel(LoraP p)
+template <bool F16> __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
 {
-    const uint32_t width = p.parts * p.rank, row = blockIdx.y, i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= width)
-        return;
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// the smallest adapter above `last` among a wave's rows (a lane's row each), or INT_MAX
+__device__ inline int next_adapter(int id, int last)
+{
+    int v = id > last ? id : 0x7fffffff;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1)
+        v = min(v, __shfl_xor(v, m));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// t = x A^T
+// ------------------------------------------------------------------------------------------------------------
+
+// Few rows: a workgroup for a row and 4 of its adapter's rows, its four waves a quarter of K each.
+constexpr uint32_t kVecI = 4;
+template <bool F16> __global__ __launch_bounds__(256) void shrink_vec(LoraP p)
+{
+    const uint32_t width = p.parts * p.rank, row = blockIdx.y, i0 = blockIdx.x * kVecI, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int a = adapter_of(p, row);
     if (a < 0)
         return;
     const uint16_t* x = p.x + int64_t(row) * p.ldx;
-    const uint16_t* w = p.a + (int64_t(a) * width + i) * p.K;
-    float s = 0.0f;
-    for (uint32_t k = lane; k < p.K; k += 64)
-        s += widen<F16>(x[k]) * widen<F16>(w[k]);
-    s = wave_sum(s);
-    if (lane == 0)
-        p.t[int64_t(row) * width + i] = s;
+    const uint16_t* w = p.a + (int64_t(a) * width + i0) * p.K;
+    float s[kVecI] = {};
+#pragma unroll 2
+    for (uint32_t k = threadIdx.x * 8; k < p.K; k += 2048) {
+        float xf[8];
+        widen8<F16>(*reinterpret_cast<const u32x4*>(x + k), xf);
+#pragma unroll
+        for (uint32_t i = 0; i < kVecI; ++i) {
+            float wf[8];
+            widen8<F16>(*reinterpret_cast<const u32x4*>(w + int64_t(i) * p.K + k), wf);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                s[i] = fmaf(xf[j], wf[j], s[i]);
+        }
+    }
+    __shared__ float red[4][kVecI];
+#pragma unroll
+    for (uint32_t i = 0; i < kVecI; ++i) {
+        const float v = wave_sum(s[i]);
+        if (lane == 0)
+            red[wave][i] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x < kVecI)
+        p.t[int64_t(row) * width + i0 + threadIdx.x] =
+            (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
 
-// c[row][n] = base[row][n] + scale t[row] . B[a][n], a thread for each
-template <bool F16, uint32_t CT> __global__ __launch_bounds__(256) void expand_kernel(LoraP p)
+// Many rows: a tile of 64 rows by 32 NB of A's rows and one split of K. Each of the four waves takes every fourth 32 k for the
+// whole tile, through three stages of LDS of its own (direct loads, two steps ahead, no barriers in the loop; nothing is read
+// from LDS twice), and the waves' sums are added at the end. A tile with rows of several adapters goes through K for each.
+constexpr int kRows = 64, kStepK = 128;
+template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(LoraP p)
 {
-    const uint32_t row = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= p.N)
-        return;
+    constexpr int XB = kRows * 64, AB = 32 * NB * 64, WB = XB + AB; // bytes of a wave's stage
+    constexpr int NX = XB / 1024, ND = WB / 1024;                   // direct loads of x, of both
+    __shared__ __attribute__((aligned(16))) uint8_t s0[4 * WB], s1[4 * WB], s2[4 * WB];
+    const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hk = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t width = p.parts * p.rank, row0 = blockIdx.x * kRows, rows = min(p.rows - row0, uint32_t(kRows));
+    const uint32_t split = blockIdx.y % p.splits, i0 = blockIdx.y / p.splits * (32 * NB);
+    const uint32_t kb = split * p.split_k, ke = min(p.K, kb + p.split_k);
+    const int steps = int((ke - kb + kStepK - 1) / kStepK);
+    const int mine = uint32_t(lane) < rows ? adapter_of(p, row0 + lane) : -1; // lane's row of the tile
+
+    const BufRes rx = buf_res(p.x + int64_t(row0) * p.ldx, uint32_t(((rows - 1) * p.ldx + p.K) * 2));
+    // byte offset of a lane's 16 bytes of each load, and their k: LDS rows of 64 bytes whose chunk c holds k chunk
+    // c ^ ((row >> 2) & 3), so the 16-byte fragment reads of 8 rows fall on all banks
+    uint32_t off[ND], kof;
+    const int slot = lane & 3;
+    {
+        const int c = slot ^ ((lane >> 4) & 3); // (row >> 2) & 3 of row 16 j + lane / 4
+        kof = uint32_t(wave * 32 + c * 8);
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+            const uint32_t r = uint32_t((j < NX ? j : j - NX) * 16 + lane / 4);
+            off[j] = j < NX ? min(r, rows - 1) * uint32_t(p.ldx) * 2 : min(r, width - i0 - 1) * p.K * 2;
+        }
+    }
+    for (int a = next_adapter(mine, -1); a != 0x7fffffff; a = next_adapter(mine, a)) {
+        const BufRes ra = buf_res(p.a + (int64_t(a) * width + i0) * p.K, uint32_t(min(uint32_t(32 * NB), width - i0) * p.K * 2));
+        auto issue = [&](int s, uint8_t* buf) {
+            // behind the split's end: past the resource, so zeros come
+            const uint32_t k = kb + uint32_t(s) * kStepK + kof, v = k < ke ? k * 2 : 0x80000000u;
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+                buf_load_lds16(j < NX ? rx : ra, (lds_void*)(buf + wave * WB + j * 1024), k < ke ? off[j] + v : v, 0);
+        };
+        f32x16 acc[2][NB];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                acc[i][j] = f32x16{};
+        auto step = [&](int s, uint8_t* cur, uint8_t* next) {
+            if (s >= steps)
+                return;
+            issue(s + 2, next);
+            __builtin_amdgcn_s_waitcnt(wait_vm(2 * ND)); // step s landed, the next two may be in flight
+            const uint8_t* b = cur + wave * WB;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const int at = (((ks * 2 + hk) ^ ((r32 >> 2) & 3)) << 4) + r32 * 64;
+                u32x4 xf[2], af[NB];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    xf[i] = *reinterpret_cast<const u32x4*>(b + at + i * 2048);
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    af[j] = *reinterpret_cast<const u32x4*>(b + XB + at + j * 2048);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+                        acc[i][j] = mfma<F16>(af[j], xf[i], acc[i][j]);
+            }
+        };
+        issue(0, s0);
+        issue(1, s1);
+        for (int s = 0; s < steps; s += 3) {
+            step(s, s0, s2);
+            step(s + 1, s1, s0);
+            step(s + 2, s2, s1);
+        }
+        __builtin_amdgcn_s_waitcnt(0); // the last (unused) loads land before the LDS is reused
+        // the waves' sums, 32 x 32 at a time: lane's values 4 g .. 4 g + 3 are A rows 8 g + 4 hk .. + 3 of x row r32
+        float* red = reinterpret_cast<float*>(s0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                __syncthreads();
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4*>(red + ((wave * 4 + g) * 64 + lane) * 4) =
+                        f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                __syncthreads();
+                f32x4 v = *reinterpret_cast<const f32x4*>(red + (wave * 64 + lane) * 4);
+#pragma unroll
+                for (int w = 1; w < 4; ++w)
+                    v += *reinterpret_cast<const f32x4*>(red + ((w * 4 + wave) * 64 + lane) * 4);
+                const uint32_t r = i * 32 + r32, n = i0 + j * 32 + wave * 8 + hk * 4;
+                if (__shfl(mine, int(r)) == a && n < width)
+                    *reinterpret_cast<f32x4*>(p.t + (int64_t(split) * p.rows + row0 + r) * width + n) = v;
+            }
+        __syncthreads(); // before the next adapter's loads
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// c = base + scale t B^T
+// ------------------------------------------------------------------------------------------------------------
+
+// the sum of the splits' partial t, 4 of a row
+__device__ inline f32x4 load_t(const LoraP& p, uint32_t row, uint32_t i)
+{
+    const int64_t width = int64_t(p.parts) * p.rank, at = int64_t(row) * width + i;
+    f32x4 v = *reinterpret_cast<const f32x4*>(p.t + at);
+    for (uint32_t s = 1; s < p.splits; ++s)
+        v += *reinterpret_cast<const f32x4*>(p.t + s * (p.rows * width) + at);
+    return v;
+}
+template <uint32_t CT> __device__ inline float load_c(const void* c, int64_t at)
+{
+    return CT == MK_F32 ? static_cast<const float*>(c)[at] : widen<CT == MK_F16>(static_cast<const uint16_t*>(c)[at]);
+}
+
+// 4 values through a buffer resource; past it zeros come, and nothing is stored
+constexpr uint32_t kOut = 0x80000000u;
+template <class V> __device__ inline V load_v(BufRes r, uint32_t voff, uint32_t soff)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (sizeof(V) == 16)
+        return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, int(voff), int(soff), 0));
+    else
+        return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, int(voff), int(soff), 0));
+#else
+    return V{};
+#endif
+}
+template <class V> __device__ inline void store_v(V v, BufRes r, uint32_t voff, uint32_t soff)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (sizeof(V) == 16)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, int(voff), int(soff), 0);
+    else
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, int(voff), int(soff), 0);
+#endif
+}
+
+// Few rows: a thread a value.
+template <bool F16, uint32_t CT> __global__ __launch_bounds__(256) void expand_vec(LoraP p)
+{
+    const uint32_t row = blockIdx.y, per = p.N / p.parts, groups = (per + 255) / 256;
+    const uint32_t part = blockIdx.x / groups, col = blockIdx.x % groups * 256 + threadIdx.x, n = part * per + col;
     const int a = adapter_of(p, row);
+    __shared__ __attribute__((aligned(16))) float st[256];
+    if (a >= 0 && threadIdx.x * 4 < p.rank)
+        *reinterpret_cast<f32x4*>(st + threadIdx.x * 4) = load_t(p, row, part * p.rank + threadIdx.x * 4);
+    __syncthreads();
+    if (col >= per)
+        return;
     float v = 0.0f;
     if (a >= 0) {
-        const uint32_t part = n / (p.N / p.parts);
-        const float* t = p.t + int64_t(row) * p.parts * p.rank + part * p.rank;
         const uint16_t* w = p.b + (int64_t(a) * p.N + n) * p.rank;
-        for (uint32_t j = 0; j < p.rank; ++j)
-            v += t[j] * widen<F16>(w[j]);
+#pragma unroll 2
+        for (uint32_t j = 0; j < p.rank; j += 8) {
+            float wf[8];
+            widen8<F16>(*reinterpret_cast<const u32x4*>(w + j), wf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v = fmaf(st[j + e], wf[e], v);
+        }
         if (p.scale)
             v *= p.scale[a];
     }
-    const int64_t ci = int64_t(row) * p.ldc + n, bi = int64_t(row) * p.ldbase + n;
-    if constexpr (CT == MK_F32) {
-        static_cast<float*>(p.c)[ci] = (p.base ? static_cast<const float*>(p.base)[bi] : 0.0f) + v;
-    } else {
-        const float o = p.base ? widen<CT == MK_F16>(static_cast<const uint16_t*>(p.base)[bi]) : 0.0f;
-        static_cast<uint16_t*>(p.c)[ci] = CT == MK_F16 ? f2h_bits(o + v) : f2bf_bits(o + v);
+    if (p.base)
+        v += load_c<CT>(p.base, int64_t(row) * p.ldbase + n);
+    const int64_t at = int64_t(row) * p.ldc + n;
+    if constexpr (CT == MK_F32)
+        static_cast<float*>(p.c)[at] = v;
+    else
+        static_cast<uint16_t*>(p.c)[at] = CT == MK_F16 ? f2h_bits(v) : f2bf_bits(v);
+}
+
+// Many rows: a workgroup has 64 rows of one part; its waves go through blocks of 128 columns. t is in LDS as 2 or 3 values
+// of the inputs' type (v = v0 + v1 (+ v2), each the rounding of what is left: 2^-16 of t, or 2^-24 with three, for fp32
+// outputs; half t after a power of two that puts the row's largest near 2^14, so that none is lost below the half range). In the product C = T B^T a wave's
+// four column tiles take columns 4 j + tile: a lane then has 4 columns next to each other of each of its rows, and base and c
+// go by 8 or 16 bytes a lane, 256 or 512 next to each other.
+template <bool F16, uint32_t CT> __global__ __launch_bounds__(256, CT == MK_F32 ? 2 : 3) void expand_tile(LoraP p)
+{
+    constexpr int NV = CT == MK_F32 && !F16 ? 3 : 2;
+    constexpr uint32_t SZ = CT == MK_F32 ? 4 : 2;
+    typedef std::conditional_t<CT == MK_F32, u32x4, u32x2> V; // 4 values of c
+    extern __shared__ __attribute__((aligned(16))) uint16_t st[]; // [NV][64][pad], then a factor a row
+    const uint32_t tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hk = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t row0 = blockIdx.x * kRows, rows = min(p.rows - row0, uint32_t(kRows));
+    const uint32_t per = p.N / p.parts, span = 512 * p.blocks, groups = (per + span - 1) / span;
+    const uint32_t part = blockIdx.y / groups, first = blockIdx.y % groups * span;
+    const uint32_t depth = (p.rank + 15) / 16 * 16, pad = depth + 8; // (rows 16 bytes off each other's banks)
+    float* factor = reinterpret_cast<float*>(st + NV * kRows * pad);
+    const int mine = lane < rows ? adapter_of(p, row0 + lane) : -2;
+    {
+        // 4 threads a row, t's values 4 (q + 4 i) .. + 3 of it in each
+        const uint32_t r = tid / 4, q = tid % 4;
+        const bool on = __shfl(mine, int(r)) >= 0;
+        float top = 0.0f;
+        if constexpr (F16) {
+            if (on)
+                for (uint32_t i = q * 4; i < p.rank; i += 16) {
+                    const f32x4 v = load_t(p, row0 + r, part * p.rank + i);
+                    top = fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), top);
+                }
+            top = fmaxf(top, __shfl_xor(top, 1));
+            top = fmaxf(top, __shfl_xor(top, 2));
+        }
+        float up = 1.0f, down = 1.0f;
+        if (F16 && top > 0.0f && top < __builtin_inff()) {
+            const int e = min(14 - ilogbf(top), 100);
+            up = ldexpf(1.0f, e);
+            down = ldexpf(1.0f, -e);
+        }
+        if (q == 0)
+            factor[r] = down;
+        for (uint32_t i = q * 4; i < depth; i += 16) {
+            const f32x4 v = on && i < p.rank ? load_t(p, row0 + r, part * p.rank + i) : f32x4{};
+            float rest[4] = {v[0] * up, v[1] * up, v[2] * up, v[3] * up};
+#pragma unroll
+            for (int s = 0; s < NV; ++s) {
+                const u32x2 h{pack_x2(rest[0], rest[1], F16), pack_x2(rest[2], rest[3], F16)};
+                *reinterpret_cast<u32x2*>(st + (s * kRows + r) * pad + i) = h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // (an infinity's or a NaN's rest is nothing)
+                    const float d = rest[e] - widen<F16>(uint16_t(h[e / 2] >> (16 * (e % 2))));
+                    rest[e] = fabsf(d) < __builtin_inff() ? d : 0.0f;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int a = next_adapter(mine, -2); a != 0x7fffffff; a = next_adapter(mine, a)) {
+        if (a < 0 && p.base == p.c)
+            continue; // rows without an adapter, in place
+        const float scale = a >= 0 && p.scale ? p.scale[a] : 1.0f;
+        const uint64_t on = __ballot(mine == a); // the adapter's rows of the tile
+        for (uint32_t blk = 0; blk < p.blocks; ++blk) {
+            const uint32_t c0 = first + (blk * 4 + wave) * 128; // column of the part
+            if (c0 >= per)
+                break;
+            const uint32_t col = c0 + r32 * 4;
+            const bool in = col < per; // (per is a multiple of 8: all 4 of a lane's columns, or none)
+#pragma unroll 1
+            for (uint32_t rt = 0; rt < 2; ++rt) {
+                const uint32_t has = uint32_t(on >> (32 * rt));
+                if (!has)
+                    continue;
+                // A lane's rows of the tile are 8 (i / 4) + 4 hk + i % 4. Their base and c by buffer loads and stores: one
+                // byte offset a lane and a scalar one a row; what is not the adapter's goes past the resource.
+                const uint32_t tr = min(rows - rt * 32, 32u);
+                const int64_t r0 = int64_t(row0) + rt * 32;
+                const BufRes rb = buf_res(p.base ? static_cast<const char*>(p.base) + (r0 * p.ldbase + part * per) * SZ : nullptr,
+                                          p.base ? uint32_t((tr - 1) * p.ldbase + per) * SZ : 0u);
+                const BufRes rc = buf_res(static_cast<const char*>(p.c) + (r0 * p.ldc + part * per) * SZ, uint32_t((tr - 1) * p.ldc + per) * SZ);
+                const uint32_t vb = (4 * hk * uint32_t(p.ldbase) + col) * SZ, vc = (4 * hk * uint32_t(p.ldc) + col) * SZ;
+                const uint32_t lane_has = in ? has >> (4 * hk) : 0u;
+                auto row_of = [](int i) { return uint32_t(8 * (i / 4) + i % 4); };
+                V basev[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    basev[i] = load_v<V>(rb, lane_has >> row_of(i) & 1 ? vb : kOut, row_of(i) * uint32_t(p.ldbase) * SZ);
+                f32x16 acc[4] = {f32x16{}, f32x16{}, f32x16{}, f32x16{}};
+                if (a >= 0) {
+                    const uint16_t* w = p.b + (int64_t(a) * p.N + part * per + col) * p.rank + hk * 8;
+                    const uint16_t* tv = st + (rt * 32 + r32) * pad + hk * 8;
+#pragma unroll 1
+                    for (uint32_t k = 0; k < depth; k += 16) {
+                        u32x4 bf[4];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            bf[t] = u32x4{};
+                            if (in && k + hk * 8 < p.rank)
+                                bf[t] = *reinterpret_cast<const u32x4*>(w + t * p.rank + k);
+                        }
+#pragma unroll
+                        for (int s = NV - 1; s >= 0; --s) {
+                            const u32x4 tf = *reinterpret_cast<const u32x4*>(tv + s * kRows * pad + k);
+#pragma unroll
+                            for (int t = 0; t < 4; ++t)
+                                acc[t] = mfma<F16>(tf, bf[t], acc[t]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float f = scale * factor[rt * 32 + 4 * hk + row_of(i)];
+                    float v[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        float o;
+                        if constexpr (CT == MK_F32)
+                            o = __builtin_bit_cast(float, uint32_t(basev[i][t]));
+                        else
+                            o = widen<CT == MK_F16>(uint16_t(basev[i][t / 2] >> (16 * (t % 2))));
+                        v[t] = a >= 0 ? fmaf(acc[t][i], f, o) : o;
+                    }
+                    V out;
+                    if constexpr (CT == MK_F32)
+                        out = __builtin_bit_cast(V, f32x4{v[0], v[1], v[2], v[3]});
+                    else
+                        out = V{pack_x2(v[0], v[1], CT == MK_F16), pack_x2(v[2], v[3], CT == MK_F16)};
+                    store_v(out, rc, lane_has >> row_of(i) & 1 ? vc : kOut, row_of(i) * uint32_t(p.ldc) * SZ);
+                }
+            }
+        }
     }
 }
+
+// ------------------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------------------
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -82,13 +430,90 @@ mk_status check_sizes(const mk_lora_rows_args* a)
         return fail(MK_ERR_ARG, "lora_rows: base and c must be f32, bf16 or f16");
     if (!a->parts || a->parts > 4 || !a->rank || a->rank % 8 || a->rank > 256 || !a->adapters || a->adapters > 0x7fffffffu)
         return fail(MK_ERR_ARG, "lora_rows: 1 to 4 parts of rank a multiple of 8 up to 256, 1 adapter or more");
-    if (!a->K || a->K % 8 || a->K > (1u << 24) || !a->N || a->N % (8 * a->parts) || a->N > (1u << 24))
-        return fail(MK_ERR_ARG, "lora_rows: K must be a multiple of 8, N of 8 parts, up to 2^24");
-    if (a->rows > 0x7fffffffu)
-        return fail(MK_ERR_ARG, "lora_rows: more than 2^31 - 1 rows");
+    if (!a->K || a->K % 8 || a->K > (1u << 22) || !a->N || a->N % (8 * a->parts) || a->N > (1u << 22))
+        return fail(MK_ERR_ARG, "lora_rows: K must be a multiple of 8, N of 8 parts, up to 2^22");
+    if (a->rows > (1u << 28)) // (64 rows a workgroup of 256: 2^30 threads)
+        return fail(MK_ERR_ARG, "lora_rows: more than 2^28 rows");
     return MK_OK;
 }
-uint64_t workspace_of(const mk_lora_rows_args* a) { return round_up(uint64_t(a->rows) * a->parts * a->rank * 4, 16); }
+
+// How the two products run, by the sizes alone (on `cus` compute units).
+struct Plan {
+    bool vec1, vec2;    // a workgroup a row (few rows) or tiles of 64 rows
+    uint32_t nb;        // the first product's tiles: 32 nb of A's rows
+    uint32_t splits, split_k;
+    uint32_t blocks;
+};
+Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
+{
+    Plan p{};
+    const uint32_t width = a->parts * a->rank, chunks = cdiv(width, 128), tiles = cdiv(a->rows, kRows);
+    const uint64_t macs = uint64_t(a->rows) * width * a->K, macs2 = uint64_t(a->rows) * a->N * a->rank;
+    p.vec1 = a->rows <= 1024 && macs <= (1u << 25);
+    p.vec2 = a->rows <= 1024 && macs2 <= (1u << 24);
+    p.nb = cdiv(cdiv(width, chunks), 32);
+    p.splits = 1;
+    p.split_k = uint32_t(round_up(a->K, kStepK));
+    if (!p.vec1) {
+        // a workgroup a compute unit at a time: the fewest rounds of the shortest splits; a split's start and end, and its
+        // partial t, cost about 4 steps
+        const uint32_t steps = cdiv(a->K, kStepK);
+        const uint64_t groups = uint64_t(tiles) * chunks;
+        double best = 1e30;
+        for (uint32_t s = 1; s <= 16 && s <= steps; ++s) {
+            const uint32_t each = cdiv(steps, s), used = cdiv(steps, each);
+            const double cost = double((groups * used + cus - 1) / cus) * (each + 4.0);
+            if (cost < best * 0.97) {
+                best = cost;
+                p.splits = used;
+                p.split_k = each * kStepK;
+            }
+        }
+    }
+    const uint32_t per = a->N / a->parts;
+    p.blocks = 1;
+    while (p.blocks < 4 && p.blocks * 512 < per && uint64_t(tiles) * a->parts * cdiv(per, 1024 * p.blocks) >= 4ull * cus)
+        p.blocks *= 2;
+    return p;
+}
+uint64_t workspace_of(const mk_lora_rows_args* a, const Plan& p)
+{
+    return round_up(uint64_t(p.splits) * a->rows * a->parts * a->rank * 4, 16);
+}
+mk_status device_cus(uint32_t* cus)
+{
+    int dev = 0, n = 0;
+    MK_HIP(hipGetDevice(&dev));
+    MK_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
+    *cus = n > 0 ? uint32_t(n) : 1u;
+    return MK_OK;
+}
+
+template <bool F16> void launch_shrink(const LoraP& p, const Plan& plan, hipStream_t s)
+{
+    const uint32_t width = p.parts * p.rank;
+    if (plan.vec1) {
+        shrink_vec<F16><<<dim3(width / kVecI, p.rows), 256, 0, s>>>(p);
+        return;
+    }
+    const dim3 grid(cdiv(p.rows, kRows), cdiv(width, 32 * plan.nb) * p.splits);
+    switch (plan.nb) {
+    case 1: shrink_tile<F16, 1><<<grid, 256, 0, s>>>(p); break;
+    case 2: shrink_tile<F16, 2><<<grid, 256, 0, s>>>(p); break;
+    case 3: shrink_tile<F16, 3><<<grid, 256, 0, s>>>(p); break;
+    default: shrink_tile<F16, 4><<<grid, 256, 0, s>>>(p); break;
+    }
+}
+template <bool F16, uint32_t CT> void launch_expand(const LoraP& p, const Plan& plan, hipStream_t s)
+{
+    const uint32_t per = p.N / p.parts;
+    if (plan.vec2) {
+        expand_vec<F16, CT><<<dim3(p.parts * cdiv(per, 256), p.rows), 256, 0, s>>>(p);
+        return;
+    }
+    const uint32_t pad = (p.rank + 15) / 16 * 16 + 8, values = CT == MK_F32 && !F16 ? 3 : 2;
+    expand_tile<F16, CT><<<dim3(cdiv(p.rows, kRows), p.parts * cdiv(per, 512 * p.blocks)), 256, (values * pad * 2 + 4) * kRows, s>>>(p);
+}
 
 } // namespace
 
@@ -103,7 +528,12 @@ mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes)
     if (!a || !bytes)
         return fail(MK_ERR_ARG, "lora_rows_workspace: null argument");
     MK_TRY(check_sizes(a));
-    *bytes = workspace_of(a);
+    *bytes = 0;
+    if (!a->rows)
+        return MK_OK;
+    uint32_t cus = 1;
+    MK_TRY(device_cus(&cus));
+    *bytes = workspace_of(a, plan_of(a, cus));
     return MK_OK;
 }
 
@@ -112,9 +542,10 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
     if (!a || !a->x || !a->a || !a->b || !a->c)
         return fail(MK_ERR_ARG, "lora_rows: null argument (x, a, b and c are required)");
     MK_TRY(check_sizes(a));
-    if (a->ldx < int64_t(a->K) || a->ldx % 8 || a->ldc < int64_t(a->N) || a->ldc % 8 ||
-        (a->base && (a->ldbase < int64_t(a->N) || a->ldbase % 8)))
-        return fail(MK_ERR_ARG, "lora_rows: ldx, ldbase and ldc must be multiples of 8, at least the row");
+    // (a tile's 64 rows of x, or 32 of c, are addressed by 31 bits)
+    auto bad = [](int64_t ld, uint32_t n) { return ld < int64_t(n) || ld % 8 || ld >= (1 << 23); };
+    if (bad(a->ldx, a->K) || bad(a->ldc, a->N) || (a->base && bad(a->ldbase, a->N)))
+        return fail(MK_ERR_ARG, "lora_rows: ldx, ldbase and ldc must be multiples of 8 below 2^23, at least the row");
     if (a->base == a->c && a->ldbase != a->ldc)
         return fail(MK_ERR_ARG, "lora_rows: in place needs ldbase == ldc");
     if (!aligned(a->x, 16) || !aligned(a->a, 16) || !aligned(a->b, 16) || !aligned(a->base, 16) || !aligned(a->c, 16) ||
@@ -122,32 +553,26 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
         return fail(MK_ERR_ARG, "lora_rows: operands and workspace must be 16-byte aligned (scale and ids 4)");
     if (!a->rows)
         return MK_OK;
-    if (!a->workspace || a->workspace_bytes < workspace_of(a))
+    if (!a->workspace || a->workspace_bytes < workspace_of(a, Plan{false, false, 1, 1, 0, 1}))
+        return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
+    uint32_t cus = 1;
+    MK_TRY(device_cus(&cus));
+    const Plan plan = plan_of(a, cus);
+    if (a->workspace_bytes < workspace_of(a, plan))
         return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
     LoraP p{static_cast<const uint16_t*>(a->x), static_cast<const uint16_t*>(a->a), static_cast<const uint16_t*>(a->b), a->scale,
             a->ids, a->base, a->c, static_cast<float*>(a->workspace), a->ldx, a->ldbase, a->ldc, a->rows, a->K, a->N, a->rank,
-            a->parts, a->adapters};
+            a->parts, a->adapters, plan.splits, plan.split_k, plan.blocks};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    // rows in the grid's second dimension, at most 65535 a launch
-    const uint32_t width = a->parts * a->rank, csize = a->c_dtype == MK_F32 ? 4 : 2;
-    for (uint32_t r0 = 0; r0 < a->rows; r0 += 65535) {
-        LoraP c = p;
-        c.rows = a->rows - r0 < 65535 ? a->rows - r0 : 65535;
-        c.x += int64_t(r0) * p.ldx;
-        c.t += int64_t(r0) * width;
-        c.ids = p.ids ? p.ids + r0 : nullptr;
-        c.base = p.base ? static_cast<const char*>(p.base) + int64_t(r0) * p.ldbase * csize : nullptr;
-        c.c = static_cast<char*>(p.c) + int64_t(r0) * p.ldc * csize;
-        const dim3 g1(cdiv(width, 4), c.rows), g2(cdiv(p.N, 256), c.rows);
-        const bool f16 = a->dtype == MK_F16;
-        f16 ? shrink_kernel<true><<<g1, 256, 0, s>>>(c) : shrink_kernel<false><<<g1, 256, 0, s>>>(c);
-        if (a->c_dtype == MK_F32)
-            f16 ? expand_kernel<true, MK_F32><<<g2, 256, 0, s>>>(c) : expand_kernel<false, MK_F32><<<g2, 256, 0, s>>>(c);
-        else if (a->c_dtype == MK_BF16)
-            f16 ? expand_kernel<true, MK_BF16><<<g2, 256, 0, s>>>(c) : expand_kernel<false, MK_BF16><<<g2, 256, 0, s>>>(c);
-        else
-            f16 ? expand_kernel<true, MK_F16><<<g2, 256, 0, s>>>(c) : expand_kernel<false, MK_F16><<<g2, 256, 0, s>>>(c);
-    }
+    const bool f16 = a->dtype == MK_F16;
+    f16 ? launch_shrink<true>(p, plan, s) : launch_shrink<false>(p, plan, s);
+    MK_LAUNCH_CHECK("lora_rows");
+    if (a->c_dtype == MK_F32)
+        f16 ? launch_expand<true, MK_F32>(p, plan, s) : launch_expand<false, MK_F32>(p, plan, s);
+    else if (a->c_dtype == MK_BF16)
+        f16 ? launch_expand<true, MK_BF16>(p, plan, s) : launch_expand<false, MK_BF16>(p, plan, s);
+    else
+        f16 ? launch_expand<true, MK_F16>(p, plan, s) : launch_expand<false, MK_F16>(p, plan, s);
     MK_LAUNCH_CHECK("lora_rows");
     return MK_OK;
 }

@@ -243,13 +243,20 @@ extern "C" mk_status mk_rope_rows(const mk_rope_rows_args* a, void* stream)
         return fail(MK_ERR_ARG, "rope_rows: more than 2^31 - 1 rows");
     RopeP p{a->q, a->k, a->q_out, a->k_out, a->ldq, a->ldk, a->ldqo, a->ldko, a->pos_ld, a->norm_q, a->norm_k, a->pos,
             a->rows, a->heads, a->kv_heads, a->d, uint32_t(turned / 2), a->eps, a->k_scale == 0.0f ? 1.0f : a->k_scale, {}, {}};
+    // theta^(-2 j / dim) radians as turns of 2^64, in extended doubles: a power for every eighth pair (150 ns each), products
+    // between them, so at most 9 roundings of 2^-64
+    const bool own = a->series == MK_ROPE_OWN;
+    const long double theta = a->theta, unit = 18446744073709551616.0L / 6.283185307179586476925286766559L;
+    long double f = 0.0L, ratio = 0.0L;
     uint32_t pair = 0;
     for (uint32_t i = 0; i < a->axes; ++i)
         for (uint32_t j = 0; j < a->axis_dims[i] / 2; ++j, ++pair) {
-            const bool own = a->series == MK_ROPE_OWN;
-            // theta^(-2 j / dim) radians as turns, in 64 bits (an extended double on the host)
-            const long double f = powl((long double)(a->theta), -2.0L * (own ? j : pair) / (own ? a->axis_dims[i] : turned));
-            p.turn[pair] = uint64_t(f / 6.283185307179586476925286766559L * 18446744073709551616.0L);
+            const uint32_t at = own ? j : pair;
+            const long double dim = own ? a->axis_dims[i] : uint32_t(turned);
+            if (at == 0)
+                ratio = powl(theta, -2.0L / dim);
+            f = at % 8 ? f * ratio : powl(theta, -2.0L * at / dim) * unit;
+            p.turn[pair] = uint64_t(f);
             p.axis[pair] = uint8_t(i);
         }
     hipStream_t s = static_cast<hipStream_t>(stream);
