@@ -303,7 +303,8 @@ mk_status mk_attention(const void* q, const void* k, const void* vt, void* out, 
  * to no others. Key c of a document has position c, its query row i position p = q_pos + i; the row sees the key iff
  *   block == 0 or p >= block or c <= p or c < prefix
  * (block 0: no mask; UINT32_MAX: causal; S: a causal text prefix, the rows behind it see every key, as mk_attention's block;
- * prefix P with a causal block: the first P keys are seen by every row). q_pos may be negative: rows may see nothing. */
+ * prefix P with a causal block: the first P keys are seen by every row). q_pos may be negative: rows may see nothing. Rows and
+ * positions stay below 2^31, a document's q_rows times heads within 2^29. */
 typedef struct mk_attn_doc {
     uint32_t q_row, q_rows;
     uint32_t k_row, k_rows;

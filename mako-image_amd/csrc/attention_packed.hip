@@ -12,79 +12,452 @@ namespace mk {
 
 namespace {
 
-constexpr uint32_t kMaxDocs = 96; // documents a launch: they go by kernel argument
+constexpr uint32_t kMaxDocs = 80; // documents a launch: they go by kernel argument, in less than 4 KB
+constexpr int kKT = 64;           // keys a tile
+// The exponentials' reference m moves only when a weight against it passes 2^8 (below).
+constexpr float kLazyP = 256.0f;
+constexpr float kLeast = -1e30f; // m of rows without a score above -inf
 
 struct Doc {
-    uint32_t first; // its first item
+    uint32_t first; // its first workgroup, a multiple of 8
     uint32_t q_row, q_rows, k_row, k_rows;
     int32_t q_pos;
     uint32_t block, prefix;
+    uint32_t blocks; // of 32 NW rows a key head
+    uint32_t splits; // workgroups that share a block's keys
+    uint32_t slot;   // its first partial result in the workspace, when splits > 1
+    uint32_t join;   // its first workgroup of the second launch
 };
 struct PackedP {
     const uint16_t *q, *k, *v;
     uint16_t* out;
     int64_t ldq, ldk, ldv, ldo;
     const float* slopes;
-    float scale, cap;
-    uint32_t heads, group, n_docs, out_f16;
+    float* part;    // workspace: [slot][32 NW][D] sums, then [slot][32 NW][2] m and l
+    float* part_ml;
+    float c;        // scale log2(e); with a cap: 2 scale log2(e) / cap
+    float cap;      // cap log2(e)
+    uint32_t heads, kv_heads, group, n_docs, out_f16;
     Doc docs[kMaxDocs];
 };
 
-template <bool F16> __device__ inline float widen(uint16_t h) { return F16 ? h2f_bits(h) : bf2f_bits(h); }
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-__device__ inline bool sees(const Doc& d, int64_t pos, int64_t key)
+template <bool F16> __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
 {
-    return d.block == 0 || pos >= int64_t(d.block) || key <= pos || key < int64_t(d.prefix);
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// 4 x 16 values of 16 bits from LDS, transposed: 16 lanes read 4 rows of 16 next to each other, 4 a lane, and each gets a column
+__device__ inline u32x2 read_tr(const uint16_t* p)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+#else
+    return u32x2{};
+#endif
 }
 
-// a wave a query row and head: a key a lane, then the head's dims a lane
-template <bool F16, int D> __global__ __launch_bounds__(64) void simple_kernel(PackedP p)
+// How many of a document's keys a row at position pos sees: they are the first ones under every mask.
+__device__ inline int seen_keys(const Doc& d, int64_t pos)
 {
-    uint32_t di = 0;
-    while (di + 1 < p.n_docs && blockIdx.x >= p.docs[di + 1].first)
-        ++di;
-    const Doc d = p.docs[di];
-    const uint32_t i = blockIdx.x - d.first, head = blockIdx.y, lane = threadIdx.x;
-    const int64_t pos = int64_t(d.q_pos) + i;
-    const uint16_t* q = p.q + (int64_t(d.q_row) + i) * p.ldq + int64_t(head) * D;
-    const uint16_t* k = p.k + int64_t(d.k_row) * p.ldk + int64_t(head / p.group) * D;
-    const uint16_t* v = p.v + int64_t(d.k_row) * p.ldv + int64_t(head / p.group) * D;
-    __shared__ float sq[D], sp[64];
-    for (int e = lane; e < D; e += 64)
-        sq[e] = widen<F16>(q[e]);
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.0f, acc[D / 64] = {};
-    for (uint32_t k0 = 0; k0 < d.k_rows; k0 += 64) {
-        const uint32_t key = k0 + lane;
-        float s = -__builtin_inff();
-        if (key < d.k_rows && sees(d, pos, key)) {
-            s = 0.0f;
-            for (int e = 0; e < D; ++e)
-                s += sq[e] * widen<F16>(k[int64_t(key) * p.ldk + e]);
-            s *= p.scale;
-            if (p.cap > 0.0f)
-                s = p.cap * tanhf(s / p.cap);
-            if (p.slopes)
-                s -= p.slopes[head] * fabsf(float(pos - int64_t(key)));
+    if (d.block == 0 || pos >= int64_t(d.block))
+        return int(d.k_rows);
+    int64_t n = pos + 1 > int64_t(d.prefix) ? pos + 1 : int64_t(d.prefix);
+    n = n < int64_t(d.k_rows) ? n : int64_t(d.k_rows);
+    return int(n > 0 ? n : 0);
+}
+__device__ inline const Doc& find_doc(const PackedP& p, uint32_t item, bool join)
+{
+    uint32_t lo = 0, hi = p.n_docs;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        ((join ? p.docs[mid].join : p.docs[mid].first) <= item ? lo : hi) = mid;
+    }
+    return p.docs[lo];
+}
+
+enum { kPlain = 0, kBias = 1, kCap = 2 /* and a bias, of slope 0 without one */ };
+
+template <int D, bool F16, int MODE, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 2 : 1, NW == 4 ? 2 : 1))) void packed_kernel(PackedP p)
+{
+    constexpr int DS = D / 16, DT = D / 32, KC = D / 8; // k steps of S, 32-dim blocks of O, 16-byte chunks of a row
+    constexpr int RL = kKT * KC / (64 * NW);            // direct loads a wave and operand
+    constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+    // the two buffers are separate objects, so that the compiler can tell a load into one from the reads of the other
+    __shared__ __attribute__((aligned(16))) uint16_t sK0[kKT * D], sK1[kKT * D], sV0[kKT * D], sV1[kKT * D];
+    __shared__ int odd_tile; // 1 + the last tile in which find_odd found any
+    auto sK = [&](int b) { return b ? sK1 : sK0; };
+    auto sV = [&](int b) { return b ? sV1 : sV0; };
+
+    const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hk = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Doc& doc = find_doc(p, blockIdx.x, false);
+    // Workgroup i runs on XCD i % 8: each XCD takes a run of a document's (key head, block, split), whose blocks share keys in
+    // its L2; later blocks, which see more under a causal mask, come first.
+    const uint32_t each = doc.blocks * doc.splits, real = each * p.kv_heads, run = (real + 7) / 8;
+    const uint32_t local = blockIdx.x - doc.first, item = local % 8 * run + local / 8;
+    if (local / 8 >= run || item >= real)
+        return;
+    const uint32_t kvh = item / each, block = doc.blocks - 1 - item % each / doc.splits, split = item % doc.splits;
+
+    // rows of a block: (query row, head of the group) pairs, so that all heads of a key head share its tiles
+    const uint32_t rows = doc.q_rows * p.group, wg0 = block * (32 * NW), w0 = wg0 + wave * 32;
+    const uint32_t wg_last = min(wg0 + 32 * NW, rows) - 1, row = min(w0 + r32, rows - 1);
+    const uint32_t qi = row / p.group, head = kvh * p.group + row % p.group;
+    const int64_t pos = int64_t(doc.q_pos) + qi;
+    const int lim = seen_keys(doc, pos);
+    const int wg_lim = seen_keys(doc, int64_t(doc.q_pos) + wg0 / p.group); // of the workgroup's first row: the least
+    const int wave_lim = seen_keys(doc, int64_t(doc.q_pos) + min(w0, rows - 1) / p.group); // of the wave's
+    const int wave_most = seen_keys(doc, int64_t(doc.q_pos) + min(w0 + 31, rows - 1) / p.group);
+    const int all_tiles = (seen_keys(doc, int64_t(doc.q_pos) + wg_last / p.group) + kKT - 1) / kKT;
+    const int t_begin = int(uint64_t(all_tiles) * split / doc.splits), t_end = int(uint64_t(all_tiles) * (split + 1) / doc.splits);
+
+    u32x4 qf[DS];
+    {
+        const uint16_t* Q = p.q + (int64_t(doc.q_row) + qi) * p.ldq + int64_t(head) * D;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+            qf[ds] = *reinterpret_cast<const u32x4*>(Q + ds * 16 + hk * 8);
+    }
+    // LDS chunks: K's so that 16 keys' fragment reads fall on all banks, V's so that the 64 bytes of 4 keys that a transposing
+    // read takes do
+    auto kswz = [](int key, int c) { return KC == 16 ? c ^ (key & 15) : c ^ ((key >> 1) & 7); };
+    auto vswz = [](int key, int c) { return KC == 16 ? c ^ ((key & 3) << 2) : c ^ ((key & 2) << 1); };
+    uint32_t ok[RL], ov[RL];
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+        const int P = (i * NW + wave) * 64 + lane, key = P / KC, c = P % KC;
+        ok[i] = (uint32_t(key) * uint32_t(p.ldk) + kswz(key, c) * 8) * 2;
+        ov[i] = (uint32_t(key) * uint32_t(p.ldv) + vswz(key, c) * 8) * 2;
+    }
+    const uint16_t* K = p.k + int64_t(doc.k_row) * p.ldk + int64_t(kvh) * D;
+    const uint16_t* V = p.v + int64_t(doc.k_row) * p.ldv + int64_t(kvh) * D;
+    // a tile's resources end with the document's last key: what lies behind it comes as zeros (a tile past the last: nothing)
+    auto tile_keys = [&](int t) { return t < t_end ? min(int(doc.k_rows) - t * kKT, kKT) : 0; };
+    auto res_of = [&](const uint16_t* base, int64_t ld, int t) {
+        const int n = tile_keys(t);
+        return buf_res(n ? base + int64_t(t) * kKT * ld : base, n ? uint32_t((n - 1) * int(ld) + D) * 2 : 0u);
+    };
+    // load i of tile t's 2 RL into buffer buf
+    auto dma = [&](const BufRes& rk, const BufRes& rv, int buf, int i) {
+        if (i < RL)
+            buf_load_lds16(rk, (lds_void*)&sK(buf)[(i * NW + wave) * 512], ok[i], 0);
+        else if (i < 2 * RL)
+            buf_load_lds16(rv, (lds_void*)&sV(buf)[((i - RL) * NW + wave) * 512], ov[i - RL], 0);
+    };
+
+    f32x16 oacc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+        oacc[dt] = f32x16{};
+    float m = kLeast, l = 0.0f;
+    const float slope = MODE != kPlain && p.slopes ? p.slopes[head] * 1.4426950408889634f : 0.0f;
+
+    // score r of a half whose first key is k0, in log2 units, less `from`
+    auto score = [&](float s, int k0, int r, float from) {
+        float x;
+        if constexpr (MODE == kCap) // cap tanh(y) = cap - 2 cap / (1 + e^2y)
+            x = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * p.c)), p.cap - from);
+        else
+            x = fmaf(s, p.c, -from);
+        if constexpr (MODE != kPlain) {
+            const float dist = float(pos - k0 - 4 * hk) - float(8 * (r / 4) + r % 4);
+            x = fmaf(-slope, fabsf(dist), x);
         }
-        const float mn = fmaxf(m, wave_max(s)), base = mn == -__builtin_inff() ? 0.0f : mn;
-        const float alpha = m == -__builtin_inff() ? 0.0f : expf(m - base), e = expf(s - base);
-        l = l * alpha + wave_sum(e);
+        return x;
+    };
+    auto masked = [&](float x, int k0, int r) { return k0 + 8 * (r / 4) + 4 * hk + r % 4 < lim ? x : -__builtin_inff(); };
+    // the weights of pair j of a half, packed, and their sum
+    auto pair = [&](const f32x16& sc, int k0, int j, uint32_t (&pw)[8], float& ls, auto edge_c) {
+        float x0 = score(sc[2 * j], k0, 2 * j, m), x1 = score(sc[2 * j + 1], k0, 2 * j + 1, m);
+        if constexpr (decltype(edge_c)::value) {
+            x0 = masked(x0, k0, 2 * j);
+            x1 = masked(x1, k0, 2 * j + 1);
+        }
+        const float e0 = __builtin_amdgcn_exp2f(x0), e1 = __builtin_amdgcn_exp2f(x1);
+        pw[j] = pack_x2(e0, e1, F16);
+        ls += e0 + e1;
+    };
+    // moves m up to a half's largest score, rescales what was summed against the old one, and makes the half's weights again
+    auto redo = [&](const f32x16& sc, int k0, uint32_t (&pw)[8], float& ls, auto edge_c) {
+        f32x16 x;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[r] = score(sc[r], k0, r, 0.0f);
+            if constexpr (decltype(edge_c)::value)
+                x[r] = masked(x[r], k0, r);
+        }
+        const float mn = fmaxf(m, max_xor32(max16(x))), alpha = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
-        __syncthreads();
-        sp[lane] = e;
-        __syncthreads();
-        for (int c = 0; c < D / 64; ++c) {
-            acc[c] *= alpha;
-            for (uint32_t j = 0; j < 64 && k0 + j < d.k_rows; ++j)
-                if (sees(d, pos, k0 + j))
-                    acc[c] += sp[j] * widen<F16>(v[int64_t(k0 + j) * p.ldv + c * 64 + lane]);
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                oacc[dt][r] *= alpha;
+        ls = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            pair(sc, k0, j, pw, ls, edge_c);
+    };
+    auto read_k = [&](int buf, int kt, int ds) {
+        const int key = kt * 32 + r32;
+        return *reinterpret_cast<const u32x4*>(&sK(buf)[key * D + kswz(key, ds * 2 + hk) * 8]);
+    };
+    // V^T fragment of 16 keys (step s2 of the tile's 4) and 32 dims: slots 4 i + j of a lane are keys 16 s2 + 8 i + 4 hk + j,
+    // those of its weights
+    auto read_v = [&](int buf, int s2, int dt) {
+        u32x4 f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int key = 16 * s2 + 8 * i + 4 * hk + ((lane & 15) >> 2), d = dt * 32 + (lane & 16) + (lane & 3) * 4;
+            const u32x2 h = read_tr(&sV(buf)[key * D + vswz(key, d / 8) * 8 + d % 8]);
+            f[2 * i] = h[0];
+            f[2 * i + 1] = h[1];
         }
+        return f;
+    };
+
+    // Infinities and NaNs of V at keys that only some of a tile's rows see must not meet the others' zero weights. Where a mask
+    // cuts a tile for some row of the workgroup, V is looked through (a quarter a wave); if there are any, they are replaced by
+    // zeros in LDS, and after the products each row adds those that it sees.
+    auto find_odd = [&](int t, auto buf_c) {
+        constexpr int buf = decltype(buf_c)::value, N = kKT * KC / (64 * NW);
+        constexpr uint32_t ODD = F16 ? 0x04000400u : 0x00800080u; // added to an exponent of all ones: a carry into bit 15
+        uint32_t any = 0;
+#pragma unroll 4
+        for (int i = 0; i < N; ++i) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(&sV(buf)[(i * 64 * NW + tid) * 8]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                any |= (v[e] & (EXP * 0x10001u)) + ODD;
+        }
+        if (any & 0x80008000u)
+            odd_tile = t + 1;
+        __syncthreads();
+        if (odd_tile != t + 1)
+            return false;
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+            u32x4* at = reinterpret_cast<u32x4*>(&sV(buf)[(i * 64 * NW + tid) * 8]);
+            u32x4 v = *at;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t c = ((v[e] & (EXP * 0x10001u)) + ODD) & 0x80008000u;
+                v[e] &= ~((c >> 15) * 0xffffu);
+            }
+            *at = v;
+        }
+        __syncthreads();
+        return true;
+    };
+    auto add_odd = [&](int t) {
+#pragma unroll 1
+        for (int key = t * kKT; key < min(t * kKT + kKT, int(doc.k_rows)); ++key) {
+            const uint16_t* v = V + int64_t(key) * p.ldv + 4 * hk;
+            if (key >= lim)
+                continue;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const u32x2 h = *reinterpret_cast<const u32x2*>(v + dt * 32 + 8 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t x = uint16_t(h[e / 2] >> (16 * (e % 2)));
+                        if ((x & EXP) == EXP)
+                            oacc[dt][4 * i + e] += F16 ? h2f_bits(x) : bf2f_bits(x);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    };
+
+    // One tile from buffer `buf`. Its fragment reads stream LA ahead of the products that use them, in a fixed order (fenced), and
+    // the next tile's loads go out between the first products. The weights are made against the m that is there, before
+    // the tile's largest score is known: those of half a between the products S^T of half b, those of half b between the
+    // products P V of half a. A lane's part of their sum decides afterwards whether a half is made again against a new m:
+    // a score more than 8 (in log2 units) above m puts that sum above 2^8.
+    constexpr int LA = 4, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
+    auto tile = [&](int t, auto buf_c, auto edge_c) {
+        constexpr int buf = decltype(buf_c)::value;
+        constexpr bool EDGE = decltype(edge_c)::value;
+        const int k0 = t * kKT;
+        const BufRes rk = res_of(K, p.ldk, t + 1), rv = res_of(V, p.ldv, t + 1);
+        if (EDGE && k0 >= wave_most) { // no row of the wave sees the tile
+#pragma unroll
+            for (int i = 0; i < 2 * RL; ++i)
+                dma(rk, rv, buf ^ 1, i);
+            return;
+        }
+        u32x4 fk[2 * DS], fv[4 * DT];
+        auto rd = [&](int g) {
+            if (g < 2 * DS)
+                fk[g] = read_k(buf, g / DS, g % DS);
+            else if (g < 2 * DS + 4 * DT)
+                fv[g - 2 * DS] = read_v(buf, (g - 2 * DS) / DT, (g - 2 * DS) % DT);
+        };
+        f32x16 s_a = f32x16{}, s_b = f32x16{};
+        uint32_t pa[8], pb[8];
+        float la = 0.0f, lb = 0.0f;
+#pragma unroll
+        for (int g = 0; g < LA; ++g)
+            rd(g);
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int ND = 2 * RL, PER = (ND + DS - 1) / DS;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            s_a = mfma<F16>(fk[ds], qf[ds], s_a);
+            __builtin_amdgcn_sched_barrier(0);
+            rd(ds + LA);
+#pragma unroll
+            for (int i = ds * PER; i < (ds + 1) * PER && i < ND; ++i)
+                dma(rk, rv, buf ^ 1, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        auto chunk = [&](const f32x16& sc, int kh, uint32_t (&pw)[8], float& ls, int c) {
+#pragma unroll
+            for (int j = c * CH; j < (c + 1) * CH; ++j) {
+                pair(sc, kh, j, pw, ls, edge_c);
+                // (pinned here: the compiler would sink the work into the path that keeps it)
+                asm volatile("" : "+v"(pw[j]), "+v"(ls));
+            }
+        };
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            s_b = mfma<F16>(fk[DS + ds], qf[ds], s_b);
+            __builtin_amdgcn_sched_barrier(0);
+            rd(DS + ds + LA);
+            __builtin_amdgcn_sched_barrier(0);
+            chunk(s_a, k0, pa, la, ds);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__any(la > kLazyP))
+            redo(s_a, k0, pa, la, edge_c);
+        l += la;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) {
+            const int st = j / DT;
+            oacc[j % DT] = mfma<F16>(fv[j], u32x4{pa[4 * st], pa[4 * st + 1], pa[4 * st + 2], pa[4 * st + 3]}, oacc[j % DT]);
+            __builtin_amdgcn_sched_barrier(0);
+            rd(2 * DS + j + LA);
+            __builtin_amdgcn_sched_barrier(0);
+            chunk(s_b, k0 + 32, pb, lb, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__any(lb > kLazyP))
+            redo(s_b, k0 + 32, pb, lb, edge_c);
+        l += lb;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) {
+            const int st = j / DT;
+            oacc[j % DT] = mfma<F16>(fv[2 * DT + j], u32x4{pb[4 * st], pb[4 * st + 1], pb[4 * st + 2], pb[4 * st + 3]}, oacc[j % DT]);
+            __builtin_amdgcn_sched_barrier(0);
+            rd(2 * DS + 2 * DT + j + LA);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto step = [&](int t, auto buf_c) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        const bool odd = wg_lim < min(t * kKT + kKT, int(doc.k_rows)) && find_odd(t, buf_c);
+        if (t * kKT + kKT > wave_lim)
+            tile(t, buf_c, std::true_type{});
+        else
+            tile(t, buf_c, std::false_type{});
+        if (odd)
+            add_odd(t);
+    };
+    if (tid == 0)
+        odd_tile = 0; // (the first step's barrier is behind it)
+    if (t_begin < t_end) {
+        const BufRes rk = res_of(K, p.ldk, t_begin), rv = res_of(V, p.ldv, t_begin);
+#pragma unroll
+        for (int i = 0; i < 2 * RL; ++i)
+            dma(rk, rv, 0, i);
     }
-    for (int c = 0; c < D / 64; ++c) {
-        const float o = l == 0.0f ? 0.0f : acc[c] / l;
-        p.out[(int64_t(d.q_row) + i) * p.ldo + int64_t(head) * D + c * 64 + lane] = p.out_f16 ? f2h_bits(o) : f2bf_bits(o);
+    for (int t = t_begin; t < t_end; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < t_end)
+            step(t + 1, std::integral_constant<int, 1>{});
     }
+    __builtin_amdgcn_s_waitcnt(0);
+
+    const float lt = add_xor32(l);
+    if (w0 + r32 >= rows)
+        return;
+    if (doc.splits > 1) {
+        const uint64_t at = (uint64_t(doc.slot) + item) * (32 * NW) + wave * 32 + r32;
+        float* o = p.part + at * D + 4 * hk;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x16& a = oacc[dt];
+                *reinterpret_cast<f32x4*>(o + dt * 32 + 8 * i) = f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]};
+            }
+        if (hk == 0) {
+            p.part_ml[2 * at] = m;
+            p.part_ml[2 * at + 1] = lt;
+        }
+        return;
+    }
+    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+    uint16_t* o = p.out + (int64_t(doc.q_row) + qi) * p.ldo + int64_t(head) * D + 4 * hk;
+    auto store = [&](auto h_c) {
+        constexpr bool H = decltype(h_c)::value;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x16& a = oacc[dt];
+                *reinterpret_cast<u32x2*>(o + dt * 32 + 8 * i) = u32x2{pack_x2(a[4 * i] * inv, a[4 * i + 1] * inv, H),
+                                                                       pack_x2(a[4 * i + 2] * inv, a[4 * i + 3] * inv, H)};
+            }
+    };
+    if (p.out_f16)
+        store(std::true_type{});
+    else
+        store(std::false_type{});
+}
+
+// The splits of a row joined: a wave a row (4 a workgroup), D / 64 dims a lane.
+template <int D, int NW> __global__ __launch_bounds__(256) void join_kernel(PackedP p)
+{
+    const Doc& doc = find_doc(p, blockIdx.x, true);
+    const uint32_t rows = doc.q_rows * p.group, lane = threadIdx.x & 63;
+    const uint32_t at = (blockIdx.x - doc.join) * 4 + (threadIdx.x >> 6);
+    if (doc.splits < 2 || at >= rows * p.kv_heads)
+        return;
+    const uint32_t kvh = at / rows, row = at % rows, block = row / (32 * NW);
+    // (blocks are numbered from the last one, as above)
+    const uint64_t item = uint64_t(doc.slot) + (uint64_t(kvh) * doc.blocks + (doc.blocks - 1 - block)) * doc.splits;
+    const uint64_t first = item * (32 * NW) + row % (32 * NW);
+    float m = kLeast;
+    for (uint32_t s = 0; s < doc.splits; ++s)
+        m = fmaxf(m, p.part_ml[2 * (first + uint64_t(s) * (32 * NW))]);
+    float l = 0.0f, o[D / 64] = {};
+    for (uint32_t s = 0; s < doc.splits; ++s) {
+        const uint64_t i = first + uint64_t(s) * (32 * NW);
+        const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * i] - m);
+        l = fmaf(w, p.part_ml[2 * i + 1], l);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e)
+            o[e] = fmaf(w, p.part[i * D + lane * (D / 64) + e], o[e]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = p.out + (int64_t(doc.q_row) + row / p.group) * p.ldo + int64_t(kvh * p.group + row % p.group) * D + lane * (D / 64);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e)
+        out[e] = p.out_f16 ? f2h_bits(o[e] * inv) : f2bf_bits(o[e] * inv);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -115,6 +488,8 @@ mk_status check_shape(const mk_attn_packed_args* a)
         const mk_attn_doc& d = a->docs[i];
         if (uint64_t(d.q_row) + d.q_rows > 0x7fffffffu || uint64_t(d.k_row) + d.k_rows > 0x7fffffffu)
             return fail(MK_ERR_ARG, "attention_packed: a document's rows end past 2^31 - 1");
+        if (uint64_t(d.q_rows) * a->heads > (1u << 29)) // (128 of them a workgroup of 256: 2^30 threads)
+            return fail(MK_ERR_ARG, "attention_packed: a document's q_rows times heads pass 2^29");
         if (int64_t(d.q_pos) + d.q_rows > 0x7fffffff)
             return fail(MK_ERR_ARG, "attention_packed: a document's positions end past 2^31 - 1");
         if (d.q_rows) {
@@ -137,6 +512,106 @@ mk_status check_shape(const mk_attn_packed_args* a)
     return MK_OK;
 }
 
+
+// One launch: up to kMaxDocs documents from docs[next] on, the longest first, and how their keys are split.
+struct Launch {
+    uint32_t nw;          // waves a workgroup (32 rows each)
+    uint32_t groups;      // workgroups
+    uint32_t joins;       // workgroups of the second launch, 0: none
+    uint64_t slots;       // partial results
+};
+
+constexpr uint64_t kMostGroups = 1u << 23; // of 256 threads: fewer than 2^32 in all
+
+// Takes documents into p; returns how many of docs were looked at.
+uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, bool split, PackedP& p, Launch& out)
+{
+    const uint32_t group = a->heads / a->kv_heads;
+    uint32_t at = next, n = 0;
+    uint64_t most_rows = 0, sum = 0;
+    for (; at < a->n_docs && n < kMaxDocs; ++at) {
+        const mk_attn_doc& d = a->docs[at];
+        if (!d.q_rows)
+            continue;
+        sum += uint64_t(cdiv(uint64_t(d.q_rows) * group, 128)) * a->kv_heads;
+        if (n && sum > kMostGroups)
+            break;
+        p.docs[n++] = Doc{0, d.q_row, d.q_rows, d.k_row, d.k_rows, d.q_pos, d.block, d.prefix, 0, 1, 0, 0};
+        most_rows = std::max(most_rows, uint64_t(d.q_rows) * group);
+    }
+    // longest first (at most kMaxDocs: an insertion sort)
+    for (uint32_t i = 1; i < n; ++i)
+        for (uint32_t j = i; j && p.docs[j].k_rows > p.docs[j - 1].k_rows; --j)
+            std::swap(p.docs[j], p.docs[j - 1]);
+    // one wave a workgroup where all rows of a key head fit it: few rows over many keys
+    out.nw = most_rows <= 32 ? 1 : 4;
+    const uint32_t resident = cus * (out.nw == 4 || a->d == 128 ? 2 : 4);
+    uint64_t groups = 0, tiles = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        Doc& d = p.docs[i];
+        d.blocks = cdiv(uint64_t(d.q_rows) * group, 32 * out.nw);
+        groups += uint64_t(d.blocks) * a->kv_heads;
+        tiles += uint64_t(d.blocks) * a->kv_heads * cdiv(d.k_rows, kKT);
+    }
+    // fewer workgroups than the chip holds: keys are split so that each has about as many tiles, at least 2
+    const uint64_t target = split && groups < resident ? std::max<uint64_t>((tiles + resident - 1) / resident, 2) : ~0ull;
+    uint64_t first = 0, join = 0;
+    out.slots = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        Doc& d = p.docs[i];
+        const uint64_t t = cdiv(d.k_rows, kKT);
+        d.splits = t > target ? uint32_t((t + target - 1) / target) : 1;
+        d.first = uint32_t(first);
+        d.join = uint32_t(join);
+        d.slot = uint32_t(out.slots);
+        const uint64_t items = uint64_t(d.blocks) * a->kv_heads * d.splits;
+        first += round_up(items, 8);
+        if (d.splits > 1) {
+            out.slots += items;
+            join += cdiv(uint64_t(d.q_rows) * a->heads, 4);
+        }
+    }
+    p.n_docs = n;
+    out.groups = uint32_t(first);
+    out.joins = uint32_t(join);
+    return at - next;
+}
+uint64_t bytes_of(const mk_attn_packed_args* a, const Launch& l) { return l.slots * (32 * l.nw) * (a->d + 2) * 4; }
+
+template <int D, bool F16, int NW> void launch_mode(const PackedP& p, int mode, uint32_t groups, hipStream_t s)
+{
+    if (mode == kPlain)
+        packed_kernel<D, F16, kPlain, NW><<<groups, 64 * NW, 0, s>>>(p);
+    else if (mode == kBias)
+        packed_kernel<D, F16, kBias, NW><<<groups, 64 * NW, 0, s>>>(p);
+    else
+        packed_kernel<D, F16, kCap, NW><<<groups, 64 * NW, 0, s>>>(p);
+}
+template <int D> void launch_all(const PackedP& p, const Launch& l, bool f16, int mode, hipStream_t s)
+{
+    if (l.nw == 4)
+        f16 ? launch_mode<D, true, 4>(p, mode, l.groups, s) : launch_mode<D, false, 4>(p, mode, l.groups, s);
+    else
+        f16 ? launch_mode<D, true, 1>(p, mode, l.groups, s) : launch_mode<D, false, 1>(p, mode, l.groups, s);
+    if (l.joins)
+        l.nw == 4 ? join_kernel<D, 4><<<l.joins, 256, 0, s>>>(p) : join_kernel<D, 1><<<l.joins, 256, 0, s>>>(p);
+}
+mk_status device_cus(uint32_t* cus)
+{
+    int dev = 0, n = 0;
+    MK_HIP(hipGetDevice(&dev));
+    MK_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
+    *cus = n > 0 ? uint32_t(n) : 1u;
+    return MK_OK;
+}
+bool any_rows(const mk_attn_packed_args* a)
+{
+    for (uint32_t i = 0; i < a->n_docs; ++i)
+        if (a->docs[i].q_rows)
+            return true;
+    return false;
+}
+
 } // namespace
 
 } // namespace mk
@@ -151,6 +626,16 @@ mk_status mk_attention_packed_workspace(const mk_attn_packed_args* a, uint64_t* 
         return fail(MK_ERR_ARG, "attention_packed_workspace: null argument");
     MK_TRY(check_shape(a));
     *bytes = 0;
+    if (!any_rows(a))
+        return MK_OK;
+    uint32_t cus = 1;
+    MK_TRY(device_cus(&cus));
+    PackedP p;
+    Launch l;
+    for (uint32_t i = 0; i < a->n_docs;) {
+        i += plan_launch(a, i, cus, true, p, l);
+        *bytes = std::max(*bytes, bytes_of(a, l)); // (launches run one after the other)
+    }
     return MK_OK;
 }
 
@@ -162,38 +647,46 @@ mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
     if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) || !aligned(a->workspace, 16) ||
         !aligned(a->slopes, 4))
         return fail(MK_ERR_ARG, "attention_packed: operands and workspace must be 16-byte aligned (slopes 4)");
-    uint64_t need = 0;
-    MK_TRY(mk_attention_packed_workspace(a, &need));
-    if (a->workspace && a->workspace_bytes < need)
-        return fail(MK_ERR_ARG, "attention_packed: the workspace is smaller than mk_attention_packed_workspace says");
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    PackedP p{static_cast<const uint16_t*>(a->q), static_cast<const uint16_t*>(a->k), static_cast<const uint16_t*>(a->v),
-              static_cast<uint16_t*>(a->out), a->ldq, a->ldk, a->ldv, a->ldo, a->slopes, a->scale, a->cap, a->heads,
-              a->heads / a->kv_heads, 0, a->out_dtype == MK_F16 ? 1u : 0u, {}};
-    uint32_t items = 0;
-    auto launch = [&]() {
-        if (!items)
-            return;
-        const dim3 grid(items, p.heads);
-        if (a->dtype == MK_F16)
-            a->d == 128 ? simple_kernel<true, 128><<<grid, 64, 0, s>>>(p) : simple_kernel<true, 64><<<grid, 64, 0, s>>>(p);
-        else
-            a->d == 128 ? simple_kernel<false, 128><<<grid, 64, 0, s>>>(p) : simple_kernel<false, 64><<<grid, 64, 0, s>>>(p);
-        p.n_docs = items = 0;
-    };
-    for (uint32_t i = 0; i < a->n_docs; ++i) {
-        const mk_attn_doc& d = a->docs[i];
-        if (!d.q_rows)
-            continue;
-        if (p.n_docs == kMaxDocs || uint64_t(items) + d.q_rows > (1u << 25))
-            launch();
-        p.docs[p.n_docs++] = Doc{items, d.q_row, d.q_rows, d.k_row, d.k_rows, d.q_pos, d.block, d.prefix};
-        items += d.q_rows;
-    }
-    if (!p.n_docs)
+    if (!any_rows(a))
         return MK_OK;
-    launch();
-    MK_LAUNCH_CHECK("attention_packed");
+    uint32_t cus = 1;
+    MK_TRY(device_cus(&cus));
+    PackedP p;
+    Launch l;
+    if (a->workspace) // before anything is launched
+        for (uint32_t i = 0; i < a->n_docs;) {
+            i += plan_launch(a, i, cus, true, p, l);
+            if (bytes_of(a, l) > a->workspace_bytes)
+                return fail(MK_ERR_ARG, "attention_packed: the workspace is smaller than mk_attention_packed_workspace says");
+        }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    constexpr float kLog2e = 1.4426950408889634f;
+    const int mode = a->cap > 0.0f ? kCap : a->slopes ? kBias : kPlain;
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.k = static_cast<const uint16_t*>(a->k);
+    p.v = static_cast<const uint16_t*>(a->v);
+    p.out = static_cast<uint16_t*>(a->out);
+    p.ldq = a->ldq;
+    p.ldk = a->ldk;
+    p.ldv = a->ldv;
+    p.ldo = a->ldo;
+    p.slopes = a->slopes;
+    p.c = mode == kCap ? 2.0f * kLog2e * a->scale / a->cap : a->scale * kLog2e;
+    p.cap = a->cap * kLog2e;
+    p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
+    p.group = a->heads / a->kv_heads;
+    p.out_f16 = a->out_dtype == MK_F16;
+    for (uint32_t i = 0; i < a->n_docs;) {
+        i += plan_launch(a, i, cus, a->workspace != nullptr, p, l);
+        if (!l.groups)
+            continue;
+        p.part = static_cast<float*>(a->workspace);
+        p.part_ml = p.part ? p.part + l.slots * (32 * l.nw) * a->d : nullptr;
+        const bool f16 = a->dtype == MK_F16;
+        a->d == 128 ? launch_all<128>(p, l, f16, mode, s) : launch_all<64>(p, l, f16, mode, s);
+        MK_LAUNCH_CHECK("attention_packed");
+    }
     return MK_OK;
 }
 

@@ -40,7 +40,7 @@ def attn(**kw):
     (dict(workspace=P + 4), "aligned"), (dict(slopes=P + 2), "aligned"),
     (dict(docs=[(0, 8, 0, 8, 0, 0, 0), (7, 2, 0, 8, 0, 0, 0)]), "share"), (dict(docs=[(10, 8, 0, 8, 0, 0, 0), (0, 11, 0, 8, 0, 0, 0)]), "share"),
     (dict(docs=[(0xFFFFFFF0, 100, 0, 8, 0, 0, 0)]), "2^31"), (dict(docs=[(0, 8, 0x7FFFFFFF, 1, 0, 0, 0)]), "2^31"),
-    (dict(docs=[(0, 8, 0, 8, 0x7FFFFFFF, 0, 0)]), "positions")])
+    (dict(docs=[(0, 8, 0, 8, 0x7FFFFFFF, 0, 0)]), "positions"), (dict(docs=[(0, (1 << 27) + 1, 0, 8, 0, 0, 0)]), "2^29")])
 def test_attention_packed_refusals(kw, match):
     if kw.get("docs", 0) is None:
         g = attn()
