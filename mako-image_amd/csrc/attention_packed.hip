@@ -12,21 +12,20 @@ namespace mk {
 
 namespace {
 
-constexpr uint32_t kMaxDocs = 80; // documents a launch: they go by kernel argument, in less than 4 KB
+constexpr uint32_t kMaxDocs = 64; // documents a launch: they go by kernel argument, in less than 4 KB
 constexpr int kKT = 64;           // keys a tile
 // The exponentials' reference m moves only when a weight against it passes 2^8 (below).
 constexpr float kLazyP = 256.0f;
 constexpr float kLeast = -1e30f; // m of rows without a score above -inf
 
 struct Doc {
-    uint32_t first; // its first workgroup, a multiple of 8
     uint32_t q_row, q_rows, k_row, k_rows;
     int32_t q_pos;
     uint32_t block, prefix;
     uint32_t blocks; // of 32 NW rows a key head
     uint32_t splits; // workgroups that share a block's keys
     uint32_t slot;   // its first partial result in the workspace, when splits > 1
-    uint32_t join;   // its first workgroup of the second launch
+    uint32_t pad;
 };
 struct PackedP {
     const uint16_t *q, *k, *v;
@@ -38,6 +37,8 @@ struct PackedP {
     float c;        // scale log2(e); with a cap: 2 scale log2(e) / cap
     float cap;      // cap log2(e)
     uint32_t heads, kv_heads, group, n_docs, out_f16;
+    uint32_t first[kMaxDocs]; // a document's first workgroup, a multiple of 8
+    uint32_t join[kMaxDocs];  // and that of the second launch
     Doc docs[kMaxDocs];
 };
 
@@ -71,14 +72,15 @@ __device__ inline int seen_keys(const Doc& d, int64_t pos)
     n = n < int64_t(d.k_rows) ? n : int64_t(d.k_rows);
     return int(n > 0 ? n : 0);
 }
-__device__ inline const Doc& find_doc(const PackedP& p, uint32_t item, bool join)
+// The document of a workgroup, by its place among their first ones (at most 64, ascending, the first 0). Arguments come from
+// host memory, 2 us and more a round trip, so all lanes compare at once: a search by halves took several.
+__device__ inline uint32_t find_doc(const uint32_t (&first)[kMaxDocs], uint32_t n, uint32_t item)
 {
-    uint32_t lo = 0, hi = p.n_docs;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        ((join ? p.docs[mid].join : p.docs[mid].first) <= item ? lo : hi) = mid;
-    }
-    return p.docs[lo];
+    static_assert(kMaxDocs <= 64, "one a lane");
+    if (n == 1)
+        return 0;
+    const uint32_t lane = threadIdx.x & 63, at = first[min(lane, n - 1)];
+    return __builtin_amdgcn_readfirstlane(uint32_t(__popcll(__ballot(lane < n && at <= item))) - 1);
 }
 
 enum { kPlain = 0, kBias = 1, kCap = 2 /* and a bias, of slope 0 without one */ };
@@ -97,11 +99,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
 
     const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hk = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Doc& doc = find_doc(p, blockIdx.x, false);
+    const uint32_t di = find_doc(p.first, p.n_docs, blockIdx.x);
+    const Doc doc = p.docs[di];
     // Workgroup i runs on XCD i % 8: each XCD takes a run of a document's (key head, block, split), whose blocks share keys in
     // its L2; later blocks, which see more under a causal mask, come first.
     const uint32_t each = doc.blocks * doc.splits, real = each * p.kv_heads, run = (real + 7) / 8;
-    const uint32_t local = blockIdx.x - doc.first, item = local % 8 * run + local / 8;
+    const uint32_t local = blockIdx.x - p.first[di], item = local % 8 * run + local / 8;
     if (local / 8 >= run || item >= real)
         return;
     const uint32_t kvh = item / each, block = doc.blocks - 1 - item % each / doc.splits, split = item % doc.splits;
@@ -429,35 +432,55 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
         store(std::false_type{});
 }
 
-// The splits of a row joined: a wave a row (4 a workgroup), D / 64 dims a lane.
+// The splits of a row joined: a workgroup a row, D / 4 lanes a split at 4 dims each, so 8 (or 16) splits at a time.
 template <int D, int NW> __global__ __launch_bounds__(256) void join_kernel(PackedP p)
 {
-    const Doc& doc = find_doc(p, blockIdx.x, true);
-    const uint32_t rows = doc.q_rows * p.group, lane = threadIdx.x & 63;
-    const uint32_t at = (blockIdx.x - doc.join) * 4 + (threadIdx.x >> 6);
+    constexpr uint32_t L = D / 4, G = 256 / L;
+    const uint32_t di = find_doc(p.join, p.n_docs, blockIdx.x);
+    const Doc doc = p.docs[di];
+    const uint32_t rows = doc.q_rows * p.group, at = blockIdx.x - p.join[di], g = threadIdx.x / L, e = threadIdx.x % L * 4;
     if (doc.splits < 2 || at >= rows * p.kv_heads)
         return;
     const uint32_t kvh = at / rows, row = at % rows, block = row / (32 * NW);
     // (blocks are numbered from the last one, as above)
     const uint64_t item = uint64_t(doc.slot) + (uint64_t(kvh) * doc.blocks + (doc.blocks - 1 - block)) * doc.splits;
     const uint64_t first = item * (32 * NW) + row % (32 * NW);
-    float m = kLeast;
-    for (uint32_t s = 0; s < doc.splits; ++s)
-        m = fmaxf(m, p.part_ml[2 * (first + uint64_t(s) * (32 * NW))]);
-    float l = 0.0f, o[D / 64] = {};
-    for (uint32_t s = 0; s < doc.splits; ++s) {
+    // each group of lanes its splits, against the largest m so far
+    float m = kLeast, l = 0.0f;
+    f32x4 o = f32x4{};
+#pragma unroll 4
+    for (uint32_t s = g; s < doc.splits; s += G) {
         const uint64_t i = first + uint64_t(s) * (32 * NW);
-        const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * i] - m);
-        l = fmaf(w, p.part_ml[2 * i + 1], l);
-#pragma unroll
-        for (int e = 0; e < D / 64; ++e)
-            o[e] = fmaf(w, p.part[i * D + lane * (D / 64) + e], o[e]);
+        const float ms = p.part_ml[2 * i], ls = p.part_ml[2 * i + 1];
+        const f32x4 os = *reinterpret_cast<const f32x4*>(p.part + i * D + e);
+        const float mn = fmaxf(m, ms), a = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(ms - mn);
+        m = mn;
+        l = l * a + w * ls;
+        o = o * a + w * os;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = p.out + (int64_t(doc.q_row) + row / p.group) * p.ldo + int64_t(kvh * p.group + row % p.group) * D + lane * (D / 64);
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e)
-        out[e] = p.out_f16 ? f2h_bits(o[e] * inv) : f2bf_bits(o[e] * inv);
+    __shared__ float sm[G], sl[G];
+    __shared__ __attribute__((aligned(16))) float so[G][D];
+    if (e == 0) {
+        sm[g] = m;
+        sl[g] = l;
+    }
+    *reinterpret_cast<f32x4*>(&so[g][e]) = o;
+    __syncthreads();
+    if (g)
+        return;
+    for (uint32_t i = 1; i < G; ++i)
+        m = fmaxf(m, sm[i]);
+    l = 0.0f;
+    o = f32x4{};
+    for (uint32_t i = 0; i < G; ++i) {
+        const float w = __builtin_amdgcn_exp2f(sm[i] - m);
+        l = fmaf(w, sl[i], l);
+        o += w * *reinterpret_cast<const f32x4*>(&so[i][e]);
+    }
+    o *= l == 0.0f ? 0.0f : 1.0f / l;
+    const bool h = p.out_f16;
+    *reinterpret_cast<u32x2*>(p.out + (int64_t(doc.q_row) + row / p.group) * p.ldo + int64_t(kvh * p.group + row % p.group) * D + e) =
+        u32x2{pack_x2(o[0], o[1], h), pack_x2(o[2], o[3], h)};
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -536,7 +559,7 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
         sum += uint64_t(cdiv(uint64_t(d.q_rows) * group, 128)) * a->kv_heads;
         if (n && sum > kMostGroups)
             break;
-        p.docs[n++] = Doc{0, d.q_row, d.q_rows, d.k_row, d.k_rows, d.q_pos, d.block, d.prefix, 0, 1, 0, 0};
+        p.docs[n++] = Doc{d.q_row, d.q_rows, d.k_row, d.k_rows, d.q_pos, d.block, d.prefix, 0, 1, 0, 0};
         most_rows = std::max(most_rows, uint64_t(d.q_rows) * group);
     }
     // longest first (at most kMaxDocs: an insertion sort)
@@ -546,29 +569,47 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
     // one wave a workgroup where all rows of a key head fit it: few rows over many keys
     out.nw = most_rows <= 32 ? 1 : 4;
     const uint32_t resident = cus * (out.nw == 4 || a->d == 128 ? 2 : 4);
-    uint64_t groups = 0, tiles = 0;
+    uint64_t tiles = 0, longest = 0;
     for (uint32_t i = 0; i < n; ++i) {
         Doc& d = p.docs[i];
         d.blocks = cdiv(uint64_t(d.q_rows) * group, 32 * out.nw);
-        groups += uint64_t(d.blocks) * a->kv_heads;
         tiles += uint64_t(d.blocks) * a->kv_heads * cdiv(d.k_rows, kKT);
+        longest = std::max<uint64_t>(longest, cdiv(d.k_rows, kKT));
     }
-    // fewer workgroups than the chip holds: keys are split so that each has about as many tiles, at least 2
-    const uint64_t target = split && groups < resident ? std::max<uint64_t>((tiles + resident - 1) / resident, 2) : ~0ull;
+    // How many tiles a workgroup takes at most: the halving of the longest document's with the least estimated time. A tile takes
+    // about 1.4 us where a compute unit has one workgroup; a split's partial results go to memory and back, at 4 TB/s, and are
+    // joined by a launch of 4 us. (us without and with splits: 1 row over 512 keys 15.7 / 9.7, 64 over 512 17.7 / 13.6, 512 over
+    // 512 18.8 / 33.7.)
+    auto items_of = [&](const Doc& d, uint64_t target) {
+        return uint64_t(d.blocks) * a->kv_heads * std::max<uint64_t>((cdiv(d.k_rows, kKT) + target - 1) / target, 1);
+    };
+    uint64_t target = std::max<uint64_t>(longest, 1);
+    double best = 1e300;
+    for (uint64_t t = target; split && t; t = t > 1 ? (t + 1) / 2 : 0) {
+        uint64_t part = 0;
+        for (uint32_t i = 0; i < n; ++i)
+            if (cdiv(p.docs[i].k_rows, kKT) > t)
+                part += items_of(p.docs[i], t);
+        const double bytes = double(part) * (32 * out.nw) * (a->d + 2) * 4;
+        const double time = std::max(double(t), double(tiles) / resident) * 1.4 + (part ? 4.0 + 2.0 * bytes / 4e6 : 0.0);
+        if (time < best) {
+            best = time;
+            target = t;
+        }
+    }
     uint64_t first = 0, join = 0;
     out.slots = 0;
     for (uint32_t i = 0; i < n; ++i) {
         Doc& d = p.docs[i];
-        const uint64_t t = cdiv(d.k_rows, kKT);
-        d.splits = t > target ? uint32_t((t + target - 1) / target) : 1;
-        d.first = uint32_t(first);
-        d.join = uint32_t(join);
+        const uint64_t items = items_of(d, target);
+        d.splits = uint32_t(items / (uint64_t(d.blocks) * a->kv_heads));
+        p.first[i] = uint32_t(first);
+        p.join[i] = uint32_t(join);
         d.slot = uint32_t(out.slots);
-        const uint64_t items = uint64_t(d.blocks) * a->kv_heads * d.splits;
         first += round_up(items, 8);
         if (d.splits > 1) {
             out.slots += items;
-            join += cdiv(uint64_t(d.q_rows) * a->heads, 4);
+            join += uint64_t(d.q_rows) * a->heads;
         }
     }
     p.n_docs = n;
