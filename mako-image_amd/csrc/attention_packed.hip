@@ -115,8 +115,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     const uint32_t qi = row / p.group, head = kvh * p.group + row % p.group;
     const int64_t pos = int64_t(doc.q_pos) + qi;
     const int lim = seen_keys(doc, pos);
-    const int wg_lim = seen_keys(doc, int64_t(doc.q_pos) + wg0 / p.group); // of the workgroup's first row: the least
-    const int wave_lim = seen_keys(doc, int64_t(doc.q_pos) + min(w0, rows - 1) / p.group); // of the wave's
+    const int64_t wg_pos = int64_t(doc.q_pos) + wg0 / p.group;
+    const int wg_lim = seen_keys(doc, wg_pos); // of the workgroup's first row: the least
     const int wave_most = seen_keys(doc, int64_t(doc.q_pos) + min(w0 + 31, rows - 1) / p.group);
     const int all_tiles = (seen_keys(doc, int64_t(doc.q_pos) + wg_last / p.group) + kKT - 1) / kKT;
     const int t_begin = int(uint64_t(all_tiles) * split / doc.splits), t_end = int(uint64_t(all_tiles) * (split + 1) / doc.splits);
@@ -132,17 +132,21 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     // read takes do
     auto kswz = [](int key, int c) { return KC == 16 ? c ^ (key & 15) : c ^ ((key >> 1) & 7); };
     auto vswz = [](int key, int c) { return KC == 16 ? c ^ ((key & 3) << 2) : c ^ ((key & 2) << 1); };
-    uint32_t ok[RL], ov[RL];
+    // A lane's byte offset of each direct load. Loads VO apart have the same swizzle, so they differ by whole rows: a scalar.
+    constexpr int VO = NW == 4 ? 1 : D / 32, VK = VO * 64 * NW / KC; // VK: rows between them
+    static_assert(VK % 16 == 0 && RL % VO == 0, "");
+    uint32_t ok[VO], ov[VO];
 #pragma unroll
-    for (int i = 0; i < RL; ++i) {
+    for (int i = 0; i < VO; ++i) {
         const int P = (i * NW + wave) * 64 + lane, key = P / KC, c = P % KC;
         ok[i] = (uint32_t(key) * uint32_t(p.ldk) + kswz(key, c) * 8) * 2;
         ov[i] = (uint32_t(key) * uint32_t(p.ldv) + vswz(key, c) * 8) * 2;
     }
+    const uint32_t sk = VK * uint32_t(p.ldk) * 2, sv = VK * uint32_t(p.ldv) * 2;
     const uint16_t* K = p.k + int64_t(doc.k_row) * p.ldk + int64_t(kvh) * D;
     const uint16_t* V = p.v + int64_t(doc.k_row) * p.ldv + int64_t(kvh) * D;
-    // a tile's resources end with the document's last key: what lies behind it comes as zeros (a tile past the last: nothing)
-    auto tile_keys = [&](int t) { return t < t_end ? min(int(doc.k_rows) - t * kKT, kKT) : 0; };
+    // a tile's resources end with the document's last key: what lies behind it comes as zeros (no tile, -1: nothing)
+    auto tile_keys = [&](int t) { return t >= 0 ? min(int(doc.k_rows) - t * kKT, kKT) : 0; };
     auto res_of = [&](const uint16_t* base, int64_t ld, int t) {
         const int n = tile_keys(t);
         return buf_res(n ? base + int64_t(t) * kKT * ld : base, n ? uint32_t((n - 1) * int(ld) + D) * 2 : 0u);
@@ -150,9 +154,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     // load i of tile t's 2 RL into buffer buf
     auto dma = [&](const BufRes& rk, const BufRes& rv, int buf, int i) {
         if (i < RL)
-            buf_load_lds16(rk, (lds_void*)&sK(buf)[(i * NW + wave) * 512], ok[i], 0);
+            buf_load_lds16(rk, (lds_void*)&sK(buf)[(i * NW + wave) * 512], ok[i % VO], i / VO * sk);
         else if (i < 2 * RL)
-            buf_load_lds16(rv, (lds_void*)&sV(buf)[((i - RL) * NW + wave) * 512], ov[i - RL], 0);
+            buf_load_lds16(rv, (lds_void*)&sV(buf)[((i - RL) * NW + wave) * 512], ov[(i - RL) % VO], (i - RL) / VO * sv);
     };
 
     f32x16 oacc[DT];
@@ -162,39 +166,46 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     float m = kLeast, l = 0.0f;
     const float slope = MODE != kPlain && p.slopes ? p.slopes[head] * 1.4426950408889634f : 0.0f;
 
-    // score r of a half whose first key is k0, in log2 units, less `from`
-    auto score = [&](float s, int k0, int r, float from) {
+    // What a lane knows of a half of a tile: its row's position less the lane's first key (values r are 8 (r / 4) + r % 4 keys
+    // further), and how many keys the row sees from that one on.
+    struct Half {
+        float rel;
+        int more;
+    };
+    auto half_of = [&](int k0) {
+        return Half{MODE == kPlain ? 0.0f : float(pos - k0 - 4 * hk), lim - k0 - 4 * hk};
+    };
+    // score r of a half in log2 units, less `from`
+    auto score = [&](float s, const Half& h, int r, float from) {
         float x;
         if constexpr (MODE == kCap) // cap tanh(y) = cap - 2 cap / (1 + e^2y)
             x = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * p.c)), p.cap - from);
         else
             x = fmaf(s, p.c, -from);
-        if constexpr (MODE != kPlain) {
-            const float dist = float(pos - k0 - 4 * hk) - float(8 * (r / 4) + r % 4);
-            x = fmaf(-slope, fabsf(dist), x);
-        }
+        if constexpr (MODE != kPlain)
+            x = fmaf(-slope, fabsf(h.rel - float(8 * (r / 4) + r % 4)), x);
         return x;
     };
-    auto masked = [&](float x, int k0, int r) { return k0 + 8 * (r / 4) + 4 * hk + r % 4 < lim ? x : -__builtin_inff(); };
+    auto masked = [](float x, const Half& h, int r) { return 8 * (r / 4) + r % 4 < h.more ? x : -__builtin_inff(); };
     // the weights of pair j of a half, packed, and their sum
-    auto pair = [&](const f32x16& sc, int k0, int j, uint32_t (&pw)[8], float& ls, auto edge_c) {
-        float x0 = score(sc[2 * j], k0, 2 * j, m), x1 = score(sc[2 * j + 1], k0, 2 * j + 1, m);
+    auto pair = [&](const f32x16& sc, const Half& h, int j, uint32_t (&pw)[8], float& ls, auto edge_c) {
+        float x0 = score(sc[2 * j], h, 2 * j, m), x1 = score(sc[2 * j + 1], h, 2 * j + 1, m);
         if constexpr (decltype(edge_c)::value) {
-            x0 = masked(x0, k0, 2 * j);
-            x1 = masked(x1, k0, 2 * j + 1);
+            x0 = masked(x0, h, 2 * j);
+            x1 = masked(x1, h, 2 * j + 1);
         }
         const float e0 = __builtin_amdgcn_exp2f(x0), e1 = __builtin_amdgcn_exp2f(x1);
         pw[j] = pack_x2(e0, e1, F16);
         ls += e0 + e1;
     };
     // moves m up to a half's largest score, rescales what was summed against the old one, and makes the half's weights again
-    auto redo = [&](const f32x16& sc, int k0, uint32_t (&pw)[8], float& ls, auto edge_c) {
+    auto redo = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, auto edge_c) {
         f32x16 x;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            x[r] = score(sc[r], k0, r, 0.0f);
+            x[r] = score(sc[r], h, r, 0.0f);
             if constexpr (decltype(edge_c)::value)
-                x[r] = masked(x[r], k0, r);
+                x[r] = masked(x[r], h, r);
         }
         const float mn = fmaxf(m, max_xor32(max16(x))), alpha = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
@@ -207,7 +218,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
         ls = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            pair(sc, k0, j, pw, ls, edge_c);
+            pair(sc, h, j, pw, ls, edge_c);
     };
     auto read_k = [&](int buf, int kt, int ds) {
         const int key = kt * 32 + r32;
@@ -288,11 +299,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     // products P V of half a. A lane's part of their sum decides afterwards whether a half is made again against a new m:
     // a score more than 8 (in log2 units) above m puts that sum above 2^8.
     constexpr int LA = 4, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
-    auto tile = [&](int t, auto buf_c, auto edge_c) {
+    auto tile = [&](int t, int next, auto buf_c, auto edge_c) {
         constexpr int buf = decltype(buf_c)::value;
         constexpr bool EDGE = decltype(edge_c)::value;
         const int k0 = t * kKT;
-        const BufRes rk = res_of(K, p.ldk, t + 1), rv = res_of(V, p.ldv, t + 1);
+        const BufRes rk = res_of(K, p.ldk, next), rv = res_of(V, p.ldv, next);
         if (EDGE && k0 >= wave_most) { // no row of the wave sees the tile
 #pragma unroll
             for (int i = 0; i < 2 * RL; ++i)
@@ -324,10 +335,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
                 dma(rk, rv, buf ^ 1, i);
             __builtin_amdgcn_sched_barrier(0);
         }
-        auto chunk = [&](const f32x16& sc, int kh, uint32_t (&pw)[8], float& ls, int c) {
+        const Half ha = half_of(k0), hb = half_of(k0 + 32);
+        auto chunk = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, int c) {
 #pragma unroll
             for (int j = c * CH; j < (c + 1) * CH; ++j) {
-                pair(sc, kh, j, pw, ls, edge_c);
+                pair(sc, h, j, pw, ls, edge_c);
                 // (pinned here: the compiler would sink the work into the path that keeps it)
                 asm volatile("" : "+v"(pw[j]), "+v"(ls));
             }
@@ -338,11 +350,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
             __builtin_amdgcn_sched_barrier(0);
             rd(DS + ds + LA);
             __builtin_amdgcn_sched_barrier(0);
-            chunk(s_a, k0, pa, la, ds);
+            chunk(s_a, ha, pa, la, ds);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (__any(la > kLazyP))
-            redo(s_a, k0, pa, la, edge_c);
+            redo(s_a, ha, pa, la, edge_c);
         l += la;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -352,11 +364,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
             __builtin_amdgcn_sched_barrier(0);
             rd(2 * DS + j + LA);
             __builtin_amdgcn_sched_barrier(0);
-            chunk(s_b, k0 + 32, pb, lb, j);
+            chunk(s_b, hb, pb, lb, j);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (__any(lb > kLazyP))
-            redo(s_b, k0 + 32, pb, lb, edge_c);
+            redo(s_b, hb, pb, lb, edge_c);
         l += lb;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -368,29 +380,52 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto step = [&](int t, auto buf_c) {
+    // Masks only cut the last keys off. The tiles that they cut for some row of the workgroup come first, the last one before the
+    // others, then those that all rows see, in a loop of its own (one loop with a branch in it spilled registers): with a
+    // bias from the tile of the first row's own position downwards and then upwards from there, so that scores fall away
+    // from the start and m seldom moves (4096 rows of 20 heads of 64 upwards throughout: 348 us).
+    const int edges = t_end - max(min(wg_lim / kKT, t_end), t_begin), fulls = t_end - t_begin - edges;
+    const int own = MODE == kPlain ? fulls - 1 : max(min(int(wg_pos / kKT) - t_begin, fulls - 1), 0);
+    auto tile_at = [&](int i) {
+        const int j = i - edges;
+        return i >= edges + fulls ? -1 : j < 0 ? t_end - 1 - i : t_begin + (j <= own ? own - j : j);
+    };
+    auto step = [&](int i, auto buf_c, auto edge_c) {
+        const int t = tile_at(i);
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        const bool odd = wg_lim < min(t * kKT + kKT, int(doc.k_rows)) && find_odd(t, buf_c);
-        if (t * kKT + kKT > wave_lim)
-            tile(t, buf_c, std::true_type{});
-        else
-            tile(t, buf_c, std::false_type{});
-        if (odd)
+        bool odd = false;
+        if constexpr (decltype(edge_c)::value)
+            odd = wg_lim < min(t * kKT + kKT, int(doc.k_rows)) && find_odd(t, buf_c);
+        tile(t, tile_at(i + 1), buf_c, edge_c);
+        if (decltype(edge_c)::value && odd)
             add_odd(t);
     };
     if (tid == 0)
         odd_tile = 0; // (the first step's barrier is behind it)
     if (t_begin < t_end) {
-        const BufRes rk = res_of(K, p.ldk, t_begin), rv = res_of(V, p.ldv, t_begin);
+        const int t = tile_at(0);
+        const BufRes rk = res_of(K, p.ldk, t), rv = res_of(V, p.ldv, t);
 #pragma unroll
         for (int i = 0; i < 2 * RL; ++i)
             dma(rk, rv, 0, i);
     }
-    for (int t = t_begin; t < t_end; t += 2) {
-        step(t, std::integral_constant<int, 0>{});
-        if (t + 1 < t_end)
-            step(t + 1, std::integral_constant<int, 1>{});
+    constexpr std::integral_constant<int, 0> b0{};
+    constexpr std::integral_constant<int, 1> b1{};
+    int i = 0;
+    for (; i + 1 < edges; i += 2) {
+        step(i, b0, std::true_type{});
+        step(i + 1, b1, std::true_type{});
+    }
+    if (i < edges) {
+        step(i++, b0, std::true_type{});
+        if (i < edges + fulls)
+            step(i++, b1, std::false_type{});
+    }
+    for (; i < edges + fulls; i += 2) {
+        step(i, b0, std::false_type{});
+        if (i + 1 < edges + fulls)
+            step(i + 1, b1, std::false_type{});
     }
     __builtin_amdgcn_s_waitcnt(0);
 
