@@ -83,10 +83,13 @@ __device__ inline uint32_t find_doc(const uint32_t (&first)[kMaxDocs], uint32_t 
     return __builtin_amdgcn_readfirstlane(uint32_t(__popcll(__ballot(lane < n && at <= item))) - 1);
 }
 
-enum { kPlain = 0, kBias = 1, kCap = 2 /* and a bias, of slope 0 without one */ };
+enum { kPlain = 0, kBias = 1, kCap = 2 /* a bit each */ };
+
+// Waves a SIMD that the registers have to leave room for.
+constexpr int waves_of(int d, int nw) { return nw == 1 ? 1 : d == 64 ? 3 : 2; }
 
 template <int D, bool F16, int MODE, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 2 : 1, NW == 4 ? 2 : 1))) void packed_kernel(PackedP p)
+__global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_waves_per_eu(waves_of(D, NW), waves_of(D, NW)))) void packed_kernel(PackedP p)
 {
     constexpr int DS = D / 16, DT = D / 32, KC = D / 8; // k steps of S, 32-dim blocks of O, 16-byte chunks of a row
     constexpr int RL = kKT * KC / (64 * NW);            // direct loads a wave and operand
@@ -164,7 +167,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     for (int dt = 0; dt < DT; ++dt)
         oacc[dt] = f32x16{};
     float m = kLeast, l = 0.0f;
-    const float slope = MODE != kPlain && p.slopes ? p.slopes[head] * 1.4426950408889634f : 0.0f;
+    const float slope = MODE & kBias ? p.slopes[head] * 1.4426950408889634f : 0.0f;
 
     // What a lane knows of a half of a tile: its row's position less the lane's first key (values r are 8 (r / 4) + r % 4 keys
     // further), and how many keys the row sees from that one on.
@@ -173,16 +176,16 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
         int more;
     };
     auto half_of = [&](int k0) {
-        return Half{MODE == kPlain ? 0.0f : float(pos - k0 - 4 * hk), lim - k0 - 4 * hk};
+        return Half{MODE & kBias ? float(pos - k0 - 4 * hk) : 0.0f, lim - k0 - 4 * hk};
     };
     // score r of a half in log2 units, less `from`
     auto score = [&](float s, const Half& h, int r, float from) {
         float x;
-        if constexpr (MODE == kCap) // cap tanh(y) = cap - 2 cap / (1 + e^2y)
+        if constexpr (MODE & kCap) // cap tanh(y) = cap - 2 cap / (1 + e^2y)
             x = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * p.c)), p.cap - from);
         else
             x = fmaf(s, p.c, -from);
-        if constexpr (MODE != kPlain)
+        if constexpr (MODE & kBias)
             x = fmaf(-slope, fabsf(h.rel - float(8 * (r / 4) + r % 4)), x);
         return x;
     };
@@ -298,7 +301,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     // the tile's largest score is known: those of half a between the products S^T of half b, those of half b between the
     // products P V of half a. A lane's part of their sum decides afterwards whether a half is made again against a new m:
     // a score more than 8 (in log2 units) above m puts that sum above 2^8.
-    constexpr int LA = 4, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
+    constexpr int LA = 3, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
     auto tile = [&](int t, int next, auto buf_c, auto edge_c) {
         constexpr int buf = decltype(buf_c)::value;
         constexpr bool EDGE = decltype(edge_c)::value;
@@ -385,7 +388,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
     // bias from the tile of the first row's own position downwards and then upwards from there, so that scores fall away
     // from the start and m seldom moves (4096 rows of 20 heads of 64 upwards throughout: 348 us).
     const int edges = t_end - max(min(wg_lim / kKT, t_end), t_begin), fulls = t_end - t_begin - edges;
-    const int own = MODE == kPlain ? fulls - 1 : max(min(int(wg_pos / kKT) - t_begin, fulls - 1), 0);
+    const int own = !(MODE & kBias) ? fulls - 1 : max(min(int(wg_pos / kKT) - t_begin, fulls - 1), 0);
     auto tile_at = [&](int i) {
         const int j = i - edges;
         return i >= edges + fulls ? -1 : j < 0 ? t_end - 1 - i : t_begin + (j <= own ? own - j : j);
@@ -428,11 +431,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
             step(i + 1, b1, std::false_type{});
     }
     __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads(); // the tiles' LDS is free
 
     const float lt = add_xor32(l);
-    if (w0 + r32 >= rows)
-        return;
     if (doc.splits > 1) {
+        if (w0 + r32 >= rows)
+            return;
         const uint64_t at = (uint64_t(doc.slot) + item) * (32 * NW) + wave * 32 + r32;
         float* o = p.part + at * D + 4 * hk;
 #pragma unroll
@@ -448,23 +452,36 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) __attribute__((amdgpu_wav
         }
         return;
     }
+    // The output through LDS (32 rows a wave, 16-byte chunks XOR-ed with the row), so that whole rows of a head leave 16 bytes a
+    // lane (8-byte pieces of 32 rows at a time: 4.4 us more of the 24 that 6453 x 20 heads of 64 over 77 to 231 keys took).
     const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-    uint16_t* o = p.out + (int64_t(doc.q_row) + qi) * p.ldo + int64_t(head) * D + 4 * hk;
-    auto store = [&](auto h_c) {
+    uint16_t* so = (wave & 2 ? sV0 : sK0) + (wave & 1) * (32 * D);
+    auto stage = [&](auto h_c) {
         constexpr bool H = decltype(h_c)::value;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x16& a = oacc[dt];
-                *reinterpret_cast<u32x2*>(o + dt * 32 + 8 * i) = u32x2{pack_x2(a[4 * i] * inv, a[4 * i + 1] * inv, H),
-                                                                       pack_x2(a[4 * i + 2] * inv, a[4 * i + 3] * inv, H)};
+                *reinterpret_cast<u32x2*>(so + r32 * D + ((dt * 4 + i) ^ (r32 % KC)) * 8 + 4 * hk) = u32x2{
+                    pack_x2(a[4 * i] * inv, a[4 * i + 1] * inv, H), pack_x2(a[4 * i + 2] * inv, a[4 * i + 3] * inv, H)};
             }
     };
     if (p.out_f16)
-        store(std::true_type{});
+        stage(std::true_type{});
     else
-        store(std::false_type{});
+        stage(std::false_type{});
+    __builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0): this wave's LDS writes done
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < KC / 2; ++j) {
+        const int r = j * (64 / KC) + lane / KC, c = lane % KC;
+        if (w0 + r >= rows)
+            continue;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(so + r * D + (c ^ (r % KC)) * 8);
+        const uint32_t rr = w0 + r, qr = p.group == 1 ? rr : rr / p.group, hh = p.group == 1 ? kvh : kvh * p.group + rr % p.group;
+        *reinterpret_cast<u32x4*>(p.out + (int64_t(doc.q_row) + qr) * p.ldo + int64_t(hh) * D + c * 8) = v;
+    }
 }
 
 // The splits of a row joined: a workgroup a row, D / 4 lanes a split at 4 dims each, so 8 (or 16) splits at a time.
@@ -660,8 +677,10 @@ template <int D, bool F16, int NW> void launch_mode(const PackedP& p, int mode, 
         packed_kernel<D, F16, kPlain, NW><<<groups, 64 * NW, 0, s>>>(p);
     else if (mode == kBias)
         packed_kernel<D, F16, kBias, NW><<<groups, 64 * NW, 0, s>>>(p);
-    else
+    else if (mode == kCap)
         packed_kernel<D, F16, kCap, NW><<<groups, 64 * NW, 0, s>>>(p);
+    else
+        packed_kernel<D, F16, kCap | kBias, NW><<<groups, 64 * NW, 0, s>>>(p);
 }
 template <int D> void launch_all(const PackedP& p, const Launch& l, bool f16, int mode, hipStream_t s)
 {
@@ -737,7 +756,7 @@ mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
         }
     hipStream_t s = static_cast<hipStream_t>(stream);
     constexpr float kLog2e = 1.4426950408889634f;
-    const int mode = a->cap > 0.0f ? kCap : a->slopes ? kBias : kPlain;
+    const int mode = (a->cap > 0.0f ? kCap : 0) | (a->slopes ? kBias : 0);
     p.q = static_cast<const uint16_t*>(a->q);
     p.k = static_cast<const uint16_t*>(a->k);
     p.v = static_cast<const uint16_t*>(a->v);
@@ -747,7 +766,7 @@ mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
     p.ldv = a->ldv;
     p.ldo = a->ldo;
     p.slopes = a->slopes;
-    p.c = mode == kCap ? 2.0f * kLog2e * a->scale / a->cap : a->scale * kLog2e;
+    p.c = mode & kCap ? 2.0f * kLog2e * a->scale / a->cap : a->scale * kLog2e;
     p.cap = a->cap * kLog2e;
     p.heads = a->heads;
     p.kv_heads = a->kv_heads;
