@@ -351,7 +351,8 @@ typedef struct mk_lora_rows_args {
     const void* base;    /* [rows][ldbase] or NULL (0); may be c itself (then ldbase == ldc) */
     void* c;             /* [rows][ldc] */
     int64_t ldx, ldbase, ldc; /* elements between rows, multiples of 8 below 2^23 */
-    uint32_t rows, K, N; /* K a multiple of 8, N of 8 parts, both up to 2^22; rows up to 2^28 */
+    uint32_t rows, K, N; /* K a multiple of 8, N of 8 parts, both up to 2^22; rows up to 2^28, rows times K
+                            below 2^41 */
     uint32_t rank;       /* of each part, a multiple of 8 up to 256 */
     uint32_t parts;      /* 1 to 4 */
     uint32_t adapters;   /* at least 1 */

@@ -52,6 +52,8 @@ template <bool F16> __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+constexpr uint32_t kOut = 0x80000000u; // a byte offset past every buffer resource here
+constexpr int kRows = 64;              // rows of a workgroup of the second product
 // the smallest adapter above `last` among a wave's rows (a lane's row each), or INT_MAX
 __device__ inline int next_adapter(int id, int last)
 {
@@ -106,11 +108,14 @@ template <bool F16> __global__ __launch_bounds__(256) void shrink_vec(LoraP p)
 // Many rows: a tile of 64 rows by 32 NB of A's rows and one split of K. Each of the four waves takes every fourth 32 k for the
 // whole tile, through three stages of LDS of its own (direct loads, two steps ahead, no barriers in the loop; nothing is read
 // from LDS twice), and the waves' sums are added at the end. A tile with rows of several adapters goes through K for each.
-constexpr int kRows = 64, kStepK = 128;
+// 16401 rows of 12288, rank 64: 128 us, 3.1 TB/s of x, of 3.6 to 4.0 TB/s that a reduction's reads reach. No faster: two or four
+// stages, 128 rows a tile (160 us), a line of 128 bytes a row and wave, K begun elsewhere in every tile, and all tiles' steps
+// shared evenly by as many workgroups as the chip holds (139 us, and more partial results to add).
+constexpr int kStepK = 128;
 template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(LoraP p)
 {
-    constexpr int XB = kRows * 64, AB = 32 * NB * 64, WB = XB + AB; // bytes of a wave's stage
-    constexpr int NX = XB / 1024, ND = WB / 1024;                   // direct loads of x, of both
+    constexpr int XB = kRows * 64, AB = NB * 2048, WB = XB + AB;   // bytes of a wave's stage
+    constexpr int NX = XB / 1024, ND = WB / 1024;                 // direct loads of x, of both
     __shared__ __attribute__((aligned(16))) uint8_t s0[4 * WB], s1[4 * WB], s2[4 * WB];
     const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hk = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -123,25 +128,21 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
     const BufRes rx = buf_res(p.x + int64_t(row0) * p.ldx, uint32_t(((rows - 1) * p.ldx + p.K) * 2));
     // byte offset of a lane's 16 bytes of each load, and their k: LDS rows of 64 bytes whose chunk c holds k chunk
     // c ^ ((row >> 2) & 3), so the 16-byte fragment reads of 8 rows fall on all banks
-    uint32_t off[ND], kof;
-    const int slot = lane & 3;
-    {
-        const int c = slot ^ ((lane >> 4) & 3); // (row >> 2) & 3 of row 16 j + lane / 4
-        kof = uint32_t(wave * 32 + c * 8);
+    uint32_t off[ND];
+    const uint32_t kof = uint32_t(wave * 32 + ((lane & 3) ^ ((lane >> 4) & 3)) * 8); // ((row >> 2) & 3 of row 16 j + lane / 4)
 #pragma unroll
-        for (int j = 0; j < ND; ++j) {
-            const uint32_t r = uint32_t((j < NX ? j : j - NX) * 16 + lane / 4);
-            off[j] = j < NX ? min(r, rows - 1) * uint32_t(p.ldx) * 2 : min(r, width - i0 - 1) * p.K * 2;
-        }
+    for (int j = 0; j < ND; ++j) {
+        const uint32_t r = uint32_t((j < NX ? j : j - NX) * 16 + lane / 4);
+        off[j] = j < NX ? min(r, rows - 1) * uint32_t(p.ldx) * 2 : min(r, width - i0 - 1) * p.K * 2;
     }
     for (int a = next_adapter(mine, -1); a != 0x7fffffff; a = next_adapter(mine, a)) {
         const BufRes ra = buf_res(p.a + (int64_t(a) * width + i0) * p.K, uint32_t(min(uint32_t(32 * NB), width - i0) * p.K * 2));
         auto issue = [&](int s, uint8_t* buf) {
             // behind the split's end: past the resource, so zeros come
-            const uint32_t k = kb + uint32_t(s) * kStepK + kof, v = k < ke ? k * 2 : 0x80000000u;
+            const uint32_t k = kb + uint32_t(s) * kStepK + kof;
 #pragma unroll
             for (int j = 0; j < ND; ++j)
-                buf_load_lds16(j < NX ? rx : ra, (lds_void*)(buf + wave * WB + j * 1024), k < ke ? off[j] + v : v, 0);
+                buf_load_lds16(j < NX ? rx : ra, (lds_void*)(buf + wave * WB + j * 1024), k < ke ? off[j] + k * 2 : kOut, 0);
         };
         f32x16 acc[2][NB];
 #pragma unroll
@@ -149,10 +150,10 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
 #pragma unroll
             for (int j = 0; j < NB; ++j)
                 acc[i][j] = f32x16{};
-        auto step = [&](int s, uint8_t* cur, uint8_t* next) {
+        auto step = [&](int s, uint8_t* cur, uint8_t* into) {
             if (s >= steps)
                 return;
-            issue(s + 2, next);
+            issue(s + 2, into);
             __builtin_amdgcn_s_waitcnt(wait_vm(2 * ND)); // step s landed, the next two may be in flight
             const uint8_t* b = cur + wave * WB;
 #pragma unroll
@@ -180,26 +181,32 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
             step(s + 2, s2, s1);
         }
         __builtin_amdgcn_s_waitcnt(0); // the last (unused) loads land before the LDS is reused
-        // the waves' sums, 32 x 32 at a time: lane's values 4 g .. 4 g + 3 are A rows 8 g + 4 hk .. + 3 of x row r32
+        // the waves' sums: a lane's values 4 g .. 4 g + 3 are A rows 8 g + 4 hk .. + 3 of x row r32
         float* red = reinterpret_cast<float*>(s0);
+        constexpr int JB = 4 * WB / 16384 < NB ? 4 * WB / 16384 : NB; // 32 x 32 sums of the four waves that a stage holds
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int ij = 0; ij < 2 * NB; ij += JB) {
+            __syncthreads();
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                __syncthreads();
+            for (int q = ij; q < ij + JB && q < 2 * NB; ++q) {
+                const f32x16& v = acc[q / NB][q % NB];
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(red + ((wave * 4 + g) * 64 + lane) * 4) =
-                        f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                __syncthreads();
-                f32x4 v = *reinterpret_cast<const f32x4*>(red + (wave * 64 + lane) * 4);
+                    *reinterpret_cast<f32x4*>(red + ((((q - ij) * 4 + wave) * 4 + g) * 64 + lane) * 4) =
+                        f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+            }
+            __syncthreads();
+#pragma unroll
+            for (int q = ij; q < ij + JB && q < 2 * NB; ++q) {
+                f32x4 v = *reinterpret_cast<const f32x4*>(red + (((q - ij) * 16 + wave) * 64 + lane) * 4);
 #pragma unroll
                 for (int w = 1; w < 4; ++w)
-                    v += *reinterpret_cast<const f32x4*>(red + ((w * 4 + wave) * 64 + lane) * 4);
-                const uint32_t r = i * 32 + r32, n = i0 + j * 32 + wave * 8 + hk * 4;
+                    v += *reinterpret_cast<const f32x4*>(red + ((((q - ij) * 4 + w) * 4 + wave) * 64 + lane) * 4);
+                const uint32_t r = q / NB * 32 + r32, n = i0 + q % NB * 32 + wave * 8 + hk * 4;
                 if (__shfl(mine, int(r)) == a && n < width)
                     *reinterpret_cast<f32x4*>(p.t + (int64_t(split) * p.rows + row0 + r) * width + n) = v;
             }
+        }
         __syncthreads(); // before the next adapter's loads
     }
 }
@@ -208,13 +215,22 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
 // c = base + scale t B^T
 // ------------------------------------------------------------------------------------------------------------
 
-// the sum of the splits' partial t, 4 of a row
+// the sum of the splits' partial t, 4 of a row, in their order; 8 loads at a time (one after the other, 16 splits took 8 us)
 __device__ inline f32x4 load_t(const LoraP& p, uint32_t row, uint32_t i)
 {
-    const int64_t width = int64_t(p.parts) * p.rank, at = int64_t(row) * width + i;
-    f32x4 v = *reinterpret_cast<const f32x4*>(p.t + at);
-    for (uint32_t s = 1; s < p.splits; ++s)
-        v += *reinterpret_cast<const f32x4*>(p.t + s * (p.rows * width) + at);
+    const int64_t width = int64_t(p.parts) * p.rank, step = p.rows * width;
+    const float* t = p.t + row * width + i;
+    f32x4 v = *reinterpret_cast<const f32x4*>(t);
+    for (uint32_t s = 1; s < p.splits; s += 8) {
+        f32x4 w[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            w[j] = *reinterpret_cast<const f32x4*>(t + min(s + j, p.splits - 1) * step);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            if (s + j < p.splits)
+                v += w[j];
+    }
     return v;
 }
 template <uint32_t CT> __device__ inline float load_c(const void* c, int64_t at)
@@ -223,7 +239,6 @@ template <uint32_t CT> __device__ inline float load_c(const void* c, int64_t at)
 }
 
 // 4 values through a buffer resource; past it zeros come, and nothing is stored
-constexpr uint32_t kOut = 0x80000000u;
 template <class V> __device__ inline V load_v(BufRes r, uint32_t voff, uint32_t soff)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -285,7 +300,8 @@ template <bool F16, uint32_t CT> __global__ __launch_bounds__(256) void expand_v
 // outputs; half t after a power of two that puts the row's largest near 2^14, so that none is lost below the half range). In the product C = T B^T a wave's
 // four column tiles take columns 4 j + tile: a lane then has 4 columns next to each other of each of its rows, and base and c
 // go by 8 or 16 bytes a lane, 256 or 512 next to each other.
-template <bool F16, uint32_t CT> __global__ __launch_bounds__(256, CT == MK_F32 ? 2 : 3) void expand_tile(LoraP p)
+// FUSE: both 32-row halves of the tile at once, so that B is read once.
+template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2) void expand_tile(LoraP p)
 {
     constexpr int NV = CT == MK_F32 && !F16 ? 3 : 2;
     constexpr uint32_t SZ = CT == MK_F32 ? 4 : 2;
@@ -349,47 +365,74 @@ template <bool F16, uint32_t CT> __global__ __launch_bounds__(256, CT == MK_F32 
                 break;
             const uint32_t col = c0 + r32 * 4;
             const bool in = col < per; // (per is a multiple of 8: all 4 of a lane's columns, or none)
-#pragma unroll 1
-            for (uint32_t rt = 0; rt < 2; ++rt) {
-                const uint32_t has = uint32_t(on >> (32 * rt));
-                if (!has)
-                    continue;
-                // A lane's rows of the tile are 8 (i / 4) + 4 hk + i % 4. Their base and c by buffer loads and stores: one
-                // byte offset a lane and a scalar one a row; what is not the adapter's goes past the resource.
-                const uint32_t tr = min(rows - rt * 32, 32u);
-                const int64_t r0 = int64_t(row0) + rt * 32;
-                const BufRes rb = buf_res(p.base ? static_cast<const char*>(p.base) + (r0 * p.ldbase + part * per) * SZ : nullptr,
-                                          p.base ? uint32_t((tr - 1) * p.ldbase + per) * SZ : 0u);
-                const BufRes rc = buf_res(static_cast<const char*>(p.c) + (r0 * p.ldc + part * per) * SZ, uint32_t((tr - 1) * p.ldc + per) * SZ);
-                const uint32_t vb = (4 * hk * uint32_t(p.ldbase) + col) * SZ, vc = (4 * hk * uint32_t(p.ldc) + col) * SZ;
-                const uint32_t lane_has = in ? has >> (4 * hk) : 0u;
-                auto row_of = [](int i) { return uint32_t(8 * (i / 4) + i % 4); };
-                V basev[16];
+            // A lane's rows of a 32-row half are 8 (i / 4) + 4 hk + i % 4. Their base and c by buffer loads and stores: one byte
+            // offset a lane and a scalar one a row; what is not the adapter's goes past the resource.
+            auto row_of = [](int i) { return uint32_t(8 * (i / 4) + i % 4); };
+            auto has_of = [&](uint32_t rt) { return in ? uint32_t(on >> (32 * rt)) >> (4 * hk) : 0u; };
+            auto res_of = [&](const void* x, int64_t ld, uint32_t rt) {
+                const uint32_t tr = rows > rt * 32 ? min(rows - rt * 32, 32u) : 0u;
+                return buf_res(static_cast<const char*>(x) + ((int64_t(row0) + rt * 32) * ld + part * per) * SZ,
+                               x && tr ? uint32_t((tr - 1) * ld + per) * SZ : 0u);
+            };
+            auto load_base = [&](uint32_t rt, V (&basev)[16]) {
+                const BufRes rb = res_of(p.base, p.ldbase, rt);
+                const uint32_t vb = (4 * hk * uint32_t(p.ldbase) + col) * SZ, has = has_of(rt);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    basev[i] = load_v<V>(rb, lane_has >> row_of(i) & 1 ? vb : kOut, row_of(i) * uint32_t(p.ldbase) * SZ);
-                f32x16 acc[4] = {f32x16{}, f32x16{}, f32x16{}, f32x16{}};
-                if (a >= 0) {
-                    const uint16_t* w = p.b + (int64_t(a) * p.N + part * per + col) * p.rank + hk * 8;
-                    const uint16_t* tv = st + (rt * 32 + r32) * pad + hk * 8;
+                    basev[i] = load_v<V>(rb, has >> row_of(i) & 1 ? vb : kOut, row_of(i) * uint32_t(p.ldbase) * SZ);
+            };
+            // RT halves from half rt on at a time: what B costs is shared by them
+            auto multiply = [&](uint32_t rt, auto& acc) {
+                constexpr int RT = sizeof(acc) / sizeof(acc[0]);
+#pragma unroll
+                for (int h = 0; h < RT; ++h)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        acc[h][t] = f32x16{};
+                if (a < 0)
+                    return;
+                // k steps in groups of 4, 2 or 1: half wave hk takes 8 G ranks next to each other of the group's 16 G (of B and of
+                // t alike), so a row of B is read by whole lines
+                const uint16_t* w = p.b + (int64_t(a) * p.N + part * per + col) * p.rank;
+                const uint16_t* tv = st + (rt * 32 + r32) * pad;
+                auto group = [&](uint32_t k, auto g_c) {
+                    constexpr int G = decltype(g_c)::value;
+                    const uint32_t at = k + hk * (8 * G);
+                    u32x4 bf[4][G];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int q = 0; q < G; ++q) {
+                            bf[t][q] = u32x4{};
+                            if (in && at + q * 8 < p.rank)
+                                bf[t][q] = *reinterpret_cast<const u32x4*>(w + t * p.rank + at + q * 8);
+                        }
+#pragma unroll
+                    for (int q = 0; q < G; ++q)
+#pragma unroll
+                        for (int s = NV - 1; s >= 0; --s)
+#pragma unroll
+                            for (int h = 0; h < RT; ++h) {
+                                const u32x4 tf = *reinterpret_cast<const u32x4*>(tv + (s * kRows + h * 32) * pad + at + q * 8);
+#pragma unroll
+                                for (int t = 0; t < 4; ++t)
+                                    acc[h][t] = mfma<F16>(tf, bf[t][q], acc[h][t]);
+                            }
+                };
+                uint32_t k = 0;
+                if constexpr (RT == 1)
 #pragma unroll 1
-                    for (uint32_t k = 0; k < depth; k += 16) {
-                        u32x4 bf[4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            bf[t] = u32x4{};
-                            if (in && k + hk * 8 < p.rank)
-                                bf[t] = *reinterpret_cast<const u32x4*>(w + t * p.rank + k);
-                        }
-#pragma unroll
-                        for (int s = NV - 1; s >= 0; --s) {
-                            const u32x4 tf = *reinterpret_cast<const u32x4*>(tv + s * kRows * pad + k);
-#pragma unroll
-                            for (int t = 0; t < 4; ++t)
-                                acc[t] = mfma<F16>(tf, bf[t], acc[t]);
-                        }
-                    }
-                }
+                    for (; k + 64 <= depth; k += 64)
+                        group(k, std::integral_constant<int, 4>{});
+#pragma unroll 1
+                for (; k + 32 <= depth; k += 32)
+                    group(k, std::integral_constant<int, 2>{});
+                if (k < depth)
+                    group(k, std::integral_constant<int, 1>{});
+            };
+            auto finish = [&](uint32_t rt, const f32x16 (&acc)[4], const V (&basev)[16]) {
+                const BufRes rc = res_of(p.c, p.ldc, rt);
+                const uint32_t vc = (4 * hk * uint32_t(p.ldc) + col) * SZ, has = has_of(rt);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float f = scale * factor[rt * 32 + 4 * hk + row_of(i)];
@@ -408,7 +451,28 @@ template <bool F16, uint32_t CT> __global__ __launch_bounds__(256, CT == MK_F32 
                         out = __builtin_bit_cast(V, f32x4{v[0], v[1], v[2], v[3]});
                     else
                         out = V{pack_x2(v[0], v[1], CT == MK_F16), pack_x2(v[2], v[3], CT == MK_F16)};
-                    store_v(out, rc, lane_has >> row_of(i) & 1 ? vc : kOut, row_of(i) * uint32_t(p.ldc) * SZ);
+                    store_v(out, rc, has >> row_of(i) & 1 ? vc : kOut, row_of(i) * uint32_t(p.ldc) * SZ);
+                }
+            };
+            if constexpr (FUSE) {
+                f32x16 acc[2][4];
+                multiply(0, acc);
+#pragma unroll
+                for (uint32_t rt = 0; rt < 2; ++rt) {
+                    V basev[16];
+                    load_base(rt, basev);
+                    finish(rt, acc[rt], basev);
+                }
+            } else {
+#pragma unroll 1
+                for (uint32_t rt = 0; rt < 2; ++rt) {
+                    if (!uint32_t(on >> (32 * rt)))
+                        continue;
+                    V basev[16];
+                    f32x16 acc[1][4];
+                    load_base(rt, basev);
+                    multiply(rt, acc);
+                    finish(rt, acc[0], basev);
                 }
             }
         }
@@ -512,7 +576,14 @@ template <bool F16, uint32_t CT> void launch_expand(const LoraP& p, const Plan& 
         return;
     }
     const uint32_t pad = (p.rank + 15) / 16 * 16 + 8, values = CT == MK_F32 && !F16 ? 3 : 2;
-    expand_tile<F16, CT><<<dim3(cdiv(p.rows, kRows), p.parts * cdiv(per, 512 * p.blocks)), 256, (values * pad * 2 + 4) * kRows, s>>>(p);
+    const dim3 grid(cdiv(p.rows, kRows), p.parts * cdiv(per, 512 * p.blocks));
+    const uint32_t lds = (values * pad * 2 + 4) * kRows;
+    // from rank 64 on B is the most of what a tile reads (us apart / shared by its two halves: 16384 x 12288 by rank 128 430 / 383
+    // with the first product, 4352 x 4096 by 64 49.3 / 47.6)
+    if (p.rank >= 64)
+        expand_tile<F16, CT, true><<<grid, 256, lds, s>>>(p);
+    else
+        expand_tile<F16, CT, false><<<grid, 256, lds, s>>>(p);
 }
 
 } // namespace
