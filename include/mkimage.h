@@ -373,7 +373,7 @@ mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes);
  * pos[r][a] f, the axes one after the other from pair 0; dims behind the last axis' (d - sum of axis_dims) are not turned.
  * series: MK_ROPE_OWN: pair j of axis a has f = theta^(-2 j / axis_dims[a]) (mk_rope_table's axes: 16, 56, 56);
  *         MK_ROPE_SHARED: pair i of all has f = theta^(-2 i / R), R the sum of axis_dims: one series cut into sections.
- * rope_mode: 1 pairs (i, i + R / 2), 2 pairs (2 i, 2 i + 1). Angles are exact to 2^-31 of a turn for int32 positions, and to
+ * rope_mode: 1 pairs (i, i + R / 2), 2 pairs (2 i, 2 i + 1). Angles are exact to 2^-30 of a turn for int32 positions, and to
  * (1 + |pos| 2^-20) times that for f32 ones up to 2^31 (an infinite or NaN position makes its pairs NaN). */
 enum mk_rope_series { MK_ROPE_OWN = 0, MK_ROPE_SHARED = 1 };
 typedef struct mk_rope_rows_args {

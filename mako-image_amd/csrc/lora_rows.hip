@@ -36,6 +36,10 @@ template <bool F16> __device__ inline void widen8(const u32x4& v, float (&f)[8])
         f[2 * j + 1] = widen<F16>(uint16_t(v[j] >> 16));
     }
 }
+template <uint32_t CT> __device__ inline float load_c(const void* c, int64_t at)
+{
+    return CT == MK_F32 ? static_cast<const float*>(c)[at] : widen<CT == MK_F16>(static_cast<const uint16_t*>(c)[at]);
+}
 // the adapter of a row, or -1
 __device__ inline int adapter_of(const LoraP& p, uint32_t row)
 {
@@ -103,6 +107,89 @@ template <bool F16> __global__ __launch_bounds__(256) void shrink_vec(LoraP p)
     if (threadIdx.x < kVecI)
         p.t[int64_t(row) * width + i0 + threadIdx.x] =
             (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+
+// Very few rows: both products in one launch. A workgroup for a row, a part and 1024 of its columns makes the part's t by itself, 8
+// values at a time over all of K, and goes on with its columns: A is read again for every 1024 columns, but a launch (2 to 3 us on
+// the host and the device each) is saved.
+constexpr uint32_t kOneThreads = 512, kOneCols = 2 * kOneThreads;
+template <bool F16, uint32_t CT> __global__ __launch_bounds__(kOneThreads) void one_kernel(LoraP p)
+{
+    const uint32_t row = blockIdx.y, per = p.N / p.parts, chunks = (per + kOneCols - 1) / kOneCols;
+    const uint32_t part = blockIdx.x / chunks, col = blockIdx.x % chunks * kOneCols + threadIdx.x * 2, n = part * per + col;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int a = adapter_of(p, row);
+    __shared__ float red[kOneThreads / 64][8];
+    __shared__ float st[256];
+    if (a >= 0) {
+        const uint16_t* x = p.x + int64_t(row) * p.ldx;
+        const uint16_t* w = p.a + (int64_t(a) * p.parts + part) * p.rank * p.K;
+        for (uint32_t i = 0; i < p.rank; i += 8, w += 8 * int64_t(p.K)) {
+            float s[8] = {};
+            for (uint32_t k = threadIdx.x * 8; k < p.K; k += kOneThreads * 8) {
+                u32x4 wv[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    wv[e] = *reinterpret_cast<const u32x4*>(w + int64_t(e) * p.K + k);
+                float xf[8];
+                widen8<F16>(*reinterpret_cast<const u32x4*>(x + k), xf);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float wf[8];
+                    widen8<F16>(wv[e], wf);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        s[e] = fmaf(xf[j], wf[j], s[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                s[e] = wave_sum(s[e]);
+            if (lane == 0)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    red[wave][e] = s[e];
+            __syncthreads();
+            if (threadIdx.x < 8) {
+                float v = 0.0f;
+#pragma unroll
+                for (uint32_t q = 0; q < kOneThreads / 64; ++q)
+                    v += red[q][threadIdx.x];
+                st[i + threadIdx.x] = v;
+            }
+            __syncthreads();
+        }
+    }
+    if (col >= per) // (per is a multiple of 8)
+        return;
+    float v[2] = {};
+    if (a >= 0) {
+        const uint16_t* w = p.b + (int64_t(a) * p.N + n) * p.rank;
+        const float scale = p.scale ? p.scale[a] : 1.0f;
+#pragma unroll 2
+        for (uint32_t j = 0; j < p.rank; j += 8)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float wf[8];
+                widen8<F16>(*reinterpret_cast<const u32x4*>(w + c * p.rank + j), wf);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[c] = fmaf(st[j + e], wf[e], v[c]);
+            }
+        v[0] *= scale;
+        v[1] *= scale;
+    }
+    if (p.base) {
+        v[0] += load_c<CT>(p.base, int64_t(row) * p.ldbase + n);
+        v[1] += load_c<CT>(p.base, int64_t(row) * p.ldbase + n + 1);
+    }
+    const int64_t at = int64_t(row) * p.ldc + n;
+    if constexpr (CT == MK_F32) {
+        static_cast<float*>(p.c)[at] = v[0];
+        static_cast<float*>(p.c)[at + 1] = v[1];
+    } else {
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.c) + at) = pack_x2(v[0], v[1], CT == MK_F16);
+    }
 }
 
 // Many rows: a tile of 64 rows by 32 NB of A's rows and one split of K. Each of the four waves takes every fourth 32 k for the
@@ -233,11 +320,6 @@ __device__ inline f32x4 load_t(const LoraP& p, uint32_t row, uint32_t i)
     }
     return v;
 }
-template <uint32_t CT> __device__ inline float load_c(const void* c, int64_t at)
-{
-    return CT == MK_F32 ? static_cast<const float*>(c)[at] : widen<CT == MK_F16>(static_cast<const uint16_t*>(c)[at]);
-}
-
 // 4 values through a buffer resource; past it zeros come, and nothing is stored
 template <class V> __device__ inline V load_v(BufRes r, uint32_t voff, uint32_t soff)
 {
@@ -250,11 +332,14 @@ template <class V> __device__ inline V load_v(BufRes r, uint32_t voff, uint32_t 
     return V{};
 #endif
 }
+// A 16-byte store has its offset in one register, with no scalar beside it: its data must not be overwritten by the very next
+// instruction, and the compiler keeps them apart only in that form (with a scalar offset, the first values of the last
+// store of a tile came out as what the next instruction wrote, in some lanes and now and then).
 template <class V> __device__ inline void store_v(V v, BufRes r, uint32_t voff, uint32_t soff)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
     if constexpr (sizeof(V) == 16)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, int(voff), int(soff), 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, int(voff + soff), 0, 0);
     else
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, int(voff), int(soff), 0);
 #endif
@@ -503,7 +588,8 @@ mk_status check_sizes(const mk_lora_rows_args* a)
 
 // How the two products run, by the sizes alone (on `cus` compute units).
 struct Plan {
-    bool vec1, vec2;    // a workgroup a row (few rows) or tiles of 64 rows
+    bool one;           // both products in one launch (very few rows)
+    bool vec1, vec2;    // else a workgroup a row (few rows) or tiles of 64 rows, each
     uint32_t nb;        // the first product's tiles: 32 nb of A's rows
     uint32_t splits, split_k;
     uint32_t blocks;
@@ -513,8 +599,16 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
     Plan p{};
     const uint32_t width = a->parts * a->rank, chunks = cdiv(width, 128), tiles = cdiv(a->rows, kRows);
     const uint64_t macs = uint64_t(a->rows) * width * a->K, macs2 = uint64_t(a->rows) * a->N * a->rank;
-    p.vec1 = a->rows <= 1024 && macs <= (1u << 25);
-    p.vec2 = a->rows <= 1024 && macs2 <= (1u << 24);
+    const uint32_t per = a->N / a->parts;
+    // (its 8 values of t at a time take 1.3 us for every 4096 k: us in two launches / in one of 1 row of 4096 to 4096 by rank 16
+    // 6.1 / 5.4, of 32 by rank 32 6.9 / 9.1, of 24 to 3 x 4096 by rank 16 6.9 / 7.6, on the device alone)
+    const uint64_t again = uint64_t(a->rows) * a->parts * cdiv(per, kOneCols) * a->rank * a->K;
+    p.one = a->rows <= 1024 && a->rank / 8 * cdiv(a->K, 8 * kOneThreads) <= 2 && again <= (1u << 25);
+    // us by rows / by tiles, rows of one adapter together: 64 x 4096 to 4096 by rank 16 6.6 / 13.6, 512 by rank 32 11.8 / 15.3, 1000 x
+    // 1280 to 3840 by rank 32 26 / 17 (2^26.9 products); in no order, where a tile takes its adapters one after the other: 6.8 / 49,
+    // 24 / 61, 41 / 72
+    p.vec1 = a->rows <= 4096 && macs <= (1u << 26);
+    p.vec2 = a->rows <= 4096 && macs2 <= (1u << 26);
     p.nb = cdiv(cdiv(width, chunks), 32);
     p.splits = 1;
     p.split_k = uint32_t(round_up(a->K, kStepK));
@@ -534,7 +628,6 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
             }
         }
     }
-    const uint32_t per = a->N / a->parts;
     p.blocks = 1;
     while (p.blocks < 4 && p.blocks * 512 < per && uint64_t(tiles) * a->parts * cdiv(per, 1024 * p.blocks) >= 4ull * cus)
         p.blocks *= 2;
@@ -553,6 +646,10 @@ mk_status device_cus(uint32_t* cus)
     return MK_OK;
 }
 
+template <bool F16, uint32_t CT> void launch_one(const LoraP& p, hipStream_t s)
+{
+    one_kernel<F16, CT><<<dim3(p.parts * cdiv(p.N / p.parts, kOneCols), p.rows), kOneThreads, 0, s>>>(p);
+}
 template <bool F16> void launch_shrink(const LoraP& p, const Plan& plan, hipStream_t s)
 {
     const uint32_t width = p.parts * p.rank;
@@ -624,7 +721,7 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
         return fail(MK_ERR_ARG, "lora_rows: operands and workspace must be 16-byte aligned (scale and ids 4)");
     if (!a->rows)
         return MK_OK;
-    if (!a->workspace || a->workspace_bytes < workspace_of(a, Plan{false, false, 1, 1, 0, 1}))
+    if (!a->workspace || a->workspace_bytes < workspace_of(a, Plan{false, false, false, 1, 1, 0, 1}))
         return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
     uint32_t cus = 1;
     MK_TRY(device_cus(&cus));
@@ -635,15 +732,28 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
             a->ids, a->base, a->c, static_cast<float*>(a->workspace), a->ldx, a->ldbase, a->ldc, a->rows, a->K, a->N, a->rank,
             a->parts, a->adapters, plan.splits, plan.split_k, plan.blocks};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool f16 = a->dtype == MK_F16;
-    f16 ? launch_shrink<true>(p, plan, s) : launch_shrink<false>(p, plan, s);
-    MK_LAUNCH_CHECK("lora_rows");
-    if (a->c_dtype == MK_F32)
-        f16 ? launch_expand<true, MK_F32>(p, plan, s) : launch_expand<false, MK_F32>(p, plan, s);
-    else if (a->c_dtype == MK_BF16)
-        f16 ? launch_expand<true, MK_BF16>(p, plan, s) : launch_expand<false, MK_BF16>(p, plan, s);
+    auto run = [&](auto f16_c, auto ct_c) {
+        constexpr bool H = decltype(f16_c)::value;
+        constexpr uint32_t CT = decltype(ct_c)::value;
+        if (plan.one) {
+            launch_one<H, CT>(p, s);
+            return;
+        }
+        launch_shrink<H>(p, plan, s);
+        launch_expand<H, CT>(p, plan, s);
+    };
+    auto with_c = [&](auto f16_c) {
+        if (a->c_dtype == MK_F32)
+            run(f16_c, std::integral_constant<uint32_t, MK_F32>{});
+        else if (a->c_dtype == MK_BF16)
+            run(f16_c, std::integral_constant<uint32_t, MK_BF16>{});
+        else
+            run(f16_c, std::integral_constant<uint32_t, MK_F16>{});
+    };
+    if (a->dtype == MK_F16)
+        with_c(std::true_type{});
     else
-        f16 ? launch_expand<true, MK_F16>(p, plan, s) : launch_expand<false, MK_F16>(p, plan, s);
+        with_c(std::false_type{});
     MK_LAUNCH_CHECK("lora_rows");
     return MK_OK;
 }

@@ -243,8 +243,8 @@ extern "C" mk_status mk_rope_rows(const mk_rope_rows_args* a, void* stream)
         return fail(MK_ERR_ARG, "rope_rows: more than 2^31 - 1 rows");
     RopeP p{a->q, a->k, a->q_out, a->k_out, a->ldq, a->ldk, a->ldqo, a->ldko, a->pos_ld, a->norm_q, a->norm_k, a->pos,
             a->rows, a->heads, a->kv_heads, a->d, uint32_t(turned / 2), a->eps, a->k_scale == 0.0f ? 1.0f : a->k_scale, {}, {}};
-    // theta^(-2 j / dim) radians as turns of 2^64, in extended doubles: a power for every eighth pair (150 ns each), products
-    // between them, so at most 9 roundings of 2^-64
+    // theta^(-2 j / dim) radians as turns of 2^64, in extended doubles: a power for every 16th pair (150 ns each), products
+    // between them, so an error below 2^-59, 2^-30 of a turn at the largest positions
     const bool own = a->series == MK_ROPE_OWN;
     const long double theta = a->theta, unit = 18446744073709551616.0L / 6.283185307179586476925286766559L;
     long double f = 0.0L, ratio = 0.0L;
@@ -255,7 +255,7 @@ extern "C" mk_status mk_rope_rows(const mk_rope_rows_args* a, void* stream)
             const long double dim = own ? a->axis_dims[i] : uint32_t(turned);
             if (at == 0)
                 ratio = powl(theta, -2.0L / dim);
-            f = at % 8 ? f * ratio : powl(theta, -2.0L * at / dim) * unit;
+            f = at % 16 ? f * ratio : powl(theta, -2.0L * at / dim) * unit;
             p.turn[pair] = uint64_t(f);
             p.axis[pair] = uint8_t(i);
         }

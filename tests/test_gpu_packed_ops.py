@@ -452,6 +452,20 @@ def test_lora_infinities_stay_with_their_rows(gpu, rows, bad):
         Lora(rows, 72, 64, 8, 1, 5, np.arange(rows) % 5, dt, M.F32, edit=edit).check()
 
 
+@pytest.mark.parametrize("dt", [M.BF16, M.F16], ids=NAME.get)
+@pytest.mark.parametrize("c_dt", [M.F32, M.BF16], ids=NAME.get)
+@pytest.mark.parametrize("rank", [32, 64, 128])
+def test_lora_the_same_bits_on_every_run_of_many_tiles(gpu, rank, c_dt, dt):
+    # (fp32 rows once came out with a few values of other registers, in some tiles of a large launch)
+    rows, K, N = 4100, 256, 2048
+    a = Lora(rows, K, N, rank, 1, 3, np.arange(rows) * 3 // rows, dt, c_dt)
+    first = a.run().result()
+    want, tol = a.want()
+    assert (np.abs(first - want) <= tol).all()
+    for _ in range(5):
+        assert np.array_equal(a.run().result(), first)
+
+
 def test_lora_half_values_of_any_size(gpu):
     # t beyond the half range, and far below it
     def edit(raw):
