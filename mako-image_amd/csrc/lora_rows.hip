@@ -604,9 +604,9 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
     // 6.1 / 5.4, of 32 by rank 32 6.9 / 9.1, of 24 to 3 x 4096 by rank 16 6.9 / 7.6, on the device alone)
     const uint64_t again = uint64_t(a->rows) * a->parts * cdiv(per, kOneCols) * a->rank * a->K;
     p.one = a->rows <= 1024 && a->rank / 8 * cdiv(a->K, 8 * kOneThreads) <= 2 && again <= (1u << 25);
-    // us by rows / by tiles, rows of one adapter together: 64 x 4096 to 4096 by rank 16 6.6 / 13.6, 512 by rank 32 11.8 / 15.3, 1000 x
-    // 1280 to 3840 by rank 32 26 / 17 (2^26.9 products); in no order, where a tile takes its adapters one after the other: 6.8 / 49,
-    // 24 / 61, 41 / 72
+    // us by rows / by tiles: 64 x 4096 to 4096 by rank 16 6.6 / 13.6, 512 by rank 32 12 to 25 / 15 to 22, 1000 x 1280 to 3840 by rank
+    // 32 (2^26.9 products) 26 / 17 where rows of one adapter are together; 6.8 / 49, 24 / 61, 41 / 72 in no order, where a tile takes
+    // its adapters one after the other. (1024 x 4096 to 4096 by rank 16, at the border: 27 / 16 and 28 / 56.)
     p.vec1 = a->rows <= 4096 && macs <= (1u << 26);
     p.vec2 = a->rows <= 4096 && macs2 <= (1u << 26);
     p.nb = cdiv(cdiv(width, chunks), 32);
