@@ -347,12 +347,11 @@ typedef struct mk_lora_rows_args {
     const void* a;       /* [adapters][parts rank][K] */
     const void* b;       /* [adapters][N][rank] */
     const float* scale;  /* device [adapters] or NULL (1) */
-    const int32_t* ids;  /* device [rows] or NULL (all 0); rows of one adapter are fastest one after the other */
+    const int32_t* ids;  /* device [rows] or NULL (all 0), in any order */
     const void* base;    /* [rows][ldbase] or NULL (0); may be c itself (then ldbase == ldc) */
     void* c;             /* [rows][ldc] */
     int64_t ldx, ldbase, ldc; /* elements between rows, multiples of 8 below 2^23 */
-    uint32_t rows, K, N; /* K a multiple of 8, N of 8 parts, both up to 2^22; rows up to 2^28, rows times K
-                            below 2^41 */
+    uint32_t rows, K, N; /* K a multiple of 8, N of 8 parts, both up to 2^22; rows up to 2^28 */
     uint32_t rank;       /* of each part, a multiple of 8 up to 256 */
     uint32_t parts;      /* 1 to 4 */
     uint32_t adapters;   /* at least 1 */
@@ -360,6 +359,8 @@ typedef struct mk_lora_rows_args {
     uint32_t c_dtype;    /* base and c: MK_F32, MK_BF16 or MK_F16 */
     void* workspace;     /* 16-byte aligned */
     uint64_t workspace_bytes; /* at least what mk_lora_rows_workspace says */
+    uint32_t grouped;    /* 1: rows of one adapter are known to be one after the other, or nearly so (a request's rows): many rows are then
+                            not looked through for their order first, 5 us. The results are the same. */
 } mk_lora_rows_args;
 /* Sums in fp32; t enters the second product as two or three values of the inputs' type (its rounding and the rest). Infinities and
  * NaNs of a row or of an adapter reach that row, or that adapter's rows, alone. All pointers 16-byte aligned (scale and ids 4). */

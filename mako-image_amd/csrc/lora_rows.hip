@@ -20,7 +20,8 @@ struct LoraP {
     const int32_t* ids;
     const void* base;
     void* c;
-    float* t; // workspace: [splits][rows][parts rank]
+    float* t;       // workspace: [splits][rows][parts rank]
+    u32x2* perm;    // workspace: [rows], the row at each place of the tiles and its adapter, or NULL: places are rows
     int64_t ldx, ldbase, ldc;
     uint32_t rows, K, N, rank, parts, adapters;
     uint32_t splits, split_k; // workgroups that share a row's K, and the k of each
@@ -58,6 +59,17 @@ template <bool F16> __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
 }
 constexpr uint32_t kOut = 0x80000000u; // a byte offset past every buffer resource here
 constexpr int kRows = 64;              // rows of a workgroup of the second product
+// the row at a place of the tiles from first on, counted from there or, in order, from row 0, and its adapter (-1: none)
+__device__ inline int row_at(const LoraP& p, uint32_t first, uint32_t i, uint32_t& row)
+{
+    if (p.perm) {
+        const u32x2 v = p.perm[first + i];
+        row = v[0];
+        return int(v[1]);
+    }
+    row = i;
+    return adapter_of(p, first + i);
+}
 // the smallest adapter above `last` among a wave's rows (a lane's row each), or INT_MAX
 __device__ inline int next_adapter(int id, int last)
 {
@@ -66,6 +78,101 @@ __device__ inline int next_adapter(int id, int last)
     for (int m = 1; m < 64; m <<= 1)
         v = min(v, __shfl_xor(v, m));
     return __builtin_amdgcn_readfirstlane(v);
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// rows in the order of their adapters
+// ------------------------------------------------------------------------------------------------------------
+
+// A tile goes through its steps for every adapter among its rows, so rows in no order cost as many times as there are adapters
+// (4096 rows of 4096 to 12288 by rank 32, 8 adapters: 232 us in no order, 63 in runs). One workgroup sorts the rows' numbers by
+// counting, where more than every second tile would have a change of adapter; rows in runs keep their places. Which
+// place a row gets among its adapter's depends on the order of atomics, its values do not: they are sums over k and rank alone.
+constexpr uint32_t kMaxOrdered = 1024; // adapters
+__global__ __launch_bounds__(1024) void order_kernel(LoraP p)
+{
+    __shared__ uint32_t count[kMaxOrdered + 1], sums[2][1024], changes;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, bins = p.adapters + 1; // the last one: rows without an adapter
+    if (tid == 0)
+        changes = 0;
+    __syncthreads();
+    // (8 loads of a thread at a time: one after the other, 16401 rows took 9 us)
+    uint32_t mine = 0;
+    for (uint32_t i0 = tid; i0 < p.rows; i0 += 8 * 1024) {
+        int id[8], before[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t i = min(i0 + j * 1024, p.rows - 1);
+            id[j] = p.ids[i];
+            before[j] = p.ids[i ? i - 1 : 0];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            mine += i0 + j * 1024 < p.rows && id[j] != before[j];
+    }
+    if (mine)
+        atomicAdd(&changes, mine);
+    __syncthreads();
+    if (changes <= p.rows / (2 * kRows)) {
+        for (uint32_t i = tid; i < p.rows; i += 1024)
+            p.perm[i] = u32x2{i, uint32_t(adapter_of(p, i))};
+        return;
+    }
+    for (uint32_t i = tid; i < bins; i += 1024)
+        count[i] = 0;
+    __syncthreads();
+    // the bins' counters up by a wave's rows, one atomic a bin; a row's place among them
+    auto place = [&](uint32_t i, int id) {
+        const bool on = i < p.rows;
+        const uint32_t bin = id >= 0 && uint32_t(id) < p.adapters ? uint32_t(id) : p.adapters;
+        uint32_t at = 0;
+        for (uint64_t todo = __ballot(on); todo;) {
+            const int first = __builtin_ctzll(todo);
+            const uint32_t b = __shfl(bin, first);
+            const uint64_t same = __ballot(on && bin == b);
+            uint32_t from = 0;
+            if (int(lane) == first)
+                from = atomicAdd(&count[b], uint32_t(__popcll(same)));
+            from = __shfl(from, first);
+            if (on && bin == b)
+                at = from + uint32_t(__popcll(same & ((1ull << lane) - 1)));
+            todo &= ~same;
+        }
+        return at;
+    };
+    auto each = [&](auto f) {
+        for (uint32_t i0 = tid - lane; i0 < p.rows; i0 += 8 * 1024) {
+            int id[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                id[j] = p.ids[min(i0 + j * 1024 + lane, p.rows - 1)];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (i0 + j * 1024 < p.rows)
+                    f(i0 + j * 1024 + lane, id[j]);
+        }
+    };
+    each([&](uint32_t i, int id) { place(i, id); });
+    __syncthreads();
+    // where each bin starts: an inclusive sum over 1024 of them, less the bin itself (the last bin of 1025 needs no more than that)
+    const uint32_t own = tid < bins ? count[tid] : 0;
+    sums[0][tid] = own;
+    int cur = 0;
+    for (uint32_t d = 1; d < 1024; d *= 2, cur ^= 1) {
+        __syncthreads();
+        sums[cur ^ 1][tid] = sums[cur][tid] + (tid >= d ? sums[cur][tid - d] : 0);
+    }
+    __syncthreads();
+    if (tid < bins)
+        count[tid] = sums[cur][tid] - own;
+    if (tid == 0 && bins > 1024)
+        count[1024] = sums[cur][1023];
+    __syncthreads();
+    each([&](uint32_t i, int id) {
+        const uint32_t at = place(i, id);
+        if (i < p.rows)
+            p.perm[at] = u32x2{i, id >= 0 && uint32_t(id) < p.adapters ? uint32_t(id) : ~0u};
+    });
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -210,9 +317,12 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
     const uint32_t split = blockIdx.y % p.splits, i0 = blockIdx.y / p.splits * (32 * NB);
     const uint32_t kb = split * p.split_k, ke = min(p.K, kb + p.split_k);
     const int steps = int((ke - kb + kStepK - 1) / kStepK);
-    const int mine = uint32_t(lane) < rows ? adapter_of(p, row0 + lane) : -1; // lane's row of the tile
+    // lane's row of the tile, from the first row of the resource on, and its adapter
+    uint32_t src;
+    int mine = row_at(p, row0, min(uint32_t(lane), rows - 1), src);
+    mine = uint32_t(lane) < rows ? mine : -1;
 
-    const BufRes rx = buf_res(p.x + int64_t(row0) * p.ldx, uint32_t(((rows - 1) * p.ldx + p.K) * 2));
+    const BufRes rx = buf_res(p.perm ? p.x : p.x + int64_t(row0) * p.ldx, uint32_t(((p.perm ? p.rows - 1 : rows - 1) * p.ldx + p.K) * 2));
     // byte offset of a lane's 16 bytes of each load, and their k: LDS rows of 64 bytes whose chunk c holds k chunk
     // c ^ ((row >> 2) & 3), so the 16-byte fragment reads of 8 rows fall on all banks
     uint32_t off[ND];
@@ -220,7 +330,7 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
 #pragma unroll
     for (int j = 0; j < ND; ++j) {
         const uint32_t r = uint32_t((j < NX ? j : j - NX) * 16 + lane / 4);
-        off[j] = j < NX ? min(r, rows - 1) * uint32_t(p.ldx) * 2 : min(r, width - i0 - 1) * p.K * 2;
+        off[j] = j < NX ? uint32_t(__shfl(src, int(r))) * uint32_t(p.ldx) * 2 : min(r, width - i0 - 1) * p.K * 2;
     }
     for (int a = next_adapter(mine, -1); a != 0x7fffffff; a = next_adapter(mine, a)) {
         const BufRes ra = buf_res(p.a + (int64_t(a) * width + i0) * p.K, uint32_t(min(uint32_t(32 * NB), width - i0) * p.K * 2));
@@ -332,16 +442,16 @@ template <class V> __device__ inline V load_v(BufRes r, uint32_t voff, uint32_t 
     return V{};
 #endif
 }
-// A 16-byte store has its offset in one register, with no scalar beside it: its data must not be overwritten by the very next
-// instruction, and the compiler keeps them apart only in that form (with a scalar offset, the first values of the last
-// store of a tile came out as what the next instruction wrote, in some lanes and now and then).
-template <class V> __device__ inline void store_v(V v, BufRes r, uint32_t voff, uint32_t soff)
+// (A 16-byte store's offset is in one register, with no scalar beside it: its data must not be overwritten by the very next
+// instruction, and the compiler keeps them apart only in that form. With a scalar offset, the first values of the last
+// store of a tile came out as what the next instruction wrote, in some lanes and now and then.)
+template <class V> __device__ inline void store_v(V v, BufRes r, uint32_t voff)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
     if constexpr (sizeof(V) == 16)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, int(voff + soff), 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, int(voff), 0, 0);
     else
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, int(voff), int(soff), 0);
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, int(voff), 0, 0);
 #endif
 }
 
@@ -392,6 +502,7 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
     constexpr uint32_t SZ = CT == MK_F32 ? 4 : 2;
     typedef std::conditional_t<CT == MK_F32, u32x4, u32x2> V; // 4 values of c
     extern __shared__ __attribute__((aligned(16))) uint16_t st[]; // [NV][64][pad], then a factor a row
+    __shared__ __attribute__((aligned(16))) uint32_t row_b[kRows], row_c[kRows]; // the rows' byte offsets in base and c
     const uint32_t tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hk = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t row0 = blockIdx.x * kRows, rows = min(p.rows - row0, uint32_t(kRows));
@@ -399,7 +510,11 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
     const uint32_t part = blockIdx.y / groups, first = blockIdx.y % groups * span;
     const uint32_t depth = (p.rank + 15) / 16 * 16, pad = depth + 8; // (rows 16 bytes off each other's banks)
     float* factor = reinterpret_cast<float*>(st + NV * kRows * pad);
-    const int mine = lane < rows ? adapter_of(p, row0 + lane) : -2;
+    uint32_t src;
+    int mine = row_at(p, row0, min(lane, rows - 1), src);
+    mine = lane < rows ? mine : -2;
+    row_b[lane] = src * uint32_t(p.ldbase) * SZ; // (every wave writes the same)
+    row_c[lane] = src * uint32_t(p.ldc) * SZ;
     {
         // 4 threads a row, t's values 4 (q + 4 i) .. + 3 of it in each
         const uint32_t r = tid / 4, q = tid % 4;
@@ -450,21 +565,20 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
                 break;
             const uint32_t col = c0 + r32 * 4;
             const bool in = col < per; // (per is a multiple of 8: all 4 of a lane's columns, or none)
-            // A lane's rows of a 32-row half are 8 (i / 4) + 4 hk + i % 4. Their base and c by buffer loads and stores: one byte
-            // offset a lane and a scalar one a row; what is not the adapter's goes past the resource.
+            // A lane's rows of a 32-row half are 8 (i / 4) + 4 hk + i % 4. Their base and c by buffer loads and stores at the rows'
+            // byte offsets; what is not the adapter's goes past the resource.
             auto row_of = [](int i) { return uint32_t(8 * (i / 4) + i % 4); };
             auto has_of = [&](uint32_t rt) { return in ? uint32_t(on >> (32 * rt)) >> (4 * hk) : 0u; };
-            auto res_of = [&](const void* x, int64_t ld, uint32_t rt) {
-                const uint32_t tr = rows > rt * 32 ? min(rows - rt * 32, 32u) : 0u;
-                return buf_res(static_cast<const char*>(x) + ((int64_t(row0) + rt * 32) * ld + part * per) * SZ,
-                               x && tr ? uint32_t((tr - 1) * ld + per) * SZ : 0u);
+            auto res_of = [&](const void* x, int64_t ld) {
+                return buf_res(static_cast<const char*>(x) + ((p.perm ? 0 : int64_t(row0)) * ld + part * per) * SZ,
+                               x ? uint32_t(((p.perm ? p.rows : rows) - 1) * ld + per) * SZ : 0u);
             };
             auto load_base = [&](uint32_t rt, V (&basev)[16]) {
-                const BufRes rb = res_of(p.base, p.ldbase, rt);
-                const uint32_t vb = (4 * hk * uint32_t(p.ldbase) + col) * SZ, has = has_of(rt);
+                const BufRes rb = res_of(p.base, p.ldbase);
+                const uint32_t has = has_of(rt);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    basev[i] = load_v<V>(rb, has >> row_of(i) & 1 ? vb : kOut, row_of(i) * uint32_t(p.ldbase) * SZ);
+                    basev[i] = load_v<V>(rb, has >> row_of(i) & 1 ? row_b[rt * 32 + 4 * hk + row_of(i)] + col * SZ : kOut, 0);
             };
             // RT halves from half rt on at a time: what B costs is shared by them
             auto multiply = [&](uint32_t rt, auto& acc) {
@@ -516,8 +630,8 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
                     group(k, std::integral_constant<int, 1>{});
             };
             auto finish = [&](uint32_t rt, const f32x16 (&acc)[4], const V (&basev)[16]) {
-                const BufRes rc = res_of(p.c, p.ldc, rt);
-                const uint32_t vc = (4 * hk * uint32_t(p.ldc) + col) * SZ, has = has_of(rt);
+                const BufRes rc = res_of(p.c, p.ldc);
+                const uint32_t has = has_of(rt);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float f = scale * factor[rt * 32 + 4 * hk + row_of(i)];
@@ -536,7 +650,7 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
                         out = __builtin_bit_cast(V, f32x4{v[0], v[1], v[2], v[3]});
                     else
                         out = V{pack_x2(v[0], v[1], CT == MK_F16), pack_x2(v[2], v[3], CT == MK_F16)};
-                    store_v(out, rc, has >> row_of(i) & 1 ? vc : kOut, row_of(i) * uint32_t(p.ldc) * SZ);
+                    store_v(out, rc, has >> row_of(i) & 1 ? row_c[rt * 32 + 4 * hk + row_of(i)] + col * SZ : kOut);
                 }
             };
             if constexpr (FUSE) {
@@ -589,6 +703,7 @@ mk_status check_sizes(const mk_lora_rows_args* a)
 // How the two products run, by the sizes alone (on `cus` compute units).
 struct Plan {
     bool one;           // both products in one launch (very few rows)
+    bool order;         // rows are taken in the order of their adapters
     bool vec1, vec2;    // else a workgroup a row (few rows) or tiles of 64 rows, each
     uint32_t nb;        // the first product's tiles: 32 nb of A's rows
     uint32_t splits, split_k;
@@ -609,6 +724,9 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
     // its adapters one after the other. (1024 x 4096 to 4096 by rank 16, at the border: 27 / 16 and 28 / 56.)
     p.vec1 = a->rows <= 4096 && macs <= (1u << 26);
     p.vec2 = a->rows <= 4096 && macs2 <= (1u << 26);
+    // (for two products by tiles alone; offsets from the first row on are below 2^31)
+    const int64_t far = std::max(std::max(a->ldx, a->base ? a->ldbase : 0) * 4, a->ldc * 4) * a->rows;
+    p.order = !p.one && !p.vec1 && !p.vec2 && a->ids && !a->grouped && a->adapters > 1 && a->adapters <= kMaxOrdered && a->rows <= (1u << 18) && far < (1ll << 31);
     p.nb = cdiv(cdiv(width, chunks), 32);
     p.splits = 1;
     p.split_k = uint32_t(round_up(a->K, kStepK));
@@ -633,10 +751,12 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
         p.blocks *= 2;
     return p;
 }
-uint64_t workspace_of(const mk_lora_rows_args* a, const Plan& p)
+// t, and the rows' order
+uint64_t bytes_of_t(const mk_lora_rows_args* a, uint32_t splits)
 {
-    return round_up(uint64_t(p.splits) * a->rows * a->parts * a->rank * 4, 16);
+    return round_up(uint64_t(splits) * a->rows * a->parts * a->rank * 4, 16);
 }
+uint64_t workspace_of(const mk_lora_rows_args* a, uint32_t splits) { return bytes_of_t(a, splits) + round_up(uint64_t(a->rows) * 8, 16); }
 mk_status device_cus(uint32_t* cus)
 {
     int dev = 0, n = 0;
@@ -701,7 +821,7 @@ mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes)
         return MK_OK;
     uint32_t cus = 1;
     MK_TRY(device_cus(&cus));
-    *bytes = workspace_of(a, plan_of(a, cus));
+    *bytes = workspace_of(a, plan_of(a, cus).splits);
     return MK_OK;
 }
 
@@ -721,15 +841,18 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
         return fail(MK_ERR_ARG, "lora_rows: operands and workspace must be 16-byte aligned (scale and ids 4)");
     if (!a->rows)
         return MK_OK;
-    if (!a->workspace || a->workspace_bytes < workspace_of(a, Plan{false, false, false, 1, 1, 0, 1}))
+    if (a->grouped > 1)
+        return fail(MK_ERR_ARG, "lora_rows: grouped is 0 or 1");
+    if (!a->workspace || a->workspace_bytes < workspace_of(a, 1))
         return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
     uint32_t cus = 1;
     MK_TRY(device_cus(&cus));
     const Plan plan = plan_of(a, cus);
-    if (a->workspace_bytes < workspace_of(a, plan))
+    if (a->workspace_bytes < workspace_of(a, plan.splits))
         return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
     LoraP p{static_cast<const uint16_t*>(a->x), static_cast<const uint16_t*>(a->a), static_cast<const uint16_t*>(a->b), a->scale,
-            a->ids, a->base, a->c, static_cast<float*>(a->workspace), a->ldx, a->ldbase, a->ldc, a->rows, a->K, a->N, a->rank,
+            a->ids, a->base, a->c, static_cast<float*>(a->workspace),
+            plan.order ? reinterpret_cast<u32x2*>(static_cast<char*>(a->workspace) + bytes_of_t(a, plan.splits)) : nullptr, a->ldx, a->ldbase, a->ldc, a->rows, a->K, a->N, a->rank,
             a->parts, a->adapters, plan.splits, plan.split_k, plan.blocks};
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto f16_c, auto ct_c) {
@@ -739,6 +862,8 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
             launch_one<H, CT>(p, s);
             return;
         }
+        if (plan.order)
+            order_kernel<<<1, 1024, 0, s>>>(p);
         launch_shrink<H>(p, plan, s);
         launch_expand<H, CT>(p, plan, s);
     };

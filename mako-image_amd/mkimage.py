@@ -67,7 +67,7 @@ class LoraRowsArgs(C.Structure):
     _fields_ = [(n, _vp) for n in ("x", "a", "b", "scale", "ids", "base", "c")] + \
                [(n, _i64) for n in ("ldx", "ldbase", "ldc")] + \
                [(n, _u32) for n in ("rows", "K", "N", "rank", "parts", "adapters", "dtype", "c_dtype")] + \
-               [("workspace", _vp), ("workspace_bytes", _u64)]
+               [("workspace", _vp), ("workspace_bytes", _u64), ("grouped", _u32)]
 
 
 class RopeRowsArgs(C.Structure):

@@ -335,8 +335,9 @@ def test_attention_output_type_and_same_bits_again(gpu):
 # ---------------------------------------------------------------------------------------------------------------------
 
 class Lora:
-    def __init__(self, rows, K, N, rank, parts, adapters, ids, dt, c_dt, seed=0, pad=0, base=True, scale=True, in_place=False, edit=None):
+    def __init__(self, rows, K, N, rank, parts, adapters, ids, dt, c_dt, seed=0, pad=0, base=True, scale=True, in_place=False, edit=None, grouped=0):
         rng = np.random.default_rng(seed)
+        self.grouped = grouped
         self.sizes, self.dt, self.c_dt, self.pad = (rows, K, N, rank, parts, adapters), dt, c_dt, pad
         raw = {"x": rng.standard_normal((rows, K)) * np.exp(rng.standard_normal(K) * 0.5), "a": rng.standard_normal((adapters, parts * rank, K)) * K ** -0.5,
                "b": rng.standard_normal((adapters, N, rank)) * rank ** -0.5, "base": rng.standard_normal((rows, N))}
@@ -364,7 +365,7 @@ class Lora:
         g.ids, g.scale = (k.p if k else None for k in self.keep)
         g.ldx, g.ldbase, g.ldc = self.buf["x"].shape[1], self.buf["base"].shape[1], self.c.shape[1]
         g.rows, g.K, g.N, g.rank, g.parts, g.adapters = self.sizes
-        g.dtype, g.c_dtype = self.dt, self.c_dt
+        g.dtype, g.c_dtype, g.grouped = self.dt, self.c_dt, self.grouped
         need = C.c_uint64()
         M.call("mk_lora_rows_workspace", C.byref(g), C.byref(need))
         self.space = M.Dev(need.value)
@@ -430,6 +431,17 @@ def test_lora_rows(gpu, rows, K, N, rank, parts, adapters, dt):
     runs[rows // 2:rows // 2 + 3] = -1
     for c_dt, ids, pad in ((dt, mixed, 8), (M.F32, runs, 0)):
         Lora(rows, K, N, rank, parts, adapters, ids, dt, c_dt, pad=pad).check()
+
+
+@pytest.mark.parametrize("c_dt", [M.F32, M.F16], ids=NAME.get)
+@pytest.mark.parametrize("adapters, seen", [(2, 2), (7, 5), (1024, 1024), (1025, 300), (64, 1)])
+def test_lora_many_rows_in_no_order(gpu, adapters, seen, c_dt):
+    # sizes whose products go by tiles: 2^26 of them and more in both
+    rows, K, N, rank = 4500, 512, 512, 32
+    rng = np.random.default_rng(adapters)
+    ids = rng.integers(-1, seen, rows) * (adapters // seen)
+    for kw in (dict(), dict(in_place=True), dict(grouped=1)):
+        Lora(rows, K, N, rank, 1, adapters, ids, M.F16, c_dt, pad=8, **kw).check()
 
 
 @pytest.mark.parametrize("rows", [3, 150])

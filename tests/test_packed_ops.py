@@ -75,7 +75,7 @@ def lora(**kw):
 @pytest.mark.parametrize("kw, match", [
     (dict(x=None), "null"), (dict(c=None), "null"), (dict(dtype=M.F32), "bf16 or f16"), (dict(c_dtype=M.I8), "base and c"), (dict(parts=0), "parts"),
     (dict(parts=5), "parts"), (dict(rank=0), "parts"), (dict(rank=12), "parts"), (dict(rank=264), "parts"), (dict(adapters=0), "adapter"), (dict(K=0), "K must"),
-    (dict(K=252), "K must"), (dict(N=88), "K must"), (dict(N=0), "K must"), (dict(rows=(1 << 28) + 1), "rows"), (dict(rows=1 << 28, K=1 << 13, ldx=1 << 13), "rows times K"), (dict(ldx=248), "ldx"), (dict(ldx=1 << 23), "ldx"), (dict(ldc=1 << 23), "ldx"), (dict(ldbase=1 << 24), "ldx"), (dict(K=(1 << 22) + 8), "K must"), (dict(ldx=260), "ldx"),
+    (dict(K=252), "K must"), (dict(N=88), "K must"), (dict(N=0), "K must"), (dict(rows=(1 << 28) + 1), "rows"), (dict(grouped=2), "grouped"), (dict(ldx=248), "ldx"), (dict(ldx=1 << 23), "ldx"), (dict(ldc=1 << 23), "ldx"), (dict(ldbase=1 << 24), "ldx"), (dict(K=(1 << 22) + 8), "K must"), (dict(ldx=260), "ldx"),
     (dict(ldc=88), "ldx"), (dict(ldbase=100), "ldx"), (dict(base=4 * P, ldbase=104), "in place"), (dict(x=P + 8), "aligned"), (dict(c=P + 4), "aligned"),
     (dict(ids=P + 1), "aligned"), (dict(workspace=P + 8), "aligned"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=16), "workspace")])
 def test_lora_rows_refusals(kw, match):
