@@ -32,7 +32,7 @@ struct PackedP {
     uint16_t* out;
     int64_t ldq, ldk, ldv, ldo;
     const float* slopes;
-    float* part;    // workspace: [slot][32 NW][D] sums, then [slot][32 NW][2] m and l
+    float* part;    // workspace: [slot][NW][32 D] sums (part_at), then [slot][NW][32][2] m and l
     float* part_ml;
     float c;        // scale log2(e); with a cap: 2 scale log2(e) / cap
     float cap;      // cap log2(e)
@@ -81,6 +81,13 @@ __device__ inline uint32_t find_doc(const uint32_t (&first)[kMaxDocs], uint32_t 
         return 0;
     const uint32_t lane = threadIdx.x & 63, at = first[min(lane, n - 1)];
     return __builtin_amdgcn_readfirstlane(uint32_t(__popcll(__ballot(lane < n && at <= item))) - 1);
+}
+
+// Where 4 dims (chunk) of one of a wave's 32 rows are in its partial results: with many rows the rows of a chunk next to each
+// other, as a wave holds them (1 KB a store: by rows, 16 bytes a lane 512 apart, was half as fast), with few by rows.
+template <int D, int NW> __device__ inline uint32_t part_at(uint32_t chunk, uint32_t r)
+{
+    return NW == 1 ? r * D + chunk * 4 : (chunk * 32 + r) * 4;
 }
 
 enum { kPlain = 0, kBias = 1, kCap = 2 /* a bit each */ };
@@ -437,18 +444,16 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     if (doc.splits > 1) {
         if (w0 + r32 >= rows)
             return;
-        const uint64_t at = (uint64_t(doc.slot) + item) * (32 * NW) + wave * 32 + r32;
-        float* o = p.part + at * D + 4 * hk;
+        const uint64_t at = (uint64_t(doc.slot) + item) * NW + wave;
+        float* o = p.part + at * (32 * D);
+        if (NW > 1 || w0 + r32 < rows) // (of a few rows the others' are not written)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x16& a = oacc[dt];
-                *reinterpret_cast<f32x4*>(o + dt * 32 + 8 * i) = f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]};
-            }
-        if (hk == 0) {
-            p.part_ml[2 * at] = m;
-            p.part_ml[2 * at + 1] = lt;
+        for (int i = 0; i < 4 * DT; ++i)
+            *reinterpret_cast<f32x4*>(o + part_at<D, NW>(2 * i + hk, r32)) =
+                f32x4{oacc[i / 4][4 * (i % 4)], oacc[i / 4][4 * (i % 4) + 1], oacc[i / 4][4 * (i % 4) + 2], oacc[i / 4][4 * (i % 4) + 3]};
+        if (hk == 0 && w0 + r32 < rows) {
+            p.part_ml[2 * (at * 32 + r32)] = m;
+            p.part_ml[2 * (at * 32 + r32) + 1] = lt;
         }
         return;
     }
@@ -484,54 +489,73 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     }
 }
 
-// The splits of a row joined: a workgroup a row, D / 4 lanes a split at 4 dims each, so 8 (or 16) splits at a time.
-template <int D, int NW> __global__ __launch_bounds__(256) void join_kernel(PackedP p)
+// The splits joined: 4 dims of a row a thread, RW rows of a wave's 32 a workgroup, its G groups every G-th split each. Many rows: as
+// many as make 256 threads, in 1 group for up to 8 splits, in 4 for more; few: one, in 8 groups (16) (32 rows of 52 splits 4.0 us, 8 rows
+// a workgroup 7.6).
+constexpr uint32_t join_rows(int d, int nw) { return nw == 1 ? 1 : 1024 / d; }
+template <int D, int NW, uint32_t G> __global__ __launch_bounds__(D / 4 * join_rows(D, NW) * G) void join_kernel(PackedP p)
 {
-    constexpr uint32_t L = D / 4, G = 256 / L;
+    constexpr uint32_t RW = join_rows(D, NW), PER = NW * 32 / RW, T = D / 4 * RW; // T: threads a group
     const uint32_t di = find_doc(p.join, p.n_docs, blockIdx.x);
     const Doc doc = p.docs[di];
-    const uint32_t rows = doc.q_rows * p.group, at = blockIdx.x - p.join[di], g = threadIdx.x / L, e = threadIdx.x % L * 4;
-    if (doc.splits < 2 || at >= rows * p.kv_heads)
-        return;
-    const uint32_t kvh = at / rows, row = at % rows, block = row / (32 * NW);
-    // (blocks are numbered from the last one, as above)
-    const uint64_t item = uint64_t(doc.slot) + (uint64_t(kvh) * doc.blocks + (doc.blocks - 1 - block)) * doc.splits;
-    const uint64_t first = item * (32 * NW) + row % (32 * NW);
-    // each group of lanes its splits, against the largest m so far
+    const uint32_t rows = doc.q_rows * p.group, at = blockIdx.x - p.join[di];
+    const uint32_t kvh = at / (doc.blocks * PER), bi = at / PER % doc.blocks, sub = at % PER; // (blocks as above, from the last one)
+    const uint32_t g = threadIdx.x / T, q = threadIdx.x % T, chunk = q / RW;
+    const uint32_t in_block = sub * RW + q % RW, row = (doc.blocks - 1 - bi) * (32 * NW) + in_block;
+    if (kvh >= p.kv_heads || (doc.blocks - 1 - bi) * (32 * NW) + sub * RW >= rows)
+        return; // (the whole workgroup)
+    const uint64_t slot = uint64_t(doc.slot) + (uint64_t(kvh) * doc.blocks + bi) * doc.splits;
+    const uint32_t wave = in_block / 32, r32 = in_block % 32;
     float m = kLeast, l = 0.0f;
     f32x4 o = f32x4{};
-#pragma unroll 4
-    for (uint32_t s = g; s < doc.splits; s += G) {
-        const uint64_t i = first + uint64_t(s) * (32 * NW);
-        const float ms = p.part_ml[2 * i], ls = p.part_ml[2 * i + 1];
-        const f32x4 os = *reinterpret_cast<const f32x4*>(p.part + i * D + e);
-        const float mn = fmaxf(m, ms), a = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(ms - mn);
-        m = mn;
-        l = l * a + w * ls;
-        o = o * a + w * os;
+    if (row < rows) {
+        // (4 splits' loads at a time)
+        constexpr uint32_t U = 4;
+        for (uint32_t s0 = g; s0 < doc.splits; s0 += U * G) {
+            float ms[U], ls[U];
+            f32x4 os[U];
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j) {
+                const uint64_t i = (slot + min(s0 + j * G, doc.splits - 1)) * NW + wave;
+                ms[j] = p.part_ml[2 * (i * 32 + r32)];
+                ls[j] = p.part_ml[2 * (i * 32 + r32) + 1];
+                os[j] = *reinterpret_cast<const f32x4*>(p.part + i * (32 * D) + part_at<D, NW>(chunk, r32));
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j) {
+                if (s0 + j * G >= doc.splits)
+                    break;
+                const float mn = fmaxf(m, ms[j]), a = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(ms[j] - mn);
+                m = mn;
+                l = l * a + w * ls[j];
+                o = o * a + w * os[j];
+            }
+        }
     }
-    __shared__ float sm[G], sl[G];
-    __shared__ __attribute__((aligned(16))) float so[G][D];
-    if (e == 0) {
-        sm[g] = m;
-        sl[g] = l;
+    if constexpr (G > 1) {
+        __shared__ __attribute__((aligned(16))) f32x4 so[G - 1][T];
+        __shared__ float sm[G - 1][T], sl[G - 1][T];
+        if (g) {
+            so[g - 1][q] = o;
+            sm[g - 1][q] = m;
+            sl[g - 1][q] = l;
+        }
+        __syncthreads();
+        if (g)
+            return;
+#pragma unroll
+        for (uint32_t i = 0; i < G - 1; ++i) {
+            const float mn = fmaxf(m, sm[i][q]), a = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(sm[i][q] - mn);
+            m = mn;
+            l = l * a + w * sl[i][q];
+            o = o * a + w * so[i][q];
+        }
     }
-    *reinterpret_cast<f32x4*>(&so[g][e]) = o;
-    __syncthreads();
-    if (g)
+    if (row >= rows)
         return;
-    for (uint32_t i = 1; i < G; ++i)
-        m = fmaxf(m, sm[i]);
-    l = 0.0f;
-    o = f32x4{};
-    for (uint32_t i = 0; i < G; ++i) {
-        const float w = __builtin_amdgcn_exp2f(sm[i] - m);
-        l = fmaf(w, sl[i], l);
-        o += w * *reinterpret_cast<const f32x4*>(&so[i][e]);
-    }
     o *= l == 0.0f ? 0.0f : 1.0f / l;
     const bool h = p.out_f16;
-    *reinterpret_cast<u32x2*>(p.out + (int64_t(doc.q_row) + row / p.group) * p.ldo + int64_t(kvh * p.group + row % p.group) * D + e) =
+    *reinterpret_cast<u32x2*>(p.out + (int64_t(doc.q_row) + row / p.group) * p.ldo + int64_t(kvh * p.group + row % p.group) * D + chunk * 4) =
         u32x2{pack_x2(o[0], o[1], h), pack_x2(o[2], o[3], h)};
 }
 
@@ -593,6 +617,7 @@ struct Launch {
     uint32_t nw;          // waves a workgroup (32 rows each)
     uint32_t groups;      // workgroups
     uint32_t joins;       // workgroups of the second launch, 0: none
+    uint32_t most_splits;
     uint64_t slots;       // partial results
 };
 
@@ -628,40 +653,46 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
         tiles += uint64_t(d.blocks) * a->kv_heads * cdiv(d.k_rows, kKT);
         longest = std::max<uint64_t>(longest, cdiv(d.k_rows, kKT));
     }
-    // How many tiles a workgroup takes at most: the halving of the longest document's with the least estimated time. A tile takes
-    // about 1.4 us where a compute unit has one workgroup; a split's partial results go to memory and back, at 4 TB/s, and are
-    // joined by a launch of 4 us. (us without and with splits: 1 row over 512 keys 15.7 / 9.7, 64 over 512 17.7 / 13.6, 512 over
-    // 512 18.8 / 33.7.)
-    auto items_of = [&](const Doc& d, uint64_t target) {
-        return uint64_t(d.blocks) * a->kv_heads * std::max<uint64_t>((cdiv(d.k_rows, kKT) + target - 1) / target, 1);
+    // How many tiles a workgroup takes at most: the part of the longest document's with the least estimated time. A tile takes about
+    // 1 us (heads of 128; 0.7 of 64) where a compute unit has one workgroup; partial results cost a launch and their way to
+    // memory and back, 2.5 us and 0.6 a MB. (us without splits / with 2 / with 8: 8 heads of 64 over 1024 rows 16.5 / 14.4 / 19.0, 20 of
+    // 128 over 1024 21.6 / 30.2 / 43.0, over 64 of 2048 43.6 / 24.5 / 14.3.)
+    auto splits_of = [](const Doc& d, uint64_t target) {
+        return std::max<uint64_t>((cdiv(d.k_rows, kKT) + target - 1) / target, 1);
     };
     uint64_t target = std::max<uint64_t>(longest, 1);
     double best = 1e300;
-    for (uint64_t t = target; split && t; t = t > 1 ? (t + 1) / 2 : 0) {
-        uint64_t part = 0;
-        for (uint32_t i = 0; i < n; ++i)
-            if (cdiv(p.docs[i].k_rows, kKT) > t)
-                part += items_of(p.docs[i], t);
-        const double bytes = double(part) * (32 * out.nw) * (a->d + 2) * 4;
-        const double time = std::max(double(t), double(tiles) / resident) * 1.4 + (part ? 4.0 + 2.0 * bytes / 4e6 : 0.0);
+    for (uint64_t parts = 1; split && parts <= std::max<uint64_t>(longest, 1); parts += 1 + parts / 4) {
+        const uint64_t t = std::max<uint64_t>((longest + parts - 1) / parts, 1);
+        double rows = 0, items = 0;
+        for (uint32_t i = 0; i < n; ++i) {
+            const Doc& d = p.docs[i];
+            items += double(d.blocks) * a->kv_heads * splits_of(d, t);
+            if (splits_of(d, t) > 1)
+                rows += double(d.q_rows) * a->heads * splits_of(d, t);
+        }
+        // (more workgroups than the chip holds: their share, and half a workgroup for the last round's end)
+        const double long_one = items <= resident ? double(t) : double(tiles) / resident + 0.5 * double(t);
+        const double time = long_one * (a->d == 128 ? 1.0 : 0.7) + (rows > 0 ? 2.5 + rows * (a->d + 2) * 4 * 0.6e-6 : 0.0);
         if (time < best) {
             best = time;
             target = t;
         }
     }
     uint64_t first = 0, join = 0;
-    out.slots = 0;
+    out.slots = out.most_splits = 0;
     for (uint32_t i = 0; i < n; ++i) {
         Doc& d = p.docs[i];
-        const uint64_t items = items_of(d, target);
-        d.splits = uint32_t(items / (uint64_t(d.blocks) * a->kv_heads));
+        d.splits = uint32_t(splits_of(d, target));
+        const uint64_t items = uint64_t(d.blocks) * a->kv_heads * d.splits;
+        out.most_splits = std::max(out.most_splits, d.splits);
         p.first[i] = uint32_t(first);
         p.join[i] = uint32_t(join);
         d.slot = uint32_t(out.slots);
         first += round_up(items, 8);
         if (d.splits > 1) {
             out.slots += items;
-            join += uint64_t(d.q_rows) * a->heads;
+            join += uint64_t(d.blocks) * a->kv_heads * (out.nw == 1 ? 32 : 128 * a->d / 1024);
         }
     }
     p.n_docs = n;
@@ -688,8 +719,14 @@ template <int D> void launch_all(const PackedP& p, const Launch& l, bool f16, in
         f16 ? launch_mode<D, true, 4>(p, mode, l.groups, s) : launch_mode<D, false, 4>(p, mode, l.groups, s);
     else
         f16 ? launch_mode<D, true, 1>(p, mode, l.groups, s) : launch_mode<D, false, 1>(p, mode, l.groups, s);
-    if (l.joins)
-        l.nw == 4 ? join_kernel<D, 4><<<l.joins, 256, 0, s>>>(p) : join_kernel<D, 1><<<l.joins, 256, 0, s>>>(p);
+    if (!l.joins)
+        return;
+    if (l.nw == 1)
+        join_kernel<D, 1, 1024 / D><<<l.joins, 256, 0, s>>>(p);
+    else if (l.most_splits <= 8)
+        join_kernel<D, 4, 1><<<l.joins, 256, 0, s>>>(p);
+    else
+        join_kernel<D, 4, 4><<<l.joins, 1024, 0, s>>>(p);
 }
 mk_status device_cus(uint32_t* cus)
 {
