@@ -92,7 +92,8 @@ template <int D, int NW> __device__ inline uint32_t part_at(uint32_t chunk, uint
 
 enum { kPlain = 0, kBias = 1, kCap = 2 /* a bit each */ };
 
-// Waves a SIMD that the registers have to leave room for.
+// Waves a SIMD that the registers have to leave room for. (Heads of 64 fit three, us of 20 heads, two documents of 4096, with
+// three / with two: with a bias 221 / 243, capped 304 / 329, neither the same. Heads of 128 would spill.)
 constexpr int waves_of(int d, int nw) { return nw == 1 ? 1 : d == 64 ? 3 : 2; }
 
 template <int D, bool F16, int MODE, int NW>
@@ -643,8 +644,10 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
     for (uint32_t i = 1; i < n; ++i)
         for (uint32_t j = i; j && p.docs[j].k_rows > p.docs[j - 1].k_rows; --j)
             std::swap(p.docs[j], p.docs[j - 1]);
-    // one wave a workgroup where all rows of a key head fit it: few rows over many keys
-    out.nw = most_rows <= 32 ? 1 : 4;
+    // One wave a workgroup where a key head has few rows in every document (us with one / with four: 1 row of 32 heads of 128 on
+    // 8 over 16411 keys 22.3 / 24.4, 16 rows of 20 heads of 64 over 4096 11.8 / 13.7; 32 rows over 77 6.2 / 5.7, 32 rows of 32 heads
+    // of 128 over 4096 25.1 / 22.6: four waves share a tile's loads).
+    out.nw = most_rows <= 16 ? 1 : 4;
     const uint32_t resident = cus * (out.nw == 4 || a->d == 128 ? 2 : 4);
     uint64_t tiles = 0, longest = 0;
     for (uint32_t i = 0; i < n; ++i) {
