@@ -320,17 +320,17 @@ typedef struct mk_attn_packed_args {
     uint32_t dtype;      /* q, k, v: MK_BF16 or MK_F16 */
     uint32_t out_dtype;  /* MK_BF16 or MK_F16 */
     uint32_t heads, kv_heads, d; /* kv_heads divides heads (at most 65535), d 64 or 128 */
-    float scale;         /* s = scale q.k; finite, >= 0 (0 is 0: every seen key weighs the same) */
-    float cap;           /* > 0: s = cap tanh(s / cap); 0: none */
+    float scale;         /* s = scale q.k; finite, >= 0 (0 is 0: every seen key weighs the same), below 2^126, as scale / cap */
+    float cap;           /* > 0: s = cap tanh(s / cap), up to 4096 (scores are then off by 2^-20 cap); 0: none */
     const float* slopes; /* device [heads] or NULL: s -= slopes[h] |p - c|, after the cap */
     const mk_attn_doc* docs; /* host [n_docs], in any order; q rows of two documents must not overlap, k rows may */
     uint32_t n_docs;
     void* workspace;     /* 16-byte aligned, or NULL: few rows over many keys then run on few compute units */
     uint64_t workspace_bytes; /* at least what mk_attention_packed_workspace says, when workspace is not NULL */
 } mk_attn_packed_args;
-/* out = softmax(s) v over the seen keys, sums and the softmax in fp32; the probabilities enter the second product in the inputs'
- * type, rounded once. A row that sees no key, or only keys of score -inf, is zero. Rows outside every document are left as they were. What a row does not see does not
- * reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees makes it NaN. All pointers
+/* out = softmax(s) v over the seen keys, scores, sums and the softmax in fp32; the probabilities enter the second product in the
+ * inputs' type, rounded once. A row that sees no key, or only keys of score -inf (below fp32's range), is zero. Rows outside every
+ * document are left as they were. What a row does not see does not reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees makes it NaN. All pointers
  * 16-byte aligned (slopes 4). A row's bits may depend on the other documents of the call (their number decides how keys are
  * split), not on their contents. */
 mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream);

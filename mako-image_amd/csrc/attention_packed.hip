@@ -16,7 +16,10 @@ constexpr uint32_t kMaxDocs = 64; // documents a launch: they go by kernel argum
 constexpr int kKT = 64;           // keys a tile
 // The exponentials' reference m moves only when a weight against it passes 2^8 (below).
 constexpr float kLazyP = 256.0f;
-constexpr float kLeast = -1e30f; // m of rows without a score above -inf
+constexpr float kLeast = -3.402823466e38f; // m of rows without a score above -inf
+// |m| from which on scores are rounded before m is taken off them. Below it one fma does both, exact against any m; from 2^31 on
+// half a step of m itself, which the largest weight would be off by, no longer fits a weight's exponent (a half's from 2^26).
+constexpr float kLargeM = 16777216.0f;
 
 struct Doc {
     uint32_t q_row, q_rows, k_row, k_rows;
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     const int64_t wg_pos = int64_t(doc.q_pos) + wg0 / p.group;
     const int wg_lim = seen_keys(doc, wg_pos); // of the workgroup's first row: the least
     const int wave_most = seen_keys(doc, int64_t(doc.q_pos) + min(w0 + 31, rows - 1) / p.group);
-    const int all_tiles = (seen_keys(doc, int64_t(doc.q_pos) + wg_last / p.group) + kKT - 1) / kKT;
+    const int all_tiles = (uint32_t(seen_keys(doc, int64_t(doc.q_pos) + wg_last / p.group)) + kKT - 1) / kKT;
     const int t_begin = int(uint64_t(all_tiles) * split / doc.splits), t_end = int(uint64_t(all_tiles) * (split + 1) / doc.splits);
 
     u32x4 qf[DS];
@@ -175,6 +178,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     for (int dt = 0; dt < DT; ++dt)
         oacc[dt] = f32x16{};
     float m = kLeast, l = 0.0f;
+    float ref = kLeast; // what the weights are first made against: m, or, where m is large, so little that they are made again
     const float slope = MODE & kBias ? p.slopes[head] * 1.4426950408889634f : 0.0f;
 
     // What a lane knows of a half of a tile: its row's position less the lane's first key (values r are 8 (r / 4) + r % 4 keys
@@ -198,9 +202,13 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         return x;
     };
     auto masked = [](float x, const Half& h, int r) { return 8 * (r / 4) + r % 4 < h.more ? x : -__builtin_inff(); };
-    // the weights of pair j of a half, packed, and their sum
-    auto pair = [&](const f32x16& sc, const Half& h, int j, uint32_t (&pw)[8], float& ls, auto edge_c) {
-        float x0 = score(sc[2 * j], h, 2 * j, m), x1 = score(sc[2 * j + 1], h, 2 * j + 1, m);
+    // the weights of pair j of a half against `from` (and then `less`), packed, and their sum
+    auto pair = [&](const f32x16& sc, const Half& h, int j, uint32_t (&pw)[8], float& ls, float from, auto less, auto edge_c) {
+        float x0 = score(sc[2 * j], h, 2 * j, from), x1 = score(sc[2 * j + 1], h, 2 * j + 1, from);
+        if constexpr (std::is_same_v<decltype(less), float>) {
+            x0 -= less;
+            x1 -= less;
+        }
         if constexpr (decltype(edge_c)::value) {
             x0 = masked(x0, h, 2 * j);
             x1 = masked(x1, h, 2 * j + 1);
@@ -220,6 +228,8 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         }
         const float mn = fmaxf(m, max_xor32(max16(x))), alpha = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
+        const bool large = fabsf(m) >= kLargeM;
+        ref = large ? kLeast : m;
         l *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -229,7 +239,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         ls = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            pair(sc, h, j, pw, ls, edge_c);
+            pair(sc, h, j, pw, ls, large ? 0.0f : m, large ? m : 0.0f, edge_c);
     };
     auto read_k = [&](int buf, int kt, int ds) {
         const int key = kt * 32 + r32;
@@ -284,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     };
     auto add_odd = [&](int t) {
 #pragma unroll 1
-        for (int key = t * kKT; key < min(t * kKT + kKT, int(doc.k_rows)); ++key) {
+        for (int key = t * kKT; key < t * kKT + tile_keys(t); ++key) {
             const uint16_t* v = V + int64_t(key) * p.ldv + 4 * hk;
             if (key >= lim)
                 continue;
@@ -350,7 +360,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         auto chunk = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, int c) {
 #pragma unroll
             for (int j = c * CH; j < (c + 1) * CH; ++j) {
-                pair(sc, h, j, pw, ls, edge_c);
+                pair(sc, h, j, pw, ls, ref, 0, edge_c);
                 // (pinned here: the compiler would sink the work into the path that keeps it)
                 asm volatile("" : "+v"(pw[j]), "+v"(ls));
             }
@@ -407,7 +417,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         __syncthreads();
         bool odd = false;
         if constexpr (decltype(edge_c)::value)
-            odd = wg_lim < min(t * kKT + kKT, int(doc.k_rows)) && find_odd(t, buf_c);
+            odd = wg_lim < t * kKT + tile_keys(t) && find_odd(t, buf_c);
         tile(t, tile_at(i + 1), buf_c, edge_c);
         if (decltype(edge_c)::value && odd)
             add_odd(t);
@@ -575,6 +585,10 @@ mk_status check_shape(const mk_attn_packed_args* a)
         return fail(MK_ERR_ARG, "attention_packed: head dim must be 64 or 128");
     if (!(a->scale >= 0.0f) || std::isinf(a->scale) || !(a->cap >= 0.0f) || std::isinf(a->cap))
         return fail(MK_ERR_ARG, "attention_packed: scale and cap must be finite and not negative");
+    // (the kernels' factors; and cap tanh(s / cap) is made as cap - 2 cap / (1 + e^(2 s / cap)), 16 u cap off: 2^-8 at 2^12)
+    constexpr float kLog2e = 1.4426950408889634f;
+    if (a->cap > 4096.0f || std::isinf(kLog2e * a->scale) || (a->cap > 0.0f && std::isinf(2.0f * kLog2e * a->scale / a->cap)))
+        return fail(MK_ERR_ARG, "attention_packed: cap up to 4096, scale and scale / cap below 2^126");
     const int64_t nq = int64_t(a->heads) * a->d, nk = int64_t(a->kv_heads) * a->d;
     constexpr int64_t most = 1 << 24;
     auto bad = [](int64_t ld, int64_t n) { return ld < n || ld % 8 || ld >= most; };

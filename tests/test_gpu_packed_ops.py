@@ -293,6 +293,26 @@ def test_attention_scores_far_apart_and_large(gpu):
             Attn(docs, nq, nk, 3, 3, 128, dt, scale=scale, edit=edit).check()
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("level", [23, 24, 26, 28, 31, 34, 60, 100, 120])
+@pytest.mark.parametrize("dt", [M.BF16, M.F16])
+def test_attention_scores_of_any_size(gpu, dt, level, sign):
+    """Scores of 1, 2 or 3 times 1 to 2 x 2^level: the largest ones' keys share the weight, however far the scores are from fp32's
+    integers (half a step of a score passes a weight's exponent range from 2^31 on)."""
+    for d, heads, kv, rows, nk, workspace, by in ((128, 4, 1, 3, 300, True, 1.1), (64, 2, 2, 40, 130, False, 1.3), (128, 2, 2, 140, 70, True, 1.7), (64, 4, 2, 40, 130, True, 1.9)):
+        def edit(raw):
+            raw["q"][:] = 0.0
+            raw["q"][:, :, 5] = 1.0
+            raw["k"][:] = 0.0
+            raw["k"][:, :, 5] = sign * (1 + np.random.default_rng(level).integers(0, 3, raw["k"].shape[:2]))
+        a = Attn([(0, rows, 0, nk, nk - rows, 0xFFFFFFFF, 0)], rows, nk, heads, kv, d, dt, scale=float(np.float32(by * 2.0 ** level)), edit=edit)
+        # the score's rounding moves all equal scores alike: the tolerance counts that of the weights and sums alone
+        want, _ = attend(a.val["q"], a.val["k"], a.val["v"], a.docs, a.scale, 0.0, None, dt, dt)
+        got = values(a.run(workspace).result()[0], dt)
+        v = np.abs(a.val["v"]).max()
+        np.testing.assert_allclose(got, want, rtol=0, atol=(2 * H[dt] + nk * u) * v)
+
+
 def test_attention_minus_infinity_scores(gpu):
     # keys whose score is -inf weigh nothing; a row of only such keys is zero
     docs, nq, nk = packed([4, 4], [80, 3])

@@ -35,7 +35,7 @@ def attn(**kw):
     (dict(q=None), "null"), (dict(out=None), "null"), (dict(dtype=M.F32), "bf16 or f16"), (dict(out_dtype=M.I8), "output"),
     (dict(heads=0), "kv_heads"), (dict(kv_heads=0), "kv_heads"), (dict(kv_heads=3), "kv_heads"), (dict(heads=65536), "kv_heads"),
     (dict(d=96), "head dim"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
-    (dict(cap=-2.0), "cap"), (dict(cap=float("inf")), "cap"), (dict(ldq=504), "rows must"), (dict(ldq=516), "rows must"), (dict(ldk=-256), "rows must"),
+    (dict(cap=-2.0), "cap"), (dict(cap=float("inf")), "cap"), (dict(cap=4097.0), "cap"), (dict(scale=1.2e38, cap=1e-3), "cap"), (dict(scale=3e38), "scale"), (dict(ldq=504), "rows must"), (dict(ldq=516), "rows must"), (dict(ldk=-256), "rows must"),
     (dict(ldv=1 << 24), "rows must"), (dict(ldo=500), "rows must"), (dict(docs=None), "null"), (dict(q=P + 8), "aligned"), (dict(out=P + 2), "aligned"),
     (dict(workspace=P + 4), "aligned"), (dict(slopes=P + 2), "aligned"),
     (dict(docs=[(0, 8, 0, 8, 0, 0, 0), (7, 2, 0, 8, 0, 0, 0)]), "share"), (dict(docs=[(10, 8, 0, 8, 0, 0, 0), (0, 11, 0, 8, 0, 0, 0)]), "share"),
