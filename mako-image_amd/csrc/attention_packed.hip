@@ -75,15 +75,23 @@ __device__ inline int seen_keys(const Doc& d, int64_t pos)
     n = n < int64_t(d.k_rows) ? n : int64_t(d.k_rows);
     return int(n > 0 ? n : 0);
 }
-// The document of a workgroup, by its place among their first ones (at most 64, ascending, the first 0). Arguments come from
-// host memory, 2 us and more a round trip, so all lanes compare at once: a search by halves took several.
-__device__ inline uint32_t find_doc(const uint32_t (&first)[kMaxDocs], uint32_t n, uint32_t item)
+// The document of a workgroup, by its place among their first ones (`table`: at most 64, ascending, the first 0), and that first
+// one. Arguments come from host memory, 2 us and more a round trip, so a lane reads each place and document in one go: a
+// search by halves took several, the place and then the document two (6453 rows over three documents 21.9 us, 21.1 so).
+__device__ inline Doc find_doc(const PackedP& p, const uint32_t (&table)[kMaxDocs], uint32_t item, uint32_t& first)
 {
     static_assert(kMaxDocs <= 64, "one a lane");
-    if (n == 1)
-        return 0;
-    const uint32_t lane = threadIdx.x & 63, at = first[min(lane, n - 1)];
-    return __builtin_amdgcn_readfirstlane(uint32_t(__popcll(__ballot(lane < n && at <= item))) - 1);
+    if (p.n_docs == 1) {
+        first = 0;
+        return p.docs[0];
+    }
+    const uint32_t lane = threadIdx.x & 63, i = min(lane, p.n_docs - 1), at = table[i];
+    const Doc d = p.docs[i];
+    const int of = int(__popcll(__ballot(lane < p.n_docs && at <= item))) - 1;
+    auto get = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), of)); };
+    first = get(at);
+    return Doc{get(d.q_row), get(d.q_rows), get(d.k_row), get(d.k_rows), int32_t(get(uint32_t(d.q_pos))), get(d.block), get(d.prefix),
+               get(d.blocks), get(d.splits), get(d.slot), 0};
 }
 
 // Where 4 dims (chunk) of one of a wave's 32 rows are in its partial results: with many rows the rows of a chunk next to each
@@ -113,12 +121,12 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
 
     const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hk = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t di = find_doc(p.first, p.n_docs, blockIdx.x);
-    const Doc doc = p.docs[di];
+    uint32_t doc_first;
+    const Doc doc = find_doc(p, p.first, blockIdx.x, doc_first);
     // Workgroup i runs on XCD i % 8: each XCD takes a run of a document's (key head, block, split), whose blocks share keys in
     // its L2; later blocks, which see more under a causal mask, come first.
     const uint32_t each = doc.blocks * doc.splits, real = each * p.kv_heads, run = (real + 7) / 8;
-    const uint32_t local = blockIdx.x - p.first[di], item = local % 8 * run + local / 8;
+    const uint32_t local = blockIdx.x - doc_first, item = local % 8 * run + local / 8;
     if (local / 8 >= run || item >= real)
         return;
     const uint32_t kvh = item / each, block = doc.blocks - 1 - item % each / doc.splits, split = item % doc.splits;
@@ -507,9 +515,9 @@ constexpr uint32_t join_rows(int d, int nw) { return nw == 1 ? 1 : 1024 / d; }
 template <int D, int NW, uint32_t G> __global__ __launch_bounds__(D / 4 * join_rows(D, NW) * G) void join_kernel(PackedP p)
 {
     constexpr uint32_t RW = join_rows(D, NW), PER = NW * 32 / RW, T = D / 4 * RW; // T: threads a group
-    const uint32_t di = find_doc(p.join, p.n_docs, blockIdx.x);
-    const Doc doc = p.docs[di];
-    const uint32_t rows = doc.q_rows * p.group, at = blockIdx.x - p.join[di];
+    uint32_t doc_first;
+    const Doc doc = find_doc(p, p.join, blockIdx.x, doc_first);
+    const uint32_t rows = doc.q_rows * p.group, at = blockIdx.x - doc_first;
     const uint32_t kvh = at / (doc.blocks * PER), bi = at / PER % doc.blocks, sub = at % PER; // (blocks as above, from the last one)
     const uint32_t g = threadIdx.x / T, q = threadIdx.x % T, chunk = q / RW;
     const uint32_t in_block = sub * RW + q % RW, row = (doc.blocks - 1 - bi) * (32 * NW) + in_block;

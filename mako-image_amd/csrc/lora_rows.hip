@@ -859,7 +859,8 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
         return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
     LoraP p{static_cast<const uint16_t*>(a->x), static_cast<const uint16_t*>(a->a), static_cast<const uint16_t*>(a->b), a->scale,
             a->ids, a->base, a->c, static_cast<float*>(a->workspace),
-            plan.order ? reinterpret_cast<u32x2*>(static_cast<char*>(a->workspace) + bytes_of_t(a, plan.splits)) : nullptr, a->ldx, a->ldbase, a->ldc, a->rows, a->K, a->N, a->rank,
+            plan.order ? reinterpret_cast<u32x2*>(static_cast<char*>(a->workspace) + bytes_of_t(a, plan.splits)) : nullptr,
+            a->ldx, a->ldbase, a->ldc, a->rows, a->K, a->N, a->rank,
             a->parts, a->adapters, plan.splits, plan.split_k, plan.blocks};
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto f16_c, auto ct_c) {
