@@ -5,7 +5,7 @@
 // partial sums of the workgroups that share a row's K (no atomics: the second launch adds them in their order). Very few rows
 // take both products in one launch, and many rows in no order are first put in the order of their adapters by one more.
 // On the device: 4352 x 4096 to 12288 by rank 32 in 3 parts 76 us (x, base and c at 3.3 TB/s), 16401 x 12288 to 4096 by rank
-// 64, fp32 rows, 260 us (3.6 TB/s), 1 row of 4096 to 4096 5.4 us.
+// 64, fp32 rows, 252 us (3.7 TB/s), 1 row of 4096 to 4096 5.4 us.
 #include "common.hpp"
 
 #include <type_traits>
@@ -447,14 +447,17 @@ template <class V> __device__ inline V load_v(BufRes r, uint32_t voff, uint32_t 
 }
 // (A 16-byte store's offset is in one register, with no scalar beside it: its data must not be overwritten by the very next
 // instruction, and the compiler keeps them apart only in that form. With a scalar offset, the first values of the last
-// store of a tile came out as what the next instruction wrote, in some lanes and now and then.)
+// store of a tile came out as what the next instruction wrote, in some lanes and now and then.) Non-temporal: c is many times a cache,
+// and leaves base and x room in it (us with / without: 16384 x 4096 to 4096 by rank 16 95 / 107, 16401 x 12288 to 4096 in fp32 252 /
+// 263, 4352 x 4096 to 12288 76 / 78; with the projection before and the rotary positions behind it the same). Base loaded so
+// is faster where it comes from memory (241) and slower where the projection has just stored it; x loaded so is slower.
 template <class V> __device__ inline void store_v(V v, BufRes r, uint32_t voff)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
     if constexpr (sizeof(V) == 16)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, int(voff), 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, int(voff), 0, 2);
     else
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, int(voff), 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, int(voff), 0, 2);
 #endif
 }
 
