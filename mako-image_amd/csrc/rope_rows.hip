@@ -40,10 +40,9 @@ template <uint32_t T> __device__ inline f32x4 load4(const void* p, int64_t at)
 template <uint32_t T> __device__ inline void store4(void* p, int64_t at, const f32x4& v)
 {
     if constexpr (T == MK_F32)
-        *reinterpret_cast<f32x4*>(static_cast<float*>(p) + at) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(static_cast<float*>(p) + at));
     else
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + at) =
-            u32x2{pack_x2(v[0], v[1], T == MK_F16), pack_x2(v[2], v[3], T == MK_F16)};
+        __builtin_nontemporal_store(u32x2{pack_x2(v[0], v[1], T == MK_F16), pack_x2(v[2], v[3], T == MK_F16)}, reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + at));
 }
 
 // The fraction of a turn, in 2^-32: an int32 position times the pair's fraction modulo 2^64 is exact; an fp32 one goes through
@@ -70,7 +69,9 @@ __device__ inline void cos_sin(uint32_t turns, float& c, float& s)
 // A lane holds 8 values of a head as two groups of 4: pairs 4 l .. 4 l + 3, with their partners R / 2 further (mode 1) or next
 // to them (mode 2), or 8 values that are not turned. So d / 8 lanes share a head, a wave holds 64 / (d / 8) heads of one row,
 // IT times: the row's cosines and sines are made once a lane for all of them. Bound by memory: every value is read and
-// written once (32760 rows of 64 heads of 128 from fp32 to bf16 300 us, 5.4 TB/s; 1333 of 40 of 64 in half 6.2 on the device).
+// written once (32760 rows of 64 heads of 128 from fp32 to bf16 290 us, 5.6 TB/s; 1333 of 40 of 64 in half 5.9 on the device).
+// Stored non-temporally, which leaves the projection's rows, still to be read, their place in the caches (16384 bf16 rows of 64 heads
+// 136 -> 110 us, 4352 38 -> 33; attention behind it takes the same time).
 template <uint32_t IN, uint32_t OUT, typename POS, int MODE, int IT> __global__ __launch_bounds__(256) void rope_kernel(RopeP p)
 {
     const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -166,8 +167,8 @@ template <uint32_t IN, uint32_t OUT, typename POS, int MODE, int IT> __global__ 
 template <uint32_t IN, uint32_t OUT, typename POS, int MODE> void launch_it(const RopeP& p, hipStream_t s)
 {
     const uint32_t wave_heads = 64 / (p.d / 8), steps = cdiv(p.heads + p.kv_heads, wave_heads);
-    // us with 4 steps a wave / with 1, heads of 128: 64 rows of 40 heads 5.2 / 3.7, 512 of 40 6.0 / 5.8; 1024 of 64 11.5 / 12.6, 4352 of
-    // 10 9.2 / 9.9, 16384 of 64 134 / 177 (a wave's sines serve four times the heads)
+    // us with 4 steps a wave / with 1, heads of 128: 64 rows of 40 heads 5.2 / 3.7, 512 of 40 5.7 / 5.5; 1024 of 64 9.2 / 11.0, 4352 of
+    // 10 8.1 / 8.8, 16384 of 64 109 / 132 (a wave's sines serve four times the heads)
     if (uint64_t(p.rows) * (p.heads + p.kv_heads) * p.d >= 1u << 22)
         rope_kernel<IN, OUT, POS, MODE, 4><<<dim3(cdiv(p.rows, 4), cdiv(steps, 4)), 256, 0, s>>>(p);
     else
