@@ -305,7 +305,7 @@ template <bool F16, uint32_t CT> __global__ __launch_bounds__(kOneThreads) void 
 // Many rows: a tile of 64 rows by 32 NB of A's rows and one split of K. Each of the four waves takes every fourth 32 k for the
 // whole tile, through three stages of LDS of its own (direct loads, two steps ahead, no barriers in the loop; nothing is read
 // from LDS twice), and the waves' sums are added at the end. A tile with rows of several adapters goes through K for each.
-// 16401 rows of 12288, rank 64: 128 us, 3.1 TB/s of x, of 3.6 to 4.0 TB/s that a reduction's reads reach. No faster: two or four
+// 16401 rows of 12288, rank 64: 117 to 134 us, 3.0 to 3.4 TB/s of x, of 3.6 to 4.0 TB/s that a reduction's reads reach. No faster: two or four
 // stages, 128 rows a tile (160 us), a line of 128 bytes a row and wave, K begun elsewhere in every tile, and all tiles' steps
 // shared evenly by as many workgroups as the chip holds (139 us, and more partial results to add).
 constexpr int kStepK = 128;
