@@ -330,7 +330,8 @@ typedef struct mk_attn_packed_args {
 } mk_attn_packed_args;
 /* out = softmax(s) v over the seen keys, scores, sums and the softmax in fp32; the probabilities enter the second product in the
  * inputs' type, rounded once. A row that sees no key, or only keys of score -inf (below fp32's range), is zero. Rows outside every
- * document are left as they were. What a row does not see does not reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees makes it NaN. All pointers
+ * document are left as they were. What a row does not see does not reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees makes it NaN, an infinity in v that
+ * infinity, or NaN where its weight is zero in the inputs' type. All pointers
  * 16-byte aligned (slopes 4). A row's bits may depend on the other documents of the call (their number decides how keys are
  * split), not on their contents. */
 mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream);

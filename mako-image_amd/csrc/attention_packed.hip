@@ -226,7 +226,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         ls += e0 + e1;
     };
     // moves m up to a half's largest score, rescales what was summed against the old one, and makes the half's weights again
-    auto redo = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, auto edge_c) {
+    auto redo = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, auto edge_c) __attribute__((always_inline)) {
         f32x16 x;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -269,8 +269,9 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
 
     // Infinities and NaNs of V at keys that only some of a tile's rows see must not meet the others' zero weights. Where a mask
     // cuts a tile for some row of the workgroup, V is looked through (a quarter a wave); if there are any, they are replaced by
-    // zeros in LDS, and after the products each row adds those that it sees.
-    auto find_odd = [&](int t, auto buf_c) {
+    // zeros in LDS, and after the products each row adds those that it sees, or a NaN where its weight is zero (0 x inf), as the
+    // product itself makes it in a tile that no mask cuts.
+    auto find_odd = [&](int t, auto buf_c) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value, N = kKT * KC / (64 * NW);
         constexpr uint32_t ODD = F16 ? 0x04000400u : 0x00800080u; // added to an exponent of all ones: a carry into bit 15
         uint32_t any = 0;
@@ -300,22 +301,27 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         __syncthreads();
         return true;
     };
-    auto add_odd = [&](int t) {
+    // `none`: a lane's weights of the tile that are zero, a bit each, those of half b above those of half a
+    auto add_odd = [&](int t, uint32_t none) __attribute__((always_inline)) {
+        const uint32_t other = uint32_t(__shfl_xor(int(none), 32)), none0 = hk ? other : none, none1 = hk ? none : other;
 #pragma unroll 1
-        for (int key = t * kKT; key < t * kKT + tile_keys(t); ++key) {
+        for (int i = 0, n = tile_keys(t); i < n; ++i) {
+            const int key = t * kKT + i;
             const uint16_t* v = V + int64_t(key) * p.ldv + 4 * hk;
             if (key >= lim)
                 continue;
+            // (key 8 r / 4 + 4 hk + r % 4 of a half is lane half hk's value r)
+            const bool zero = (i & 4 ? none1 : none0) >> (i / 32 * 16 + i % 32 / 8 * 4 + i % 4) & 1;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const u32x2 h = *reinterpret_cast<const u32x2*>(v + dt * 32 + 8 * i);
+                for (int j = 0; j < 4; ++j) {
+                    const u32x2 h = *reinterpret_cast<const u32x2*>(v + dt * 32 + 8 * j);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint16_t x = uint16_t(h[e / 2] >> (16 * (e % 2)));
                         if ((x & EXP) == EXP)
-                            oacc[dt][4 * i + e] += F16 ? h2f_bits(x) : bf2f_bits(x);
+                            oacc[dt][4 * j + e] += zero ? __builtin_nanf("") : F16 ? h2f_bits(x) : bf2f_bits(x);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     // products P V of half a. A lane's part of their sum decides afterwards whether a half is made again against a new m:
     // a score more than 8 (in log2 units) above m puts that sum above 2^8.
     constexpr int LA = 3, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
-    auto tile = [&](int t, int next, auto buf_c, auto edge_c) {
+    auto tile = [&](int t, int next, auto buf_c, auto edge_c, bool odd, uint32_t& none) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value;
         constexpr bool EDGE = decltype(edge_c)::value;
         const int k0 = t * kKT;
@@ -365,6 +371,15 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             __builtin_amdgcn_sched_barrier(0);
         }
         const Half ha = half_of(k0), hb = half_of(k0 + 32);
+        auto zeros = [&](const uint32_t (&pw)[8], int half) {
+            if constexpr (EDGE) {
+                if (!odd)
+                    return;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    none |= (uint32_t(!(pw[j] & 0xffffu)) | uint32_t(!(pw[j] >> 16)) << 1) << (16 * half + 2 * j);
+            }
+        };
         auto chunk = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, int c) {
 #pragma unroll
             for (int j = c * CH; j < (c + 1) * CH; ++j) {
@@ -385,6 +400,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         if (__any(la > kLazyP))
             redo(s_a, ha, pa, la, edge_c);
         l += la;
+        zeros(pa, 0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
@@ -399,6 +415,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         if (__any(lb > kLazyP))
             redo(s_b, hb, pb, lb, edge_c);
         l += lb;
+        zeros(pb, 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
@@ -419,16 +436,17 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         const int j = i - edges;
         return i >= edges + fulls ? -1 : j < 0 ? t_end - 1 - i : t_begin + (j <= own ? own - j : j);
     };
-    auto step = [&](int i, auto buf_c, auto edge_c) {
+    auto step = [&](int i, auto buf_c, auto edge_c) __attribute__((always_inline)) {
         const int t = tile_at(i);
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         bool odd = false;
+        uint32_t none = 0;
         if constexpr (decltype(edge_c)::value)
             odd = wg_lim < t * kKT + tile_keys(t) && find_odd(t, buf_c);
-        tile(t, tile_at(i + 1), buf_c, edge_c);
+        tile(t, tile_at(i + 1), buf_c, edge_c, odd, none);
         if (decltype(edge_c)::value && odd)
-            add_odd(t);
+            add_odd(t, none);
     };
     if (tid == 0)
         odd_tile = 0; // (the first step's barrier is behind it)
