@@ -14,8 +14,11 @@ namespace {
 
 constexpr uint32_t kMaxDocs = 64; // documents a launch: they go by kernel argument, in less than 4 KB
 constexpr int kKT = 64;           // keys a tile
-// The exponentials' reference m moves only when a weight against it passes 2^8 (below).
-constexpr float kLazyP = 256.0f;
+// The exponentials' reference m moves only when a weight against it passes 2^8, in half 2^15 (below). For half weights it lies 7 under
+// the largest score's next whole number: a weight loses 2^-25 below half's normal range, so 2^-31 of the largest (with m
+// the largest score itself, 2^17 keys of 2^-25.5 each, 0.3% of their row, came out as nothing). bf16 has fp32's range.
+constexpr float kUp = 7.0f;
+template <bool F16> constexpr float kLazyP = F16 ? 32768.0f : 256.0f;
 constexpr float kLeast = -3.402823466e38f; // m of rows without a score above -inf
 // |m| from which on scores are rounded before m is taken off them. Below it one fma does both, exact against any m; from 2^31 on
 // half a step of m itself, which the largest weight would be off by, no longer fits a weight's exponent (a half's from 2^26).
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         pw[j] = pack_x2(e0, e1, F16);
         ls += e0 + e1;
     };
-    // moves m up to a half's largest score, rescales what was summed against the old one, and makes the half's weights again
+    // moves m up to a half's largest score (less kUp), rescales what was summed against the old one, and makes the half's weights again
     auto redo = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, auto edge_c) __attribute__((always_inline)) {
         f32x16 x;
 #pragma unroll
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             if constexpr (decltype(edge_c)::value)
                 x[r] = masked(x[r], h, r);
         }
-        const float mn = fmaxf(m, max_xor32(max16(x))), alpha = __builtin_amdgcn_exp2f(m - mn);
+        const float top = max_xor32(max16(x)), mn = fmaxf(m, F16 ? ceilf(top) - kUp : top), alpha = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         const bool large = fabsf(m) >= kLargeM;
         ref = large ? kLeast : m;
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     // the next tile's loads go out between the first products. The weights are made against the m that is there, before
     // the tile's largest score is known: those of half a between the products S^T of half b, those of half b between the
     // products P V of half a. A lane's part of their sum decides afterwards whether a half is made again against a new m:
-    // a score more than 8 (in log2 units) above m puts that sum above 2^8.
+    // a score more than 8 (in log2 units) above m puts that sum above kLazyP.
     constexpr int LA = 3, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
     auto tile = [&](int t, int next, auto buf_c, auto edge_c, bool odd, uint32_t& none) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value;
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             chunk(s_a, ha, pa, la, ds);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (__any(la > kLazyP))
+        if (__any(la > kLazyP<F16>))
             redo(s_a, ha, pa, la, edge_c);
         l += la;
         zeros(pa, 0);
@@ -412,7 +415,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             chunk(s_b, hb, pb, lb, j);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (__any(lb > kLazyP))
+        if (__any(lb > kLazyP<F16>))
             redo(s_b, hb, pb, lb, edge_c);
         l += lb;
         zeros(pb, 1);

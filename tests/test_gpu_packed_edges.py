@@ -41,3 +41,23 @@ def test_infinite_values_without_weight(gpu, block, rows, heads, kv, d, workspac
     got = values(a.result()[0], dt)
     assert (got[:, 0, 9] == np.inf).all() and np.isnan(got[:, 0, 40]).all() and np.isnan(got[-1, 0, 3]) and got[-1, 0, 7] == -np.inf
     assert block == 0 or np.isfinite(got[0, 0, 3])
+
+
+@pytest.mark.parametrize("rows, heads, kv, d, workspace", [(1, 1, 1, 128, False), (3, 4, 1, 64, True), (40, 1, 1, 64, False)])
+def test_half_weights_far_below_the_largest(gpu, rows, heads, kv, d, workspace):
+    """2^17 keys that each weigh about 2^-25.5 of one: together 0.3% of it. A weight loses 2^-31 of the largest at most."""
+    n = (1 << 17) + 1
+
+    def edit(raw):
+        one_dim(raw)
+        raw["k"][:, :, 5] = -17.675
+        raw["v"][:] = 1.0
+        # (the last key's tile is the first one taken)
+        raw["k"][-1, :, 5] = raw["v"][-1] = 0.0
+
+    a = Attn([(0, rows, 0, n, n - 1, 0, 0)], rows, n, heads, kv, d, M.F16, scale=1.0, edit=edit)
+    got = values(a.run(workspace).result()[0], M.F16)
+    p = np.exp(a.val["k"][0, 0, 5]) * (n - 1)
+    want = p / (1 + p)
+    assert 2.0 ** -9 < want < 2.0 ** -8
+    assert np.abs(got - want).max() <= (2 * H[M.F16] + (n + 2 * d) * u) * want + n * 2.0 ** -31
