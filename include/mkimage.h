@@ -325,17 +325,19 @@ typedef struct mk_attn_packed_args {
     const float* slopes; /* device [heads] or NULL: s -= slopes[h] |p - c|, after the cap */
     const mk_attn_doc* docs; /* host [n_docs], in any order; q rows of two documents must not overlap, k rows may */
     uint32_t n_docs;
-    void* workspace;     /* 16-byte aligned, or NULL: few rows over many keys then run on few compute units */
-    uint64_t workspace_bytes; /* at least what mk_attention_packed_workspace says, when workspace is not NULL */
+    void* workspace;     /* 16-byte aligned, or NULL */
+    uint64_t workspace_bytes; /* of any size: with less than mk_attention_packed_workspace says (or NULL), few rows over many keys run on
+                            fewer compute units */
 } mk_attn_packed_args;
 /* out = softmax(s) v over the seen keys, scores, sums and the softmax in fp32; the probabilities enter the second product in the
  * inputs' type, rounded once. A row that sees no key, or only keys of score -inf (below fp32's range), is zero. Rows outside every
  * document are left as they were. What a row does not see does not reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees makes it NaN, an infinity in v that
  * infinity, or NaN where its weight is zero in the inputs' type. All pointers
- * 16-byte aligned (slopes 4). A row's bits may depend on the other documents of the call (their number decides how keys are
- * split), not on their contents. */
+ * 16-byte aligned (slopes 4). A row's bits may depend on the sizes and the number of the other documents of the call and on
+ * the workspace's (they decide how keys are split), not on what the documents hold. */
 mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream);
-/* The workspace of that call on the current device, in bytes (0: none). Reads all of the arguments but the operands. */
+/* The workspace with which that call is fastest on the current device, in bytes (0: none). A smaller batch may ask for more than
+ * a larger one, whose rows fill the chip by themselves. Reads all of the arguments but the operands. */
 mk_status mk_attention_packed_workspace(const mk_attn_packed_args* a, uint64_t* bytes);
 
 /* Low-rank adapters of many requests beside a shared projection: with a = ids[r], and column n in part p = n / (N / parts),

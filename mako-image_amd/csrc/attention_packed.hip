@@ -668,8 +668,11 @@ struct Launch {
 
 constexpr uint64_t kMostGroups = 1u << 23; // of 256 threads: fewer than 2^32 in all
 
-// Takes documents into p; returns how many of docs were looked at.
-uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, bool split, PackedP& p, Launch& out)
+uint64_t bytes_of(const mk_attn_packed_args* a, uint64_t slots, uint32_t nw) { return slots * (32 * nw) * (a->d + 2) * 4; }
+
+// Takes documents into p, their keys split as far as `room` bytes of workspace hold the partial results; returns how many of docs
+// were looked at. With all the room that the best split needs it is the same split as with any more.
+uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, uint64_t room, PackedP& p, Launch& out)
 {
     const uint32_t group = a->heads / a->kv_heads;
     uint32_t at = next, n = 0;
@@ -709,15 +712,21 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
     };
     uint64_t target = std::max<uint64_t>(longest, 1);
     double best = 1e300;
-    for (uint64_t parts = 1; split && parts <= std::max<uint64_t>(longest, 1); parts += 1 + parts / 4) {
+    for (uint64_t parts = 1; room && parts <= std::max<uint64_t>(longest, 1); parts += 1 + parts / 4) {
         const uint64_t t = std::max<uint64_t>((longest + parts - 1) / parts, 1);
         double rows = 0, items = 0;
+        uint64_t slots = 0;
         for (uint32_t i = 0; i < n; ++i) {
             const Doc& d = p.docs[i];
-            items += double(d.blocks) * a->kv_heads * splits_of(d, t);
-            if (splits_of(d, t) > 1)
-                rows += double(d.q_rows) * a->heads * splits_of(d, t);
+            const uint64_t splits = splits_of(d, t), of = uint64_t(d.blocks) * a->kv_heads * splits;
+            items += double(of);
+            if (splits > 1) {
+                rows += double(d.q_rows) * a->heads * splits;
+                slots += of;
+            }
         }
+        if (bytes_of(a, slots, out.nw) > room)
+            continue;
         // (more workgroups than the chip holds: their share, and half a workgroup for the last round's end)
         const double long_one = items <= resident ? double(t) : double(tiles) / resident + 0.5 * double(t);
         const double time = long_one * (a->d == 128 ? 1.0 : 0.7) + (rows > 0 ? 2.5 + rows * (a->d + 2) * 4 * 0.6e-6 : 0.0);
@@ -747,8 +756,6 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
     out.joins = uint32_t(join);
     return at - next;
 }
-uint64_t bytes_of(const mk_attn_packed_args* a, const Launch& l) { return l.slots * (32 * l.nw) * (a->d + 2) * 4; }
-
 template <int D, bool F16, int NW> void launch_mode(const PackedP& p, int mode, uint32_t groups, hipStream_t s)
 {
     if (mode == kPlain)
@@ -812,8 +819,8 @@ mk_status mk_attention_packed_workspace(const mk_attn_packed_args* a, uint64_t* 
     PackedP p;
     Launch l;
     for (uint32_t i = 0; i < a->n_docs;) {
-        i += plan_launch(a, i, cus, true, p, l);
-        *bytes = std::max(*bytes, bytes_of(a, l)); // (launches run one after the other)
+        i += plan_launch(a, i, cus, UINT64_MAX, p, l);
+        *bytes = std::max(*bytes, bytes_of(a, l.slots, l.nw)); // (launches run one after the other)
     }
     return MK_OK;
 }
@@ -832,12 +839,6 @@ mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
     MK_TRY(device_cus(&cus));
     PackedP p;
     Launch l;
-    if (a->workspace) // before anything is launched
-        for (uint32_t i = 0; i < a->n_docs;) {
-            i += plan_launch(a, i, cus, true, p, l);
-            if (bytes_of(a, l) > a->workspace_bytes)
-                return fail(MK_ERR_ARG, "attention_packed: the workspace is smaller than mk_attention_packed_workspace says");
-        }
     hipStream_t s = static_cast<hipStream_t>(stream);
     constexpr float kLog2e = 1.4426950408889634f;
     const int mode = (a->cap > 0.0f ? kCap : 0) | (a->slopes ? kBias : 0);
@@ -857,7 +858,7 @@ mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
     p.group = a->heads / a->kv_heads;
     p.out_f16 = a->out_dtype == MK_F16;
     for (uint32_t i = 0; i < a->n_docs;) {
-        i += plan_launch(a, i, cus, a->workspace != nullptr, p, l);
+        i += plan_launch(a, i, cus, a->workspace ? a->workspace_bytes : 0, p, l);
         if (!l.groups)
             continue;
         p.part = static_cast<float*>(a->workspace);

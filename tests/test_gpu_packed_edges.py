@@ -61,3 +61,40 @@ def test_half_weights_far_below_the_largest(gpu, rows, heads, kv, d, workspace):
     want = p / (1 + p)
     assert 2.0 ** -9 < want < 2.0 ** -8
     assert np.abs(got - want).max() <= (2 * H[M.F16] + (n + 2 * d) * u) * want + n * 2.0 ** -31
+
+
+@pytest.mark.parametrize("part", [0.0, 0.3, 0.9])
+def test_attention_takes_the_workspace_that_it_is_given(gpu, part):
+    """A workspace of a part of what the keys' best split needs, none of it among them: fewer splits, the same rows."""
+    docs, nq, nk = packed([1, 3, 7], [4099, 777, 1500], mask="causal")
+    for heads, kv, d in ((8, 1, 128), (8, 8, 64), (40, 2, 64)):
+        a = Attn(docs, nq, nk, heads, kv, d, M.BF16)
+        g, need = a.args(), C.c_uint64()
+        M.call("mk_attention_packed_workspace", C.byref(g), C.byref(need))
+        assert need.value > 4096
+        size = int(need.value * part) // 16 * 16
+        space, guard = M.Dev(need.value), np.full(need.value - size, 0x5A, np.uint8)
+        M.call("mk_memset", space.p, 0xFF, need.value)
+        space.write(guard, size)
+        g.workspace, g.workspace_bytes = space.p, size
+        M.call("mk_attention_packed", C.byref(g), None)
+        got, mine = a.result()
+        assert np.array_equal(space.to_array(np.uint8, (need.value,))[size:], guard)
+        want, tol = attend(a.val["q"], a.val["k"], a.val["v"], docs, a.scale, 0.0, None, M.BF16, M.BF16)
+        assert (np.abs(values(got, M.BF16) - want)[mine] <= tol[mine]).all()
+
+
+def test_attention_one_workspace_for_a_large_batch_and_small_ones(gpu):
+    # the rows of four images fill the chip without splits, so they need none
+    big, need = Attn(packed([2176, 1101, 2377, 1801])[0], 1, 1, 32, 32, 64, M.BF16), C.c_uint64(7)
+    M.call("mk_attention_packed_workspace", C.byref(big.args()), C.byref(need))
+    space = M.Dev(max(need.value, 16))
+    for lens_q, lens_k in (([1], [16411]), ([1, 1, 1], [5000, 77, 900]), ([40], [3000])):
+        docs, nq, nk = packed(lens_q, lens_k, mask="causal")
+        a = Attn(docs, nq, nk, 8, 2, 64, M.BF16)
+        g = a.args()
+        g.workspace, g.workspace_bytes = space.p, need.value
+        M.call("mk_attention_packed", C.byref(g), None)
+        got, mine = a.result()
+        want, tol = attend(a.val["q"], a.val["k"], a.val["v"], docs, a.scale, 0.0, None, M.BF16, M.BF16)
+        assert (np.abs(values(got, M.BF16) - want)[mine] <= tol[mine]).all()
