@@ -370,6 +370,11 @@ typedef struct mk_lora_rows_args {
 mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream);
 /* The workspace of that call on the current device, in bytes. Reads the sizes and types alone. */
 mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes);
+/* How that call runs on a device of cus compute units, without running it (host only; a test hook): out[0] 1: both products in
+ * one launch; out[1] rows of A a tile of the first product (0: a workgroup a row, without tiles), out[2] columns of c that a
+ * workgroup of the second goes through (0: without tiles), out[3] workgroups that share a row's K, out[4] 1: the rows are put in the order of
+ * their adapters first, out[5] 1: a tile's two halves share what they read of B. Reads no operand. */
+mk_status mk_lora_rows_plan(const mk_lora_rows_args* a, uint32_t cus, uint32_t* out);
 
 /* Rotary positions of several axes (text: one; an image's rows: height and width; a video's: time, height and width) on the
  * query and key heads of packed rows, each head RMS-normed before (v rsqrt(mean v^2 + eps) w) where norm_q / norm_k is given:

@@ -8,6 +8,7 @@
 // 64, fp32 rows, 252 us (3.7 TB/s), 1 row of 4096 to 4096 5.4 us.
 #include "common.hpp"
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -714,6 +715,7 @@ struct Plan {
     uint32_t nb;        // the first product's tiles: 32 nb of A's rows
     uint32_t splits, split_k;
     uint32_t blocks;
+    bool fuse;          // both halves of a tile share what they read of B
 };
 Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
 {
@@ -759,6 +761,9 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
     p.blocks = 1;
     while (p.blocks < 4 && p.blocks * 512 < per && uint64_t(tiles) * a->parts * cdiv(per, 1024 * p.blocks) >= 4ull * cus)
         p.blocks *= 2;
+    // from rank 64 on B is the most of what a tile reads (us apart / shared by its two halves: 16384 x 12288 by rank 128 430 / 383
+    // with the first product, 4352 x 4096 by 64 49.3 / 47.6)
+    p.fuse = a->rank >= 64;
     return p;
 }
 // t, and the rows' order
@@ -805,9 +810,7 @@ template <bool F16, uint32_t CT> void launch_expand(const LoraP& p, const Plan& 
     const uint32_t pad = (p.rank + 15) / 16 * 16 + 8, values = CT == MK_F32 && !F16 ? 3 : 2;
     const dim3 grid(cdiv(p.rows, kRows), p.parts * cdiv(per, 512 * p.blocks));
     const uint32_t lds = (values * pad * 2 + 4) * kRows;
-    // from rank 64 on B is the most of what a tile reads (us apart / shared by its two halves: 16384 x 12288 by rank 128 430 / 383
-    // with the first product, 4352 x 4096 by 64 49.3 / 47.6)
-    if (p.rank >= 64)
+    if (plan.fuse)
         expand_tile<F16, CT, true><<<grid, 256, lds, s>>>(p);
     else
         expand_tile<F16, CT, false><<<grid, 256, lds, s>>>(p);
@@ -832,6 +835,20 @@ mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes)
     uint32_t cus = 1;
     MK_TRY(device_cus(&cus));
     *bytes = workspace_of(a, plan_of(a, cus).splits);
+    return MK_OK;
+}
+
+mk_status mk_lora_rows_plan(const mk_lora_rows_args* a, uint32_t cus, uint32_t* out)
+{
+    if (!a || !out || !cus)
+        return fail(MK_ERR_ARG, "lora_rows_plan: null argument or no compute units");
+    MK_TRY(check_sizes(a));
+    if (!a->rows)
+        return fail(MK_ERR_ARG, "lora_rows_plan: no rows");
+    const Plan p = plan_of(a, cus);
+    const uint32_t o[6] = {p.one, p.one || p.vec1 ? 0 : 32 * p.nb, p.one || p.vec2 ? 0 : 512 * p.blocks, p.one || p.vec1 ? 1 : p.splits, p.order,
+                           !p.one && !p.vec2 && p.fuse};
+    std::copy(o, o + 6, out);
     return MK_OK;
 }
 

@@ -142,6 +142,7 @@ _SIGS = {
     "mk_attention_packed_workspace": (_i, [C.POINTER(AttnPackedArgs), C.POINTER(_u64)]),
     "mk_lora_rows": (_i, [C.POINTER(LoraRowsArgs), _vp]),
     "mk_lora_rows_workspace": (_i, [C.POINTER(LoraRowsArgs), C.POINTER(_u64)]),
+    "mk_lora_rows_plan": (_i, [C.POINTER(LoraRowsArgs), _u32, C.POINTER(_u32)]),
     "mk_rope_rows": (_i, [C.POINTER(RopeRowsArgs), _vp]),
     "mk_silu": (_i, [_vp, _sz, _vp]),
     "mk_gelu_tanh": (_i, [_vp, _sz, _vp]),

@@ -1,0 +1,53 @@
+"""Which kernels a mk_lora_rows call takes, by its sizes alone, on 256 compute units (no GPU)."""
+import ctypes as C
+
+import pytest
+
+import mkimage as M
+import test_gpu_lora_tiles
+import test_gpu_packed_ops
+
+P = 1 << 20  # an aligned address that no call may touch
+ONE, A_TILE, COLUMNS, SPLITS, ORDER, FUSE = range(6)
+
+
+def args(rows, K, N, rank, parts=1, adapters=4, **kw):
+    g = M.LoraRowsArgs()
+    g.x = g.a = g.b = g.base = g.c = g.ids = P
+    g.ldx, g.ldbase, g.ldc = K, N, N
+    g.rows, g.K, g.N, g.rank, g.parts, g.adapters, g.dtype, g.c_dtype = rows, K, N, rank, parts, adapters, M.BF16, M.BF16
+    for k, v in kw.items():
+        setattr(g, k, v)
+    return g
+
+
+def plan(*a, cus=256, **kw):
+    out = (C.c_uint32 * 6)(*[99] * 6)
+    M.call("mk_lora_rows_plan", C.byref(args(*a, **kw)), cus, out)
+    return list(out)
+
+
+def test_plan_refusals():
+    f, out = M.lib().mk_lora_rows_plan, (C.c_uint32 * 6)()
+    assert f(None, 256, out) == 1 and f(C.byref(args(5, 64, 64, 8)), 256, None) == 1
+    assert f(C.byref(args(5, 64, 64, 8)), 0, out) == 1
+    assert f(C.byref(args(0, 64, 64, 8)), 256, out) == 1 and b"no rows" in M.lib().mk_last_error()
+    assert f(C.byref(args(5, 64, 64, 12)), 256, out) == 1 and b"rank" in M.lib().mk_last_error()
+
+
+@pytest.mark.parametrize("size, takes", test_gpu_lora_tiles.TILES)
+def test_the_tests_of_tiles_take_tiles(size, takes):
+    got = plan(*size)
+    assert got[ONE] == 0 and tuple(got[i] for i in (A_TILE, COLUMNS, SPLITS, FUSE)) == takes
+
+
+def test_the_tests_of_few_rows_take_the_other_kernels():
+    kinds = {(p[ONE], p[A_TILE] > 0, p[COLUMNS] > 0) for p in (plan(*size) for size in test_gpu_packed_ops.LORA_SIZES)}
+    assert kinds == {(1, False, False), (0, False, False)}
+
+
+def test_rows_in_no_order_are_sorted_where_both_products_take_tiles():
+    assert plan(4352, 4096, 12288, 32, 3)[ORDER] == 1
+    for kw in (dict(ids=None), dict(grouped=1), dict(adapters=1), dict(adapters=1025)):
+        assert plan(4352, 4096, 12288, 32, 3, **kw)[ORDER] == 0
+    assert plan(24, 4096, 12288, 16, 3)[ORDER] == 0
