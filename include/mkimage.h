@@ -361,16 +361,19 @@ typedef struct mk_lora_rows_args {
     uint32_t dtype;      /* x, a, b: MK_BF16 or MK_F16 */
     uint32_t c_dtype;    /* base and c: MK_F32, MK_BF16 or MK_F16 */
     void* workspace;     /* 16-byte aligned */
-    uint64_t workspace_bytes; /* at least what mk_lora_rows_workspace says */
+    uint64_t workspace_bytes; /* at least (4 parts rank + 8) rows, rounded up to 16; with less than mk_lora_rows_workspace says, fewer
+                            workgroups share a row's K */
     uint32_t grouped;    /* 1: rows of one adapter are known to be one after the other, or nearly so (a request's rows): many rows are then
                             not looked through for their order first, 5 us. The results are the same. */
 } mk_lora_rows_args;
 /* Sums in fp32; t enters the second product as two or three values of the inputs' type (its rounding and the rest). Infinities and
  * NaNs of a row or of an adapter reach that row, or that adapter's rows, alone. All pointers 16-byte aligned (scale and ids 4). */
 mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream);
-/* The workspace of that call on the current device, in bytes. Reads the sizes and types alone. */
+/* The workspace with which that call is fastest on the current device, in bytes: fewer rows can ask for more than many, whose tiles fill
+ * the chip by themselves. Reads the sizes and types alone. */
 mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes);
-/* How that call runs on a device of cus compute units, without running it (host only; a test hook): out[0] 1: both products in
+/* How that call runs on a device of cus compute units, without running it, with its workspace or (NULL) with all that
+ * mk_lora_rows_workspace asks for (host only; a test hook): out[0] 1: both products in
  * one launch; out[1] rows of A a tile of the first product (0: a workgroup a row, without tiles), out[2] columns of c that a
  * workgroup of the second goes through (0: without tiles), out[3] workgroups that share a row's K, out[4] 1: the rows are put in the order of
  * their adapters first, out[5] 1: a tile's two halves share what they read of B. Reads no operand. */

@@ -707,7 +707,7 @@ mk_status check_sizes(const mk_lora_rows_args* a)
     return MK_OK;
 }
 
-// How the two products run, by the sizes alone (on `cus` compute units).
+// How the two products run, by the sizes alone (on `cus` compute units; `room` bytes of workspace bound the splits of K).
 struct Plan {
     bool one;           // both products in one launch (very few rows)
     bool order;         // rows are taken in the order of their adapters
@@ -717,7 +717,13 @@ struct Plan {
     uint32_t blocks;
     bool fuse;          // both halves of a tile share what they read of B
 };
-Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
+// t, and the rows' order
+uint64_t bytes_of_t(const mk_lora_rows_args* a, uint32_t splits)
+{
+    return round_up(uint64_t(splits) * a->rows * a->parts * a->rank * 4, 16);
+}
+uint64_t workspace_of(const mk_lora_rows_args* a, uint32_t splits) { return bytes_of_t(a, splits) + round_up(uint64_t(a->rows) * 8, 16); }
+Plan plan_of(const mk_lora_rows_args* a, uint32_t cus, uint64_t room)
 {
     Plan p{};
     const uint32_t width = a->parts * a->rank, chunks = cdiv(width, 128), tiles = cdiv(a->rows, kRows);
@@ -747,6 +753,8 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
         double best = 1e30;
         for (uint32_t s = 1; s <= 16 && s <= steps; ++s) {
             const uint32_t each = cdiv(steps, s), used = cdiv(steps, each);
+            if (used > 1 && workspace_of(a, used) > room)
+                break;
             const double cost = double((groups * used + cus - 1) / cus) * (each + 4.0);
             if (cost < best * 0.97) {
                 best = cost;
@@ -766,12 +774,6 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus)
     p.fuse = a->rank >= 64;
     return p;
 }
-// t, and the rows' order
-uint64_t bytes_of_t(const mk_lora_rows_args* a, uint32_t splits)
-{
-    return round_up(uint64_t(splits) * a->rows * a->parts * a->rank * 4, 16);
-}
-uint64_t workspace_of(const mk_lora_rows_args* a, uint32_t splits) { return bytes_of_t(a, splits) + round_up(uint64_t(a->rows) * 8, 16); }
 mk_status device_cus(uint32_t* cus)
 {
     int dev = 0, n = 0;
@@ -834,7 +836,7 @@ mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes)
         return MK_OK;
     uint32_t cus = 1;
     MK_TRY(device_cus(&cus));
-    *bytes = workspace_of(a, plan_of(a, cus).splits);
+    *bytes = workspace_of(a, plan_of(a, cus, UINT64_MAX).splits);
     return MK_OK;
 }
 
@@ -845,7 +847,7 @@ mk_status mk_lora_rows_plan(const mk_lora_rows_args* a, uint32_t cus, uint32_t* 
     MK_TRY(check_sizes(a));
     if (!a->rows)
         return fail(MK_ERR_ARG, "lora_rows_plan: no rows");
-    const Plan p = plan_of(a, cus);
+    const Plan p = plan_of(a, cus, a->workspace ? a->workspace_bytes : UINT64_MAX);
     const uint32_t o[6] = {p.one, p.one || p.vec1 ? 0 : 32 * p.nb, p.one || p.vec2 ? 0 : 512 * p.blocks, p.one || p.vec1 ? 1 : p.splits, p.order,
                            !p.one && !p.vec2 && p.fuse};
     std::copy(o, o + 6, out);
@@ -871,12 +873,10 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
     if (a->grouped > 1)
         return fail(MK_ERR_ARG, "lora_rows: grouped is 0 or 1");
     if (!a->workspace || a->workspace_bytes < workspace_of(a, 1))
-        return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
+        return fail(MK_ERR_ARG, "lora_rows: the workspace holds less than (4 parts rank + 8) rows bytes");
     uint32_t cus = 1;
     MK_TRY(device_cus(&cus));
-    const Plan plan = plan_of(a, cus);
-    if (a->workspace_bytes < workspace_of(a, plan.splits))
-        return fail(MK_ERR_ARG, "lora_rows: the workspace is smaller than mk_lora_rows_workspace says");
+    const Plan plan = plan_of(a, cus, a->workspace_bytes);
     LoraP p{static_cast<const uint16_t*>(a->x), static_cast<const uint16_t*>(a->a), static_cast<const uint16_t*>(a->b), a->scale,
             a->ids, a->base, a->c, static_cast<float*>(a->workspace),
             plan.order ? reinterpret_cast<u32x2*>(static_cast<char*>(a->workspace) + bytes_of_t(a, plan.splits)) : nullptr,

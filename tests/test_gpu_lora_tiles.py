@@ -194,3 +194,27 @@ def test_lora_tiles_of_rows_past_32_bits(gpu, c_dt):
         tol[r] = ((K / 8 + 16) * u * ta + (H[M.BF16] ** 2 + (rank + 8) * u) * np.abs(t)) @ np.abs(b[i]).T
     tol += (H[c_dt] + 2 * u) * np.abs(want) + 2 * u * np.abs(base)
     assert (np.abs(values(got, c_dt) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("size", [(4161, 1160, 72, 16, 1, 9), (130, 12296, 2072, 256, 1, 2), (77, 20000, 40, 48, 1, 3)])
+def test_lora_takes_the_workspace_that_it_is_given(gpu, size):
+    """From one split of K, the least that is taken, to all of them: the same rows, nothing behind the workspace, 16 bytes less refused."""
+    rows, K, N, rank, parts, adapters = size
+    least = -(-rows * (4 * parts * rank + 8) // 16) * 16
+    a = Lora(*size, ids_of("mixed", rows, adapters), M.BF16, M.BF16)
+    full = plan(a)[SPLITS]
+    want, tol = a.want()
+    for splits in (1, 2, full):
+        g = a.args()
+        size = least + (splits - 1) * rows * 4 * parts * rank
+        space, guard = M.Dev(size + 4096), np.full(4096, 0x5A, np.uint8)
+        M.call("mk_memset", space.p, 0xFF, size)
+        space.write(guard, size)
+        g.workspace, g.workspace_bytes = space.p, size
+        assert plan(g)[SPLITS] <= splits and (splits < full or plan(g)[SPLITS] == full)
+        M.call("mk_lora_rows", C.byref(g), None)
+        assert (np.abs(a.result() - want) <= tol).all()
+        assert np.array_equal(space.to_array(np.uint8, (size + 4096,))[size:], guard)
+    g.workspace_bytes = least - 16
+    with pytest.raises(M.MkError, match="workspace"):
+        M.call("mk_lora_rows", C.byref(g), None)

@@ -51,3 +51,20 @@ def test_rows_in_no_order_are_sorted_where_both_products_take_tiles():
     for kw in (dict(ids=None), dict(grouped=1), dict(adapters=1), dict(adapters=1025)):
         assert plan(4352, 4096, 12288, 32, 3, **kw)[ORDER] == 0
     assert plan(24, 4096, 12288, 16, 3)[ORDER] == 0
+
+
+def test_k_is_split_as_far_as_the_workspace_reaches():
+    size = (2048, 12288, 4096, 64)
+    full = plan(*size)[SPLITS]
+    one = 2048 * (4 * 64 + 8)
+    assert full >= 8
+    for splits in range(1, full + 2):
+        room = one + (splits - 1) * 2048 * 4 * 64
+        a, b = plan(*size, workspace=P, workspace_bytes=room)[SPLITS], plan(*size, workspace=P, workspace_bytes=room - 16)[SPLITS]
+        assert 1 <= b <= a <= splits and b < max(splits, 2)
+    assert a == full
+    # the workspace of many rows (one split) serves fewer, which would have taken more of it
+    many = 16384 * (4 * 64 + 8)
+    assert plan(16384, 12288, 4096, 64, workspace=P, workspace_bytes=many)[SPLITS] == 1
+    assert 1 < plan(13056, 12288, 4096, 64, workspace=P, workspace_bytes=4 * many)[SPLITS]
+    assert plan(13056, 12288, 4096, 64, workspace=P, workspace_bytes=many)[SPLITS] == 1
