@@ -364,7 +364,9 @@ typedef struct mk_lora_rows_args {
     uint64_t workspace_bytes; /* at least (4 parts rank + 8) rows, rounded up to 16; with less than mk_lora_rows_workspace says, fewer
                             workgroups share a row's K */
     uint32_t grouped;    /* 1: rows of one adapter are known to be one after the other, or nearly so (a request's rows): many rows are then
-                            not looked through for their order first, 5 us. The results are the same. */
+                            not looked through for their order first, 5 us. The results are the same. (Rows in no order are sorted up
+                            to 2^18 rows, 1024 adapters and 2 GiB from the first row of x, base or c to the last: beyond, each tile of 64 rows
+                            takes its adapters one after the other.) */
 } mk_lora_rows_args;
 /* Sums in fp32; t enters the second product as two or three values of the inputs' type (its rounding and the rest). Infinities and
  * NaNs of a row or of an adapter reach that row, or that adapter's rows, alone. All pointers 16-byte aligned (scale and ids 4). */

@@ -738,8 +738,8 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus, uint64_t room)
     // its adapters one after the other. (1024 x 4096 to 4096 by rank 16, at the border: 27 / 16 and 28 / 56.)
     p.vec1 = a->rows <= 4096 && macs <= (1u << 26);
     p.vec2 = a->rows <= 4096 && macs2 <= (1u << 26);
-    // (for two products by tiles alone; offsets from the first row on are below 2^31)
-    const int64_t far = std::max(std::max(a->ldx, a->base ? a->ldbase : 0) * 4, a->ldc * 4) * a->rows;
+    // (for two products by tiles alone; byte offsets from the first row on are below 2^31)
+    const int64_t far = std::max(a->ldx * 2, std::max(a->base ? a->ldbase : 0, a->ldc) * (a->c_dtype == MK_F32 ? 4 : 2)) * a->rows;
     p.order = !p.one && !p.vec1 && !p.vec2 && a->ids && !a->grouped && a->adapters > 1 && a->adapters <= kMaxOrdered && a->rows <= (1u << 18) && far < (1ll << 31);
     p.nb = cdiv(cdiv(width, chunks), 32);
     p.splits = 1;

@@ -218,3 +218,36 @@ def test_lora_takes_the_workspace_that_it_is_given(gpu, size):
     g.workspace_bytes = least - 16
     with pytest.raises(M.MkError, match="workspace"):
         M.call("mk_lora_rows", C.byref(g), None)
+
+
+def test_lora_rows_in_no_order_up_to_the_sort_s_reach(gpu):
+    # 40000 rows of 26840 bf16 elements: 2147200000 bytes, the last row's offset just below 2^31
+    rows, ld, K, N, rank = 40000, 26840, 16, 8, 8
+    rng = np.random.default_rng(3)
+    (xb, x), (ab, a), (bb, b) = (stored(rng.standard_normal(s), M.BF16) for s in ((rows, K), (3, rank, K), (3, N, rank)))
+    ids = rng.integers(-1, 3, rows).astype(np.int32)
+    keep = [dev(v) for v in (ab, bb, ids)]
+    xs, cs = M.Dev(((rows - 1) * ld + K) * 2), M.Dev(((rows - 1) * ld + N) * 2)
+    for r in range(rows):
+        xs.write(xb[r], r * ld * 2)
+    g = M.LoraRowsArgs()
+    g.x, g.a, g.b, g.ids, g.c, g.ldx, g.ldc = xs.p, keep[0].p, keep[1].p, keep[2].p, cs.p, ld, ld
+    g.rows, g.K, g.N, g.rank, g.parts, g.adapters, g.dtype, g.c_dtype = rows, K, N, rank, 1, 3, M.BF16, M.BF16
+    assert plan(g)[ORDER] == 1 and plan(g, ldc=ld + 8)[ORDER] == 0
+    g.ldc = ld
+    need = C.c_uint64()
+    M.call("mk_lora_rows_workspace", C.byref(g), C.byref(need))
+    space = M.Dev(need.value)
+    g.workspace, g.workspace_bytes = space.p, need.value
+    M.call("mk_lora_rows", C.byref(g), None)
+    M.sync()
+    got = np.empty((rows, N), np.uint16)
+    for r in range(rows):
+        M.call("mk_memcpy_d2h", got[r].ctypes.data, cs.p + r * ld * 2, N * 2)
+    want, tol = np.zeros((rows, N)), np.zeros((rows, N))
+    for i in range(3):
+        r = ids == i
+        t, ta = x[r] @ a[i].T, np.abs(x[r]) @ np.abs(a[i]).T
+        want[r] = t @ b[i].T
+        tol[r] = ((K / 8 + 16) * u * ta + (H[M.BF16] ** 2 + (rank + 8) * u) * np.abs(t)) @ np.abs(b[i]).T
+    assert (np.abs(values(got, M.BF16) - want) <= tol + (H[M.BF16] + 2 * u) * np.abs(want)).all()

@@ -68,3 +68,13 @@ def test_k_is_split_as_far_as_the_workspace_reaches():
     assert plan(16384, 12288, 4096, 64, workspace=P, workspace_bytes=many)[SPLITS] == 1
     assert 1 < plan(13056, 12288, 4096, 64, workspace=P, workspace_bytes=4 * many)[SPLITS]
     assert plan(13056, 12288, 4096, 64, workspace=P, workspace_bytes=many)[SPLITS] == 1
+
+
+def test_rows_are_sorted_as_far_as_byte_offsets_reach():
+    # below 2^31 bytes from the first row on, of x (16 bits), base and c (their type's)
+    for rows, kw, sorted_ in ((87000, dict(), 1), (87500, dict(), 0), (43600, dict(c_dtype=M.F32), 1), (43800, dict(c_dtype=M.F32), 0),
+                              (43600, dict(ldx=24576), 1), (43800, dict(ldx=24576), 0), (43800, dict(ldbase=24576), 0), (43800, dict(ldbase=24576, base=None), 1),
+                              (1 << 18, dict(ldx=4096, ldc=4088, ldbase=4088), 0), (1 << 18, dict(ldx=4088, ldc=4088, ldbase=4088), 1),
+                              ((1 << 18) + 1, dict(ldx=8, ldc=8, ldbase=8), 0)):
+        kw = dict(dict(ldx=4096, ldc=12288, ldbase=12288), **kw)
+        assert plan(rows, 8, 8, 8, **kw)[ORDER] == sorted_, (rows, kw)
