@@ -24,7 +24,7 @@ struct LoraP {
     const int32_t* ids;
     const void* base;
     void* c;
-    float* t;       // workspace: [splits][rows][parts rank]
+    float* t;       // workspace: [splits][rows][parts rank], a row's at its own number
     u32x2* perm;    // workspace: [rows], the row at each place of the tiles and its adapter, or NULL: places are rows
     int64_t ldx, ldbase, ldc;
     uint32_t rows, K, N, rank, parts, adapters;
@@ -63,7 +63,8 @@ template <bool F16> __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
 }
 constexpr uint32_t kOut = 0x80000000u; // a byte offset past every buffer resource here
 constexpr int kRows = 64;              // rows of a workgroup of the second product
-// the row at a place of the tiles from first on, counted from there or, in order, from row 0, and its adapter (-1: none)
+// the row at a place of the tiles from first on, counted from there or, in order, from row 0 (row_base), and its adapter (-1: none)
+__device__ inline uint32_t row_base(const LoraP& p, uint32_t first) { return p.perm ? 0 : first; }
 __device__ inline int row_at(const LoraP& p, uint32_t first, uint32_t i, uint32_t& row)
 {
     if (p.perm) {
@@ -404,8 +405,9 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
                 for (int w = 1; w < 4; ++w)
                     v += *reinterpret_cast<const f32x4*>(red + ((((q - ij) * 4 + w) * 4 + wave) * 64 + lane) * 4);
                 const uint32_t r = q / NB * 32 + r32, n = i0 + q % NB * 32 + wave * 8 + hk * 4;
+                const uint32_t row = row_base(p, row0) + uint32_t(__shfl(int(src), int(r)));
                 if (__shfl(mine, int(r)) == a && n < width)
-                    *reinterpret_cast<f32x4*>(p.t + (int64_t(split) * p.rows + row0 + r) * width + n) = v;
+                    *reinterpret_cast<f32x4*>(p.t + (int64_t(split) * p.rows + row) * width + n) = v;
             }
         }
         __syncthreads(); // before the next adapter's loads
@@ -524,13 +526,13 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
     row_c[lane] = src * uint32_t(p.ldc) * SZ;
     {
         // 4 threads a row, t's values 4 (q + 4 i) .. + 3 of it in each
-        const uint32_t r = tid / 4, q = tid % 4;
+        const uint32_t r = tid / 4, q = tid % 4, row = row_base(p, row0) + uint32_t(__shfl(int(src), int(r)));
         const bool on = __shfl(mine, int(r)) >= 0;
         float top = 0.0f;
         if constexpr (F16) {
             if (on)
                 for (uint32_t i = q * 4; i < p.rank; i += 16) {
-                    const f32x4 v = load_t(p, row0 + r, part * p.rank + i);
+                    const f32x4 v = load_t(p, row, part * p.rank + i);
                     top = fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), top);
                 }
             top = fmaxf(top, __shfl_xor(top, 1));
@@ -545,7 +547,7 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
         if (q == 0)
             factor[r] = down;
         for (uint32_t i = q * 4; i < depth; i += 16) {
-            const f32x4 v = on && i < p.rank ? load_t(p, row0 + r, part * p.rank + i) : f32x4{};
+            const f32x4 v = on && i < p.rank ? load_t(p, row, part * p.rank + i) : f32x4{};
             float rest[4] = {v[0] * up, v[1] * up, v[2] * up, v[3] * up};
 #pragma unroll
             for (int s = 0; s < NV; ++s) {
@@ -738,9 +740,11 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus, uint64_t room)
     // its adapters one after the other. (1024 x 4096 to 4096 by rank 16, at the border: 27 / 16 and 28 / 56.)
     p.vec1 = a->rows <= 4096 && macs <= (1u << 26);
     p.vec2 = a->rows <= 4096 && macs2 <= (1u << 26);
-    // (for two products by tiles alone; byte offsets from the first row on are below 2^31)
-    const int64_t far = std::max(a->ldx * 2, std::max(a->base ? a->ldbase : 0, a->ldc) * (a->c_dtype == MK_F32 ? 4 : 2)) * a->rows;
-    p.order = !p.one && !p.vec1 && !p.vec2 && a->ids && !a->grouped && a->adapters > 1 && a->adapters <= kMaxOrdered && a->rows <= (1u << 18) && far < (1ll << 31);
+    // Where a product goes by tiles, the other one by rows or not (us in no order without / with, and in runs, where finding that out
+    // is all it does: 2000 x 1280 to 5120 by rank 16 58 / 35 and 24 / 27, 2000 x 256 to 12288 99 / 46 and 35 / 38, 600 x 12288 to 640 32 / 22 and
+    // 14 / 19; byte offsets from the first row on are below 2^31).
+    const int64_t far = std::max(p.vec1 ? 0 : a->ldx * 2, p.vec2 ? 0 : std::max(a->base ? a->ldbase : 0, a->ldc) * (a->c_dtype == MK_F32 ? 4 : 2)) * a->rows;
+    p.order = !p.one && !(p.vec1 && p.vec2) && a->ids && !a->grouped && a->adapters > 1 && a->adapters <= kMaxOrdered && a->rows <= (1u << 18) && far < (1ll << 31);
     p.nb = cdiv(cdiv(width, chunks), 32);
     p.splits = 1;
     p.split_k = uint32_t(round_up(a->K, kStepK));

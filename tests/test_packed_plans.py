@@ -46,11 +46,19 @@ def test_the_tests_of_few_rows_take_the_other_kernels():
     assert kinds == {(1, False, False), (0, False, False)}
 
 
-def test_rows_in_no_order_are_sorted_where_both_products_take_tiles():
+def test_rows_in_no_order_are_sorted_where_a_product_takes_tiles():
     assert plan(4352, 4096, 12288, 32, 3)[ORDER] == 1
     for kw in (dict(ids=None), dict(grouped=1), dict(adapters=1), dict(adapters=1025)):
         assert plan(4352, 4096, 12288, 32, 3, **kw)[ORDER] == 0
-    assert plan(24, 4096, 12288, 16, 3)[ORDER] == 0
+    # one of the products by rows
+    for size, tiles in (((2000, 1280, 5120, 16), (0, 512)), ((600, 12288, 640, 16), (32, 0)), ((300, 4096, 24576, 16, 2), (0, 512))):
+        got = plan(*size)
+        assert (got[A_TILE], got[COLUMNS]) == tiles and got[ORDER] == 1
+        assert plan(*size, grouped=1)[ORDER] == 0
+    # (only what goes by tiles has to be in reach)
+    assert plan(600, 12288, 640, 16, ldc=(1 << 23) - 8, c_dtype=M.F32)[ORDER] == 1
+    assert plan(600, 12288, 640, 16, ldx=(1 << 23) - 8)[ORDER] == 0
+    assert plan(24, 4096, 12288, 16, 3)[ORDER] == 0 and plan(1000, 1280, 1280, 16)[ORDER] == 0
 
 
 def test_k_is_split_as_far_as_the_workspace_reaches():
