@@ -296,7 +296,8 @@ mk_status mk_attention(const void* q, const void* k, const void* vt, void* out, 
  * They allocate nothing and keep nothing between calls: what they need besides their operands is the caller's workspace. They
  * may be captured, and may run on several streams at once, with a workspace each. They run on the current device. Host arrays
  * are read during the call only (a graph keeps what they held at its capture). No output overlaps an input (but for the
- * in-place forms named below), another output or the workspace. A call whose sizes leave nothing to do returns MK_OK.
+ * in-place forms named below), another output or the workspace. A call whose sizes leave nothing to do returns MK_OK, with null
+ * operands too.
  * ------------------------------------------------------------------------------------------------------------ */
 
 /* Attention of packed documents: query rows q_row .. q_row + q_rows - 1 attend to key rows k_row .. k_row + k_rows - 1, and

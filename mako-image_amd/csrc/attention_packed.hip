@@ -790,12 +790,17 @@ mk_status device_cus(uint32_t* cus)
     *cus = n > 0 ? uint32_t(n) : 1u;
     return MK_OK;
 }
-bool any_rows(const mk_attn_packed_args* a)
+// whether a document has query rows, and (keys) one of those keys
+bool any_rows(const mk_attn_packed_args* a, bool* keys = nullptr)
 {
+    bool any = false;
     for (uint32_t i = 0; i < a->n_docs; ++i)
-        if (a->docs[i].q_rows)
-            return true;
-    return false;
+        if (a->docs[i].q_rows) {
+            any = true;
+            if (keys && a->docs[i].k_rows)
+                *keys = true;
+        }
+    return any;
 }
 
 } // namespace
@@ -827,14 +832,17 @@ mk_status mk_attention_packed_workspace(const mk_attn_packed_args* a, uint64_t* 
 
 mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
 {
-    if (!a || !a->q || !a->k || !a->v || !a->out)
-        return fail(MK_ERR_ARG, "attention_packed: null argument (q, k, v and out are required)");
+    if (!a)
+        return fail(MK_ERR_ARG, "attention_packed: null argument");
     MK_TRY(check_shape(a));
     if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) || !aligned(a->workspace, 16) ||
         !aligned(a->slopes, 4))
         return fail(MK_ERR_ARG, "attention_packed: operands and workspace must be 16-byte aligned (slopes 4)");
-    if (!any_rows(a))
+    bool keys = false;
+    if (!any_rows(a, &keys))
         return MK_OK;
+    if (!a->q || !a->out || (keys && (!a->k || !a->v)))
+        return fail(MK_ERR_ARG, "attention_packed: null argument (q and out are required, k and v for documents with keys)");
     uint32_t cus = 1;
     MK_TRY(device_cus(&cus));
     PackedP p;

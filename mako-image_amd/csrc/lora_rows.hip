@@ -860,22 +860,24 @@ mk_status mk_lora_rows_plan(const mk_lora_rows_args* a, uint32_t cus, uint32_t* 
 
 mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
 {
-    if (!a || !a->x || !a->a || !a->b || !a->c)
-        return fail(MK_ERR_ARG, "lora_rows: null argument (x, a, b and c are required)");
+    if (!a)
+        return fail(MK_ERR_ARG, "lora_rows: null argument");
     MK_TRY(check_sizes(a));
     // (a tile's 64 rows of x, or 32 of c, are addressed by 31 bits)
     auto bad = [](int64_t ld, uint32_t n) { return ld < int64_t(n) || ld % 8 || ld >= (1 << 23); };
     if (bad(a->ldx, a->K) || bad(a->ldc, a->N) || (a->base && bad(a->ldbase, a->N)))
         return fail(MK_ERR_ARG, "lora_rows: ldx, ldbase and ldc must be multiples of 8 below 2^23, at least the row");
-    if (a->base == a->c && a->ldbase != a->ldc)
+    if (a->base && a->base == a->c && a->ldbase != a->ldc)
         return fail(MK_ERR_ARG, "lora_rows: in place needs ldbase == ldc");
     if (!aligned(a->x, 16) || !aligned(a->a, 16) || !aligned(a->b, 16) || !aligned(a->base, 16) || !aligned(a->c, 16) ||
         !aligned(a->workspace, 16) || !aligned(a->scale, 4) || !aligned(a->ids, 4))
         return fail(MK_ERR_ARG, "lora_rows: operands and workspace must be 16-byte aligned (scale and ids 4)");
-    if (!a->rows)
-        return MK_OK;
     if (a->grouped > 1)
         return fail(MK_ERR_ARG, "lora_rows: grouped is 0 or 1");
+    if (!a->rows)
+        return MK_OK;
+    if (!a->x || !a->a || !a->b || !a->c)
+        return fail(MK_ERR_ARG, "lora_rows: null argument (x, a, b and c are required)");
     if (!a->workspace || a->workspace_bytes < workspace_of(a, 1))
         return fail(MK_ERR_ARG, "lora_rows: the workspace holds less than (4 parts rank + 8) rows bytes");
     uint32_t cus = 1;

@@ -203,9 +203,11 @@ using namespace mk;
 
 extern "C" mk_status mk_rope_rows(const mk_rope_rows_args* a, void* stream)
 {
-    if (!a || !a->q || !a->q_out || !a->pos)
+    if (!a)
+        return fail(MK_ERR_ARG, "rope_rows: null argument");
+    if (a->rows && (!a->q || !a->q_out || !a->pos))
         return fail(MK_ERR_ARG, "rope_rows: null argument (q, q_out and pos are required)");
-    if (!!a->k != !!a->k_out || !!a->k != !!a->kv_heads)
+    if (a->rows && (!!a->k != !!a->k_out || !!a->k != !!a->kv_heads))
         return fail(MK_ERR_ARG, "rope_rows: k, k_out and kv_heads come together");
     if (!a->heads || a->heads > 65535 || a->kv_heads > 65535 || (a->d != 64 && a->d != 128))
         return fail(MK_ERR_ARG, "rope_rows: 1 to 65535 heads of dim 64 or 128");
@@ -237,7 +239,7 @@ extern "C" mk_status mk_rope_rows(const mk_rope_rows_args* a, void* stream)
     if (!aligned(a->q, in) || !aligned(a->k, in) || !aligned(a->q_out, out) || !aligned(a->k_out, out) || !aligned(a->pos, 4) ||
         !aligned(a->norm_q, 4) || !aligned(a->norm_k, 4))
         return fail(MK_ERR_ARG, "rope_rows: q, k and their outputs must be aligned for 4 elements, the rest for one");
-    if ((a->q == a->q_out && (a->dtype != a->out_dtype || a->ldq != a->ldqo)) ||
+    if ((a->q && a->q == a->q_out && (a->dtype != a->out_dtype || a->ldq != a->ldqo)) ||
         (a->k && a->k == a->k_out && (a->dtype != a->out_dtype || a->ldk != a->ldko)))
         return fail(MK_ERR_ARG, "rope_rows: in place needs equal types and strides");
     if (!a->rows)

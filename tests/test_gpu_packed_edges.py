@@ -98,3 +98,12 @@ def test_attention_one_workspace_for_a_large_batch_and_small_ones(gpu):
         got, mine = a.result()
         want, tol = attend(a.val["q"], a.val["k"], a.val["v"], docs, a.scale, 0.0, None, M.BF16, M.BF16)
         assert (np.abs(values(got, M.BF16) - want)[mine] <= tol[mine]).all()
+
+
+def test_no_keys_and_null_k_and_v(gpu):
+    a = Attn([(0, 5, 0, 0, 0, 0, 0), (7, 140, 3, 0, 4, CAUSAL, 0)], 150, 1, 2, 2, 64, M.BF16)
+    g = a.args()
+    g.k = g.v = None
+    M.call("mk_attention_packed", C.byref(g), None)
+    got, mine = a.result()
+    assert (got[mine] == 0).all() and mine.sum() == 145
