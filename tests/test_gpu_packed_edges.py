@@ -100,6 +100,58 @@ def test_attention_one_workspace_for_a_large_batch_and_small_ones(gpu):
         assert (np.abs(values(got, M.BF16) - want)[mine] <= tol[mine]).all()
 
 
+@pytest.mark.parametrize("dt", [M.BF16, M.F16], ids=NAME.get)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("form", ["one wave", "four waves", "split, one wave", "split, four waves"])
+def test_unseen_values_reach_nothing_on_any_variant(gpu, form, where, bad, dt):
+    """As test_attention_unseen_rows_reach_nothing, in half too, with up to 16 rows a key head (one wave a workgroup) and with keys
+    split over workgroups, capped and with a bias; every row behind a document is bad for 70 rows, more than a tile."""
+    one, split = "one" in form, "split" in form
+    lens_q = [3, 7, 1, 5] if one else [3, 40, 100, 33]
+    lens_k = [1500, 1200, 17, 2050] if split else [65, 33, 1, 130] if one else [65, 100, 101, 33]
+    docs, nq, nk = packed(lens_q, lens_k, mask="causal", gap=70)
+    nq, nk = nq + 70, nk + 70
+
+    def edit(raw):
+        x = raw[where]
+        for doc in docs:
+            end = doc[2] + doc[3]
+            x[end:end + 70] = bad
+            if doc[3] > 1:
+                x[end - 1, 0] = bad
+                x[end - 1 - doc[1] // 2, 1, 3] = bad
+
+    for heads, kv, d, cap, slopes in ((2, 2, 64, 0.0, None), (4, 2, 128, 0.0, np.float32([0.5, 0.25, 0.0, 0.01])), (2, 2, 64, 9.0, None)):
+        a = Attn(docs, nq, nk, heads, kv, d, dt, cap=cap, slopes=slopes, edit=edit, seed=len(form))
+        g, need = a.args(), C.c_uint64()
+        M.call("mk_attention_packed_workspace", C.byref(g), C.byref(need))
+        assert (need.value > 0) == split, need.value
+        got, mine = a.run().result()
+        got = values(got, dt)
+        want, tol = attend(a.val["q"], a.val["k"], a.val["v"], docs, a.scale, cap, slopes, dt, dt)
+        with np.errstate(all="ignore"):
+            fine = np.isfinite(want) & mine[:, None, None]
+            assert (np.abs(got - want)[fine] <= tol[fine]).all()
+            rest = ~np.isfinite(want) & mine[:, None, None]
+            assert not np.isfinite(got[rest]).any()
+            # a seen NaN makes its row NaN: all dims of it in K, its own in V
+            assert rest.any() and (not np.isnan(bad) or np.isnan(got[rest]).all())
+
+
+def test_seen_scores_of_infinity_make_the_row_nan(gpu):
+    for dt in (M.BF16, M.F16):
+        for rows, nk in ((5, 90), (40, 300)):
+            def edit(raw):
+                one_dim(raw)
+                raw["k"][nk - rows + 2, :, 5] = np.inf
+
+            docs = [(0, rows, 0, nk, nk - rows, CAUSAL, 0)]
+            a = Attn(docs, rows, nk, 2, 2, 64, dt, edit=edit)
+            got = values(a.run().result()[0], dt)
+            assert np.isnan(got[2:]).all() and np.isfinite(got[:2]).all()
+
+
 def test_no_keys_and_null_k_and_v(gpu):
     a = Attn([(0, 5, 0, 0, 0, 0, 0), (7, 140, 3, 0, 4, CAUSAL, 0)], 150, 1, 2, 2, 64, M.BF16)
     g = a.args()
