@@ -731,15 +731,18 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus, uint64_t room)
     const uint32_t width = a->parts * a->rank, chunks = cdiv(width, 128), tiles = cdiv(a->rows, kRows);
     const uint64_t macs = uint64_t(a->rows) * width * a->K, macs2 = uint64_t(a->rows) * a->N * a->rank;
     const uint32_t per = a->N / a->parts;
-    // (its 8 values of t at a time take 1.3 us for every 4096 k: us in two launches / in one of 1 row of 4096 to 4096 by rank 16
-    // 6.1 / 5.4, of 32 by rank 32 6.9 / 9.1, of 24 to 3 x 4096 by rank 16 6.9 / 7.6, on the device alone)
+    // (its 8 values of t at a time take 1.3 us for every 4096 k: us in two launches / in one, on the device alone, of 1 row of 4096 to 4096
+    // by rank 16 5.7 / 5.2, of 32 by rank 32 6.9 / 9.1, of 64 by rank 16 5.9 / 5.1 in runs and 6.5 / 5.6 in no order, of 256 x 1280 to 5120 6.8 /
+    // 4.7 and 9.1 / 11.6. 24 rows of 16 adapters to 3 x 4096 by rank 16 6.5 / 8.0, but 9.4 / 8.9 a call through the Python binding, whose
+    // time is the host's: one launch, and a captured graph of that call is the slower for it.)
     const uint64_t again = uint64_t(a->rows) * a->parts * cdiv(per, kOneCols) * a->rank * a->K;
     p.one = a->rows <= 1024 && a->rank / 8 * cdiv(a->K, 8 * kOneThreads) <= 2 && again <= (1u << 25);
-    // us by rows / by tiles: 64 x 4096 to 4096 by rank 16 6.6 / 13.6, 512 by rank 32 12 to 25 / 15 to 22, 1000 x 1280 to 3840 by rank
-    // 32 (2^26.9 products) 26 / 17 where rows of one adapter are together; 6.8 / 49, 24 / 61, 41 / 72 in no order, where a tile takes
-    // its adapters one after the other. (1024 x 4096 to 4096 by rank 16, at the border: 27 / 16 and 28 / 56.)
-    p.vec1 = a->rows <= 4096 && macs <= (1u << 26);
-    p.vec2 = a->rows <= 4096 && macs2 <= (1u << 26);
+    // us by rows / by tiles in runs that are said to be grouped, and in no order (8 adapters, sorted for the tiles): 512 x 4096 to 4096 by
+    // rank 16 (2^25 products each) 9.6 / 14.2, 14 / 29; 1024 (2^26) 24 / 14, 27 / 28; 512 x 1280 to 3840 by rank 32 in 3 parts (2^25.9)
+    // 10 / 17, 22 / 37; 1024 (2^26.9) 17 / 17, 42 / 34; 256 x 4096 to 12288 by rank 32 in 3 parts (2^26.6) 20 / 20, 31 / 40; 2048 x 12288
+    // to 4096 by rank 64 228 / 30, 261 / 59.
+    p.vec1 = a->rows <= 4096 && macs < (1u << 26);
+    p.vec2 = a->rows <= 4096 && macs2 < (1u << 26);
     // Where a product goes by tiles, the other one by rows or not (us in no order without / with, and in runs, where finding that out
     // is all it does: 2000 x 1280 to 5120 by rank 16 58 / 35 and 24 / 27, 2000 x 256 to 12288 99 / 46 and 35 / 38, 600 x 12288 to 640 32 / 22 and
     // 14 / 19; byte offsets from the first row on are below 2^31).

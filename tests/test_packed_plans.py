@@ -86,3 +86,10 @@ def test_rows_are_sorted_as_far_as_byte_offsets_reach():
                               ((1 << 18) + 1, dict(ldx=8, ldc=8, ldbase=8), 0)):
         kw = dict(dict(ldx=4096, ldc=12288, ldbase=12288), **kw)
         assert plan(rows, 8, 8, 8, **kw)[ORDER] == sorted_, (rows, kw)
+
+
+def test_a_product_of_2_to_26_and_more_goes_by_tiles():
+    assert plan(1024, 4096, 4088, 16)[A_TILE:COLUMNS + 1] == [32, 0]
+    assert plan(1024, 4088, 4096, 16)[A_TILE:COLUMNS + 1] == [0, 512]
+    assert plan(1024, 4096, 4096, 16)[A_TILE:COLUMNS + 1] == [32, 512]
+    assert plan(1023, 4096, 4096, 16)[:3] == [0, 0, 0]
