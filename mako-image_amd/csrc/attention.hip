@@ -56,7 +56,6 @@ __device__ inline uint32_t cvt_bf16x2(float a, float b)
 // kernel over either: the 32 x 32 x 16 MFMA, the packed conversion (v_cvt_pk_bf16_f32 / v_cvt_pk_f16_f32, both
 // round to nearest even), the two-deep dot product the row sums use, and the rounding that keeps the running max
 // exactly representable.
-typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
 typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2;
 template <bool F16> struct Elem;
 template <> struct Elem<false> {

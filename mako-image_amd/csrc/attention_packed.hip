@@ -31,7 +31,6 @@ struct Doc {
     uint32_t blocks; // of 32 NW rows a key head
     uint32_t splits; // workgroups that share a block's keys
     uint32_t slot;   // its first partial result in the workspace, when splits > 1
-    uint32_t pad;
 };
 struct PackedP {
     const uint16_t *q, *k, *v;
@@ -42,23 +41,15 @@ struct PackedP {
     float* part_ml;
     float c;        // scale log2(e); with a cap: 2 scale log2(e) / cap
     float cap;      // cap log2(e)
-    uint32_t heads, kv_heads, group, n_docs, out_f16;
+    uint32_t kv_heads, group, n_docs, out_f16;
     uint32_t first[kMaxDocs]; // a document's first workgroup, a multiple of 8
     uint32_t join[kMaxDocs];  // and that of the second launch
     Doc docs[kMaxDocs];
 };
 
-typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-template <bool F16> __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
-{
-    if constexpr (F16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 // 4 x 16 values of 16 bits from LDS, transposed: 16 lanes read 4 rows of 16 next to each other, 4 a lane, and each gets a column
 __device__ inline u32x2 read_tr(const uint16_t* p)
 {
@@ -94,7 +85,7 @@ __device__ inline Doc find_doc(const PackedP& p, const uint32_t (&table)[kMaxDoc
     auto get = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), of)); };
     first = get(at);
     return Doc{get(d.q_row), get(d.q_rows), get(d.k_row), get(d.k_rows), int32_t(get(uint32_t(d.q_pos))), get(d.block), get(d.prefix),
-               get(d.blocks), get(d.splits), get(d.slot), 0};
+               get(d.blocks), get(d.splits), get(d.slot)};
 }
 
 // Where 4 dims (chunk) of one of a wave's 32 rows are in its partial results: with many rows the rows of a chunk next to each
@@ -365,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         constexpr int ND = 2 * RL, PER = (ND + DS - 1) / DS;
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds) {
-            s_a = mfma<F16>(fk[ds], qf[ds], s_a);
+            s_a = mfma_32x32x16<F16>(fk[ds], qf[ds], s_a);
             __builtin_amdgcn_sched_barrier(0);
             rd(ds + LA);
 #pragma unroll
@@ -393,7 +384,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         };
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds) {
-            s_b = mfma<F16>(fk[DS + ds], qf[ds], s_b);
+            s_b = mfma_32x32x16<F16>(fk[DS + ds], qf[ds], s_b);
             __builtin_amdgcn_sched_barrier(0);
             rd(DS + ds + LA);
             __builtin_amdgcn_sched_barrier(0);
@@ -408,7 +399,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
             const int st = j / DT;
-            oacc[j % DT] = mfma<F16>(fv[j], u32x4{pa[4 * st], pa[4 * st + 1], pa[4 * st + 2], pa[4 * st + 3]}, oacc[j % DT]);
+            oacc[j % DT] = mfma_32x32x16<F16>(fv[j], u32x4{pa[4 * st], pa[4 * st + 1], pa[4 * st + 2], pa[4 * st + 3]}, oacc[j % DT]);
             __builtin_amdgcn_sched_barrier(0);
             rd(2 * DS + j + LA);
             __builtin_amdgcn_sched_barrier(0);
@@ -423,7 +414,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
             const int st = j / DT;
-            oacc[j % DT] = mfma<F16>(fv[2 * DT + j], u32x4{pb[4 * st], pb[4 * st + 1], pb[4 * st + 2], pb[4 * st + 3]}, oacc[j % DT]);
+            oacc[j % DT] = mfma_32x32x16<F16>(fv[2 * DT + j], u32x4{pb[4 * st], pb[4 * st + 1], pb[4 * st + 2], pb[4 * st + 3]}, oacc[j % DT]);
             __builtin_amdgcn_sched_barrier(0);
             rd(2 * DS + 2 * DT + j + LA);
             __builtin_amdgcn_sched_barrier(0);
@@ -483,15 +474,14 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     const float lt = add_xor32(l);
     if (doc.splits > 1) {
         if (w0 + r32 >= rows)
-            return;
+            return; // (rows that are not there write nothing)
         const uint64_t at = (uint64_t(doc.slot) + item) * NW + wave;
         float* o = p.part + at * (32 * D);
-        if (NW > 1 || w0 + r32 < rows) // (of a few rows the others' are not written)
 #pragma unroll
         for (int i = 0; i < 4 * DT; ++i)
             *reinterpret_cast<f32x4*>(o + part_at<D, NW>(2 * i + hk, r32)) =
                 f32x4{oacc[i / 4][4 * (i % 4)], oacc[i / 4][4 * (i % 4) + 1], oacc[i / 4][4 * (i % 4) + 2], oacc[i / 4][4 * (i % 4) + 3]};
-        if (hk == 0 && w0 + r32 < rows) {
+        if (hk == 0) {
             p.part_ml[2 * (at * 32 + r32)] = m;
             p.part_ml[2 * (at * 32 + r32) + 1] = lt;
         }
@@ -543,7 +533,7 @@ template <int D, int NW, uint32_t G> __global__ __launch_bounds__(D / 4 * join_r
     const uint32_t kvh = at / (doc.blocks * PER), bi = at / PER % doc.blocks, sub = at % PER; // (blocks as above, from the last one)
     const uint32_t g = threadIdx.x / T, q = threadIdx.x % T, chunk = q / RW;
     const uint32_t in_block = sub * RW + q % RW, row = (doc.blocks - 1 - bi) * (32 * NW) + in_block;
-    if (kvh >= p.kv_heads || (doc.blocks - 1 - bi) * (32 * NW) + sub * RW >= rows)
+    if ((doc.blocks - 1 - bi) * (32 * NW) + sub * RW >= rows)
         return; // (the whole workgroup)
     const uint64_t slot = uint64_t(doc.slot) + (uint64_t(kvh) * doc.blocks + bi) * doc.splits;
     const uint32_t wave = in_block / 32, r32 = in_block % 32;
@@ -600,8 +590,6 @@ template <int D, int NW, uint32_t G> __global__ __launch_bounds__(D / 4 * join_r
         u32x2{pack_x2(o[0], o[1], h), pack_x2(o[2], o[3], h)};
 }
 
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
 // everything but the operands' addresses, for the call and for its workspace's size
 mk_status check_shape(const mk_attn_packed_args* a)
 {
@@ -656,7 +644,6 @@ mk_status check_shape(const mk_attn_packed_args* a)
     return MK_OK;
 }
 
-
 // One launch: up to kMaxDocs documents from docs[next] on, the longest first, and how their keys are split.
 struct Launch {
     uint32_t nw;          // waves a workgroup (32 rows each)
@@ -684,7 +671,7 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
         sum += uint64_t(cdiv(uint64_t(d.q_rows) * group, 128)) * a->kv_heads;
         if (n && sum > kMostGroups)
             break;
-        p.docs[n++] = Doc{d.q_row, d.q_rows, d.k_row, d.k_rows, d.q_pos, d.block, d.prefix, 0, 1, 0, 0};
+        p.docs[n++] = Doc{d.q_row, d.q_rows, d.k_row, d.k_rows, d.q_pos, d.block, d.prefix, 0, 1, 0};
         most_rows = std::max(most_rows, uint64_t(d.q_rows) * group);
     }
     // longest first (at most kMaxDocs: an insertion sort)
@@ -782,14 +769,6 @@ template <int D> void launch_all(const PackedP& p, const Launch& l, bool f16, in
     else
         join_kernel<D, 4, 4><<<l.joins, 1024, 0, s>>>(p);
 }
-mk_status device_cus(uint32_t* cus)
-{
-    int dev = 0, n = 0;
-    MK_HIP(hipGetDevice(&dev));
-    MK_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
-    *cus = n > 0 ? uint32_t(n) : 1u;
-    return MK_OK;
-}
 // whether a document has query rows, and (keys) one of those keys
 bool any_rows(const mk_attn_packed_args* a, bool* keys = nullptr)
 {
@@ -820,7 +799,7 @@ mk_status mk_attention_packed_workspace(const mk_attn_packed_args* a, uint64_t* 
     if (!any_rows(a))
         return MK_OK;
     uint32_t cus = 1;
-    MK_TRY(device_cus(&cus));
+    MK_TRY(compute_units(cus));
     PackedP p;
     Launch l;
     for (uint32_t i = 0; i < a->n_docs;) {
@@ -844,7 +823,7 @@ mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
     if (!a->q || !a->out || (keys && (!a->k || !a->v)))
         return fail(MK_ERR_ARG, "attention_packed: null argument (q and out are required, k and v for documents with keys)");
     uint32_t cus = 1;
-    MK_TRY(device_cus(&cus));
+    MK_TRY(compute_units(cus));
     PackedP p;
     Launch l;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -861,7 +840,6 @@ mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream)
     p.slopes = a->slopes;
     p.c = mode & kCap ? 2.0f * kLog2e * a->scale / a->cap : a->scale * kLog2e;
     p.cap = a->cap * kLog2e;
-    p.heads = a->heads;
     p.kv_heads = a->kv_heads;
     p.group = a->heads / a->kv_heads;
     p.out_f16 = a->out_dtype == MK_F16;

@@ -2,6 +2,7 @@
 #include "common.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <mutex>
 #include <vector>
@@ -42,6 +43,23 @@ bool capturing(const void* stream)
         return true;
     }
     return cap != hipStreamCaptureStatusNone;
+}
+
+mk_status compute_units(uint32_t& n)
+{
+    static std::atomic<int> known[64];
+    int dev = 0, cus = 0;
+    MK_HIP(hipGetDevice(&dev));
+    if (dev >= 0 && dev < 64)
+        cus = known[dev].load(std::memory_order_relaxed);
+    if (!cus) {
+        MK_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+        cus = std::max(cus, 1);
+        if (dev >= 0 && dev < 64)
+            known[dev].store(cus, std::memory_order_relaxed);
+    }
+    n = uint32_t(cus);
+    return MK_OK;
 }
 
 void set_error(const std::string& msg) { g_error = msg; }

@@ -14,6 +14,7 @@ namespace mk {
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
 typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 bf16x4;
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
 typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
@@ -48,6 +49,15 @@ __device__ inline void buf_load_lds16(BufRes, lds_void*, uint32_t, uint32_t) {}
 __device__ inline u32x4 buf_load16(BufRes, uint32_t, uint32_t) { return u32x4{}; }
 #endif
 
+// c + a b of 32 x 32 x 16, 8 values of bf16 or half a lane and operand
+template <bool F16> __device__ inline f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c)
+{
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
 // ---- GEMM dispatch plan (gemm.hip), shared with the engine's launch-grouping cost model ----
 struct GemmPlan {
     int bm;          // tile height in tokens (256, or 128 for launches of few tiles)
@@ -75,6 +85,8 @@ bool known_stream(const void* stream);
 void forget_stream(const void* stream);
 // Whether a stream is being captured into a graph (or cannot be asked because another one is).
 bool capturing(const void* stream);
+// compute units of the current device, asked once a device (the question costs as much as a launch)
+mk_status compute_units(uint32_t& n);
 // To be called before a stream is destroyed: waits for its last stream-K, split-K and group norm launches and frees their
 // workspaces for other streams (an event must not be asked after the stream it was recorded on is gone).
 void release_stream(const void* stream);
@@ -347,6 +359,7 @@ uint64_t tensor_key(uint64_t seed, const char* name);
 __host__ __device__ inline uint32_t vt_col(uint32_t k) { return (k & ~12u) | ((k & 4u) << 1) | ((k & 8u) >> 1); }
 
 inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
+inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 inline uint64_t round_up(uint64_t a, uint64_t b) { return (a + b - 1) / b * b; }
 
 } // namespace mk

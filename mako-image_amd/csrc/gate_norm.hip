@@ -447,7 +447,6 @@ void launch_rows(const mk_gate_norm_args& g, hipStream_t s)
         launch_gate_norm<16, 3, 4>(g, s);
 }
 
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool float_type(uint32_t t) { return t == MK_F32 || t == MK_BF16 || t == MK_F16; }
 
 } // namespace

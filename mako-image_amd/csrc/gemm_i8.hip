@@ -11,7 +11,6 @@
 #include "common.hpp"
 
 #include <algorithm>
-#include <atomic>
 #include <string>
 #include <type_traits>
 #include <utility>
@@ -876,26 +875,6 @@ template <int EC> mk_status launch(const I8P& p, uint32_t cus, hipStream_t s)
     MK_LAUNCH_CHECK("gemm_i8");
     return MK_OK;
 }
-
-// Compute units of the current device, asked once a device (the question costs as much as a launch).
-mk_status compute_units(uint32_t& n)
-{
-    static std::atomic<int> known[64];
-    int dev = 0, cus = 0;
-    MK_HIP(hipGetDevice(&dev));
-    if (dev >= 0 && dev < 64)
-        cus = known[dev].load(std::memory_order_relaxed);
-    if (!cus) {
-        MK_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-        cus = std::max(cus, 1);
-        if (dev >= 0 && dev < 64)
-            known[dev].store(cus, std::memory_order_relaxed);
-    }
-    n = uint32_t(cus);
-    return MK_OK;
-}
-
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // The checks of a call's arguments, and the kernels' (an empty product's, M or batch 0, too).
 mk_status prepare(const mk_gemm_args* a, const float* ascale, I8P& p)

@@ -16,8 +16,6 @@ namespace mk {
 
 namespace {
 
-typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
-
 struct LoraP {
     const uint16_t *x, *a, *b;
     const float* scale;
@@ -54,13 +52,6 @@ __device__ inline int adapter_of(const LoraP& p, uint32_t row)
 // s_waitcnt immediate: vmcnt vm, lgkmcnt 0 (vmcnt's bits 3:0 and 15:14, expcnt not waited for)
 constexpr int wait_vm(int vm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4); }
 
-template <bool F16> __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
-{
-    if constexpr (F16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 constexpr uint32_t kOut = 0x80000000u; // a byte offset past every buffer resource here
 constexpr int kRows = 64;              // rows of a workgroup of the second product
 // the row at a place of the tiles from first on, counted from there or, in order, from row 0 (row_base), and its adapter (-1: none)
@@ -372,7 +363,7 @@ template <bool F16, int NB> __global__ __launch_bounds__(256) void shrink_tile(L
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < NB; ++j)
-                        acc[i][j] = mfma<F16>(af[j], xf[i], acc[i][j]);
+                        acc[i][j] = mfma_32x32x16<F16>(af[j], xf[i], acc[i][j]);
             }
         };
         issue(0, s0);
@@ -624,7 +615,7 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
                                 const u32x4 tf = *reinterpret_cast<const u32x4*>(tv + (s * kRows + h * 32) * pad + at + q * 8);
 #pragma unroll
                                 for (int t = 0; t < 4; ++t)
-                                    acc[h][t] = mfma<F16>(tf, bf[t][q], acc[h][t]);
+                                    acc[h][t] = mfma_32x32x16<F16>(tf, bf[t][q], acc[h][t]);
                             }
                 };
                 uint32_t k = 0;
@@ -690,8 +681,6 @@ template <bool F16, uint32_t CT, bool FUSE> __global__ __launch_bounds__(256, 2)
 // ------------------------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------------------------
-
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // sizes and types, for the call and for its workspace's size
 mk_status check_sizes(const mk_lora_rows_args* a)
@@ -781,14 +770,6 @@ Plan plan_of(const mk_lora_rows_args* a, uint32_t cus, uint64_t room)
     p.fuse = a->rank >= 64;
     return p;
 }
-mk_status device_cus(uint32_t* cus)
-{
-    int dev = 0, n = 0;
-    MK_HIP(hipGetDevice(&dev));
-    MK_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
-    *cus = n > 0 ? uint32_t(n) : 1u;
-    return MK_OK;
-}
 
 template <bool F16, uint32_t CT> void launch_one(const LoraP& p, hipStream_t s)
 {
@@ -842,7 +823,7 @@ mk_status mk_lora_rows_workspace(const mk_lora_rows_args* a, uint64_t* bytes)
     if (!a->rows)
         return MK_OK;
     uint32_t cus = 1;
-    MK_TRY(device_cus(&cus));
+    MK_TRY(compute_units(cus));
     *bytes = workspace_of(a, plan_of(a, cus, UINT64_MAX).splits);
     return MK_OK;
 }
@@ -884,7 +865,7 @@ mk_status mk_lora_rows(const mk_lora_rows_args* a, void* stream)
     if (!a->workspace || a->workspace_bytes < workspace_of(a, 1))
         return fail(MK_ERR_ARG, "lora_rows: the workspace holds less than (4 parts rank + 8) rows bytes");
     uint32_t cus = 1;
-    MK_TRY(device_cus(&cus));
+    MK_TRY(compute_units(cus));
     const Plan plan = plan_of(a, cus, a->workspace_bytes);
     LoraP p{static_cast<const uint16_t*>(a->x), static_cast<const uint16_t*>(a->a), static_cast<const uint16_t*>(a->b), a->scale,
             a->ids, a->base, a->c, static_cast<float*>(a->workspace),

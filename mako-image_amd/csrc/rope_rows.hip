@@ -191,7 +191,6 @@ template <uint32_t IN> void launch_out(const RopeP& p, uint32_t out, bool f32_po
         launch_mode<IN, MK_F16>(p, f32_pos, mode, s);
 }
 
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int64_t size_of(uint32_t t) { return t == MK_F32 ? 4 : 2; }
 bool float_type(uint32_t t) { return t == MK_F32 || t == MK_BF16 || t == MK_F16; }
 
