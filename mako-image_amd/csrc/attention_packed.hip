@@ -20,8 +20,9 @@ constexpr int kKT = 64;           // keys a tile
 constexpr float kUp = 7.0f;
 template <bool F16> constexpr float kLazyP = F16 ? 32768.0f : 256.0f;
 constexpr float kLeast = -3.402823466e38f; // m of rows without a score above -inf
-// |m| from which on scores are rounded before m is taken off them. Below it one fma does both, exact against any m; from 2^31 on
-// half a step of m itself, which the largest weight would be off by, no longer fits a weight's exponent (a half's from 2^26).
+// |m| from which on scores are rounded before m is taken off them. Below it one fma does both, exact against any m (without a bias or
+// a cap: with them s - m or cap - m is rounded first, by up to half a step of m, as a score in fp32 of m's size is); from 2^31 on half
+// a step of m itself, which the largest weight would be off by, no longer fits a weight's exponent (a half's from 2^26).
 constexpr float kLargeM = 16777216.0f;
 
 struct Doc {
@@ -204,7 +205,10 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         return x;
     };
     auto masked = [](float x, const Half& h, int r) { return 8 * (r / 4) + r % 4 < h.more ? x : -__builtin_inff(); };
-    // the weights of pair j of a half against `from` (and then `less`), packed, and their sum
+    // The weights of pair j of a half against `from` (and then `less`), packed, and their sum. The second product takes them rounded to the
+    // inputs' type, the matrix instruction's: of the output's error against 64 bits of 0.0023 (16411 keys, bf16; its own rounding alone
+    // 0.0016) that is 0.0016. A sum of the rounded weights changes nothing (0.0023), and a second product of what the rounding left
+    // would take half as many matrix instructions more and make NaN of infinities in V (0 x inf).
     auto pair = [&](const f32x16& sc, const Half& h, int j, uint32_t (&pw)[8], float& ls, float from, auto less, auto edge_c) {
         float x0 = score(sc[2 * j], h, 2 * j, from), x1 = score(sc[2 * j + 1], h, 2 * j + 1, from);
         if constexpr (std::is_same_v<decltype(less), float>) {
@@ -680,7 +684,9 @@ uint32_t plan_launch(const mk_attn_packed_args* a, uint32_t next, uint32_t cus, 
             std::swap(p.docs[j], p.docs[j - 1]);
     // One wave a workgroup where a key head has few rows in every document (us with one / with four: 1 row of 32 heads of 128 on
     // 8 over 16411 keys 22.3 / 24.4, 16 rows of 20 heads of 64 over 4096 11.8 / 13.7; 32 rows over 77 6.2 / 5.7, 32 rows of 32 heads
-    // of 128 over 4096 25.1 / 22.6: four waves share a tile's loads).
+    // of 128 over 4096 25.1 / 22.6: four waves share a tile's loads). Single rows next to a prompt take its four waves, three of them
+    // idle, in the prompt's launch (us so / in a launch of their own behind the prompt's: 31 rows over 2000 keys, 32 heads of 128 on 8, and
+    // a prompt of 512 63 / 69, of 128 67 / 64, of 2048 99 / 104; 20 heads of 64, 512 86 / 106, 17 121 / 98; 7 rows over 16411 and 512 119 / 113).
     out.nw = most_rows <= 16 ? 1 : 4;
     const uint32_t resident = cus * (out.nw == 4 || a->d == 128 ? 2 : 4);
     uint64_t tiles = 0, longest = 0;
