@@ -49,6 +49,7 @@ struct PackedP {
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // 4 x 16 values of 16 bits from LDS, transposed: 16 lanes read 4 rows of 16 next to each other, 4 a lane, and each gets a column
@@ -299,9 +300,9 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         __syncthreads();
         return true;
     };
-    // `none`: a lane's weights of the tile that are zero, a bit each, those of half b above those of half a
-    auto add_odd = [&](int t, uint32_t none) __attribute__((always_inline)) {
-        const uint32_t other = uint32_t(__shfl_xor(int(none), 32)), none0 = hk ? other : none, none1 = hk ? none : other;
+    // `some`: a lane's weights of the tile that are not zero: of pair j of half h bits 8 h + j and 16 + 8 h + j
+    auto add_odd = [&](int t, uint32_t some) __attribute__((always_inline)) {
+        const uint32_t other = uint32_t(__shfl_xor(int(some), 32)), some0 = hk ? other : some, some1 = hk ? some : other;
 #pragma unroll 1
         for (int i = 0, n = tile_keys(t); i < n; ++i) {
             const int key = t * kKT + i;
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             if (key >= lim)
                 continue;
             // (key 8 r / 4 + 4 hk + r % 4 of a half is lane half hk's value r)
-            const bool zero = (i & 4 ? none1 : none0) >> (i / 32 * 16 + i % 32 / 8 * 4 + i % 4) & 1;
+            const bool zero = !((i & 4 ? some1 : some0) >> (i % 2 * 16 + i / 32 * 8 + i % 32 / 8 * 2 + i % 4 / 2) & 1);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     // products P V of half a. A lane's part of their sum decides afterwards whether a half is made again against a new m:
     // a score more than 8 (in log2 units) above m puts that sum above kLazyP.
     constexpr int LA = 3, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
-    auto tile = [&](int t, int next, auto buf_c, auto edge_c, bool odd, uint32_t& none) __attribute__((always_inline)) {
+    auto tile = [&](int t, int next, auto buf_c, auto edge_c, bool odd, uint32_t& some) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value;
         constexpr bool EDGE = decltype(edge_c)::value;
         const int k0 = t * kKT;
@@ -369,13 +370,13 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             __builtin_amdgcn_sched_barrier(0);
         }
         const Half ha = half_of(k0), hb = half_of(k0 + 32);
-        auto zeros = [&](const uint32_t (&pw)[8], int half) {
+        auto not_zero = [&](const uint32_t (&pw)[8], int half) {
             if constexpr (EDGE) {
                 if (!odd)
                     return;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    none |= (uint32_t(!(pw[j] & 0xffffu)) | uint32_t(!(pw[j] >> 16)) << 1) << (16 * half + 2 * j);
+                    some |= __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, pw[j]), u16x2{1, 1})) << (8 * half + j);
             }
         };
         auto chunk = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, int c) {
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         if (__any(la > kLazyP<F16>))
             redo(s_a, ha, pa, la, edge_c);
         l += la;
-        zeros(pa, 0);
+        not_zero(pa, 0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         if (__any(lb > kLazyP<F16>))
             redo(s_b, hb, pb, lb, edge_c);
         l += lb;
-        zeros(pb, 1);
+        not_zero(pb, 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
@@ -439,12 +440,12 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         bool odd = false;
-        uint32_t none = 0;
+        uint32_t some = 0;
         if constexpr (decltype(edge_c)::value)
             odd = wg_lim < t * kKT + tile_keys(t) && find_odd(t, buf_c);
-        tile(t, tile_at(i + 1), buf_c, edge_c, odd, none);
+        tile(t, tile_at(i + 1), buf_c, edge_c, odd, some);
         if (decltype(edge_c)::value && odd)
-            add_odd(t, none);
+            add_odd(t, some);
     };
     if (tid == 0)
         odd_tile = 0; // (the first step's barrier is behind it)
