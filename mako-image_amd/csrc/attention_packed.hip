@@ -15,8 +15,8 @@ namespace {
 constexpr uint32_t kMaxDocs = 64; // documents a launch: they go by kernel argument, in less than 4 KB
 constexpr int kKT = 64;           // keys a tile
 // The exponentials' reference m moves only when a weight against it passes 2^8, in half 2^15 (below). For half weights it lies 7 under
-// the largest score's next whole number: a weight loses 2^-25 below half's normal range, so 2^-31 of the largest (with m
-// the largest score itself, 2^17 keys of 2^-25.5 each, 0.3% of their row, came out as nothing). bf16 has fp32's range.
+// the largest score, whose own weight is then 2^7, unrounded: a weight loses 2^-25 below half's normal range, so 2^-32 of the largest (with
+// m the largest score itself, 2^17 keys of 2^-25.5 each, 0.3% of their row, came out as nothing). bf16 has fp32's range.
 constexpr float kUp = 7.0f;
 template <bool F16> constexpr float kLazyP = F16 ? 32768.0f : 256.0f;
 constexpr float kLeast = -3.402823466e38f; // m of rows without a score above -inf
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             if constexpr (decltype(edge_c)::value)
                 x[r] = masked(x[r], h, r);
         }
-        const float top = max_xor32(max16(x)), mn = fmaxf(m, F16 ? ceilf(top) - kUp : top), alpha = __builtin_amdgcn_exp2f(m - mn);
+        const float top = max_xor32(max16(x)), mn = fmaxf(m, F16 ? top - kUp : top), alpha = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         const bool large = fabsf(m) >= kLargeM;
         ref = large ? kLeast : m;

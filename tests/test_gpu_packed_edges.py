@@ -159,3 +159,24 @@ def test_no_keys_and_null_k_and_v(gpu):
     M.call("mk_attention_packed", C.byref(g), None)
     got, mine = a.result()
     assert (got[mine] == 0).all() and mine.sum() == 145
+
+
+@pytest.mark.parametrize("dt", [M.BF16, M.F16], ids=NAME.get)
+@pytest.mark.parametrize("rows, nk, workspace", [(1, 1, False), (3, 130, True), (3, 2000, True), (70, 300, False)])
+def test_a_row_with_one_key_of_weight_is_its_value(gpu, rows, nk, workspace, dt):
+    """The largest score's own weight is a power of two, with no rounding: scores up to 1000, off by 2^-14 at most (2^-25 of them in log2
+    units), move the weight and the sum alike by far less than half a step of the output's type."""
+    for d, heads, kv, slopes in ((64, 3, 3, None), (128, 4, 1, None), (64, 2, 2, np.float32([0.25, 0.0]))):
+        def edit(raw):
+            one_dim(raw)
+            raw["k"][:, :, 5] = -900.0
+            for g in range(kv):
+                raw["k"][(7 * g + 5) % nk, g, 5] = 0.37 * 2 ** (4 * g)
+
+        a = Attn([(0, rows, 0, nk, nk - rows, 0, 0)], rows, nk, heads, kv, d, dt, scale=1.0, slopes=slopes, edit=edit)
+        got = a.run(workspace).result()[0]
+        bits = M.bf16_bits if dt == M.BF16 else M.f16_bits
+        for h in range(heads):
+            g = h // (heads // kv)
+            want = bits(a.val["v"][(7 * g + 5) % nk, g].astype(np.float32))
+            assert (got[:, h] == want).all(), (d, h)
