@@ -112,6 +112,8 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     // the two buffers are separate objects, so that the compiler can tell a load into one from the reads of the other
     __shared__ __attribute__((aligned(16))) uint16_t sK0[kKT * D], sK1[kKT * D], sV0[kKT * D], sV1[kKT * D];
     __shared__ int odd_tile; // 1 + the last tile in which find_odd found any
+    // there: which of a lane's weights of a half are not zero, those of pair j in bits j and 16 + j (not in registers, which are full)
+    __shared__ uint32_t weighty[2][64 * NW];
     auto sK = [&](int b) { return b ? sK1 : sK0; };
     auto sV = [&](int b) { return b ? sV1 : sV0; };
 
@@ -301,17 +303,15 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         __syncthreads();
         return true;
     };
-    // `some`: a lane's weights of the tile that are not zero: of pair j of half h bits 8 h + j and 16 + 8 h + j
-    auto add_odd = [&](int t, uint32_t some) __attribute__((always_inline)) {
-        const uint32_t other = uint32_t(__shfl_xor(int(some), 32)), some0 = hk ? other : some, some1 = hk ? some : other;
+    auto add_odd = [&](int t) __attribute__((always_inline)) {
 #pragma unroll 1
         for (int i = 0, n = tile_keys(t); i < n; ++i) {
             const int key = t * kKT + i;
             const uint16_t* v = V + int64_t(key) * p.ldv + 4 * hk;
             if (key >= lim)
                 continue;
-            // (key 8 r / 4 + 4 hk + r % 4 of a half is lane half hk's value r)
-            const bool zero = !((i & 4 ? some1 : some0) >> (i % 2 * 16 + i / 32 * 8 + i % 32 / 8 * 2 + i % 4 / 2) & 1);
+            // (key 8 (r / 4) + 4 hk + r % 4 of a half is lane half hk's value r, of its pair r / 2)
+            const bool zero = !(weighty[i / 32][wave * 64 + (i & 4) * 8 + r32] >> (i % 2 * 16 + i % 32 / 8 * 2 + i % 4 / 2) & 1);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
     // products P V of half a. A lane's part of their sum decides afterwards whether a half is made again against a new m:
     // a score more than 8 (in log2 units) above m puts that sum above kLazyP.
     constexpr int LA = 3, CH = 8 / DS; // fragments ahead; pairs of weights behind a product
-    auto tile = [&](int t, int next, auto buf_c, auto edge_c, bool odd, uint32_t& some) __attribute__((always_inline)) {
+    auto tile = [&](int t, int next, auto buf_c, auto edge_c, bool odd) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value;
         constexpr bool EDGE = decltype(edge_c)::value;
         const int k0 = t * kKT;
@@ -375,9 +375,11 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
             if constexpr (EDGE) {
                 if (!odd)
                     return;
+                uint32_t some = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    some |= __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, pw[j]), u16x2{1, 1})) << (8 * half + j);
+                    some |= __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, pw[j]), u16x2{1, 1})) << j;
+                weighty[half][tid] = some;
             }
         };
         auto chunk = [&](const f32x16& sc, const Half& h, uint32_t (&pw)[8], float& ls, int c) {
@@ -441,12 +443,11 @@ __global__ __launch_bounds__(64 * NW, waves_of(D, NW)) __attribute__((amdgpu_wav
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         bool odd = false;
-        uint32_t some = 0;
         if constexpr (decltype(edge_c)::value)
             odd = wg_lim < t * kKT + tile_keys(t) && find_odd(t, buf_c);
-        tile(t, tile_at(i + 1), buf_c, edge_c, odd, some);
+        tile(t, tile_at(i + 1), buf_c, edge_c, odd);
         if (decltype(edge_c)::value && odd)
-            add_odd(t, some);
+            add_odd(t);
     };
     if (tid == 0)
         odd_tile = 0; // (the first step's barrier is behind it)
