@@ -251,3 +251,21 @@ def test_lora_rows_in_no_order_up_to_the_sort_s_reach(gpu):
         want[r] = t @ b[i].T
         tol[r] = ((K / 8 + 16) * u * ta + (H[M.BF16] ** 2 + (rank + 8) * u) * np.abs(t)) @ np.abs(b[i]).T
     assert (np.abs(values(got, M.BF16) - want) <= tol + (H[M.BF16] + 2 * u) * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_lora_random_sizes(gpu, seed):
+    """Any sizes, on whichever kernels they take; tens of thousands of rows with short rows, few rows with long ones."""
+    rng = np.random.default_rng(2000 + seed)
+    parts, rank = int(rng.integers(1, 5)), 8 * int(rng.choice([1, 2, 3, 4, 5, 8, 9, 16, 20, 32]))
+    rows = int(np.exp(rng.uniform(0, np.log(12000))))
+    most = int(min(4096, 6e6 // rows, 3e8 // (rows * parts * rank)))
+    K = 8 * int(rng.integers(1, max(most // 8, 1) + 1))
+    N = 8 * parts * int(rng.integers(1, max(min(most, 3e8 / (rows * rank)) // (8 * parts), 1) + 1))
+    adapters = int(rng.choice([1, 2, 3, 9, 40]))
+    dt = int(rng.choice([M.BF16, M.F16]))
+    in_place = bool(rng.random() < 0.3)
+    a = Lora(rows, K, N, rank, parts, adapters, ids_of(str(rng.choice(["mixed", "runs", "none"])), rows, adapters, seed), dt, int(rng.choice([dt, M.F32])), seed=seed,
+             pad=8 * int(rng.integers(0, 3)), base=in_place or bool(rng.random() < 0.8), scale=bool(rng.random() < 0.7), in_place=in_place, grouped=int(rng.random() < 0.3))
+    print(a.sizes, plan(a), flush=True)
+    a.check()
