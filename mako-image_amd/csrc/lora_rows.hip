@@ -4,8 +4,8 @@
 // and c once each, with 2 rank flops a value. t is a few values a row, so it goes through memory in fp32, as the
 // partial sums of the workgroups that share a row's K (no atomics: the second launch adds them in their order). Very few rows
 // take both products in one launch, and many rows in no order are first put in the order of their adapters by one more.
-// On the device: 4352 x 4096 to 12288 by rank 32 in 3 parts 76 us (x, base and c at 3.3 TB/s), 16401 x 12288 to 4096 by rank
-// 64, fp32 rows, 252 us (3.7 TB/s), 1 row of 4096 to 4096 5.4 us.
+// On the device: 4352 x 4096 to 12288 by rank 32 in 3 parts 75 us (x, base and c at 3.3 TB/s; 84 through single calls), 16401 x 12288 to
+// 4096 by rank 64, fp32 rows, 250 to 277 us (3.4 to 3.7 TB/s), 1 row of 4096 to 4096 5.1 us.
 #include "common.hpp"
 
 #include <algorithm>
