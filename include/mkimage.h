@@ -332,9 +332,9 @@ typedef struct mk_attn_packed_args {
 } mk_attn_packed_args;
 /* out = softmax(s) v over the seen keys, scores, sums and the softmax in fp32; the probabilities enter the second product in the
  * inputs' type, rounded once. A row that sees no key, or only keys of score -inf (below fp32's range), is zero. Rows outside every
- * document are left as they were. What a row does not see does not reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees makes it NaN, an infinity in v that
- * infinity, or NaN where its weight is zero in the inputs' type. All pointers
- * 16-byte aligned (slopes 4). A row's bits may depend on the sizes and the number of the other documents of the call and on
+ * document are left as they were. What a row does not see does not reach it, whatever it holds (infinities and NaN too); a NaN, or a score of +inf, in what it sees
+ * makes it NaN, an infinity in v that infinity, or NaN where its weight is zero in the inputs' type. All pointers 16-byte
+ * aligned (slopes 4). A row's bits may depend on the sizes and the number of the other documents of the call and on
  * the workspace's (they decide how keys are split), not on what the documents hold. */
 mk_status mk_attention_packed(const mk_attn_packed_args* a, void* stream);
 /* The workspace with which that call is fastest on the current device, in bytes (0: none). A smaller batch may ask for more than
@@ -363,7 +363,7 @@ typedef struct mk_lora_rows_args {
     uint32_t c_dtype;    /* base and c: MK_F32, MK_BF16 or MK_F16 */
     void* workspace;     /* 16-byte aligned */
     uint64_t workspace_bytes; /* at least (4 parts rank + 8) rows, rounded up to 16; with less than mk_lora_rows_workspace says, fewer
-                            workgroups share a row's K */
+                            workgroups share a row's K (its sums are then added in another order) */
     uint32_t grouped;    /* 1: rows of one adapter are known to be one after the other, or nearly so (a request's rows): many rows are then
                             not looked through for their order first, 5 us. The results are the same. (Rows in no order are sorted up
                             to 2^18 rows, 1024 adapters and 2 GiB from the first row of x, base or c to the last: beyond, each tile of 64 rows

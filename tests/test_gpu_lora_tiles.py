@@ -269,3 +269,14 @@ def test_lora_random_sizes(gpu, seed):
              pad=8 * int(rng.integers(0, 3)), base=in_place or bool(rng.random() < 0.8), scale=bool(rng.random() < 0.7), in_place=in_place, grouped=int(rng.random() < 0.3))
     print(a.sizes, plan(a), flush=True)
     a.check()
+
+
+@pytest.mark.parametrize("size", [(4161, 520, 264, 24, 3, 5), (300, 1032, 24616, 16, 1, 3), (600, 8200, 64, 16, 1, 4)])
+def test_lora_said_to_be_grouped_or_not_the_same_bits(gpu, size):
+    for ids in ("mixed", "runs"):
+        got = []
+        for grouped in (0, 1):
+            a = Lora(*size, ids_of(ids, size[0], size[5]), M.BF16, M.F32, grouped=grouped)
+            assert plan(a)[ORDER] == 1 - grouped
+            got.append(a.run().result())
+        assert np.array_equal(*got)
